@@ -68,6 +68,8 @@ extern "C" {
 #define ONYX_STATUS_WAIT_TIMEOUT 16u  /* a bounded wait inside the kernel for the row's
                                          partial results gave up (a hardware fault): the
                                          row's output is not valid */
+#define ONYX_STATUS_BAD_POLICY 32u    /* policy sampling: a policy value, a uniform number or
+                                         a draft length of the row is outside its range */
 
 ONYX_API int onyx_abi_version(void);
 ONYX_API const char* onyx_error_string(int code);
@@ -193,6 +195,75 @@ ONYX_API int onyx_masked_sample(const void* logits, int dtype, int64_t rows, int
                                 int64_t row_stride, const uint32_t* mask, int64_t mask_stride,
                                 double temperature, double top_p, uint64_t seed, uint64_t call,
                                 int32_t* out_idx, uint32_t* out_status, void* stream);
+
+/*
+ * Sampling under a policy of its own for each row, with given random numbers. A policy is
+ * four doubles in device memory: temperature (finite, >= 0), top_k (a whole number >= 0, 0:
+ * off), top_p (0 < top_p <= 1) and min_p (0 <= min_p <= 1); row r's is at policies +
+ * r * policy_stride (0: one policy for every row, else >= 4).
+ *
+ * The distribution of a row. Ids are the mask's (NULL: every id). Weights are
+ * exp((v - max) / temperature) in float64; where any value is +inf the +inf ids share the
+ * mass alone; temperature 0 keeps the first maximum alone. Ids are ranked by value, the
+ * lowest id first among equals. top_k keeps the first k of the ranking; top_p the shortest
+ * prefix of those whose mass reaches top_p times their mass (1: off); min_p the ids whose
+ * weight is at least min_p times the largest. With top_k = 0 and min_p = 0 this is the
+ * distribution of onyx_masked_sample, the reference's _filtered_reference_weights
+ * (onyx_cuda/src/onyx_cuda/selection.py); only where the mass reaches top_p exactly (equal
+ * values) that one's sum of rounded shares may keep one id more.
+ *
+ * onyx_policy_sample: out_idx[r] is the first kept id, in id order, whose cumulative weight
+ * exceeds u times the kept total, u = uniforms[r * uniform_stride] in [0, 1), float or
+ * double (uniform_dtype ONYX_DTYPE_F32 or ONYX_DTYPE_F64). Status as for onyx_masked_sample,
+ * and BAD_POLICY for a policy or a uniform outside its range (the row's logits are not
+ * looked at); the id is -1 with any of them.
+ */
+ONYX_API int onyx_policy_sample(const void* logits, int dtype, int64_t rows, int64_t vocab,
+                                int64_t row_stride, const uint32_t* mask, int64_t mask_stride,
+                                const double* policies, int64_t policy_stride,
+                                const void* uniforms, int uniform_dtype, int64_t uniform_stride,
+                                int32_t* out_idx, uint32_t* out_status, void* stream);
+
+/*
+ * The distribution itself: out + r * out_stride gets row r's vocab probabilities, rounded
+ * once to float, 0 for the ids that are not kept and for every id of a row with a status.
+ */
+ONYX_API int onyx_policy_probs(const void* logits, int dtype, int64_t rows, int64_t vocab,
+                               int64_t row_stride, const uint32_t* mask, int64_t mask_stride,
+                               const double* policies, int64_t policy_stride, float* out,
+                               int64_t out_stride, uint32_t* out_status, void* stream);
+
+/*
+ * Speculative sampling of `batch` entries with up to `gamma` drafted tokens each (rows,
+ * masks and drafts laid out as for onyx_spec_verify; masks may be NULL). Entry b's policy is
+ * at policies + b * policy_stride and holds for all its rows; uniforms + b * uniform_stride
+ * are its gamma + 1 numbers. With p the row's distribution and q the draft's, draft i of the
+ * entry's draft_lens[b] (NULL: gamma) is accepted iff uniforms[i] * q(draft) < p(draft). At
+ * the first refusal the token is drawn from max(p - q, 0), after the last acceptance from
+ * the p of the row that follows, each by uniforms[gamma] and the rule of onyx_policy_sample.
+ * So the tokens follow the target's distribution whatever the draft's.
+ * q of draft i: draft_probs + b * dp_batch_stride + i * dp_row_stride, vocab floats (negative
+ * values and NaN count as 0); NULL: each draft was certain (q = 1 at the draft, 0 elsewhere).
+ * Where max(p - q, 0) leaves nothing the draw is from p. A draft outside [0, vocab) is
+ * refused, its row's q still taken off where draft_probs is given.
+ * accept_len[b]: drafts accepted; token[b]: the drawn token; out_status[b]: 0, or the status
+ * of the row that ended the decision (token -1); BAD_POLICY also for a draft length outside
+ * [0, gamma]. The workspace (16-byte aligned, onyx_spec_sample_workspace_size bytes) needs no
+ * initial value; calls that may run at once need separate ones. gamma in [1, 255], batch at
+ * most 2^23 - 1.
+ */
+ONYX_API size_t onyx_spec_sample_workspace_size(int64_t batch, int64_t gamma);
+ONYX_API int onyx_spec_sample(const void* logits, int dtype, int64_t batch, int64_t gamma,
+                              int64_t vocab, int64_t batch_stride, int64_t row_stride,
+                              const uint32_t* masks, int64_t mask_batch_stride,
+                              int64_t mask_row_stride, const int32_t* drafts,
+                              int64_t draft_stride, const float* draft_probs,
+                              int64_t dp_batch_stride, int64_t dp_row_stride,
+                              const int32_t* draft_lens, const double* policies,
+                              int64_t policy_stride, const void* uniforms, int uniform_dtype,
+                              int64_t uniform_stride, int32_t* accept_len, int32_t* token,
+                              uint32_t* out_status, void* workspace, size_t workspace_bytes,
+                              void* stream);
 
 /*
  * Valid-token bitmasks of DFA states (the mask producer): row r of `out` (out_stride >=

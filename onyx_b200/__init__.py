@@ -10,6 +10,8 @@ Python boundary kept as a drop-in:
 * :mod:`onyx_b200.torch_backend` -- ``select_cuda_argmax``;
 * :mod:`onyx_b200.masked_selection` -- batched ``masked_argmax``, ``spec_verify``,
   ``gather_masked_argmax``, ``mask_apply`` on torch tensors;
+* :mod:`onyx_b200.policy_sampling` -- ``policy_sample``, ``policy_probs``, ``spec_sample``:
+  sampling and speculative sampling under a policy per row, from given uniforms;
 * :mod:`onyx_b200.vocab_parallel` -- batch- and vocabulary-sharded multi-GPU selection.
 """
 
@@ -31,6 +33,14 @@ from .masked_selection import (
     masked_argmax,
     spec_verify,
     vocab_partial_keys,
+)
+from .policy_sampling import (
+    STATUS_BAD_POLICY,
+    SamplingPolicy,
+    pack_policies,
+    policy_probs,
+    policy_sample,
+    spec_sample,
 )
 from .torch_backend import select_cuda_argmax, select_masked_cuda_argmax
 from .torch_grammar_mask import TorchCUDAGrammarLogitMask, create_cuda_grammar_logit_mask
@@ -61,4 +71,10 @@ __all__ = [
     "TemperatureTopPSelection",
     "create_cuda_sampler",
     "masked_sample",
+    "SamplingPolicy",
+    "pack_policies",
+    "policy_sample",
+    "policy_probs",
+    "spec_sample",
+    "STATUS_BAD_POLICY",
 ]

@@ -36,6 +36,7 @@ STATUS_ALL_NEG_INF = 2
 STATUS_NAN_IN_SUPPORT = 4
 STATUS_BAD_STATE = 8
 STATUS_WAIT_TIMEOUT = 16
+STATUS_BAD_POLICY = 32
 
 # every symbol include/onyx_b200.h declares, with its ctypes signature
 _i64, _i32, _vp, _sz = ctypes.c_int64, ctypes.c_int, ctypes.c_void_p, ctypes.c_size_t
@@ -67,6 +68,14 @@ SIGNATURES: dict[str, tuple[object, list]] = {
     "onyx_masked_sample": (
         _i32, [_vp, _i32, _i64, _i64, _i64, _vp, _i64, ctypes.c_double, ctypes.c_double,
                ctypes.c_uint64, ctypes.c_uint64, _vp, _vp, _vp]),
+    "onyx_policy_sample": (
+        _i32, [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i32, _i64, _vp, _vp, _vp]),
+    "onyx_policy_probs": (
+        _i32, [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp]),
+    "onyx_spec_sample_workspace_size": (_sz, [_i64, _i64]),
+    "onyx_spec_sample": (
+        _i32, [_vp, _i32, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64,
+               _i64, _vp, _vp, _i64, _vp, _i32, _i64, _vp, _vp, _vp, _vp, _sz, _vp]),
     "onyx_dfa_state_masks": (
         _i32, [_vp, _i32, _i32, _i32, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp]),
     "onyx_ipc_handle_bytes": (_sz, []),

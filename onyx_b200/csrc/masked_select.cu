@@ -23,6 +23,7 @@
 // with one atomicAdd; the CTA that draws the final ticket combines the partials, writes the
 // outputs and resets the counter to zero for the next call. Nothing ever waits on another
 // CTA, so no schedule can hang.
+#include "host_common.h"
 #include "onyx_common.cuh"
 #include "../../include/onyx_b200.h"
 
@@ -1294,7 +1295,7 @@ static cudaError_t dispatch(int dt, bool fast, const ScanParams& p, cudaStream_t
 
 static bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 
-static int finish_launch(cudaError_t e) {
+int finish_launch(cudaError_t e) {
   if (e != cudaSuccess) {
     g_last_cuda_error = (int)e;
     return ONYX_ERR_CUDA;
@@ -1307,7 +1308,7 @@ static int finish_launch(cudaError_t e) {
   return ONYX_OK;
 }
 
-static bool pdl_enabled() { return option(ONYX_OPTION_PDL) != 0; }
+bool pdl_enabled() { return option(ONYX_OPTION_PDL) != 0; }
 
 static int bind_workspace(ScanParams& p, void* ws, size_t ws_bytes, size_t need,
                           int64_t groups) {

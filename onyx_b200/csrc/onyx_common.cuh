@@ -30,6 +30,7 @@ constexpr uint32_t kStatusAllNegInf = 2u;
 constexpr uint32_t kStatusNanInSupport = 4u;
 constexpr uint32_t kStatusBadState = 8u;
 constexpr uint32_t kStatusWaitTimeout = 16u;
+constexpr uint32_t kStatusBadPolicy = 32u;
 
 // partial-result flags
 constexpr uint32_t kFlagAny = 1u;        // the segment holds at least one valid token

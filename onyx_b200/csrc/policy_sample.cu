@@ -1,0 +1,218 @@
+// C entry points of sampling under per-row policies (include/onyx_b200.h): argument checks,
+// the choice of the cluster size, launches.
+#include "host_common.h"
+#include "policy_sample.cuh"
+
+#include "../../include/onyx_b200.h"
+
+#include <algorithm>
+#include <atomic>
+
+namespace onyx {
+
+// Streaming multiprocessors of the current device, asked once per device; 0 on an error.
+static int device_sms(cudaError_t* err) {
+  static std::atomic<int> known[64];
+  int dev = 0;
+  *err = cudaGetDevice(&dev);
+  if (*err != cudaSuccess) return 0;
+  if (dev >= 0 && dev < 64) {
+    const int n = known[dev].load(std::memory_order_relaxed);
+    if (n) return n;
+  }
+  int sms = 0;
+  *err = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (*err != cudaSuccess) return 0;
+  if (dev >= 0 && dev < 64) known[dev].store(sms, std::memory_order_relaxed);
+  return sms;
+}
+
+// CTAs per row: a power of two, as many as the SMs hold two of, at least 4,096 ids each.
+static int cluster_size(int64_t rows, int64_t vocab, int sms) {
+  int k = 1;
+  while (k < kPsMaxCluster && rows * k * 2 <= 2ll * sms && vocab >= 2ll * k * 4096) k *= 2;
+  return k;
+}
+
+template <int OP>
+static int launch_policy(int dtype, PolicyParams& p, int64_t rows, cudaStream_t stream) {
+  cudaError_t e;
+  const int sms = device_sms(&e);
+  if (!sms) return finish_launch(e);
+  p.k = cluster_size(rows, p.vocab, sms);
+  if (rows * p.k > 0x7FFFFFFFll) return ONYX_ERR_INVALID_ARGUMENT;
+  const int64_t per = (int64_t)p.k * kPsWarps * kPsChunk;
+  p.warp_ids = (int32_t)((p.vocab + per - 1) / per * kPsChunk);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(rows * p.k), 1, 1);
+  cfg.blockDim = dim3(kPsThreads, 1, 1);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (p.k > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = (unsigned)p.k;
+    attr[n].val.clusterDim.y = 1;
+    attr[n++].val.clusterDim.z = 1;
+  }
+  if (pdl_enabled()) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  switch (dtype) {
+    case kBF16: e = cudaLaunchKernelEx(&cfg, policy_kernel<kBF16, OP>, p); break;
+    case kF16: e = cudaLaunchKernelEx(&cfg, policy_kernel<kF16, OP>, p); break;
+    default: e = cudaLaunchKernelEx(&cfg, policy_kernel<kF32, OP>, p); break;
+  }
+  return finish_launch(e);
+}
+
+static bool policy_dtype(int dt) { return dt == kF32 || dt == kF16 || dt == kBF16; }
+
+// The checks that the three entry points share; `rows` entries of the policies.
+static int policy_checks(const void* logits, int dtype, int64_t rows, int64_t vocab,
+                         const double* policies, int64_t policy_stride) {
+  if (!policy_dtype(dtype)) return ONYX_ERR_UNSUPPORTED_DTYPE;
+  if (rows < 0 || rows > 0x7FFFFFFFll || vocab <= 0 || vocab > 0x7FFFFFFFll - 1)
+    return ONYX_ERR_INVALID_ARGUMENT;
+  if (rows > 0 && (!logits || !policies)) return ONYX_ERR_INVALID_ARGUMENT;
+  if (policy_stride != 0 && policy_stride < 4) return ONYX_ERR_INVALID_ARGUMENT;
+  return ONYX_OK;
+}
+
+static bool uniform_dtype(int dt) { return dt == kF32 || dt == kF64; }
+
+}  // namespace onyx
+
+using namespace onyx;
+
+extern "C" {
+
+int onyx_policy_sample(const void* logits, int dtype, int64_t rows, int64_t vocab,
+                       int64_t row_stride, const uint32_t* mask, int64_t mask_stride,
+                       const double* policies, int64_t policy_stride, const void* uniforms,
+                       int uniform_dtype_code, int64_t uniform_stride, int32_t* out_idx,
+                       uint32_t* out_status, void* stream) {
+  const int rc = policy_checks(logits, dtype, rows, vocab, policies, policy_stride);
+  if (rc != ONYX_OK) return rc;
+  if (!uniform_dtype(uniform_dtype_code)) return ONYX_ERR_UNSUPPORTED_DTYPE;
+  if (rows == 0) return ONYX_OK;
+  if (!uniforms || !out_idx || !out_status) return ONYX_ERR_INVALID_ARGUMENT;
+  if (rows > 1 && (row_stride < vocab || (mask && mask_stride < (vocab + 31) / 32) ||
+                   uniform_stride < 1))
+    return ONYX_ERR_INVALID_ARGUMENT;
+  PolicyParams p = {};
+  p.logits = logits;
+  p.group_stride = row_stride;
+  p.vocab = vocab;
+  p.mask = mask;
+  p.mask_group_stride = mask_stride;
+  p.policies = policies;
+  p.policy_stride = policy_stride;
+  p.uniforms = uniforms;
+  p.uniform_stride = uniform_stride;
+  p.uniform_f64 = uniform_dtype_code == kF64;
+  p.per_group = 1;
+  p.out_idx = out_idx;
+  p.out_status = out_status;
+  return launch_policy<kOpDraw>(dtype, p, rows, (cudaStream_t)stream);
+}
+
+int onyx_policy_probs(const void* logits, int dtype, int64_t rows, int64_t vocab,
+                      int64_t row_stride, const uint32_t* mask, int64_t mask_stride,
+                      const double* policies, int64_t policy_stride, float* out,
+                      int64_t out_stride, uint32_t* out_status, void* stream) {
+  const int rc = policy_checks(logits, dtype, rows, vocab, policies, policy_stride);
+  if (rc != ONYX_OK) return rc;
+  if (rows == 0) return ONYX_OK;
+  if (!out || !out_status) return ONYX_ERR_INVALID_ARGUMENT;
+  if (rows > 1 && (row_stride < vocab || (mask && mask_stride < (vocab + 31) / 32) ||
+                   out_stride < vocab))
+    return ONYX_ERR_INVALID_ARGUMENT;
+  PolicyParams p = {};
+  p.logits = logits;
+  p.group_stride = row_stride;
+  p.vocab = vocab;
+  p.mask = mask;
+  p.mask_group_stride = mask_stride;
+  p.policies = policies;
+  p.policy_stride = policy_stride;
+  p.per_group = 1;
+  p.out_probs = out;
+  p.out_stride = out_stride;
+  p.out_status = out_status;
+  return launch_policy<kOpProbs>(dtype, p, rows, (cudaStream_t)stream);
+}
+
+size_t onyx_spec_sample_workspace_size(int64_t batch, int64_t gamma) {
+  if (batch <= 0 || gamma < 1 || gamma > 255) return 0;
+  return (size_t)batch * (size_t)(gamma + 1) * sizeof(int4);
+}
+
+int onyx_spec_sample(const void* logits, int dtype, int64_t batch, int64_t gamma, int64_t vocab,
+                     int64_t batch_stride, int64_t row_stride, const uint32_t* masks,
+                     int64_t mask_batch_stride, int64_t mask_row_stride, const int32_t* drafts,
+                     int64_t draft_stride, const float* draft_probs, int64_t dp_batch_stride,
+                     int64_t dp_row_stride, const int32_t* draft_lens, const double* policies,
+                     int64_t policy_stride, const void* uniforms, int uniform_dtype_code,
+                     int64_t uniform_stride, int32_t* accept_len, int32_t* token,
+                     uint32_t* out_status, void* workspace, size_t workspace_bytes,
+                     void* stream) {
+  const int rc = policy_checks(logits, dtype, batch, vocab, policies, policy_stride);
+  if (rc != ONYX_OK) return rc;
+  if (!uniform_dtype(uniform_dtype_code)) return ONYX_ERR_UNSUPPORTED_DTYPE;
+  if (gamma < 1 || gamma > 255 || batch > 0x7FFFFFFFll / 256) return ONYX_ERR_INVALID_ARGUMENT;
+  if (batch == 0) return ONYX_OK;
+  if (!drafts || !uniforms || !accept_len || !token || !out_status)
+    return ONYX_ERR_INVALID_ARGUMENT;
+  const int64_t words = (vocab + 31) / 32;
+  if (row_stride < vocab || (masks && mask_row_stride < words) ||
+      (draft_probs && gamma > 1 && dp_row_stride < vocab))
+    return ONYX_ERR_INVALID_ARGUMENT;
+  if (batch > 1 &&
+      (batch_stride < 0 || (masks && mask_batch_stride < 0) || draft_stride < gamma ||
+       (draft_probs && dp_batch_stride < 0) || uniform_stride < gamma + 1))
+    return ONYX_ERR_INVALID_ARGUMENT;
+  if (!workspace || ((uintptr_t)workspace & 15u) ||
+      workspace_bytes < onyx_spec_sample_workspace_size(batch, gamma))
+    return ONYX_ERR_WORKSPACE;
+  PolicyParams p = {};
+  p.logits = logits;
+  p.group_stride = batch_stride;
+  p.row_stride = row_stride;
+  p.vocab = vocab;
+  p.mask = masks;
+  p.mask_group_stride = mask_batch_stride;
+  p.mask_row_stride = mask_row_stride;
+  p.policies = policies;
+  p.policy_stride = policy_stride;
+  p.uniforms = uniforms;
+  p.uniform_stride = uniform_stride;
+  p.uniform_f64 = uniform_dtype_code == kF64;
+  p.per_group = (int32_t)gamma + 1;
+  p.drafts = drafts;
+  p.draft_stride = draft_stride;
+  p.draft_probs = draft_probs;
+  p.dp_group_stride = dp_batch_stride;
+  p.dp_row_stride = dp_row_stride;
+  p.draft_lens = draft_lens;
+  p.results = static_cast<int4*>(workspace);
+  const int rc2 = launch_policy<kOpSpec>(dtype, p, batch * (gamma + 1), (cudaStream_t)stream);
+  if (rc2 != ONYX_OK) return rc2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((batch + 127) / 128), 1, 1);
+  cfg.blockDim = dim3(128, 1, 1);
+  cfg.stream = (cudaStream_t)stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 1 : 0;
+  return finish_launch(cudaLaunchKernelEx(&cfg, spec_join_kernel, (const int4*)p.results, batch,
+                                          (int)gamma + 1, draft_lens, accept_len, token,
+                                          out_status));
+}
+
+}  // extern "C"

@@ -1,0 +1,704 @@
+// Sampling under a policy of its own for each row: temperature, top-k, top-p and min-p, with
+// the random numbers given by the caller. Three operators share the row's distribution:
+//   draw   one id per row;
+//   probs  the filtered, renormalised probabilities of every id;
+//   spec   speculative sampling of drafted tokens (rows gamma + 1 to an entry).
+//
+// Mathematics. For the valid ids of a row with maximum m, weight w(v) = exp((v - m) / T)
+// (T = 0: the first maximum alone; any +inf: the +inf ids alone, with equal weights). Ids are
+// ranked by (value falling, id rising). top-k keeps the first k; top-p keeps the shortest
+// prefix of those whose mass reaches p times their mass; min-p keeps w >= min_p. All three
+// keep a prefix of the ranking, so the kept set is given by a cut (an order code), the number
+// of ids equal to it that are kept in id order (`take`) and the bound w >= min_p. The draw is
+// the first kept id, in id order, whose cumulative weight exceeds u times the kept total.
+//
+// Sums and weights are float64: whether a cumulative mass reaches p, or an id's interval holds
+// u, decides a whole number, and float32 sums over 10^5 ids would decide it differently for
+// about one row in a hundred.
+//
+// Shape of the work. One cluster of k CTAs per row (k = 1, 2, 4 or 8, the more the fewer the
+// rows); CTA ranks, the warps of a CTA and the 256-id chunks of a warp follow id order, a lane
+// holding 8 consecutive ids. A row is streamed from HBM by the first pass and from L2 by the
+// later ones, so no row length is bound to shared memory. Cluster-wide sums: every CTA stores
+// its part into every CTA's box (distributed shared memory), one cluster barrier publishes
+// them, and all CTAs combine the boxes in rank order, so all hold identical totals and take
+// the same branches.
+#pragma once
+
+#include <cfloat>
+
+#include "onyx_common.cuh"
+
+namespace onyx {
+
+constexpr int kPsThreads = 512;
+constexpr int kPsWarps = kPsThreads / 32;
+constexpr int kPsMaxCluster = 8;
+constexpr int kPsEntries = kPsMaxCluster * kPsWarps;
+constexpr int kPsChunk = 256;  // ids a warp handles at a time, 8 to a lane
+
+enum PolicyOp : int { kOpDraw = 0, kOpProbs = 1, kOpSpec = 2 };
+
+struct PolicyParams {
+  const void* logits;
+  int64_t group_stride;  // elements between entries (spec) or rows
+  int64_t row_stride;    // elements between the rows of one entry (spec)
+  int64_t vocab;
+  const uint32_t* mask;  // nullptr: every id valid
+  int64_t mask_group_stride, mask_row_stride;  // words
+  const double* policies;  // temperature, top_k, top_p, min_p
+  int64_t policy_stride;   // doubles between entries, 0: one policy for all
+  const void* uniforms;
+  int64_t uniform_stride;
+  int32_t uniform_f64;
+  int32_t per_group;  // rows per entry: 1, or gamma + 1
+  int32_t* out_idx;
+  uint32_t* out_status;
+  float* out_probs;
+  int64_t out_stride;
+  const int32_t* drafts;
+  int64_t draft_stride;
+  const float* draft_probs;  // nullptr: each draft has probability 1
+  int64_t dp_group_stride, dp_row_stride;
+  const int32_t* draft_lens;  // nullptr: gamma drafts for every entry
+  int4* results;              // spec: {verdict, token, status, 0} of every row
+  int32_t warp_ids;  // ids per warp, a multiple of kPsChunk
+  int32_t k;         // CTAs per row
+};
+
+enum Verdict : int { kAccepted = 0, kDecided = 1 };
+
+struct RowPolicy {
+  double temperature, top_p, min_p;
+  uint32_t top_k;  // 0: off
+  bool ok;
+};
+
+__device__ __forceinline__ RowPolicy load_policy(const double* p) {
+  RowPolicy r;
+  r.temperature = p[0];
+  const double k = p[1];
+  r.top_p = p[2];
+  r.min_p = p[3];
+  // comparisons are written so that a NaN fails them
+  r.ok = r.temperature >= 0.0 && r.temperature < INFINITY && k >= 0.0 && k < INFINITY &&
+         r.top_p > 0.0 && r.top_p <= 1.0 && r.min_p >= 0.0 && r.min_p <= 1.0 && k == floor(k);
+  r.top_k = r.ok ? (k < 4294967295.0 ? (uint32_t)k : 0xFFFFFFFFu) : 0u;
+  return r;
+}
+
+__device__ __forceinline__ double load_uniform(const PolicyParams& p, int64_t i) {
+  return p.uniform_f64 ? static_cast<const double*>(p.uniforms)[i]
+                       : (double)static_cast<const float*>(p.uniforms)[i];
+}
+
+__device__ __forceinline__ void ps_cluster_arrive() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void ps_cluster_wait() {
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t ps_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+template <class T>
+__device__ __forceinline__ T* ps_remote(T* p, uint32_t rank) {
+  unsigned long long out;
+  asm("mapa.u64 %0, %1, %2;" : "=l"(out) : "l"(p), "r"(rank));
+  return reinterpret_cast<T*>(out);
+}
+
+__device__ __forceinline__ double warp_sum(double v) {
+#pragma unroll
+  for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(~0u, v, d);
+  return v;
+}
+__device__ __forceinline__ double warp_scan(double v, int lane) {  // inclusive
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const double o = __shfl_up_sync(~0u, v, d);
+    if (lane >= d) v += o;
+  }
+  return v;
+}
+__device__ __forceinline__ uint32_t warp_scan(uint32_t v, int lane) {  // inclusive
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const uint32_t o = __shfl_up_sync(~0u, v, d);
+    if (lane >= d) v += o;
+  }
+  return v;
+}
+
+struct PsBox {  // one CTA's part of a cluster-wide reduction
+  double mass;
+  uint32_t count, top;
+};
+
+struct PsShared {
+  PsBox box[2][kPsMaxCluster];  // used alternately: one may still be read as the next is written
+  double part_mass[kPsWarps];
+  uint32_t part_count[kPsWarps], part_top[kPsWarps];
+  // one entry per warp of the cluster, in id order
+  double entry_mass[kPsEntries];
+  uint32_t entry_ties[kPsEntries], entry_before[kPsEntries];
+  double scan_mass[kPsEntries];    // kept mass before the entry
+  uint32_t scan_ties[kPsEntries];  // ties before the entry
+  double total;
+  int owner;
+  uint32_t before;
+};
+
+// The part of a row that one warp owns, and how it is read.
+template <int DT>
+struct RowView {
+  using S = typename Elem<DT>::storage;
+  const S* row;
+  const uint32_t* mask;
+  uint32_t begin, end, vocab;
+  bool vec;  // 16-byte loads: the row starts on a 16-byte boundary
+
+  // f(id of the lane's first element, values, valid bits); every lane of the warp makes every
+  // call, so f may use warp-wide instructions
+  template <class F>
+  __device__ __forceinline__ void each(int lane, F&& f) const {
+    for (uint32_t at = begin; at < end; at += kPsChunk) {
+      const uint32_t id = at + 8u * lane;
+      float v[8];
+      uint32_t bits = 0;
+      if (id < vocab) {
+        const uint32_t left = vocab - id;
+        bits = mask ? (mask[id >> 5] >> (id & 31u)) & 0xFFu : 0xFFu;
+        if (left < 8u) bits &= (1u << left) - 1u;
+        if (vec && left >= 8u) {
+          if constexpr (DT == kF32) {
+            const float4 a = *reinterpret_cast<const float4*>(row + id);
+            const float4 b = *reinterpret_cast<const float4*>(row + id + 4);
+            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+            v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+          } else {
+            const uint4 a = *reinterpret_cast<const uint4*>(row + id);
+            const uint32_t u[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const uint32_t h = (u[j >> 1] >> (16 * (j & 1))) & 0xFFFFu;
+              v[j] = DT == kBF16 ? bf16_bits_to_f32(h) : f16_bits_to_f32(h);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = (uint32_t)j < left ? Elem<DT>::to_f32(row, id + j) : 0.0f;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = 0.0f;
+      }
+      f(id, v, bits);
+    }
+  }
+};
+
+// What decides which ids of the row are kept, and their weights.
+struct RowCut {
+  double top, inv_t, min_p;
+  uint32_t cut, take;  // ids above `cut`, and the first `take` ids equal to it
+  bool flat;           // every kept id weighs 1 (T = 0, or +inf present)
+
+  __device__ __forceinline__ double weight(float v) const {
+    return flat ? 1.0 : exp(((double)v - top) * inv_t);
+  }
+};
+
+template <int DT>
+struct PolicyRow {
+  PsShared& sh;
+  RowView<DT> view;
+  uint32_t rank, k;
+  int warp, lane, entry;
+  int parity = 0;
+
+  __device__ PolicyRow(PsShared& s) : sh(s) {}
+
+  __device__ __forceinline__ void publish() {
+    if (k > 1) {
+      ps_cluster_arrive();
+      ps_cluster_wait();
+    } else {
+      __syncthreads();
+    }
+  }
+
+  // cluster-wide sums of `mass` and `count` and maximum of `top`
+  __device__ PsBox reduce(double mass, uint32_t count, uint32_t top) {
+    mass = warp_sum(mass);
+    count = __reduce_add_sync(~0u, count);
+    top = __reduce_max_sync(~0u, top);
+    if (lane == 0) sh.part_mass[warp] = mass, sh.part_count[warp] = count, sh.part_top[warp] = top;
+    __syncthreads();
+    if (warp == 0) {
+      PsBox b = {0.0, 0u, 0u};
+      for (int i = 0; i < kPsWarps; ++i) {
+        b.mass += sh.part_mass[i];
+        b.count += sh.part_count[i];
+        b.top = max(b.top, sh.part_top[i]);
+      }
+      if ((uint32_t)lane < k) *ps_remote(&sh.box[parity][rank], lane) = b;
+    }
+    publish();
+    PsBox r = {0.0, 0u, 0u};
+    for (uint32_t i = 0; i < k; ++i) {
+      const PsBox b = sh.box[parity][i];
+      r.mass += b.mass;
+      r.count += b.count;
+      r.top = max(r.top, b.top);
+    }
+    parity ^= 1;
+    return r;
+  }
+
+  // mass and count of the valid ids whose order code is at least `code`
+  __device__ PsBox at_least(const RowCut& c, uint32_t code) {
+    double mass = 0.0;
+    uint32_t count = 0;
+    view.each(lane, [&](uint32_t, const float* v, uint32_t bits) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if ((bits >> j & 1u) && ord32(v[j]) >= code) {
+          mass += c.weight(v[j]);
+          ++count;
+        }
+    });
+    return reduce(mass, count, 0u);
+  }
+
+  // fills c.cut and c.take from the policy; `top` is the row's largest order code
+  __device__ void find_cut(RowCut& c, const RowPolicy& pol, uint32_t top) {
+    const uint32_t base = c.flat ? top - 1u : 0u;  // +inf present: those ids alone
+    c.cut = base;
+    c.take = 0;
+    PsBox above = {0.0, 0u, 0u};  // of the ids above the cut
+    bool by_k = false;
+    if (!(pol.temperature > 0.0)) {
+      c.cut = top;
+      c.take = 1;
+      return;
+    }
+    if (pol.top_k && pol.top_k < view.vocab) {
+      uint32_t lo = base, hi = top + 1u;
+      while (hi - lo > 1u) {
+        const uint32_t mid = lo + (hi - lo) / 2u;
+        const PsBox b = at_least(c, mid);
+        if (b.count >= pol.top_k) {
+          lo = mid;
+        } else {
+          hi = mid;
+          above = b;
+        }
+      }
+      if (lo > base) {
+        by_k = true;
+        c.cut = lo;
+        c.take = pol.top_k - above.count;
+      }
+    }
+    if (pol.top_p < 1.0) {
+      const double w_cut = by_k ? c.weight(code_value(c.cut)) : 0.0;
+      const double total = by_k ? above.mass + (double)c.take * w_cut : at_least(c, base + 1u).mass;
+      const double goal = pol.top_p * total;
+      uint32_t lo = c.cut, hi = top + 1u;
+      PsBox over = {0.0, 0u, 0u}, level = {0.0, 0u, 0u};
+      bool have = false;
+      while (hi - lo > 1u) {
+        const uint32_t mid = lo + (hi - lo) / 2u;
+        const PsBox b = at_least(c, mid);
+        if (b.mass >= goal) {
+          lo = mid;
+          level = b;
+          have = true;
+        } else {
+          hi = mid;
+          over = b;
+        }
+      }
+      const uint32_t most = have ? level.count - over.count : c.take;
+      if (by_k || have) {
+        const double w = c.weight(code_value(lo));
+        double t = ceil((goal - over.mass) / w);
+        t = t < 1.0 ? 1.0 : t > (double)most ? (double)most : t;
+        while (t > 1.0 && over.mass + (t - 1.0) * w >= goal) t -= 1.0;
+        while (t < (double)most && over.mass + t * w < goal) t += 1.0;
+        c.cut = lo;
+        c.take = (uint32_t)t;
+      }
+    }
+    if (c.take && !c.flat && c.weight(code_value(c.cut)) < c.min_p) c.take = 0;
+  }
+
+  __device__ static float code_value(uint32_t code) {
+    return __uint_as_float((code & 0x80000000u) ? code & 0x7FFFFFFFu : ~code);
+  }
+
+  // Publishes one entry per warp and scans them: scan_ties, scan_mass, total, before. `w_tie`
+  // is the weight of an id at the cut; entries hold the mass above it.
+  __device__ void scan_entries(double mass, uint32_t ties, uint32_t before, double w_tie,
+                               uint32_t take) {
+    if ((uint32_t)lane < k) {
+      PsShared* r = ps_remote(&sh, lane);
+      r->entry_mass[entry] = mass;
+      r->entry_ties[entry] = ties;
+      r->entry_before[entry] = before;
+    }
+    publish();
+    if (warp == 0) {
+      const int n = (int)k * kPsWarps, per = (n + 31) / 32;
+      const int lo = min(n, lane * per), hi = min(n, lo + per);
+      uint32_t t = 0, b = 0;
+      for (int i = lo; i < hi; ++i) t += sh.entry_ties[i], b += sh.entry_before[i];
+      uint32_t run = warp_scan(t, lane) - t;
+      b = __reduce_add_sync(~0u, b);
+      double m = 0.0;
+      for (int i = lo; i < hi; ++i) {
+        const uint32_t n_tie = sh.entry_ties[i];
+        const uint32_t kept = run < take ? min(n_tie, take - run) : 0u;
+        sh.scan_ties[i] = run;
+        run += n_tie;
+        const double e = sh.entry_mass[i] + (double)kept * w_tie;
+        sh.entry_mass[i] = e;
+        m += e;
+      }
+      const double incl = warp_scan(m, lane);
+      const double prev = __shfl_up_sync(~0u, incl, 1);
+      double acc = lane ? prev : 0.0;  // summed, not subtracted: never below 0
+      for (int i = lo; i < hi; ++i) {
+        sh.scan_mass[i] = acc;
+        acc += sh.entry_mass[i];
+      }
+      if (lane == 31) sh.total = acc;
+      if (lane == 0) sh.before = b;
+    }
+    __syncthreads();
+  }
+
+  // the entry whose interval of kept mass holds `goal` (the last with mass, if rounding leaves
+  // none)
+  __device__ int find_owner(double goal) {
+    if (warp == 0) {
+      const int n = (int)k * kPsWarps;
+      int first = n, last = 0;
+      for (int i = lane; i < n; i += 32) {
+        const double m = sh.entry_mass[i];
+        if (m > 0.0) {
+          last = max(last, i);
+          if (sh.scan_mass[i] + m > goal) first = min(first, i);
+        }
+      }
+      first = __reduce_min_sync(~0u, first);
+      last = __reduce_max_sync(~0u, last);
+      if (lane == 0) sh.owner = first < n ? first : last;
+    }
+    __syncthreads();
+    return sh.owner;
+  }
+
+  // f(id, weights of the lane's 8 ids: 0 where not kept) over this warp's ids
+  template <class F>
+  __device__ __forceinline__ void each_kept(const RowCut& c, F&& f) {
+    uint32_t run = sh.scan_ties[entry];
+    view.each(lane, [&](uint32_t id, const float* v, uint32_t bits) {
+      double w[8];
+      uint32_t tie = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t code = ord32(v[j]);
+        const bool valid = bits >> j & 1u;
+        w[j] = 0.0;
+        if (valid && code == c.cut) tie |= 1u << j;
+        if (valid && code > c.cut) {
+          const double x = c.weight(v[j]);
+          if (x >= c.min_p) w[j] = x;
+        }
+      }
+      if (c.take && __any_sync(~0u, tie)) {
+        const uint32_t n = __popc(tie);
+        const uint32_t incl = warp_scan(n, lane);
+        uint32_t at = run + incl - n;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (tie >> j & 1u) {
+            if (at < c.take) w[j] = c.weight(v[j]);
+            ++at;
+          }
+        run += __shfl_sync(~0u, incl, 31);
+      }
+      f(id, w);
+    });
+  }
+
+  // first id, in id order, whose cumulative weight exceeds `goal`; `start` is the mass before
+  // this warp; weigh(id, w[8]) may replace the kept weights. Whole warp; all lanes return it.
+  template <class W>
+  __device__ int pick(const RowCut& c, double start, double goal, W&& weigh) {
+    int found = -1, last = -1;
+    double run = start;
+    each_kept(c, [&](uint32_t id, double* w) {
+      if (found >= 0) return;  // uniform over the warp
+      weigh(id, w);
+      double s = 0.0;
+      int mine = -1;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        s += w[j];
+        if (w[j] > 0.0) mine = (int)id + j;
+      }
+      const double incl = warp_scan(s, lane);
+      const uint32_t over = __ballot_sync(~0u, s > 0.0 && run + incl > goal);
+      if (over) {
+        const int src = __ffs(over) - 1;
+        const double prev = __shfl_up_sync(~0u, incl, 1);
+        int at = mine;
+        if (lane == src) {
+          double acc = run + (lane ? prev : 0.0);
+#pragma unroll
+          for (int j = 7; j >= 0; --j) {
+            // cumulative weight up to and with j, in the order of a forward walk
+            double x = acc;
+#pragma unroll
+            for (int i = 0; i <= j; ++i) x += w[i];
+            if (w[j] > 0.0 && x > goal) at = (int)id + j;
+          }
+        }
+        found = __shfl_sync(~0u, at, src);
+        return;
+      }
+      last = max(last, mine);
+      run += __shfl_sync(~0u, incl, 31);
+    });
+    if (found < 0) found = __reduce_max_sync(~0u, last);
+    return found;
+  }
+};
+
+template <int DT, int OP>
+__global__ void __launch_bounds__(kPsThreads) policy_kernel(const PolicyParams p) {
+  __shared__ PsShared sh;
+  const uint32_t k = (uint32_t)p.k;
+  // the barrier's first phase: every CTA of the cluster runs before its boxes are written
+  if (k > 1) ps_cluster_arrive();
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+
+  const int64_t item = (int64_t)(blockIdx.x / k);
+  const int64_t group = OP == kOpSpec ? item / p.per_group : item;
+  const int sub = OP == kOpSpec ? (int)(item - group * p.per_group) : 0;
+
+  PolicyRow<DT> row(sh);
+  row.rank = k > 1 ? ps_rank() : 0u;
+  row.k = k;
+  row.warp = threadIdx.x >> 5;
+  row.lane = threadIdx.x & 31;
+  row.entry = (int)row.rank * kPsWarps + row.warp;
+  using S = typename Elem<DT>::storage;
+  row.view.row = static_cast<const S*>(p.logits) + group * p.group_stride + sub * p.row_stride;
+  row.view.mask =
+      p.mask ? p.mask + group * p.mask_group_stride + sub * p.mask_row_stride : nullptr;
+  row.view.vocab = (uint32_t)p.vocab;
+  const uint64_t begin = (uint64_t)row.entry * (uint32_t)p.warp_ids;
+  row.view.begin = (uint32_t)min(begin, (uint64_t)p.vocab);
+  row.view.end = (uint32_t)min(begin + (uint32_t)p.warp_ids, (uint64_t)p.vocab);
+  row.view.vec = (reinterpret_cast<uintptr_t>(row.view.row) & 15u) == 0;
+
+  const RowPolicy pol = load_policy(p.policies + group * p.policy_stride);
+  bool ok = pol.ok;
+  double u = 0.0, u_accept = 0.0;
+  int len = 0;
+  if (OP == kOpDraw) u = load_uniform(p, group * p.uniform_stride);
+  if (OP == kOpSpec) {
+    len = p.draft_lens ? p.draft_lens[group] : p.per_group - 1;
+    u = load_uniform(p, group * p.uniform_stride + p.per_group - 1);
+    if (sub < len && sub < p.per_group - 1)
+      u_accept = load_uniform(p, group * p.uniform_stride + sub);
+    ok = ok && len >= 0 && len < p.per_group && u_accept >= 0.0 && u_accept < 1.0;
+  }
+  if (OP != kOpProbs) ok = ok && u >= 0.0 && u < 1.0;
+  if (k > 1) ps_cluster_wait();
+
+  const bool first = row.rank == 0 && threadIdx.x == 0;
+  uint32_t status = ok ? 0u : kStatusBadPolicy;
+  if (OP == kOpSpec && ok && sub > len) return;  // a row past the entry's drafts
+
+  RowCut c = {};
+  if (ok) {
+    uint32_t top = 0;
+    row.view.each(row.lane, [&](uint32_t, const float* v, uint32_t bits) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (bits >> j & 1u) top = max(top, ord32(v[j]));
+    });
+    top = row.reduce(0.0, 0u, top).top;
+    if (top == 0u) status = kStatusEmptyMask;
+    if (top == kOrd32NaN) status = kStatusNanInSupport;
+    if (top == kOrd32NegInf) status = kStatusAllNegInf;
+    if (!status) {
+      const float best = PolicyRow<DT>::code_value(top);
+      c.flat = !(pol.temperature > 0.0) || best == INFINITY;
+      c.top = best;
+      c.inv_t = fmin(1.0 / pol.temperature, DBL_MAX);  // 0 * inv_t stays 0
+      c.min_p = pol.min_p;
+      row.find_cut(c, pol, top);
+    }
+  }
+
+  if (status) {
+    if (OP == kOpProbs) {
+      for (uint32_t i = row.view.begin + row.lane; i < row.view.end; i += 32u)
+        p.out_probs[group * p.out_stride + i] = 0.0f;
+      if (first) p.out_status[item] = status;
+    } else if (first) {
+      if (OP == kOpDraw) {
+        p.out_idx[item] = -1;
+        p.out_status[item] = status;
+      } else {
+        p.results[item] = make_int4(kDecided, -1, (int)status, 0);
+      }
+    }
+    return;
+  }
+
+  // the kept mass and the ties at the cut, by warps; for a drafted row also the ties before it
+  uint32_t draft = 0;
+  bool drafted = false;
+  if (OP == kOpSpec && sub < len) {
+    const int32_t d = p.drafts[group * p.draft_stride + sub];
+    drafted = d >= 0 && d < (int64_t)p.vocab;
+    draft = drafted ? (uint32_t)d : 0u;
+  }
+  double mass = 0.0;
+  uint32_t ties = 0, before = 0;
+  row.view.each(row.lane, [&](uint32_t id, const float* v, uint32_t bits) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (!(bits >> j & 1u)) continue;
+      const uint32_t code = ord32(v[j]);
+      if (code == c.cut) {
+        ++ties;
+        if (OP == kOpSpec && id + j < draft) ++before;
+      } else if (code > c.cut) {
+        const double w = c.weight(v[j]);
+        if (w >= c.min_p) mass += w;
+      }
+    }
+  });
+  mass = warp_sum(mass);
+  ties = __reduce_add_sync(~0u, ties);
+  before = __reduce_add_sync(~0u, before);
+  const double w_tie = c.take ? c.weight(PolicyRow<DT>::code_value(c.cut)) : 0.0;
+  row.scan_entries(mass, ties, before, w_tie, c.take);
+  const double total = sh.total;
+
+  if (OP == kOpProbs) {
+    float* out = p.out_probs + group * p.out_stride;
+    const double inv = 1.0 / total;
+    row.each_kept(c, [&](uint32_t id, double* w) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (id + j < row.view.vocab) out[id + j] = (float)(w[j] * inv);
+    });
+    if (first) p.out_status[item] = 0u;
+    return;
+  }
+
+  bool residual = false;
+  const float* q = nullptr;
+  if (OP == kOpSpec && sub < len) {
+    double p_d = 0.0, q_d = drafted ? 1.0 : 0.0;
+    if (p.draft_probs) q = p.draft_probs + group * p.dp_group_stride + sub * p.dp_row_stride;
+    if (drafted) {
+      if (q) q_d = fmax((double)q[draft], 0.0);
+      const bool valid = !row.view.mask || (row.view.mask[draft >> 5] >> (draft & 31u) & 1u);
+      const float v = Elem<DT>::to_f32(row.view.row, draft);
+      const uint32_t code = ord32(v);
+      if (valid && (code > c.cut || (code == c.cut && sh.before < c.take))) {
+        const double w = c.weight(v);
+        if (w >= c.min_p) p_d = w / total;
+      }
+    }
+    if (drafted && u_accept * q_d < p_d) {
+      if (first) p.results[item] = make_int4(kAccepted, -1, 0, 0);
+      return;
+    }
+    residual = true;
+  }
+
+  // what remains of p where the draft's probability is taken off
+  const double inv = 1.0 / total;
+  auto rest = [&](uint32_t id, double* w) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (w[j] > 0.0) {
+        const double qj = q ? fmax((double)q[id + j], 0.0)
+                            : (drafted && id + j == draft ? 1.0 : 0.0);
+        w[j] = fmax(w[j] * inv - qj, 0.0);
+      }
+  };
+  if (OP == kOpSpec && residual) {
+    double sum = 0.0;
+    row.each_kept(c, [&](uint32_t id, double* w) {
+      rest(id, w);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sum += w[j];
+    });
+    sum = warp_sum(sum);
+    __syncthreads();
+    if (k > 1) {  // every CTA has read the first scan before its entries are overwritten
+      ps_cluster_arrive();
+      ps_cluster_wait();
+    }
+    row.scan_entries(sum, ties, 0u, 0.0, 0u);
+    if (!(sh.total > 0.0)) {  // the draft covers p everywhere: draw from p itself
+      residual = false;
+      __syncthreads();
+      if (k > 1) {
+        ps_cluster_arrive();
+        ps_cluster_wait();
+      }
+      row.scan_entries(mass, ties, 0u, w_tie, c.take);
+    }
+  }
+  const double goal = u * sh.total;
+  const int owner = row.find_owner(goal);
+  if (owner == row.entry) {
+    const double start = sh.scan_mass[owner];
+    const int id = OP == kOpSpec && residual
+                       ? row.pick(c, start, goal, rest)
+                       : row.pick(c, start, goal, [](uint32_t, double*) {});
+    if (row.lane == 0) {
+      if (OP == kOpDraw) {
+        p.out_idx[item] = id;
+        p.out_status[item] = 0u;
+      } else {
+        p.results[item] = make_int4(kDecided, id, 0, 0);
+      }
+    }
+  }
+}
+
+// Joins the rows of every entry: the first row that decides ends it.
+__global__ void spec_join_kernel(const int4* results, int64_t batch, int per_group,
+                                 const int32_t* draft_lens, int32_t* accept_len,
+                                 int32_t* token, uint32_t* status) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int64_t b = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  if (b >= batch) return;
+  const int4* r = results + b * per_group;
+  int len = draft_lens ? draft_lens[b] : per_group - 1;
+  len = len < 0 || len >= per_group ? 0 : len;
+  int i = 0;
+  int4 x = r[0];
+  while (x.x == kAccepted && i < len) x = r[++i];
+  accept_len[b] = i;
+  token[b] = x.y;
+  status[b] = (uint32_t)x.z;
+}
+
+}  // namespace onyx

@@ -1,0 +1,610 @@
+"""GPU parity of policy sampling against the float64 oracle (oracle/policy.py).
+
+Token ids, accepted lengths and status words are whole numbers and must be equal, but for one
+case. The kernel's float64 sums are trees, the oracle's sequential; each is within (n - 1) 2^-53
+of the exact sum of n weights, relative (every addition rounds by at most 2^-53 and no weight is
+negative). So where u times the total lies within 2 n 2^-53 of the total from the boundary
+between two kept ids, either of the two is right: rows made of a few repeated values reach that
+(four ids of weight 1, 2812 of weight e^-2 and u = 1/4 put it on the boundary exactly). The
+weights max(p - q, 0) of a refused draft have errors of their own, at most 4 2^-53 p each (the
+weight, the total, the quotient, the difference), so there the bound is 2 (n + 4) 2^-53 of p's
+whole mass, which is 1.
+
+Probabilities are float64 values rounded once to float32: within 2^-24 of the oracle's,
+relative, plus its sums' error and, below float32's smallest normal number, 2^-150."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+import onyx_b200 as ox
+from onyx_b200 import workloads
+from oracle import policy as opol
+from oracle import sampling as osamp
+from tests.gpu_util import host, masks_to_device, requires_cuda, to_device
+
+pytestmark = [pytest.mark.gpu, requires_cuda]
+
+POLICIES = {
+    "plain": (1.0, 0, 1.0, 0.0),
+    "greedy": (0.0, 7, 0.5, 0.3),
+    "top_k": (0.9, 50, 1.0, 0.0),
+    "top_k1": (1.0, 1, 1.0, 0.0),
+    "top_p": (0.8, 0, 0.9, 0.0),
+    "top_p_small": (1.0, 0, 0.02, 0.0),
+    "top_p_hot": (2.0, 0, 0.99, 0.0),
+    "min_p": (1.0, 0, 1.0, 0.05),
+    "min_p_all": (1.0, 0, 1.0, 1.0),
+    "all": (0.7, 40, 0.95, 0.02),
+    "k_wide": (1.5, 1000, 0.9, 0.0),
+}
+
+
+def f64(x: np.ndarray, dtype: str) -> np.ndarray:
+    if dtype == "bf16":
+        return (x.astype(np.uint32) << 16).view(np.float32).astype(np.float64)
+    return x.astype(np.float64)
+
+
+def rounded(x: np.ndarray, dtype: str) -> np.ndarray:
+    x = np.asarray(x, np.float32)
+    return workloads.bf16_bits(x) if dtype == "bf16" else x.astype(
+        np.float16 if dtype == "f16" else np.float32)
+
+
+def normal(rng, shape, dtype, scale=3.0):
+    return rounded(rng.standard_normal(shape) * scale, dtype)
+
+
+def table(policy, rows):
+    return np.tile(np.asarray(policy, np.float64), (rows, 1))
+
+
+def gpu(a, dtype=torch.float64):
+    return torch.as_tensor(np.asarray(a), dtype=dtype).cuda()
+
+
+def assert_probs(got: torch.Tensor, expected: np.ndarray):
+    got = host(got).astype(np.float64)
+    np.testing.assert_array_equal(got > 0, expected.astype(np.float32) > 0)
+    err = np.abs(got - expected)
+    assert (err <= expected * (2.0**-24 + 1e-10) + 2.0**-150).all(), err.max()
+
+
+def on_boundary(w, u, a: int, b: int) -> bool:
+    """Whether rounding decides between the ids a and b of the weights w (the module's bound;
+    weights max(p - q, 0) sum to less than 1, all others to at least 1)."""
+    ids = np.flatnonzero(w)
+    at = np.searchsorted(ids, min(a, b))
+    if at + 1 >= ids.size or (ids[at], ids[at + 1]) != (min(a, b), max(a, b)):
+        return False
+    cum = np.cumsum(w[ids])
+    return abs(cum[at] - u * cum[-1]) <= 2 * (ids.size + 4) * 2.0**-53 * max(1.0, cum[-1])
+
+
+def check(x, m, dtype, policies, u, *, probs=True):
+    """Draw and probabilities of oracle-layout rows against the oracle."""
+    xt, mt = to_device(x, dtype), None if m is None else masks_to_device(m)
+    pol = gpu(policies)
+    r = ox.policy_sample(xt, mt, pol, torch.as_tensor(u).cuda())
+    v = f64(x, dtype)
+    ids, status = opol.sample(v, m, policies, np.asarray(u, np.float64))
+    np.testing.assert_array_equal(host(r.status).astype(np.uint32), status)
+    got = host(r.token_ids)
+    for i in np.flatnonzero(got != ids):
+        valid = np.ones(v.shape[1], bool) if m is None else osamp.unpack_mask(m[i], v.shape[1])
+        w = opol.kept_weights(v[i], valid, policies[i])[1]
+        assert on_boundary(w, float(u[i]), got[i], ids[i]), (i, got, ids)
+    if probs:
+        p, st = ox.policy_probs(xt, mt, pol)
+        p_ref, st_ref = opol.probs(v, m, policies)
+        np.testing.assert_array_equal(host(st).astype(np.uint32), st_ref)
+        assert_probs(p, p_ref)
+    return host(r.token_ids)
+
+
+@pytest.mark.parametrize("policy", list(POLICIES))
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+def test_random_rows(dtype, policy, cuda_lib):
+    rng = np.random.default_rng(len(dtype) * 100 + list(POLICIES).index(policy))
+    rows, vocab = 12, 5003
+    x = normal(rng, (rows, vocab), dtype)
+    m = workloads.bernoulli_masks(rng, rng.uniform(0.002, 0.5, rows), vocab)
+    check(x, m, dtype, table(POLICIES[policy], rows), rng.random(rows))
+    check(x, None, dtype, table(POLICIES[policy], rows), rng.random(rows, dtype=np.float32))
+
+
+@pytest.mark.parametrize("vocab", [1, 2, 7, 8, 9, 31, 33, 255, 256, 257, 4095, 4097, 8193, 32769])
+def test_odd_vocabularies(vocab, cuda_lib):
+    """Rows that end inside a vector, a mask word, a chunk and a CTA's part."""
+    rng = np.random.default_rng(vocab)
+    for dtype, rows in (("bf16", 3), ("f32", 1)):
+        x = normal(rng, (rows, vocab), dtype)
+        m = workloads.bernoulli_masks(rng, np.full(rows, 0.7), vocab)
+        for policy in ("plain", "all", "top_p", "greedy"):
+            check(x, m, dtype, table(POLICIES[policy], rows), rng.random(rows))
+            check(x, None, dtype, table(POLICIES[policy], rows), rng.random(rows))
+
+
+@pytest.mark.parametrize("rows", [1, 2, 5, 16, 40, 75, 149, 300])
+def test_batches(rows, cuda_lib):
+    """Every cluster size, each row under a policy of its own."""
+    rng = np.random.default_rng(rows)
+    vocab = 40000 if rows <= 40 else 9001
+    x = normal(rng, (rows, vocab), "bf16")
+    m = workloads.bernoulli_masks(rng, rng.uniform(0.01, 0.9, rows), vocab)
+    names = list(POLICIES)
+    policies = np.stack([POLICIES[names[i]] for i in rng.integers(0, len(names), rows)])
+    check(x, m, "bf16", policies, rng.random(rows))
+
+
+def test_full_vocabulary_rows(cuda_lib):
+    w = workloads.batched(rows=6)
+    rng = np.random.default_rng(6)
+    for policy in ("top_p", "all", "plain", "top_p_hot", "k_wide"):
+        check(w["logits_bf16"], w["masks"], "bf16", table(POLICIES[policy], 6), rng.random(6))
+        check(w["logits_bf16"][:3], None, "bf16", table(POLICIES[policy], 3), rng.random(3))
+
+
+def test_rows_longer_than_shared_memory(cuda_lib):
+    rng = np.random.default_rng(8)
+    for dtype in ("f32", "bf16"):
+        x = normal(rng, (2, 1500001), dtype)
+        check(x, None, dtype, np.stack([POLICIES["top_p"], POLICIES["all"]]), rng.random(2))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+def test_wide_value_ranges(dtype, cuda_lib):
+    """Values from a hundredth to thousands, temperatures from 0.001 to 1000."""
+    rng = np.random.default_rng(77)
+    scales = np.array([[0.01], [0.3], [1.0], [8.0], [30.0], [3000.0], [1e-6], [3.0]])
+    x = rounded(rng.standard_normal((8, 9001)) * scales, dtype)
+    m = workloads.bernoulli_masks(rng, rng.uniform(0.05, 1.0, 8), 9001)
+    for policy in ((1000.0, 0, 0.9, 0.0), (5.0, 0, 0.999, 0.0), (0.001, 0, 0.5, 0.0),
+                   (0.05, 200, 0.95, 0.0), (1000.0, 3000, 0.7, 0.0), (1.0, 0, 0.5, 1e-6),
+                   (1e-310, 0, 0.9, 0.0), (50.0, 5, 1.0, 0.99)):
+        check(x, m, dtype, table(policy, 8), rng.random(8))
+        check(x, None, dtype, table(policy, 8), rng.random(8))
+
+
+def test_extreme_finite_values(cuda_lib):
+    """The largest and lowest finite values of a type, as masks of other programs write them."""
+    for dtype, big in (("f32", 3.4028234e38), ("f16", 65504.0), ("bf16", 3.3895314e38)):
+        x = np.zeros((3, 700), np.float32)
+        x[:, 100:] = -big
+        x[0, :100] = np.linspace(-3, 3, 100)
+        x[1, :] = -big  # nothing but the lowest value: a flat row
+        x[2, 5] = big
+        x = rounded(x, dtype)
+        for policy in ("plain", "top_p", "all", "top_k"):
+            check(x, None, dtype, table(POLICIES[policy], 3), [0.1, 0.5, 0.9])
+
+
+def test_special_rows(cuda_lib):
+    vocab = 300
+    rng = np.random.default_rng(3)
+    x = (rng.standard_normal((12, vocab)) * 2).astype(np.float32)
+    m = np.full((12, (vocab + 31) // 32), 0xFFFFFFFF, np.uint32)
+    x[0, [3, 40, 41, 299]] = 50.0            # ties among the leaders
+    x[1, [7, 100, 101, 280]] = np.inf        # +inf ids share the mass
+    x[2, 17] = np.nan                        # a valid NaN
+    x[3, :] = -np.inf
+    m[4, :] = 0                              # no valid id
+    m[4, -1] = np.uint32(0xFFFFFFFF) << np.uint32(vocab % 32)  # bits past the vocabulary only
+    x[5, :] = 0.5                            # flat
+    x[6, ::3] = -np.inf
+    x[7, 250] = 1e30                         # one id takes all the mass
+    x[8, [0, 31, 299]] = [np.nan, np.inf, -np.inf]
+    m[8] = 0
+    m[8, 0] = 0b110                          # NaN and infinities in masked places
+    x[9, :] = -0.0
+    x[9, ::2] = 0.0                          # signed zeros tie
+    m[10] = 0
+    m[10, 9] = 1 << 11                       # the last id alone
+    x[11, [20, 200]] = [np.inf, np.nan]
+    for policy in list(POLICIES.values()) + [(1.0, 2, 1.0, 0.0), (1.0, 3, 0.5, 0.0)]:
+        for u in (0.0, 0.3, 0.74, 1.0 - 2.0**-24):
+            check(x, m, "f32", table(policy, 12), np.full(12, u, np.float32))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_ties_at_the_cut(dtype, cuda_lib):
+    """Thousands of ids share the value the cut falls on: the first in id order are kept."""
+    vocab = 20000
+    x = np.full((4, vocab), -5.0, np.float32)
+    x[:, ::7] = 1.0
+    x[1, 100] = 2.0
+    x[2, ::5000] = 3.0
+    x[3, :] = 0.25
+    x = rounded(x, dtype)
+    for policy in ((1.0, 0, 0.1, 0.0), (1.0, 0, 0.5, 0.0), (1.0, 0, 0.97, 0.0), (1.0, 5, 1.0, 0.0),
+                   (1.0, 1000, 1.0, 0.0), (1.0, 2861, 0.9, 0.0), (1.0, 19999, 0.5, 0.2)):
+        for u in (0.0, 0.25, 0.6, 0.999):
+            check(x, None, dtype, table(policy, 4), np.full(4, u), probs=u == 0.25)
+
+
+def test_nearly_equal_float32_values(cuda_lib):
+    """float32 values that agree in all but their last bits, thousands in the same place."""
+    rng = np.random.default_rng(12)
+    x = np.full((3, 30000), 7.0, np.float32)
+    x += rng.integers(0, 64, x.shape).astype(np.float32) * np.float32(2.0**-21)
+    x[1] = -x[1]
+    x[2] = x[2] * np.float32(2.0**-20)
+    for policy in ((1.0, 0, 0.5, 0.0), (1.0, 12345, 0.9, 0.0), (1e-6, 0, 0.3, 0.0),
+                   (1.0, 100, 1.0, 0.0)):
+        check(x, None, "f32", table(policy, 3), rng.random(3))
+
+
+def test_edge_numbers(cuda_lib):
+    """u = 0 draws the first kept id, u next to 1 the last that rounding allows."""
+    rng = np.random.default_rng(9)
+    x = normal(rng, (6, 2000), "bf16")
+    for dtype in (np.float32, np.float64):
+        for u in (0.0, np.nextafter(dtype(1), dtype(0)), np.finfo(dtype).tiny):
+            check(x, None, "bf16", table(POLICIES["top_p"], 6), np.full(6, u, dtype))
+
+
+def test_bad_policies_and_numbers_are_reported(cuda_lib):
+    rng = np.random.default_rng(10)
+    bad = [(-1, 0, 1, 0), (np.nan, 0, 1, 0), (np.inf, 0, 1, 0), (1, -1, 1, 0), (1, 1.5, 1, 0),
+           (1, np.nan, 1, 0), (1, 0, 0, 0), (1, 0, 1.1, 0), (1, 0, np.nan, 0), (1, 0, 1, -0.1),
+           (1, 0, 1, 1.1), (1, 0, 1, np.nan), (1, np.inf, 1, 0), (1, 1e300, 1, 0), (1, 0, 1, 0)]
+    n = len(bad)
+    x = normal(rng, (n, 900), "f32")
+    x[0] = np.nan  # not looked at
+    check(x, None, "f32", np.asarray(bad, np.float64), np.full(n, 0.5))
+    u = np.array([1.0, -0.1, np.nan, np.inf, 0.5] * 3)
+    check(x[1:], None, "f32", table(POLICIES["plain"], n - 1), u[: n - 1], probs=False)
+    r = ox.policy_sample(to_device(x[1:3], "f32"), None, gpu(table(POLICIES["plain"], 2)),
+                         gpu([1.0, 0.5]))
+    assert host(r.status).tolist() == [ox.STATUS_BAD_POLICY, 0]
+
+
+def test_strides(cuda_lib):
+    """Column slices, padded and repeated rows, wide policy tables, strided numbers."""
+    rng = np.random.default_rng(5)
+    full = normal(rng, (4, 3011), "bf16")
+    m = workloads.bernoulli_masks(rng, np.array([0.5, 0.1, 1.0, 0.02]), 3000)
+    policies = np.stack([POLICIES[n] for n in ("top_p", "all", "plain", "top_k")])
+    u = rng.random(4)
+    wide = torch.zeros(4, 6, dtype=torch.float64, device="cuda")
+    wide[:, :4] = gpu(policies)
+    us = torch.zeros(4, 3, dtype=torch.float64, device="cuda")
+    us[:, 1] = gpu(u)
+    for off in (0, 1, 3, 8, 11):
+        x = np.ascontiguousarray(full[:, off:off + 3000])
+        r = ox.policy_sample(to_device(full, "bf16")[:, off:off + 3000], masks_to_device(m),
+                             wide[:, :4], us[:, 1])
+        ids, status = opol.sample(f64(x, "bf16"), m, policies, u)
+        np.testing.assert_array_equal(host(r.token_ids), ids)
+        np.testing.assert_array_equal(host(r.status).astype(np.uint32), status)
+        out = torch.full((4, 3009), 7.0, device="cuda")
+        p, _ = ox.policy_probs(to_device(full, "bf16")[:, off:off + 3000], masks_to_device(m),
+                               wide[:, :4], out=out[:, 4:3004])
+        assert p.data_ptr() == out[:, 4:].data_ptr()
+        assert_probs(p, opol.probs(f64(x, "bf16"), m, policies)[0])
+        assert (host(out[:, :4]) == 7).all() and (host(out[:, 3004:]) == 7).all()
+    # one row seen four times, one mask row, one policy, one number; transposed logits
+    row = to_device(full[:1, :3000], "bf16")
+    one = ox.policy_sample(row.expand(4, 3000), masks_to_device(m[:1]).expand(4, -1),
+                           gpu(policies[0]), gpu(u[:1]).expand(4))
+    ref = opol.sample(f64(full[:1, :3000], "bf16"), m[:1], policies[:1], u[:1])[0]
+    assert host(one.token_ids).tolist() == [int(ref[0])] * 4
+    t = to_device(full[:, :3000], "bf16").t().contiguous().t()
+    r = ox.policy_sample(t, masks_to_device(m), gpu(policies), gpu(u))
+    np.testing.assert_array_equal(
+        host(r.token_ids), opol.sample(f64(full[:, :3000], "bf16"), m, policies, u)[0])
+    # a single row [V]
+    r = ox.policy_sample(row[0], masks_to_device(m[:1])[0], gpu(policies[0]), gpu(u[:1]))
+    assert host(r.token_ids).tolist() == [int(ref[0])]
+
+
+def test_offsets_past_32_bits(cuda_lib):
+    """Rows more than 2^31 elements apart."""
+    rng = np.random.default_rng(21)
+    x = normal(rng, (3, 5000), "bf16")
+    big = torch.empty((3, 1_200_000_008), dtype=torch.bfloat16, device="cuda")
+    view = big[:, :5000]
+    view.copy_(to_device(x, "bf16"))
+    policies, u = table(POLICIES["all"], 3), rng.random(3)
+    r = ox.policy_sample(view, None, gpu(policies), gpu(u))
+    np.testing.assert_array_equal(host(r.token_ids),
+                                  opol.sample(f64(x, "bf16"), None, policies, u)[0])
+    del view, big
+    out = torch.empty((3, 800_000_000), dtype=torch.float32, device="cuda")[:, :5000]
+    ox.policy_probs(to_device(x, "bf16"), None, gpu(policies), out=out)
+    assert_probs(out, opol.probs(f64(x, "bf16"), None, policies)[0])
+
+
+def test_empty_batches(cuda_lib):
+    x = torch.zeros(0, 50, device="cuda")
+    pol = torch.zeros(0, 4, dtype=torch.float64, device="cuda")
+    r = ox.policy_sample(x, None, pol, torch.zeros(0, device="cuda"))
+    assert r.token_ids.shape == (0,) and r.status.shape == (0,)
+    p, st = ox.policy_probs(x, None, pol)
+    assert p.shape == (0, 50) and st.shape == (0,)
+    s = ox.spec_sample(torch.zeros(0, 3, 50, device="cuda"), None,
+                       torch.zeros(0, 2, dtype=torch.int32, device="cuda"), pol,
+                       torch.zeros(0, 3, device="cuda"))
+    assert s.accept_len.shape == (0,)
+
+
+def test_refusals(cuda_lib):
+    x = torch.zeros(2, 64, device="cuda")
+    pol = gpu(table(POLICIES["plain"], 2))
+    u = torch.zeros(2, device="cuda")
+    m = torch.zeros(2, 2, dtype=torch.int32, device="cuda")
+    for err, args in (
+        (TypeError, (x.double(), None, pol, u)), (TypeError, (x.int(), None, pol, u)),
+        (ValueError, (x[None], None, pol, u)), (ValueError, (x[:, :0], None, pol, u)),
+        (ValueError, (x, m[:, :1], pol, u)), (ValueError, (x, m[:1], pol, u)),
+        (TypeError, (x, m.long(), pol, u)), (TypeError, (x, None, pol.float(), u)),
+        (ValueError, (x, None, pol[:1], u)), (ValueError, (x, None, pol[:, :3], u)),
+        (ValueError, (x, None, pol.cpu(), u)), (ValueError, (x, None, pol, u[:1])),
+        (TypeError, (x, None, pol, u.half())), (ValueError, (x, None, pol, u.cpu())),
+        (TypeError, (x, None, [1.0], u)), (ValueError, (x, None, pol, u[:, None])),
+    ):
+        with pytest.raises(err):
+            ox.policy_sample(*args)
+    for out in (torch.zeros(2, 63, device="cuda"), torch.zeros(2, 64, device="cuda").double(),
+                torch.zeros(1, 64, device="cuda").expand(2, 64), torch.zeros(2, 64),
+                torch.zeros(64, 2, device="cuda").t(), x):
+        with pytest.raises(ValueError):
+            ox.policy_probs(x, None, pol, out=out)
+    y = torch.zeros(2, 3, 64, device="cuda")
+    d = torch.zeros(2, 2, dtype=torch.int32, device="cuda")
+    u = torch.zeros(2, 3, device="cuda")
+    for err, args, kw in (
+        (ValueError, (y[0], None, d, pol, u), {}), (ValueError, (y[:, :1], None, d, pol, u), {}),
+        (TypeError, (y.double(), None, d, pol, u), {}), (ValueError, (y, m, d, pol, u), {}),
+        (ValueError, (y, None, d.long(), pol, u), {}), (ValueError, (y, None, d[:, :1], pol, u), {}),
+        (ValueError, (y, None, d, pol, u[:, :2]), {}), (ValueError, (y, None, d, pol[:1], u), {}),
+        (ValueError, (y, None, d, pol, u), dict(draft_probs=y)),
+        (ValueError, (y, None, d, pol, u), dict(draft_probs=y[:, :2].double())),
+        (ValueError, (y, None, d, pol, u), dict(draft_lens=d[:, 0].long())),
+        (ValueError, (y, None, d, pol, u), dict(draft_lens=d)),
+        (ValueError, (y, None, d.cpu(), pol, u), {}),
+    ):
+        with pytest.raises(err):
+            ox.spec_sample(*args, **kw)
+
+
+def test_same_draw_as_masked_sample(cuda_lib):
+    """Temperature and top-p alone, with the numbers masked_sample makes for itself."""
+    w = workloads.batched(rows=8)
+    x, m = to_device(w["logits_bf16"], "bf16"), masks_to_device(w["masks"])
+    for call in range(3):
+        u = [osamp.uniform(11, call, r) for r in range(8)]
+        a = ox.masked_sample(x, m, temperature=0.8, top_p=0.9, seed=11, call=call)
+        pol = ox.pack_policies(ox.SamplingPolicy(temperature=0.8, top_p=0.9))
+        b = ox.policy_sample(x, m, pol, gpu(u))
+        assert torch.equal(a.token_ids, b.token_ids) and torch.equal(a.status, b.status)
+
+
+# --------------------------------------------------------------------------------------
+# speculative sampling
+# --------------------------------------------------------------------------------------
+def spec_inputs(rng, batch, gamma, vocab, dtype, masked=True, noise=0.5, temperature=1.0):
+    x = rng.standard_normal((batch, gamma + 1, vocab)) * 3
+    m = None
+    valid = np.ones((batch, gamma, vocab), bool)
+    if masked:
+        m = workloads.bernoulli_masks(rng, rng.uniform(0.05, 0.6, batch * (gamma + 1)), vocab)
+        m = m.reshape(batch, gamma + 1, -1)
+        valid = np.stack([[osamp.unpack_mask(m[b, i], vocab) for i in range(gamma)]
+                          for b in range(batch)])
+    z = x[:, :gamma] + rng.standard_normal((batch, gamma, vocab)) * noise
+    z = np.where(valid, z / temperature, -np.inf)
+    q = np.exp(z - z.max(-1, keepdims=True))
+    q = (q / q.sum(-1, keepdims=True)).astype(np.float32)
+    d = np.array([[opol.choose(q[b, i].astype(np.float64), rng.random()) for i in range(gamma)]
+                  for b in range(batch)], np.int32)
+    return rounded(x, dtype), m, q, d, rng.random((batch, gamma + 1))
+
+
+def check_spec(x, m, d, policies, u, dtype, q=None, lens=None):
+    r = ox.spec_sample(
+        to_device(x, dtype), None if m is None else masks_to_device(m), torch.from_numpy(d).cuda(),
+        gpu(policies), torch.as_tensor(u).cuda(), draft_probs=None if q is None else
+        torch.from_numpy(q).cuda(), draft_lens=None if lens is None else
+        torch.as_tensor(lens, dtype=torch.int32).cuda())
+    drawn = {}
+    taken, token, status = opol.spec(f64(x, dtype), m, d, policies, np.asarray(u, np.float64), q,
+                                     lens, drawn)
+    np.testing.assert_array_equal(host(r.accept_len), taken)
+    got = host(r.correction)
+    for b in np.flatnonzero(got != token):
+        assert b in drawn and on_boundary(drawn[b], float(u[b, -1]), got[b], token[b]), (
+            b, got, token)
+    np.testing.assert_array_equal(host(r.status).astype(np.uint32), status)
+    return taken
+
+
+@pytest.mark.parametrize("policy", list(POLICIES))
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+def test_spec_random(dtype, policy, cuda_lib):
+    rng = np.random.default_rng(len(dtype) * 1000 + list(POLICIES).index(policy))
+    batch, gamma, vocab = 7, 4, 2003
+    t = POLICIES[policy][0] or 0.3
+    for masked in (True, False):
+        x, m, q, d, u = spec_inputs(rng, batch, gamma, vocab, dtype, masked, temperature=t)
+        pol = table(POLICIES[policy], batch)
+        check_spec(x, m, d, pol, u, dtype, q)
+        check_spec(x, m, d, pol, u.astype(np.float32), dtype, None)
+        lens = rng.integers(0, gamma + 1, batch)
+        check_spec(x, m, d, pol, u, dtype, q, lens)
+
+
+def test_spec_accepts_and_refuses(cuda_lib):
+    """A draft model near the target: every accepted length occurs, 0 to gamma."""
+    rng = np.random.default_rng(2)
+    x, m, q, d, u = spec_inputs(rng, 60, 3, 801, "f32", noise=0.7)
+    taken = check_spec(x, m, d, table(POLICIES["plain"], 60), u, "f32", q)
+    assert set(taken.tolist()) == {0, 1, 2, 3}
+
+
+@pytest.mark.parametrize("batch,gamma,vocab", [(1, 1, 5), (1, 1, 40000), (1, 7, 20000),
+                                               (3, 255, 70), (150, 1, 300), (40, 4, 9001)])
+def test_spec_shapes(batch, gamma, vocab, cuda_lib):
+    rng = np.random.default_rng(batch * 1000 + gamma)
+    x, m, q, d, u = spec_inputs(rng, batch, gamma, vocab, "bf16", noise=0.1)
+    names = list(POLICIES)
+    policies = np.stack([POLICIES[names[i]] for i in rng.integers(0, len(names), batch)])
+    policies[:, 0] = np.where(policies[:, 0] == 0, 0, 1.0)
+    check_spec(x, m, d, policies, u, "bf16", q)
+    check_spec(x, None, d, policies, u, "bf16", q)
+
+
+def test_spec_special_rows(cuda_lib):
+    rng = np.random.default_rng(31)
+    x, m, q, d, u = spec_inputs(rng, 14, 3, 500, "f32", noise=0.0)
+    u[:, :3] = 0.01  # every draft accepted, unless the row says otherwise
+    lens = np.full(14, 3)
+    m[0, 0] = 0                      # no valid id at the first row
+    x[1, 2] = np.nan                 # a bad row behind two accepted drafts
+    x[2, 3, :] = -np.inf             # the row after the last draft
+    x[3, 1, :] = np.nan
+    u[3, 0] = 1.0 - 2.0**-53         # refused before the bad row is reached
+    q[3, 0, d[3, 0]] = 1.0
+    lens[4], lens[5] = -1, 4         # lengths outside [0, gamma]
+    u[6, 3] = 1.0                    # the drawing number outside [0, 1)
+    u[7, 1] = np.nan
+    d[8, 1] = 500                    # drafts outside the vocabulary
+    d[9, 0] = -3
+    q[10, 0] = np.nan                # probabilities that are none
+    q[11, 0] = -1.0
+    q[12, 0] = 2.0                   # nothing remains: the draw is from p
+    u[12, 0] = 0.9
+    x[13, 0, :] = 0.0
+    x[13, 0, d[13, 0]] = np.inf
+    m[13, 0] = 0xFFFFFFFF
+    check_spec(x, m, d, table(POLICIES["plain"], 14), u, "f32", q, lens)
+    check_spec(x, m, d, table(POLICIES["all"], 14), u, "f32", q, lens)
+    check_spec(x, m, d, table(POLICIES["plain"], 14), u, "f32", None, lens)
+    bad = table(POLICIES["plain"], 14)
+    bad[5:8, 2] = 0.0
+    check_spec(x, m, d, bad, u, "f32", q, lens)
+
+
+def test_spec_ties_at_the_cut(cuda_lib):
+    """A draft that ties with the cut is kept or not by its place among the ties."""
+    x = np.zeros((6, 2, 3000), np.float32)
+    x[:, :, 2000:] = -1.0
+    d = np.array([[0], [99], [100], [101], [1999], [2500]], np.int32)
+    q = np.full((6, 1, 3000), 1.0 / 3000, np.float32)
+    for k in (100, 101, 2000):
+        for u0 in (0.0, 0.05, 0.9):
+            u = np.full((6, 2), 0.37)
+            u[:, 0] = u0
+            check_spec(x, None, d, table((1.0, k, 1.0, 0.0), 6), u, "f32", q)
+            check_spec(x, None, d, table((1.0, k, 1.0, 0.0), 6), u, "f32", None)
+
+
+def test_spec_strides(cuda_lib):
+    rng = np.random.default_rng(14)
+    x, m, q, d, u = spec_inputs(rng, 5, 3, 1999, "bf16")
+    pol = table(POLICIES["all"], 5)
+    ref = opol.spec(f64(x, "bf16"), m, d, pol, u, q)
+    xt = torch.zeros(6, 5, 2050, dtype=torch.bfloat16, device="cuda")
+    xt[1:, :4, 7:2006] = to_device(x, "bf16")
+    qt = torch.zeros(5, 4, 2001, device="cuda")
+    qt[:, 1:, 1:2000] = torch.from_numpy(q).cuda()
+    mt = torch.zeros(5, 5, m.shape[2] + 3, dtype=torch.int32, device="cuda")
+    mt[:, 1:, : m.shape[2]] = masks_to_device(m)
+    dt = torch.zeros(5, 9, dtype=torch.int32, device="cuda")
+    dt[:, 2:8:2] = torch.from_numpy(d).cuda()
+    ut = torch.zeros(4, 5, dtype=torch.float64, device="cuda")
+    ut.copy_(torch.from_numpy(u).t())
+    r = ox.spec_sample(xt[1:, :4, 7:2006], mt[:, 1:], dt[:, 2:8:2], gpu(pol), ut.t(),
+                       draft_probs=qt[:, 1:, 1:2000])
+    for got, want in zip((r.accept_len, r.correction, r.status), ref):
+        np.testing.assert_array_equal(host(got).astype(np.int64), want.astype(np.int64))
+
+
+# --------------------------------------------------------------------------------------
+# a run of them together, streams and graphs
+# --------------------------------------------------------------------------------------
+def test_speculative_step_together(cuda_lib):
+    """Draft with policy_probs and policy_sample, verify with spec_sample, as one step."""
+    rng = np.random.default_rng(40)
+    batch, gamma, vocab = 9, 3, 12000
+    target = normal(rng, (batch, gamma + 1, vocab), "bf16")
+    draft = rounded(f64(target[:, :gamma], "bf16") + rng.standard_normal(
+        (batch, gamma, vocab)) * 0.3, "bf16")
+    m = workloads.bernoulli_masks(rng, rng.uniform(0.02, 0.3, batch * (gamma + 1)), vocab)
+    m = m.reshape(batch, gamma + 1, -1)
+    names = [n for n in POLICIES if n not in ("top_p_small", "min_p_all")]
+    policies = np.stack([POLICIES[names[b % len(names)]] for b in range(batch)])
+    u_draft, u = rng.random((batch, gamma)), rng.random((batch, gamma + 1))
+    pol = ox.pack_policies([ox.SamplingPolicy(float(t), int(k), float(p), float(mp))
+                            for t, k, p, mp in policies])
+    xd, mt = to_device(draft, "bf16"), masks_to_device(m)
+    q = torch.empty(batch, gamma, vocab, device="cuda")
+    drafts = torch.empty(batch, gamma, dtype=torch.int32, device="cuda")
+    for i in range(gamma):
+        ox.policy_probs(xd[:, i], mt[:, i], pol, out=q[:, i])
+        drafts[:, i] = ox.policy_sample(xd[:, i], mt[:, i], pol, gpu(u_draft[:, i])).token_ids
+    for i in range(gamma):
+        ids, _ = opol.sample(f64(draft[:, i], "bf16"), m[:, i], policies, u_draft[:, i])
+        np.testing.assert_array_equal(host(drafts[:, i]), ids)
+        assert_probs(q[:, i], opol.probs(f64(draft[:, i], "bf16"), m[:, i], policies)[0])
+    r = ox.spec_sample(to_device(target, "bf16"), mt, drafts, pol, gpu(u), draft_probs=q)
+    ref = opol.spec(f64(target, "bf16"), m, host(drafts), policies, u, host(q))
+    for got, want in zip((r.accept_len, r.correction, r.status), ref):
+        np.testing.assert_array_equal(host(got).astype(np.int64), want.astype(np.int64))
+
+
+def test_streams_and_graph_replay(cuda_lib):
+    """Captured calls replay on changed logits, policies and numbers, beside eager calls on
+    another stream."""
+    rng = np.random.default_rng(50)
+    batch, gamma, vocab = 4, 2, 30011
+    sets = []
+    for i in range(3):
+        x, m, q, d, u = spec_inputs(rng, batch, gamma, vocab, "bf16", noise=0.2)
+        policies = np.stack([POLICIES[n] for n in (("top_p", "all", "plain", "top_k"),
+                                                   ("min_p", "greedy", "all", "top_p"),
+                                                   ("k_wide", "top_p", "greedy", "plain"))[i]])
+        sets.append((to_device(x, "bf16"), masks_to_device(m), torch.from_numpy(q).cuda(),
+                     torch.from_numpy(d).cuda(), gpu(u), gpu(policies)))
+
+    def run(x, m, q, d, u, pol):
+        a = ox.policy_sample(x[:, 0], m[:, 0], pol, u[:, 0])
+        p, st = ox.policy_probs(x[:, 1], m[:, 1], pol)
+        s = ox.spec_sample(x, m, d, pol, u, draft_probs=q)
+        return [a.token_ids, a.status, p, st, s.accept_len, s.correction, s.status]
+
+    eager = [[t.clone() for t in run(*s)] for s in sets]
+    static = [t.clone() for t in sets[0]]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run(*static)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = run(*static)
+    for i in (1, 2, 0, 1):
+        for t, new in zip(static, sets[i]):
+            t.copy_(new)
+        torch.cuda.synchronize()
+        side.wait_stream(torch.cuda.current_stream())
+        graph.replay()
+        with torch.cuda.stream(side):
+            other = run(*sets[2])
+        torch.cuda.synchronize()
+        for got, want in zip(held, eager[i]):
+            assert torch.equal(got, want)
+        for got, want in zip(other, eager[2]):
+            assert torch.equal(got, want)
+
+
+def test_repeated_calls_give_the_same_bits(cuda_lib):
+    rng = np.random.default_rng(60)
+    x = to_device(normal(rng, (20, 50021), "f32"), "f32")
+    pol = gpu(table((1.1, 0, 0.97, 0.0), 20))
+    first = ox.policy_probs(x, None, pol)[0].clone()
+    for _ in range(5):
+        assert torch.equal(ox.policy_probs(x, None, pol)[0], first)

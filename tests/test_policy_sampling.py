@@ -1,0 +1,182 @@
+"""Policy sampling without a GPU: the policy object, the oracle against the reference's
+fixtures and by brute force, and the refusals of the C entry points and the Python calls."""
+
+from __future__ import annotations
+
+import itertools
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import onyx_b200 as ox
+from onyx_b200 import _lib
+from oracle import policy as opol
+from oracle import sampling as osamp
+from tests.conftest import golden_values, load_golden
+
+
+def test_policy_checks():
+    p = ox.SamplingPolicy()
+    assert p.values() == (1.0, 0.0, 1.0, 0.0)
+    assert ox.SamplingPolicy(0, 50, 0.9, 0.1).values() == (0.0, 50.0, 0.9, 0.1)
+    for kw, err in (
+        (dict(temperature=-0.1), ValueError), (dict(temperature=math.nan), ValueError),
+        (dict(temperature=math.inf), ValueError), (dict(temperature="1"), TypeError),
+        (dict(temperature=True), TypeError), (dict(top_k=-1), ValueError),
+        (dict(top_k=1.5), TypeError), (dict(top_k=True), TypeError),
+        (dict(top_k=1 << 31), ValueError), (dict(top_p=0.0), ValueError),
+        (dict(top_p=1.01), ValueError), (dict(top_p=math.nan), ValueError),
+        (dict(min_p=-0.1), ValueError), (dict(min_p=1.1), ValueError),
+        (dict(min_p=None), TypeError),
+    ):
+        with pytest.raises(err):
+            ox.SamplingPolicy(**kw)
+
+
+def test_pack_policies():
+    rows = ox.pack_policies([ox.SamplingPolicy(0.7, 40), ox.SamplingPolicy(top_p=0.9)], "cpu")
+    assert rows.dtype == torch.float64
+    assert rows.tolist() == [[0.7, 40.0, 1.0, 0.0], [1.0, 0.0, 0.9, 0.0]]
+    assert ox.pack_policies(ox.SamplingPolicy(min_p=0.5), "cpu").tolist() == [1.0, 0.0, 1.0, 0.5]
+    assert ox.pack_policies([], "cpu").shape == (0, 4)
+    with pytest.raises(TypeError):
+        ox.pack_policies([(1.0, 0, 1.0, 0.0)], "cpu")
+
+
+@pytest.mark.parametrize("case", load_golden("sampling_cases.json")["cases"],
+                         ids=lambda c: c["name"])
+def test_oracle_keeps_the_reference_set(case):
+    """Temperature and top-p alone: the reference's kept ids and probabilities. The reference
+    adds rounded shares, the weights here are added as they are: where the mass reaches top_p
+    exactly (equal values, top_p 1/2) the reference's sum may fall an ulp short of it, and it
+    keeps one id more."""
+    x = golden_values(case["bits"], case["dtype"])
+    if case["dtype"] == "bf16":
+        x = (x.astype(np.uint32) << 16).view(np.float32)
+    valid = osamp.unpack_mask(np.asarray(case["mask_words"], np.uint32), x.size)
+    policy = (case["temperature"], 0, case["top_p"], 0.0)
+    status, w = opol.kept_weights(x, valid, policy)
+    if case["expected_status"] != "ok":
+        assert status
+        return
+    expected = {i: float.fromhex(h) for i, h in case["expected_kept"]}
+    whole = opol.kept_weights(x, valid, (case["temperature"], 0, 1.0, 0.0))[1].sum()
+    if abs(w.sum() - case["top_p"] * whole) > 1e-12 * whole:
+        assert set(np.flatnonzero(w > 0)) == set(expected)
+    else:
+        extra = set(expected) - set(np.flatnonzero(w > 0))
+        assert len(extra) <= 1 and set(np.flatnonzero(w > 0)) <= set(expected)
+        return
+    # the reference's probabilities are shares of the whole mass, not of the kept one
+    p = w / w.sum() * sum(expected.values())
+    for i, e in expected.items():
+        assert p[i] == pytest.approx(e, rel=1e-12)
+
+
+def test_oracle_by_brute_force():
+    """Five ids, every policy of a grid: the kept set from the definition, id by id."""
+    rng = np.random.default_rng(0)
+    for _ in range(40):
+        v = rng.integers(-2, 3, 5) * 0.5
+        valid = rng.random(5) < 0.8
+        if not valid.any():
+            continue
+        for t, k, p, m in itertools.product((0.5, 2.0), (0, 1, 3), (0.3, 0.75, 1.0), (0.0, 0.4)):
+            _, w = opol.kept_weights(v, valid, (t, k, p, m))
+            ranked = sorted(np.flatnonzero(valid), key=lambda i: (-v[i], i))
+            weight = {i: math.exp((v[i] - v[ranked[0]]) / t) for i in ranked}
+            if k:
+                ranked = ranked[:k]
+            total, run, kept = sum(weight[i] for i in ranked), 0.0, []
+            for i in ranked:
+                if p < 1.0 and run >= p * total:
+                    break
+                run += weight[i]
+                if weight[i] >= m:
+                    kept.append(i)
+            assert sorted(kept) == list(np.flatnonzero(w)), (v, valid, t, k, p, m)
+
+
+def test_speculation_keeps_the_target_distribution():
+    """Over a fine grid of numbers, the first token of speculative sampling has the target's
+    distribution: q(d) of the drafts d, then acceptance or the remaining mass."""
+    p_x, q_x = np.array([0.1, 1.2, 0.4, -0.3]), np.array([1.0, 0.2, 0.4, 0.0])
+    policy = (1.0, 0, 1.0, 0.0)
+    w = opol.kept_weights(p_x, np.ones(4, bool), policy)[1]
+    q = np.exp(q_x) / np.exp(q_x).sum()
+    n = 400
+    got = np.zeros(4)
+    for d in range(4):
+        for a, b in itertools.product(range(n), range(40)):
+            u = np.array([[(a + 0.5) / n, (b + 0.5) / 40]])
+            taken, token, _ = opol.spec(np.stack([p_x, p_x])[None], None, np.array([[d]]),
+                                        [policy], u, q[None, None])
+            got[d if taken[0] else token[0]] += q[d] / (n * 40)
+    # the grid places each acceptance within 1/n and each draw within 1/40 of its share
+    np.testing.assert_allclose(got, w / w.sum(), atol=1 / n + 1 / 40)
+
+
+def test_c_refusals(cuda_lib):
+    """Every call is refused on the host before anything is launched (or is empty)."""
+    f = cuda_lib.onyx_policy_sample
+    one = 0x1000  # a pointer that is never read: refusals come first
+    ok = [one, 2, 4, 100, 100, None, 0, one, 4, one, 0, 1, one, one, None]
+
+    def call(fn, base, **change):
+        args = list(base)
+        for at, v in change.items():
+            args[int(at[1:])] = v
+        return fn(*args)
+
+    bad, dtype = _lib.ERR_INVALID_ARGUMENT, _lib.ERR_UNSUPPORTED_DTYPE
+    assert call(f, ok, a2=0) == _lib.OK
+    for change, code in (
+        (dict(a1=3), dtype), (dict(a1=9), dtype), (dict(a10=1), dtype), (dict(a10=2), dtype),
+        (dict(a0=None), bad), (dict(a7=None), bad), (dict(a9=None), bad), (dict(a12=None), bad),
+        (dict(a13=None), bad), (dict(a3=0), bad), (dict(a3=-5), bad), (dict(a3=1 << 31), bad),
+        (dict(a2=-1), bad), (dict(a2=1 << 31), bad), (dict(a4=99), bad), (dict(a8=3), bad),
+        (dict(a8=-4), bad), (dict(a11=0), bad), (dict(a5=one, a6=3), bad),
+    ):
+        assert call(f, ok, **change) == code, change
+    f = cuda_lib.onyx_policy_probs
+    ok = [one, 0, 4, 100, 100, None, 0, one, 0, one, 100, one, None]
+    assert call(f, ok, a2=0) == _lib.OK
+    for change, code in (
+        (dict(a1=3), dtype), (dict(a9=None), bad), (dict(a11=None), bad), (dict(a10=99), bad),
+        (dict(a4=1), bad), (dict(a8=2), bad), (dict(a5=one, a6=3), bad), (dict(a3=0), bad),
+    ):
+        assert call(f, ok, **change) == code, change
+    f = cuda_lib.onyx_spec_sample
+    need = cuda_lib.onyx_spec_sample_workspace_size(4, 3)
+    assert need == 4 * 4 * 16
+    assert cuda_lib.onyx_spec_sample_workspace_size(4, 0) == 0
+    assert cuda_lib.onyx_spec_sample_workspace_size(4, 256) == 0
+    assert cuda_lib.onyx_spec_sample_workspace_size(0, 3) == 0
+    #     logits dt B  G  V    bs   rs   masks mb mr drafts ds  q   qb   qr   lens
+    ok = [one, 2, 4, 3, 100, 400, 100, None, 0, 0, one, 3, one, 300, 100, None,
+          one, 4, one, 0, 4, one, one, one, one, need, None]
+    assert call(f, ok, a2=0) == _lib.OK
+    for change, code in (
+        (dict(a1=3), dtype), (dict(a19=2), dtype), (dict(a3=0), bad), (dict(a3=256), bad),
+        (dict(a2=-1), bad), (dict(a2=1 << 23), bad), (dict(a4=0), bad), (dict(a6=99), bad),
+        (dict(a7=one, a8=16, a9=3), bad), (dict(a10=None), bad), (dict(a11=2), bad),
+        (dict(a14=99), bad), (dict(a16=None), bad), (dict(a17=1), bad), (dict(a18=None), bad),
+        (dict(a20=3), bad), (dict(a21=None), bad), (dict(a22=None), bad), (dict(a23=None), bad),
+        (dict(a24=None), _lib.ERR_WORKSPACE), (dict(a24=one + 4), _lib.ERR_WORKSPACE),
+        (dict(a25=need - 1), _lib.ERR_WORKSPACE),
+    ):
+        assert call(f, ok, **change) == code, change
+
+
+def test_calls_refuse_host_tensors():
+    x, pol = torch.zeros(2, 10), ox.pack_policies(ox.SamplingPolicy(), "cpu")
+    with pytest.raises(ValueError, match="CUDA"):
+        ox.policy_sample(x, None, pol, torch.zeros(2))
+    with pytest.raises(ValueError, match="CUDA"):
+        ox.policy_probs(x, None, pol)
+    with pytest.raises(ValueError, match="CUDA"):
+        ox.spec_sample(x[None], None, torch.zeros(1, 1, dtype=torch.int32), pol, torch.zeros(1, 2))
+    with pytest.raises(TypeError):
+        ox.policy_sample([1.0], None, pol, torch.zeros(1))
