@@ -34,6 +34,30 @@ static int cluster_size(int64_t rows, int64_t vocab, int sms) {
   return k;
 }
 
+// Shared memory spent on peaks at most; longer parts of rows do without.
+constexpr size_t kPsMostPeaks = 96 * 1024;
+
+template <int OP>
+static const void* policy_fn(int dtype) {
+  return dtype == kBF16 ? (const void*)policy_kernel<kBF16, OP>
+         : dtype == kF16 ? (const void*)policy_kernel<kF16, OP>
+                         : (const void*)policy_kernel<kF32, OP>;
+}
+
+// Lets kernel number `which` use the dynamic shared memory it may ask for, once per device.
+static cudaError_t allow_shared(const void* fn, int which) {
+  static std::atomic<uint16_t> done[64];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev >= 0 && dev < 64 && (done[dev].load(std::memory_order_acquire) >> which & 1)) return e;
+  e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           (int)(kPsBins * sizeof(uint32_t) + kPsMostPeaks));
+  if (e == cudaSuccess && dev >= 0 && dev < 64)
+    done[dev].fetch_or((uint16_t)(1u << which), std::memory_order_release);
+  return e;
+}
+
 template <int OP>
 static int launch_policy(int dtype, PolicyParams& p, int64_t rows, cudaStream_t stream) {
   cudaError_t e;
@@ -43,9 +67,17 @@ static int launch_policy(int dtype, PolicyParams& p, int64_t rows, cudaStream_t 
   if (rows * p.k > 0x7FFFFFFFll) return ONYX_ERR_INVALID_ARGUMENT;
   const int64_t per = (int64_t)p.k * kPsWarps * kPsChunk;
   p.warp_ids = (int32_t)((p.vocab + per - 1) / per * kPsChunk);
+  size_t smem = kPsBins * sizeof(uint32_t);
+  const size_t peaks = (size_t)p.warp_ids / 8 * kPsWarps * sizeof(uint16_t);
+  p.peaks = peaks <= kPsMostPeaks;
+  if (p.peaks) smem += peaks;
+  const void* fn = policy_fn<OP>(dtype);
+  e = allow_shared(fn, OP * 3 + (dtype == kBF16 ? 0 : dtype == kF16 ? 1 : 2));
+  if (e != cudaSuccess) return finish_launch(e);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(rows * p.k), 1, 1);
   cfg.blockDim = dim3(kPsThreads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   int n = 0;
@@ -61,12 +93,8 @@ static int launch_policy(int dtype, PolicyParams& p, int64_t rows, cudaStream_t 
   }
   cfg.attrs = attr;
   cfg.numAttrs = n;
-  switch (dtype) {
-    case kBF16: e = cudaLaunchKernelEx(&cfg, policy_kernel<kBF16, OP>, p); break;
-    case kF16: e = cudaLaunchKernelEx(&cfg, policy_kernel<kF16, OP>, p); break;
-    default: e = cudaLaunchKernelEx(&cfg, policy_kernel<kF32, OP>, p); break;
-  }
-  return finish_launch(e);
+  void* args[] = {&p};
+  return finish_launch(cudaLaunchKernelExC(&cfg, fn, args));
 }
 
 static bool policy_dtype(int dt) { return dt == kF32 || dt == kF16 || dt == kBF16; }

@@ -36,6 +36,14 @@ constexpr int kPsWarps = kPsThreads / 32;
 constexpr int kPsMaxCluster = 8;
 constexpr int kPsEntries = kPsMaxCluster * kPsWarps;
 constexpr int kPsChunk = 256;  // ids a warp handles at a time, 8 to a lane
+constexpr int kPsAhead = 4;    // chunks whose loads the streaming pass has in flight
+
+// The value histogram: one bin for every bf16 value with 2^-7 <= |v| < 2^9, in falling order
+// of value; positive ones first.
+constexpr int kPsBins = 4096;
+constexpr int kPsHalf = kPsBins / 2;
+constexpr uint32_t kPsLow = 0x3C00u;  // bf16 bits of 2^-7
+constexpr int kPsOwn = kPsBins / kPsThreads;  // bins a thread scans
 
 enum PolicyOp : int { kOpDraw = 0, kOpProbs = 1, kOpSpec = 2 };
 
@@ -64,6 +72,7 @@ struct PolicyParams {
   int4* results;              // spec: {verdict, token, status, 0} of every row
   int32_t warp_ids;  // ids per warp, a multiple of kPsChunk
   int32_t k;         // CTAs per row
+  int32_t peaks;     // shared memory holds the maximum of every 8 ids
 };
 
 enum Verdict : int { kAccepted = 0, kDecided = 1 };
@@ -135,6 +144,14 @@ __device__ __forceinline__ uint32_t warp_scan(uint32_t v, int lane) {  // inclus
 struct PsBox {  // one CTA's part of a cluster-wide reduction
   double mass;
   uint32_t count, top;
+  uint32_t large, low;
+};
+
+struct PsCross {  // the bin in which a count or a mass is reached
+  double mass;    // ahead of it
+  uint32_t count;  // ahead of it
+  uint32_t n;      // ids of it that are kept
+  int bin;
 };
 
 struct PsShared {
@@ -149,53 +166,105 @@ struct PsShared {
   double total;
   int owner;
   uint32_t before;
+  uint32_t part_large[kPsWarps], part_low[kPsWarps];
+  PsCross cross[2];  // of top-k, of top-p
 };
+
+// dynamic shared memory: the histogram, then the peaks of this CTA's ids
+extern __shared__ __align__(16) unsigned char ps_dynamic[];
+__device__ __forceinline__ uint32_t* ps_hist() { return reinterpret_cast<uint32_t*>(ps_dynamic); }
+__device__ __forceinline__ uint16_t* ps_peaks() {
+  return reinterpret_cast<uint16_t*>(ps_dynamic + kPsBins * sizeof(uint32_t));
+}
 
 // The part of a row that one warp owns, and how it is read.
 template <int DT>
 struct RowView {
   using S = typename Elem<DT>::storage;
   const S* row;
-  const uint32_t* mask;
+  const uint8_t* mask;  // bit t & 7 of byte t >> 3
+  uint16_t* peaks;      // of this warp: order code >> 16 of the maximum of every 8 ids, or null
   uint32_t begin, end, vocab;
   bool vec;  // 16-byte loads: the row starts on a 16-byte boundary
 
-  // f(id of the lane's first element, values, valid bits); every lane of the warp makes every
-  // call, so f may use warp-wide instructions
+  struct Raw {  // 8 consecutive ids as loaded
+    uint4 a, b;
+    uint32_t bits;
+  };
+
+  __device__ __forceinline__ Raw load(uint32_t id) const {
+    Raw r;
+    r.a = make_uint4(0u, 0u, 0u, 0u);
+    if (DT == kF32) r.b = r.a;
+    r.bits = 0u;
+    if (id >= end) return r;
+    const uint32_t left = vocab - id;
+    r.bits = mask ? mask[id >> 3] : 0xFFu;
+    if (left < 8u) r.bits &= (1u << left) - 1u;
+    if (vec && left >= 8u) {
+      r.a = *reinterpret_cast<const uint4*>(row + id);
+      if (DT == kF32) r.b = *reinterpret_cast<const uint4*>(row + id + 4);
+    } else {
+      uint32_t u[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        u[j] = 0u;
+        if ((uint32_t)j < left) {
+          if constexpr (DT == kF32) u[j] = __float_as_uint(row[id + j]);
+          else u[j] = row[id + j];
+        }
+      }
+      if constexpr (DT == kF32) {
+        r.a = make_uint4(u[0], u[1], u[2], u[3]);
+        r.b = make_uint4(u[4], u[5], u[6], u[7]);
+      } else {
+        r.a = make_uint4(u[0] | u[1] << 16, u[2] | u[3] << 16, u[4] | u[5] << 16,
+                         u[6] | u[7] << 16);
+      }
+    }
+    return r;
+  }
+
+  // float32 bits of value j
+  __device__ __forceinline__ static uint32_t bits_of(const Raw& r, int j) {
+    const uint32_t a[4] = {r.a.x, r.a.y, r.a.z, r.a.w};
+    if constexpr (DT == kF32) {
+      const uint32_t b[4] = {r.b.x, r.b.y, r.b.z, r.b.w};
+      return j < 4 ? a[j & 3] : b[j & 3];
+    } else if constexpr (DT == kBF16) {
+      return j & 1 ? a[j >> 1] & 0xFFFF0000u : a[j >> 1] << 16;
+    } else {
+      return __float_as_uint(f16_bits_to_f32(a[j >> 1] >> (16 * (j & 1)) & 0xFFFFu));
+    }
+  }
+  __device__ __forceinline__ static float value_of(const Raw& r, int j) {
+    return __uint_as_float(bits_of(r, j));
+  }
+
+  // f(id of the lane's first value, its raw values): the pass that reads the row from HBM.
+  // Every lane of the warp makes every call.
   template <class F>
-  __device__ __forceinline__ void each(int lane, F&& f) const {
+  __device__ __forceinline__ void stream(int lane, F&& f) const {
+    uint32_t at = begin;
+    for (; at < end; at += kPsAhead * kPsChunk) {
+      Raw r[kPsAhead];
+#pragma unroll
+      for (int i = 0; i < kPsAhead; ++i) r[i] = load(at + i * kPsChunk + 8u * lane);
+#pragma unroll
+      for (int i = 0; i < kPsAhead; ++i)
+        if (at + i * kPsChunk < end) f(at + i * kPsChunk + 8u * lane, r[i]);
+    }
+  }
+
+  // f(id, raw values) over the chunks that may hold order codes of at least `code`; lanes whose
+  // 8 ids hold none get no valid ids. Every lane of the warp makes every call.
+  template <class F>
+  __device__ __forceinline__ void each(int lane, uint32_t code, F&& f) const {
     for (uint32_t at = begin; at < end; at += kPsChunk) {
       const uint32_t id = at + 8u * lane;
-      float v[8];
-      uint32_t bits = 0;
-      if (id < vocab) {
-        const uint32_t left = vocab - id;
-        bits = mask ? (mask[id >> 5] >> (id & 31u)) & 0xFFu : 0xFFu;
-        if (left < 8u) bits &= (1u << left) - 1u;
-        if (vec && left >= 8u) {
-          if constexpr (DT == kF32) {
-            const float4 a = *reinterpret_cast<const float4*>(row + id);
-            const float4 b = *reinterpret_cast<const float4*>(row + id + 4);
-            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
-            v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-          } else {
-            const uint4 a = *reinterpret_cast<const uint4*>(row + id);
-            const uint32_t u[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const uint32_t h = (u[j >> 1] >> (16 * (j & 1))) & 0xFFFFu;
-              v[j] = DT == kBF16 ? bf16_bits_to_f32(h) : f16_bits_to_f32(h);
-            }
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = (uint32_t)j < left ? Elem<DT>::to_f32(row, id + j) : 0.0f;
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = 0.0f;
-      }
-      f(id, v, bits);
+      const bool need = !peaks || peaks[(id - begin) >> 3] >= (code >> 16);
+      if (!__any_sync(~0u, need)) continue;
+      f(id, load(need ? id : end));
     }
   }
 };
@@ -209,10 +278,14 @@ struct RowCut {
   __device__ __forceinline__ double weight(float v) const {
     return flat ? 1.0 : exp(((double)v - top) * inv_t);
   }
+  // the lowest order code that is kept
+  __device__ __forceinline__ uint32_t least() const { return take ? cut : cut + 1u; }
 };
 
 template <int DT>
 struct PolicyRow {
+  using View = RowView<DT>;
+  using Raw = typename View::Raw;
   PsShared& sh;
   RowView<DT> view;
   uint32_t rank, k;
@@ -230,29 +303,38 @@ struct PolicyRow {
     }
   }
 
-  // cluster-wide sums of `mass` and `count` and maximum of `top`
-  __device__ PsBox reduce(double mass, uint32_t count, uint32_t top) {
+  // cluster-wide sums of the counts and of `mass`, and maximum of `top`
+  __device__ PsBox reduce(double mass, uint32_t count, uint32_t top, uint32_t large, uint32_t low) {
     mass = warp_sum(mass);
     count = __reduce_add_sync(~0u, count);
     top = __reduce_max_sync(~0u, top);
-    if (lane == 0) sh.part_mass[warp] = mass, sh.part_count[warp] = count, sh.part_top[warp] = top;
+    large = __reduce_add_sync(~0u, large);
+    low = __reduce_add_sync(~0u, low);
+    if (lane == 0) {
+      sh.part_mass[warp] = mass, sh.part_count[warp] = count, sh.part_top[warp] = top;
+      sh.part_large[warp] = large, sh.part_low[warp] = low;
+    }
     __syncthreads();
     if (warp == 0) {
-      PsBox b = {0.0, 0u, 0u};
+      PsBox b = {};
       for (int i = 0; i < kPsWarps; ++i) {
         b.mass += sh.part_mass[i];
         b.count += sh.part_count[i];
         b.top = max(b.top, sh.part_top[i]);
+        b.large += sh.part_large[i];
+        b.low += sh.part_low[i];
       }
       if ((uint32_t)lane < k) *ps_remote(&sh.box[parity][rank], lane) = b;
     }
     publish();
-    PsBox r = {0.0, 0u, 0u};
+    PsBox r = {};
     for (uint32_t i = 0; i < k; ++i) {
       const PsBox b = sh.box[parity][i];
       r.mass += b.mass;
       r.count += b.count;
       r.top = max(r.top, b.top);
+      r.large += b.large;
+      r.low += b.low;
     }
     parity ^= 1;
     return r;
@@ -262,15 +344,15 @@ struct PolicyRow {
   __device__ PsBox at_least(const RowCut& c, uint32_t code) {
     double mass = 0.0;
     uint32_t count = 0;
-    view.each(lane, [&](uint32_t, const float* v, uint32_t bits) {
+    view.each(lane, code, [&](uint32_t, const Raw& r) {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if ((bits >> j & 1u) && ord32(v[j]) >= code) {
-          mass += c.weight(v[j]);
+        if ((r.bits >> j & 1u) && ord32(View::value_of(r, j)) >= code) {
+          mass += c.weight(View::value_of(r, j));
           ++count;
         }
     });
-    return reduce(mass, count, 0u);
+    return reduce(mass, count, 0u, 0u, 0u);
   }
 
   // fills c.cut and c.take from the policy; `top` is the row's largest order code
@@ -334,6 +416,153 @@ struct PolicyRow {
       }
     }
     if (c.take && !c.flat && c.weight(code_value(c.cut)) < c.min_p) c.take = 0;
+  }
+
+  // ---- the cut from the value histogram (bf16: a bin is one value) ----------------------
+  __device__ static float bin_value(int bin) {
+    const uint32_t bits = bin < kPsHalf ? kPsLow + (kPsHalf - 1 - bin)
+                                        : 0x8000u | (kPsLow + (bin - kPsHalf));
+    return __uint_as_float(bits << 16);
+  }
+
+  // counts a value's bin; false for the values that have none
+  __device__ __forceinline__ static bool count_bin(uint32_t* hist, uint32_t f32_bits) {
+    const uint32_t i = ((f32_bits >> 16) & 0x7FFFu) - kPsLow;
+    if (i >= (uint32_t)kPsHalf) return false;
+    const uint32_t positive = (uint32_t)((int32_t)~f32_bits >> 31);
+    atomicAdd(hist + kPsHalf + (int)(i ^ positive), 1u);
+    return true;
+  }
+
+  // Sets c.cut and c.take from the counts of every value; `sum` holds what lies outside the
+  // bins: `count` and `mass` of |v| < 2^-7, `large` of v >= 2^9, `low` of v <= -2^9. False
+  // where the bins do not decide the cut. Every CTA adds up the bins of all CTAs and finds the
+  // same cut for itself.
+  __device__ bool find_cut_by_values(RowCut& c, const RowPolicy& pol, const PsBox& sum) {
+    if (c.flat || sum.large) return false;
+    const int mine = threadIdx.x * kPsOwn;  // this thread's bins, in falling order of value
+    uint32_t n[kPsOwn] = {};
+    for (uint32_t r = 0; r < k; ++r) {
+      const uint4* h =
+          reinterpret_cast<const uint4*>((k > 1 ? ps_remote(ps_hist(), r) : ps_hist()) + mine);
+#pragma unroll
+      for (int i = 0; i < kPsOwn / 4; ++i) {
+        const uint4 x = h[i];
+        n[4 * i] += x.x, n[4 * i + 1] += x.y, n[4 * i + 2] += x.z, n[4 * i + 3] += x.w;
+      }
+    }
+    double w[kPsOwn], mass = 0.0;
+    uint32_t count = 0;
+    int deepest = -1;
+#pragma unroll
+    for (int j = 0; j < kPsOwn; ++j) {
+      w[j] = n[j] ? c.weight(bin_value(mine + j)) : 0.0;
+      mass += (double)n[j] * w[j];
+      count += n[j];
+      if (n[j] && w[j] >= c.min_p) deepest = mine + j;
+    }
+    deepest = __reduce_max_sync(~0u, deepest);
+    if (lane == 0) sh.part_top[warp] = (uint32_t)(deepest + 1);
+    if (threadIdx.x < 2) sh.cross[threadIdx.x].bin = -1;
+    double mass_end = block_scan(mass, sh.part_mass);
+    uint32_t count_before = block_scan(count, sh.part_count) - count;
+    double mass_before = __shfl_up_sync(~0u, mass_end, 1);
+    if (lane == 0) mass_before = warp ? sh.part_mass[warp - 1] : 0.0;
+    if (mine >= kPsHalf) {  // the values next to zero lie between the halves
+      mass_before += sum.mass;
+      mass_end += sum.mass;
+      count_before += sum.count;
+    }
+    const uint32_t in_bins = sh.part_count[kPsWarps - 1] + sum.count;
+    const double all_mass = sh.part_mass[kPsWarps - 1] + sum.mass;
+    // the values below -2^9 lie behind the bins; they may weigh nothing next to the rest
+    const bool low = sum.low && (c.top + 512.0) * c.inv_t < 60.0;
+
+    int cut_bin = kPsBins;
+    uint32_t take = 0;
+    double above = 0.0;
+    if (pol.top_k && pol.top_k < in_bins + sum.low) {
+      if (pol.top_k > in_bins) return false;
+      if (count_before < pol.top_k && pol.top_k <= count_before + count) {
+        PsCross x = {mass_before, count_before, 0u, -1};
+#pragma unroll
+        for (int j = 0; j < kPsOwn; ++j)
+          if (x.bin < 0) {
+            if (pol.top_k <= x.count + n[j]) {
+              x.bin = mine + j;
+            } else {
+              x.count += n[j];
+              x.mass += (double)n[j] * w[j];
+            }
+          }
+        sh.cross[0] = x;
+      }
+      __syncthreads();
+      if (sh.cross[0].bin < 0) return false;  // among the values next to zero
+      cut_bin = sh.cross[0].bin;
+      take = pol.top_k - sh.cross[0].count;
+      above = sh.cross[0].mass;
+    }
+    if (pol.top_p < 1.0) {
+      const bool by_k = cut_bin < kPsBins;
+      if (!by_k && low) return false;
+      const double total = by_k ? above + (double)take * c.weight(bin_value(cut_bin)) : all_mass;
+      const double goal = pol.top_p * total;
+      if (count && mine <= cut_bin && mass_before < goal &&
+          (goal <= mass_end || cut_bin < mine + kPsOwn)) {
+        PsCross x = {mass_before, 0u, 0u, -1};  // the bin that reaches the goal, else the last
+        double run = mass_before, weight = 0.0;
+#pragma unroll
+        for (int j = 0; j < kPsOwn; ++j)
+          if (n[j] && mine + j <= cut_bin && run < goal) {
+            x = {run, 0u, mine + j == cut_bin ? take : n[j], mine + j};
+            weight = w[j];
+            run += (double)x.n * w[j];
+          }
+        double t = ceil((goal - x.mass) / weight);
+        t = t < 1.0 ? 1.0 : t > (double)x.n ? (double)x.n : t;
+        while (t > 1.0 && x.mass + (t - 1.0) * weight >= goal) t -= 1.0;
+        while (t < (double)x.n && x.mass + t * weight < goal) t += 1.0;
+        x.n = (uint32_t)t;
+        sh.cross[1] = x;
+      }
+      __syncthreads();
+      if (sh.cross[1].bin < 0) return false;  // among the values next to zero
+      cut_bin = sh.cross[1].bin;
+      take = sh.cross[1].n;
+    }
+    c.cut = cut_bin < kPsBins ? ord32(bin_value(cut_bin)) : 0u;
+    c.take = cut_bin < kPsBins ? take : 0u;
+    if (c.min_p > 0.0 && !low) {
+      // weights below min_p are dropped one by one where they are summed; here the bound only
+      // spares looking at them
+      for (int i = 0; i < kPsWarps; ++i) deepest = max(deepest, (int)sh.part_top[i] - 1);
+      const float edge = __uint_as_float(kPsLow << 16);
+      uint32_t bound = 0;
+      if (deepest >= kPsHalf) bound = ord32(bin_value(deepest)) - 1u;
+      else if (sum.count && c.weight(edge) >= c.min_p) bound = ord32(-edge);
+      else if (deepest >= 0) bound = ord32(bin_value(deepest)) - 1u;
+      if (bound >= c.cut && bound) {
+        c.cut = bound;
+        c.take = 0u;
+      }
+    }
+    return true;
+  }
+
+  // inclusive scan over the CTA; part[w] becomes the sum up to and with warp w
+  template <class T>
+  __device__ T block_scan(T v, T* part) {
+    T incl = warp_scan(v, lane);
+    if (lane == 31) part[warp] = incl;
+    __syncthreads();
+    if (warp == 0) {
+      const T x = lane < kPsWarps ? part[lane] : T(0);
+      const T y = warp_scan(x, lane);
+      if (lane < kPsWarps) part[lane] = y;
+    }
+    __syncthreads();
+    return warp ? part[warp - 1] + incl : incl;
   }
 
   __device__ static float code_value(uint32_t code) {
@@ -406,17 +635,17 @@ struct PolicyRow {
   template <class F>
   __device__ __forceinline__ void each_kept(const RowCut& c, F&& f) {
     uint32_t run = sh.scan_ties[entry];
-    view.each(lane, [&](uint32_t id, const float* v, uint32_t bits) {
+    view.each(lane, c.least(), [&](uint32_t id, const Raw& r) {
       double w[8];
       uint32_t tie = 0;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const uint32_t code = ord32(v[j]);
-        const bool valid = bits >> j & 1u;
+        const uint32_t code = ord32(View::value_of(r, j));
+        const bool valid = r.bits >> j & 1u;
         w[j] = 0.0;
         if (valid && code == c.cut) tie |= 1u << j;
         if (valid && code > c.cut) {
-          const double x = c.weight(v[j]);
+          const double x = c.weight(View::value_of(r, j));
           if (x >= c.min_p) w[j] = x;
         }
       }
@@ -427,7 +656,7 @@ struct PolicyRow {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
           if (tie >> j & 1u) {
-            if (at < c.take) w[j] = c.weight(v[j]);
+            if (at < c.take) w[j] = c.weight(View::value_of(r, j));
             ++at;
           }
         run += __shfl_sync(~0u, incl, 31);
@@ -481,7 +710,7 @@ struct PolicyRow {
 };
 
 template <int DT, int OP>
-__global__ void __launch_bounds__(kPsThreads) policy_kernel(const PolicyParams p) {
+__global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParams p) {
   __shared__ PsShared sh;
   const uint32_t k = (uint32_t)p.k;
   // the barrier's first phase: every CTA of the cluster runs before its boxes are written
@@ -500,13 +729,14 @@ __global__ void __launch_bounds__(kPsThreads) policy_kernel(const PolicyParams p
   row.entry = (int)row.rank * kPsWarps + row.warp;
   using S = typename Elem<DT>::storage;
   row.view.row = static_cast<const S*>(p.logits) + group * p.group_stride + sub * p.row_stride;
-  row.view.mask =
-      p.mask ? p.mask + group * p.mask_group_stride + sub * p.mask_row_stride : nullptr;
+  row.view.mask = reinterpret_cast<const uint8_t*>(
+      p.mask ? p.mask + group * p.mask_group_stride + sub * p.mask_row_stride : nullptr);
   row.view.vocab = (uint32_t)p.vocab;
   const uint64_t begin = (uint64_t)row.entry * (uint32_t)p.warp_ids;
   row.view.begin = (uint32_t)min(begin, (uint64_t)p.vocab);
   row.view.end = (uint32_t)min(begin + (uint32_t)p.warp_ids, (uint64_t)p.vocab);
   row.view.vec = (reinterpret_cast<uintptr_t>(row.view.row) & 15u) == 0;
+  row.view.peaks = p.peaks ? ps_peaks() + row.warp * (p.warp_ids >> 3) : nullptr;
 
   const RowPolicy pol = load_policy(p.policies + group * p.policy_stride);
   bool ok = pol.ok;
@@ -528,14 +758,43 @@ __global__ void __launch_bounds__(kPsThreads) policy_kernel(const PolicyParams p
   if (OP == kOpSpec && ok && sub > len) return;  // a row past the entry's drafts
 
   RowCut c = {};
+  c.inv_t = fmin(1.0 / pol.temperature, DBL_MAX);  // 0 * inv_t stays 0
+  c.min_p = pol.min_p;
   if (ok) {
-    uint32_t top = 0;
-    row.view.each(row.lane, [&](uint32_t, const float* v, uint32_t bits) {
+    // one pass over the row: its maximum, the peaks, and for bf16 the count of every value
+    const bool values = DT == kBF16 && pol.temperature > 0.0 && (pol.top_k || pol.top_p < 1.0);
+    uint32_t* hist = ps_hist();
+    if (values) {
+      for (int i = threadIdx.x; i < kPsBins / 4; i += kPsThreads)
+        reinterpret_cast<uint4*>(hist)[i] = make_uint4(0u, 0u, 0u, 0u);
+      __syncthreads();
+    }
+    uint32_t top = 0, small = 0, large = 0, low = 0;
+    double small_mass = 0.0;  // relative to a value of 0
+    row.view.stream(row.lane, [&](uint32_t id, const auto& r) {
+      using View = RowView<DT>;
+      uint32_t peak = 0;
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (bits >> j & 1u) top = max(top, ord32(v[j]));
+        if (r.bits >> j & 1u) {
+          peak = max(peak, ord32(View::value_of(r, j)));
+          if (DT == kBF16 && values && !PolicyRow<DT>::count_bin(hist, View::bits_of(r, j))) {
+            const float v = View::value_of(r, j);
+            if (fabsf(v) < 1.0f) {
+              ++small;
+              small_mass += exp((double)v * c.inv_t);
+            } else if (v > 0.0f) {
+              ++large;
+            } else {
+              ++low;
+            }
+          }
+        }
+      if (row.view.peaks) row.view.peaks[(id - row.view.begin) >> 3] = (uint16_t)(peak >> 16);
+      top = max(top, peak);
     });
-    top = row.reduce(0.0, 0u, top).top;
+    PsBox sum = row.reduce(small_mass, small, top, large, low);
+    top = sum.top;
     if (top == 0u) status = kStatusEmptyMask;
     if (top == kOrd32NaN) status = kStatusNanInSupport;
     if (top == kOrd32NegInf) status = kStatusAllNegInf;
@@ -543,9 +802,13 @@ __global__ void __launch_bounds__(kPsThreads) policy_kernel(const PolicyParams p
       const float best = PolicyRow<DT>::code_value(top);
       c.flat = !(pol.temperature > 0.0) || best == INFINITY;
       c.top = best;
-      c.inv_t = fmin(1.0 / pol.temperature, DBL_MAX);  // 0 * inv_t stays 0
-      c.min_p = pol.min_p;
-      row.find_cut(c, pol, top);
+      sum.mass = sum.count ? sum.mass * exp(-c.top * c.inv_t) : 0.0;
+      // a small mass that left the range of doubles on the way
+      const bool lost = !(sum.mass >= 0.0 && sum.mass < INFINITY);
+      if (!(values && !lost && row.find_cut_by_values(c, pol, sum))) {
+        __syncthreads();  // the scans' results have been read
+        row.find_cut(c, pol, top);
+      }
     }
   }
 
@@ -575,16 +838,17 @@ __global__ void __launch_bounds__(kPsThreads) policy_kernel(const PolicyParams p
   }
   double mass = 0.0;
   uint32_t ties = 0, before = 0;
-  row.view.each(row.lane, [&](uint32_t id, const float* v, uint32_t bits) {
+  row.view.each(row.lane, c.least(), [&](uint32_t id, const auto& r) {
+    using View = RowView<DT>;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      if (!(bits >> j & 1u)) continue;
-      const uint32_t code = ord32(v[j]);
+      if (!(r.bits >> j & 1u)) continue;
+      const uint32_t code = ord32(View::value_of(r, j));
       if (code == c.cut) {
         ++ties;
         if (OP == kOpSpec && id + j < draft) ++before;
       } else if (code > c.cut) {
-        const double w = c.weight(v[j]);
+        const double w = c.weight(View::value_of(r, j));
         if (w >= c.min_p) mass += w;
       }
     }
@@ -599,10 +863,12 @@ __global__ void __launch_bounds__(kPsThreads) policy_kernel(const PolicyParams p
   if (OP == kOpProbs) {
     float* out = p.out_probs + group * p.out_stride;
     const double inv = 1.0 / total;
+    for (uint32_t i = row.view.begin + row.lane; i < row.view.end; i += 32u) out[i] = 0.0f;
+    __syncwarp();
     row.each_kept(c, [&](uint32_t id, double* w) {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (id + j < row.view.vocab) out[id + j] = (float)(w[j] * inv);
+        if (w[j] > 0.0) out[id + j] = (float)(w[j] * inv);
     });
     if (first) p.out_status[item] = 0u;
     return;
@@ -615,7 +881,7 @@ __global__ void __launch_bounds__(kPsThreads) policy_kernel(const PolicyParams p
     if (p.draft_probs) q = p.draft_probs + group * p.dp_group_stride + sub * p.dp_row_stride;
     if (drafted) {
       if (q) q_d = fmax((double)q[draft], 0.0);
-      const bool valid = !row.view.mask || (row.view.mask[draft >> 5] >> (draft & 31u) & 1u);
+      const bool valid = !row.view.mask || (row.view.mask[draft >> 3] >> (draft & 7u) & 1u);
       const float v = Elem<DT>::to_f32(row.view.row, draft);
       const uint32_t code = ord32(v);
       if (valid && (code > c.cut || (code == c.cut && sh.before < c.take))) {
