@@ -72,7 +72,7 @@ struct PolicyParams {
   int4* results;              // spec: {verdict, token, status, 0} of every row
   int32_t warp_ids;  // ids per warp, a multiple of kPsChunk
   int32_t k;         // CTAs per row
-  int32_t peaks;     // shared memory holds the maximum of every 8 ids
+  int32_t peaks;     // where in dynamic shared memory the peaks of every 8 ids lie (0: nowhere)
 };
 
 enum Verdict : int { kAccepted = 0, kDecided = 1 };
@@ -141,6 +141,11 @@ __device__ __forceinline__ uint32_t warp_scan(uint32_t v, int lane) {  // inclus
   return v;
 }
 
+// 2^(j/16), filled by every CTA when it starts.
+struct PsPowers {
+  double at[16];
+};
+
 struct PsBox {  // one CTA's part of a cluster-wide reduction
   double mass;
   uint32_t count, top;
@@ -158,23 +163,21 @@ struct PsShared {
   PsBox box[2][kPsMaxCluster];  // used alternately: one may still be read as the next is written
   double part_mass[kPsWarps];
   uint32_t part_count[kPsWarps], part_top[kPsWarps];
-  // one entry per warp of the cluster, in id order
-  double entry_mass[kPsEntries];
+  // one entry per warp of the cluster, in id order; the second set holds what max(p - q, 0)
+  // leaves
+  double entry_mass[2][kPsEntries];
   uint32_t entry_ties[kPsEntries], entry_before[kPsEntries];
-  double scan_mass[kPsEntries];    // kept mass before the entry
-  uint32_t scan_ties[kPsEntries];  // ties before the entry
-  double total;
-  int owner;
-  uint32_t before;
+  PsPowers powers;
   uint32_t part_large[kPsWarps], part_low[kPsWarps];
   PsCross cross[2];  // of top-k, of top-p
 };
 
-// dynamic shared memory: the histogram, then the peaks of this CTA's ids
+// dynamic shared memory: the histogram, the weights of its bins, the peaks of this CTA's ids
 extern __shared__ __align__(16) unsigned char ps_dynamic[];
 __device__ __forceinline__ uint32_t* ps_hist() { return reinterpret_cast<uint32_t*>(ps_dynamic); }
-__device__ __forceinline__ uint16_t* ps_peaks() {
-  return reinterpret_cast<uint16_t*>(ps_dynamic + kPsBins * sizeof(uint32_t));
+// weights of the bins: over the histogram where no other CTA reads it, else behind it
+__device__ __forceinline__ double* ps_table(int k) {
+  return reinterpret_cast<double*>(ps_dynamic + (k > 1 ? kPsBins * sizeof(uint32_t) : 0));
 }
 
 // The part of a row that one warp owns, and how it is read.
@@ -241,6 +244,32 @@ struct RowView {
     return __uint_as_float(bits_of(r, j));
   }
 
+  // order code of the largest valid value, 0 without one; NaN above all
+  __device__ __forceinline__ static uint32_t peak_of(const Raw& r) {
+    if (!r.bits) return 0u;
+    float m;
+    if constexpr (DT == kF32) {
+      m = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        m = max_nan_f32(m, r.bits >> j & 1u ? value_of(r, j) : -INFINITY);
+    } else {
+      const uint32_t none = DT == kBF16 ? 0xFF80FF80u : 0xFC00FC00u;  // -inf twice
+      uint32_t m01, m23, m45, m67;
+      expand8_16(r.bits, m01, m23, m45, m67);
+      const uint32_t a = (r.a.x & m01) | (none & ~m01), b = (r.a.y & m23) | (none & ~m23);
+      const uint32_t d = (r.a.z & m45) | (none & ~m45), e = (r.a.w & m67) | (none & ~m67);
+      if constexpr (DT == kBF16) {
+        const uint32_t x = max_nan_bf16x2(max_nan_bf16x2(a, b), max_nan_bf16x2(d, e));
+        m = max_nan_f32(bf16_bits_to_f32(x & 0xFFFFu), bf16_bits_to_f32(x >> 16));
+      } else {
+        const uint32_t x = max_nan_f16x2(max_nan_f16x2(a, b), max_nan_f16x2(d, e));
+        m = max_nan_f32(f16_bits_to_f32(x & 0xFFFFu), f16_bits_to_f32(x >> 16));
+      }
+    }
+    return ord32(m);
+  }
+
   // f(id of the lane's first value, its raw values): the pass that reads the row from HBM.
   // Every lane of the warp makes every call.
   template <class F>
@@ -269,17 +298,53 @@ struct RowView {
   }
 };
 
+// 2^y for y <= 0 (below -1000: 0). Table-driven in the manner of Tang (ACM TOMS 15, 1989):
+// y = e + j/16 + f with |f| <= 1/32, 2^f by its Taylor polynomial of degree 6 (the next term
+// is below 5e-16 there), so about 1e-15 of the value. 12 float64 operations; the 16 entries
+// take the 16 pairs of banks, so lookups of a warp do not conflict.
+__device__ __forceinline__ double exp2_neg(double y, const PsPowers& powers) {
+  if (!(y > -1000.0)) return 0.0;
+  const double shift = 0x1.8p48;  // its last place is 1/16
+  const double t = y + shift;
+  const int n = __double2loint(t);
+  const double f = y - (t - shift);
+  const double f2 = f * f;
+  // ln 2^k / k!
+  const double a = fma(0.2402265069591007, f, 0.6931471805599453);
+  const double b = fma(0.009618129107628477, f, 0.05550410866482158);
+  const double d = fma(0.00015403530393381608, f, 0.0013333558146428443);
+  const double q = fma(fma(d, f2, b), f2, a) * f;
+  const double w = powers.at[n & 15];
+  const double r = fma(w, q, w);
+  return __hiloint2double(__double2hiint(r) + (n >> 4) * (1 << 20), __double2loint(r));
+}
+
 // What decides which ids of the row are kept, and their weights.
 struct RowCut {
-  double top, inv_t, min_p;
+  double top, scale, inv_t, min_p;  // scale = log2(e) / T
+  const PsPowers* powers;
   uint32_t cut, take;  // ids above `cut`, and the first `take` ids equal to it
   bool flat;           // every kept id weighs 1 (T = 0, or +inf present)
 
   __device__ __forceinline__ double weight(float v) const {
-    return flat ? 1.0 : exp(((double)v - top) * inv_t);
+    return flat ? 1.0 : exp2_neg(((double)v - top) * scale, *powers);
   }
   // the lowest order code that is kept
   __device__ __forceinline__ uint32_t least() const { return take ? cut : cut + 1u; }
+
+  // Weights below min_p are dropped one by one where they are summed; this raises the cut to
+  // a bound below which none passes, which spares looking at them.
+  __device__ __forceinline__ void bound_by_min_p() {
+    if (flat || !(min_p > 0.0)) return;
+    const double low = top + log(min_p) / inv_t * (1.0 + 1e-9) - fabs(top) * 1e-9;
+    const uint32_t code = ord32(__double2float_rd(low)) - 1u;
+    if (code >= cut) {
+      cut = code;
+      take = 0u;
+    }
+    if (take && weight(__uint_as_float(cut & 0x80000000u ? cut & 0x7FFFFFFFu : ~cut)) < min_p)
+      take = 0u;
+  }
 };
 
 template <int DT>
@@ -288,6 +353,7 @@ struct PolicyRow {
   using Raw = typename View::Raw;
   PsShared& sh;
   RowView<DT> view;
+  double* table = nullptr;  // weights of the kept bins, where the cut came from them
   uint32_t rank, k;
   int warp, lane, entry;
   int parity = 0;
@@ -415,7 +481,6 @@ struct PolicyRow {
         c.take = (uint32_t)t;
       }
     }
-    if (c.take && !c.flat && c.weight(code_value(c.cut)) < c.min_p) c.take = 0;
   }
 
   // ---- the cut from the value histogram (bf16: a bin is one value) ----------------------
@@ -437,8 +502,9 @@ struct PolicyRow {
   // Sets c.cut and c.take from the counts of every value; `sum` holds what lies outside the
   // bins: `count` and `mass` of |v| < 2^-7, `large` of v >= 2^9, `low` of v <= -2^9. False
   // where the bins do not decide the cut. Every CTA adds up the bins of all CTAs and finds the
-  // same cut for itself.
-  __device__ bool find_cut_by_values(RowCut& c, const RowPolicy& pol, const PsBox& sum) {
+  // same cut for itself. `tab` gets the weights of the kept bins; with one CTA it may lie over
+  // the histogram.
+  __device__ bool find_cut_by_values(RowCut& c, const RowPolicy& pol, const PsBox& sum, double* tab) {
     if (c.flat || sum.large) return false;
     const int mine = threadIdx.x * kPsOwn;  // this thread's bins, in falling order of value
     uint32_t n[kPsOwn] = {};
@@ -453,28 +519,28 @@ struct PolicyRow {
     }
     double w[kPsOwn], mass = 0.0;
     uint32_t count = 0;
-    int deepest = -1;
+    const bool by_mass = pol.top_p < 1.0;
 #pragma unroll
     for (int j = 0; j < kPsOwn; ++j) {
-      w[j] = n[j] ? c.weight(bin_value(mine + j)) : 0.0;
+      w[j] = by_mass && n[j] ? c.weight(bin_value(mine + j)) : 0.0;
       mass += (double)n[j] * w[j];
       count += n[j];
-      if (n[j] && w[j] >= c.min_p) deepest = mine + j;
     }
-    deepest = __reduce_max_sync(~0u, deepest);
-    if (lane == 0) sh.part_top[warp] = (uint32_t)(deepest + 1);
     if (threadIdx.x < 2) sh.cross[threadIdx.x].bin = -1;
-    double mass_end = block_scan(mass, sh.part_mass);
+    double mass_before = 0.0, mass_end = 0.0;
+    if (by_mass) {
+      mass_end = block_scan(mass, sh.part_mass);
+      mass_before = __shfl_up_sync(~0u, mass_end, 1);
+      if (lane == 0) mass_before = warp ? sh.part_mass[warp - 1] : 0.0;
+    }
     uint32_t count_before = block_scan(count, sh.part_count) - count;
-    double mass_before = __shfl_up_sync(~0u, mass_end, 1);
-    if (lane == 0) mass_before = warp ? sh.part_mass[warp - 1] : 0.0;
     if (mine >= kPsHalf) {  // the values next to zero lie between the halves
       mass_before += sum.mass;
       mass_end += sum.mass;
       count_before += sum.count;
     }
     const uint32_t in_bins = sh.part_count[kPsWarps - 1] + sum.count;
-    const double all_mass = sh.part_mass[kPsWarps - 1] + sum.mass;
+    const double all_mass = by_mass ? sh.part_mass[kPsWarps - 1] + sum.mass : 0.0;
     // the values below -2^9 lie behind the bins; they may weigh nothing next to the rest
     const bool low = sum.low && (c.top + 512.0) * c.inv_t < 60.0;
 
@@ -503,7 +569,7 @@ struct PolicyRow {
       take = pol.top_k - sh.cross[0].count;
       above = sh.cross[0].mass;
     }
-    if (pol.top_p < 1.0) {
+    if (by_mass) {
       const bool by_k = cut_bin < kPsBins;
       if (!by_k && low) return false;
       const double total = by_k ? above + (double)take * c.weight(bin_value(cut_bin)) : all_mass;
@@ -533,20 +599,13 @@ struct PolicyRow {
     }
     c.cut = cut_bin < kPsBins ? ord32(bin_value(cut_bin)) : 0u;
     c.take = cut_bin < kPsBins ? take : 0u;
-    if (c.min_p > 0.0 && !low) {
-      // weights below min_p are dropped one by one where they are summed; here the bound only
-      // spares looking at them
-      for (int i = 0; i < kPsWarps; ++i) deepest = max(deepest, (int)sh.part_top[i] - 1);
-      const float edge = __uint_as_float(kPsLow << 16);
-      uint32_t bound = 0;
-      if (deepest >= kPsHalf) bound = ord32(bin_value(deepest)) - 1u;
-      else if (sum.count && c.weight(edge) >= c.min_p) bound = ord32(-edge);
-      else if (deepest >= 0) bound = ord32(bin_value(deepest)) - 1u;
-      if (bound >= c.cut && bound) {
-        c.cut = bound;
-        c.take = 0u;
-      }
-    }
+    // the weights of the kept bins, for the passes that follow
+    table = tab;
+#pragma unroll
+    for (int j = 0; j < kPsOwn; ++j)
+      if (n[j] && mine + j <= cut_bin)
+        table[mine + j] = by_mass ? w[j] : c.weight(bin_value(mine + j));
+    __syncthreads();
     return true;
   }
 
@@ -569,72 +628,120 @@ struct PolicyRow {
     return __uint_as_float((code & 0x80000000u) ? code & 0x7FFFFFFFu : ~code);
   }
 
-  // Publishes one entry per warp and scans them: scan_ties, scan_mass, total, before. `w_tie`
-  // is the weight of an id at the cut; entries hold the mass above it.
-  __device__ void scan_entries(double mass, uint32_t ties, uint32_t before, double w_tie,
-                               uint32_t take) {
+  struct Scan {  // of the entries of all warps, as this warp sees them
+    double total, mass_before;  // kept mass; of it, before this warp
+    uint32_t ties_before, draft_before;
+  };
+
+  // Kept mass of the entries that lane `lane` holds: `per` of them, in id order.
+  static constexpr int kPer = kPsEntries / 32;
+  struct Held {
+    double mass[kPer];
+    int first, n;
+  };
+  __device__ __forceinline__ Held held(int set, uint32_t take, double w_tie, uint32_t* ties_run,
+                                       uint32_t* ties_at) {
+    Held h;
+    const int n = (int)k * kPsWarps, per = (n + 31) / 32;
+    h.first = lane * per;
+    h.n = max(0, min(per, n - h.first));
+    uint32_t t[kPer], sum = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      t[i] = i < h.n ? sh.entry_ties[h.first + i] : 0u;
+      h.mass[i] = i < h.n ? sh.entry_mass[set][h.first + i] : 0.0;
+      sum += t[i];
+    }
+    uint32_t run = warp_scan(sum, lane) - sum;
+    *ties_run = run;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      ties_at[i] = run;
+      const uint32_t kept = run < take ? min(t[i], take - run) : 0u;
+      if (kept) h.mass[i] += (double)kept * w_tie;
+      run += t[i];
+    }
+    return h;
+  }
+
+  // Publishes this warp's entry to the cluster and scans all of them; every warp does so for
+  // itself. `w_tie` is the weight of an id at the cut, `mass` that above it.
+  __device__ Scan scan_entries(int set, double mass, uint32_t ties, uint32_t before,
+                               uint32_t take, double w_tie) {
     if ((uint32_t)lane < k) {
       PsShared* r = ps_remote(&sh, lane);
-      r->entry_mass[entry] = mass;
-      r->entry_ties[entry] = ties;
-      r->entry_before[entry] = before;
+      r->entry_mass[set][entry] = mass;
+      if (set == 0) {
+        r->entry_ties[entry] = ties;
+        r->entry_before[entry] = before;
+      }
     }
     publish();
-    if (warp == 0) {
-      const int n = (int)k * kPsWarps, per = (n + 31) / 32;
-      const int lo = min(n, lane * per), hi = min(n, lo + per);
-      uint32_t t = 0, b = 0;
-      for (int i = lo; i < hi; ++i) t += sh.entry_ties[i], b += sh.entry_before[i];
-      uint32_t run = warp_scan(t, lane) - t;
-      b = __reduce_add_sync(~0u, b);
-      double m = 0.0;
-      for (int i = lo; i < hi; ++i) {
-        const uint32_t n_tie = sh.entry_ties[i];
-        const uint32_t kept = run < take ? min(n_tie, take - run) : 0u;
-        sh.scan_ties[i] = run;
-        run += n_tie;
-        const double e = sh.entry_mass[i] + (double)kept * w_tie;
-        sh.entry_mass[i] = e;
-        m += e;
-      }
-      const double incl = warp_scan(m, lane);
-      const double prev = __shfl_up_sync(~0u, incl, 1);
-      double acc = lane ? prev : 0.0;  // summed, not subtracted: never below 0
-      for (int i = lo; i < hi; ++i) {
-        sh.scan_mass[i] = acc;
-        acc += sh.entry_mass[i];
-      }
-      if (lane == 31) sh.total = acc;
-      if (lane == 0) sh.before = b;
+    uint32_t run, at[kPer];
+    const Held h = held(set, take, w_tie, &run, at);
+    double sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) sum += h.mass[i];
+    const double incl = warp_scan(sum, lane);
+    double acc = __shfl_up_sync(~0u, incl, 1);
+    if (lane == 0) acc = 0.0;
+    Scan s;
+    s.total = __shfl_sync(~0u, incl, 31);
+    const int per = ((int)k * kPsWarps + 31) / 32, src = entry / per;
+    double mine = 0.0;
+    uint32_t mine_ties = 0;
+    uint32_t b = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      if (h.first + i == entry) mine = acc, mine_ties = at[i];
+      if (i < h.n) b += sh.entry_before[h.first + i];
+      acc += h.mass[i];
     }
-    __syncthreads();
+    s.mass_before = __shfl_sync(~0u, mine, src);
+    s.ties_before = __shfl_sync(~0u, mine_ties, src);
+    s.draft_before = __reduce_add_sync(~0u, b);
+    return s;
   }
 
   // the entry whose interval of kept mass holds `goal` (the last with mass, if rounding leaves
   // none)
-  __device__ int find_owner(double goal) {
-    if (warp == 0) {
-      const int n = (int)k * kPsWarps;
-      int first = n, last = 0;
-      for (int i = lane; i < n; i += 32) {
-        const double m = sh.entry_mass[i];
-        if (m > 0.0) {
-          last = max(last, i);
-          if (sh.scan_mass[i] + m > goal) first = min(first, i);
-        }
+  __device__ int find_owner(int set, uint32_t take, double w_tie, double goal) {
+    uint32_t run, at[kPer];
+    const Held h = held(set, take, w_tie, &run, at);
+    double sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) sum += h.mass[i];
+    const double incl = warp_scan(sum, lane);
+    double acc = __shfl_up_sync(~0u, incl, 1);
+    if (lane == 0) acc = 0.0;
+    int first = kPsEntries, last = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (h.mass[i] > 0.0) {
+        last = h.first + i;
+        if (acc + h.mass[i] > goal) first = min(first, h.first + i);
+        acc += h.mass[i];
       }
-      first = __reduce_min_sync(~0u, first);
-      last = __reduce_max_sync(~0u, last);
-      if (lane == 0) sh.owner = first < n ? first : last;
-    }
-    __syncthreads();
-    return sh.owner;
+    first = __reduce_min_sync(~0u, first);
+    last = __reduce_max_sync(~0u, last);
+    return first < kPsEntries ? first : last;
   }
 
-  // f(id, weights of the lane's 8 ids: 0 where not kept) over this warp's ids
+  // weight of a kept value
+  __device__ __forceinline__ double weight(const RowCut& c, uint32_t f32_bits) const {
+    if (DT == kBF16 && table) {
+      const uint32_t i = ((f32_bits >> 16) & 0x7FFFu) - kPsLow;
+      const uint32_t positive = (uint32_t)((int32_t)~f32_bits >> 31);
+      if (i < (uint32_t)kPsHalf) return table[kPsHalf + (int)(i ^ positive)];
+    }
+    return c.weight(__uint_as_float(f32_bits));
+  }
+
+  // f(id, weights of the lane's 8 ids: 0 where not kept) over this warp's ids;
+  // `ties_before`: ids at the cut before this warp
   template <class F>
-  __device__ __forceinline__ void each_kept(const RowCut& c, F&& f) {
-    uint32_t run = sh.scan_ties[entry];
+  __device__ __forceinline__ void each_kept(const RowCut& c, uint32_t ties_before, F&& f) {
+    uint32_t run = ties_before;
     view.each(lane, c.least(), [&](uint32_t id, const Raw& r) {
       double w[8];
       uint32_t tie = 0;
@@ -645,7 +752,7 @@ struct PolicyRow {
         w[j] = 0.0;
         if (valid && code == c.cut) tie |= 1u << j;
         if (valid && code > c.cut) {
-          const double x = c.weight(View::value_of(r, j));
+          const double x = weight(c, View::bits_of(r, j));
           if (x >= c.min_p) w[j] = x;
         }
       }
@@ -656,7 +763,7 @@ struct PolicyRow {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
           if (tie >> j & 1u) {
-            if (at < c.take) w[j] = c.weight(View::value_of(r, j));
+            if (at < c.take) w[j] = weight(c, View::bits_of(r, j));
             ++at;
           }
         run += __shfl_sync(~0u, incl, 31);
@@ -668,10 +775,11 @@ struct PolicyRow {
   // first id, in id order, whose cumulative weight exceeds `goal`; `start` is the mass before
   // this warp; weigh(id, w[8]) may replace the kept weights. Whole warp; all lanes return it.
   template <class W>
-  __device__ int pick(const RowCut& c, double start, double goal, W&& weigh) {
+  __device__ int pick(const RowCut& c, uint32_t ties_before, double start, double goal,
+                      W&& weigh) {
     int found = -1, last = -1;
     double run = start;
-    each_kept(c, [&](uint32_t id, double* w) {
+    each_kept(c, ties_before, [&](uint32_t id, double* w) {
       if (found >= 0) return;  // uniform over the warp
       weigh(id, w);
       double s = 0.0;
@@ -681,24 +789,20 @@ struct PolicyRow {
         s += w[j];
         if (w[j] > 0.0) mine = (int)id + j;
       }
+      if (!__any_sync(~0u, mine >= 0)) return;
       const double incl = warp_scan(s, lane);
       const uint32_t over = __ballot_sync(~0u, s > 0.0 && run + incl > goal);
       if (over) {
         const int src = __ffs(over) - 1;
         const double prev = __shfl_up_sync(~0u, incl, 1);
-        int at = mine;
-        if (lane == src) {
-          double acc = run + (lane ? prev : 0.0);
+        double acc = run + (lane ? prev : 0.0);
+        int at = -1;
 #pragma unroll
-          for (int j = 7; j >= 0; --j) {
-            // cumulative weight up to and with j, in the order of a forward walk
-            double x = acc;
-#pragma unroll
-            for (int i = 0; i <= j; ++i) x += w[i];
-            if (w[j] > 0.0 && x > goal) at = (int)id + j;
-          }
+        for (int j = 0; j < 8; ++j) {
+          acc += w[j];
+          if (at < 0 && w[j] > 0.0 && acc > goal) at = (int)id + j;
         }
-        found = __shfl_sync(~0u, at, src);
+        found = __shfl_sync(~0u, at < 0 ? mine : at, src);
         return;
       }
       last = max(last, mine);
@@ -708,6 +812,18 @@ struct PolicyRow {
     return found;
   }
 };
+
+// zeros for a lane's 8 ids
+__device__ __forceinline__ void clear_probs(float* out, uint32_t id, uint32_t end) {
+  if (id + 8u <= end && (reinterpret_cast<uintptr_t>(out) & 15u) == 0) {
+    reinterpret_cast<float4*>(out + id)[0] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    reinterpret_cast<float4*>(out + id)[1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (id + j < end) out[id + j] = 0.0f;
+  }
+}
 
 template <int DT, int OP>
 __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParams p) {
@@ -736,7 +852,7 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
   row.view.begin = (uint32_t)min(begin, (uint64_t)p.vocab);
   row.view.end = (uint32_t)min(begin + (uint32_t)p.warp_ids, (uint64_t)p.vocab);
   row.view.vec = (reinterpret_cast<uintptr_t>(row.view.row) & 15u) == 0;
-  row.view.peaks = p.peaks ? ps_peaks() + row.warp * (p.warp_ids >> 3) : nullptr;
+  row.view.peaks = p.peaks ? reinterpret_cast<uint16_t*>(ps_dynamic + p.peaks) + row.warp * (p.warp_ids >> 3) : nullptr;
 
   const RowPolicy pol = load_policy(p.policies + group * p.policy_stride);
   bool ok = pol.ok;
@@ -758,7 +874,10 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
   if (OP == kOpSpec && ok && sub > len) return;  // a row past the entry's drafts
 
   RowCut c = {};
-  c.inv_t = fmin(1.0 / pol.temperature, DBL_MAX);  // 0 * inv_t stays 0
+  c.inv_t = fmin(1.0 / pol.temperature, 1e300);  // 0 times it stays 0
+  c.scale = c.inv_t * 1.4426950408889634;
+  c.powers = &sh.powers;
+  if (threadIdx.x < 16) sh.powers.at[threadIdx.x] = exp2((double)threadIdx.x / 16.0);
   c.min_p = pol.min_p;
   if (ok) {
     // one pass over the row: its maximum, the peaks, and for bf16 the count of every value
@@ -773,25 +892,32 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
     double small_mass = 0.0;  // relative to a value of 0
     row.view.stream(row.lane, [&](uint32_t id, const auto& r) {
       using View = RowView<DT>;
-      uint32_t peak = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (r.bits >> j & 1u) {
-          peak = max(peak, ord32(View::value_of(r, j)));
-          if (DT == kBF16 && values && !PolicyRow<DT>::count_bin(hist, View::bits_of(r, j))) {
-            const float v = View::value_of(r, j);
-            if (fabsf(v) < 1.0f) {
-              ++small;
-              small_mass += exp((double)v * c.inv_t);
-            } else if (v > 0.0f) {
-              ++large;
-            } else {
-              ++low;
-            }
-          }
-        }
+      const uint32_t peak = View::peak_of(r);
       if (row.view.peaks) row.view.peaks[(id - row.view.begin) >> 3] = (uint16_t)(peak >> 16);
       top = max(top, peak);
+      if (OP == kOpProbs) clear_probs(p.out_probs + group * p.out_stride, id, row.view.end);
+      if (DT == kBF16 && values) {
+        uint32_t odd = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (r.bits >> j & 1u)
+            if (!PolicyRow<DT>::count_bin(hist, View::bits_of(r, j))) odd |= 1u << j;
+        if (odd) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (odd >> j & 1u) {
+              const float v = View::value_of(r, j);
+              if (fabsf(v) < 1.0f) {
+                ++small;
+                small_mass += exp((double)v * c.inv_t);
+              } else if (v > 0.0f) {
+                ++large;
+              } else {
+                ++low;
+              }
+            }
+        }
+      }
     });
     PsBox sum = row.reduce(small_mass, small, top, large, low);
     top = sum.top;
@@ -805,17 +931,19 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
       sum.mass = sum.count ? sum.mass * exp(-c.top * c.inv_t) : 0.0;
       // a small mass that left the range of doubles on the way
       const bool lost = !(sum.mass >= 0.0 && sum.mass < INFINITY);
-      if (!(values && !lost && row.find_cut_by_values(c, pol, sum))) {
+      if (!(values && !lost && row.find_cut_by_values(c, pol, sum, ps_table(p.k)))) {
         __syncthreads();  // the scans' results have been read
         row.find_cut(c, pol, top);
       }
+      c.bound_by_min_p();
     }
   }
 
   if (status) {
     if (OP == kOpProbs) {
-      for (uint32_t i = row.view.begin + row.lane; i < row.view.end; i += 32u)
-        p.out_probs[group * p.out_stride + i] = 0.0f;
+      if (!ok)  // the other rows were cleared as they were read
+        for (uint32_t i = row.view.begin + row.lane; i < row.view.end; i += 32u)
+          p.out_probs[group * p.out_stride + i] = 0.0f;
       if (first) p.out_status[item] = status;
     } else if (first) {
       if (OP == kOpDraw) {
@@ -848,7 +976,7 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
         ++ties;
         if (OP == kOpSpec && id + j < draft) ++before;
       } else if (code > c.cut) {
-        const double w = c.weight(View::value_of(r, j));
+        const double w = row.weight(c, View::bits_of(r, j));
         if (w >= c.min_p) mass += w;
       }
     }
@@ -857,15 +985,13 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
   ties = __reduce_add_sync(~0u, ties);
   before = __reduce_add_sync(~0u, before);
   const double w_tie = c.take ? c.weight(PolicyRow<DT>::code_value(c.cut)) : 0.0;
-  row.scan_entries(mass, ties, before, w_tie, c.take);
-  const double total = sh.total;
+  auto scan = row.scan_entries(0, mass, ties, before, c.take, w_tie);
+  const double total = scan.total;
 
   if (OP == kOpProbs) {
     float* out = p.out_probs + group * p.out_stride;
     const double inv = 1.0 / total;
-    for (uint32_t i = row.view.begin + row.lane; i < row.view.end; i += 32u) out[i] = 0.0f;
-    __syncwarp();
-    row.each_kept(c, [&](uint32_t id, double* w) {
+    row.each_kept(c, scan.ties_before, [&](uint32_t id, double* w) {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
         if (w[j] > 0.0) out[id + j] = (float)(w[j] * inv);
@@ -884,7 +1010,7 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
       const bool valid = !row.view.mask || (row.view.mask[draft >> 3] >> (draft & 7u) & 1u);
       const float v = Elem<DT>::to_f32(row.view.row, draft);
       const uint32_t code = ord32(v);
-      if (valid && (code > c.cut || (code == c.cut && sh.before < c.take))) {
+      if (valid && (code > c.cut || (code == c.cut && scan.draft_before < c.take))) {
         const double w = c.weight(v);
         if (w >= c.min_p) p_d = w / total;
       }
@@ -909,35 +1035,24 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
   };
   if (OP == kOpSpec && residual) {
     double sum = 0.0;
-    row.each_kept(c, [&](uint32_t id, double* w) {
+    row.each_kept(c, scan.ties_before, [&](uint32_t id, double* w) {
       rest(id, w);
 #pragma unroll
       for (int j = 0; j < 8; ++j) sum += w[j];
     });
     sum = warp_sum(sum);
-    __syncthreads();
-    if (k > 1) {  // every CTA has read the first scan before its entries are overwritten
-      ps_cluster_arrive();
-      ps_cluster_wait();
-    }
-    row.scan_entries(sum, ties, 0u, 0.0, 0u);
-    if (!(sh.total > 0.0)) {  // the draft covers p everywhere: draw from p itself
-      residual = false;
-      __syncthreads();
-      if (k > 1) {
-        ps_cluster_arrive();
-        ps_cluster_wait();
-      }
-      row.scan_entries(mass, ties, 0u, w_tie, c.take);
-    }
+    const auto left = row.scan_entries(1, sum, ties, 0u, 0u, 0.0);
+    residual = left.total > 0.0;  // else the draft covers p everywhere: draw from p itself
+    if (residual) scan.total = left.total, scan.mass_before = left.mass_before;
   }
-  const double goal = u * sh.total;
-  const int owner = row.find_owner(goal);
+  const double goal = u * scan.total;
+  const int owner = residual ? row.find_owner(1, 0u, 0.0, goal)
+                             : row.find_owner(0, c.take, w_tie, goal);
   if (owner == row.entry) {
-    const double start = sh.scan_mass[owner];
     const int id = OP == kOpSpec && residual
-                       ? row.pick(c, start, goal, rest)
-                       : row.pick(c, start, goal, [](uint32_t, double*) {});
+                       ? row.pick(c, scan.ties_before, scan.mass_before, goal, rest)
+                       : row.pick(c, scan.ties_before, scan.mass_before, goal,
+                                  [](uint32_t, double*) {});
     if (row.lane == 0) {
       if (OP == kOpDraw) {
         p.out_idx[item] = id;
