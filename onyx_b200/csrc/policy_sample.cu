@@ -37,13 +37,6 @@ static int cluster_size(int64_t rows, int64_t vocab, int sms) {
 // Shared memory spent on peaks at most; longer parts of rows do without.
 constexpr size_t kPsMostPeaks = 96 * 1024;
 
-// Shared memory ahead of the peaks: the histogram of values and the weights of its bins (one
-// over the other where a row has one CTA). Peaks at offset 0 mean none, so it is never 0.
-static size_t policy_shared(int dtype, int k) {
-  if (dtype != kBF16) return 16;
-  return kPsBins * sizeof(double) + (k > 1 ? kPsBins * sizeof(uint32_t) : 0);
-}
-
 template <int OP>
 static const void* policy_fn(int dtype) {
   return dtype == kBF16 ? (const void*)policy_kernel<kBF16, OP>
@@ -59,7 +52,7 @@ static cudaError_t allow_shared(const void* fn, int which) {
   if (e != cudaSuccess) return e;
   if (dev >= 0 && dev < 64 && (done[dev].load(std::memory_order_acquire) >> which & 1)) return e;
   e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           (int)(kPsBins * (sizeof(double) + sizeof(uint32_t)) + kPsMostPeaks));
+                           (int)(2 * kPsArea + kPsMostPeaks));
   if (e == cudaSuccess && dev >= 0 && dev < 64)
     done[dev].fetch_or((uint16_t)(1u << which), std::memory_order_release);
   return e;
@@ -74,7 +67,7 @@ static int launch_policy(int dtype, PolicyParams& p, int64_t rows, cudaStream_t 
   if (rows * p.k > 0x7FFFFFFFll) return ONYX_ERR_INVALID_ARGUMENT;
   const int64_t per = (int64_t)p.k * kPsWarps * kPsChunk;
   p.warp_ids = (int32_t)((p.vocab + per - 1) / per * kPsChunk);
-  size_t smem = policy_shared(dtype, p.k);
+  size_t smem = 2 * kPsArea;
   const size_t peaks = (size_t)p.warp_ids / 8 * kPsWarps * sizeof(uint16_t);
   p.peaks = 0;
   if (peaks <= kPsMostPeaks) {

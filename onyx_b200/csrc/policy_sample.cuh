@@ -8,9 +8,9 @@
 // (T = 0: the first maximum alone; any +inf: the +inf ids alone, with equal weights). Ids are
 // ranked by (value falling, id rising). top-k keeps the first k; top-p keeps the shortest
 // prefix of those whose mass reaches p times their mass; min-p keeps w >= min_p. All three
-// keep a prefix of the ranking, so the kept set is given by a cut (an order code), the number
-// of ids equal to it that are kept in id order (`take`) and the bound w >= min_p. The draw is
-// the first kept id, in id order, whose cumulative weight exceeds u times the kept total.
+// keep a prefix of the ranking, so the kept set is a cut: the values above `cut`, of the ids
+// equal to it the first `take` in id order, and w >= min_p. The draw is the first kept id, in
+// id order, whose cumulative weight exceeds u times the kept total.
 //
 // Sums and weights are float64: whether a cumulative mass reaches p, or an id's interval holds
 // u, decides a whole number, and float32 sums over 10^5 ids would decide it differently for
@@ -18,11 +18,25 @@
 //
 // Shape of the work. One cluster of k CTAs per row (k = 1, 2, 4 or 8, the more the fewer the
 // rows); CTA ranks, the warps of a CTA and the 256-id chunks of a warp follow id order, a lane
-// holding 8 consecutive ids. A row is streamed from HBM by the first pass and from L2 by the
-// later ones, so no row length is bound to shared memory. Cluster-wide sums: every CTA stores
-// its part into every CTA's box (distributed shared memory), one cluster barrier publishes
-// them, and all CTAs combine the boxes in rank order, so all hold identical totals and take
-// the same branches.
+// holding 8 consecutive ids.
+//   1  One pass reads the row from HBM: its maximum, the maximum of every 8 ids (the peaks,
+//      kept in shared memory), and a histogram with a bin for every value of bfloat16
+//      precision, |v| in [2^-9, 2^7) -- 4,096 bins. For float32 and float16 rows whose top-p
+//      needs the whole mass it also sums the weights.
+//   2  The histograms of the CTAs are added up (each CTA a part of the bins, over distributed
+//      shared memory) and every CTA scans all bins in falling order of value. For bfloat16 a
+//      bin is one value, count times weight its mass, and the scan yields the cut. For the
+//      other types it yields the few bins that hold the cut.
+//   3  Those bins' ids (a few dozen as a rule) are listed, sorted by value and id and summed
+//      exactly. Where the list would be long the same histogram is taken again over the
+//      remaining range of order codes, a 4096th of it to a bin.
+//   4  The kept mass is summed by warps (the peaks name the vectors to read again, from L1 or
+//      L2), the warps' sums are scanned, and the warp whose interval holds u draws.
+// Rows that step 2 cannot serve (values of 2^7 and more, a cut among values next to zero)
+// start step 3 from the whole range of codes. No row length is bound to shared memory.
+//
+// Every CTA of a cluster computes the same totals from the same parts in the same order, so
+// all take the same branches, and the result does not depend on timing.
 #pragma once
 
 #include <cfloat>
@@ -38,12 +52,14 @@ constexpr int kPsEntries = kPsMaxCluster * kPsWarps;
 constexpr int kPsChunk = 256;  // ids a warp handles at a time, 8 to a lane
 constexpr int kPsAhead = 4;    // chunks whose loads the streaming pass has in flight
 
-// The value histogram: one bin for every bf16 value with 2^-7 <= |v| < 2^9, in falling order
-// of value; positive ones first.
+// The value histogram: one bin for every bf16 value with 2^-9 <= |v| < 2^7, in falling order
+// of value; positive ones first. The values next to zero, |v| < 2^-9, lie between the halves.
 constexpr int kPsBins = 4096;
 constexpr int kPsHalf = kPsBins / 2;
-constexpr uint32_t kPsLow = 0x3C00u;  // bf16 bits of 2^-7
+constexpr uint32_t kPsLow = 0x3B00u;  // bf16 bits of 2^-9
+constexpr float kPsSmall = 0x1p-9f, kPsLarge = 0x1p7f;
 constexpr int kPsOwn = kPsBins / kPsThreads;  // bins a thread scans
+constexpr uint32_t kPsList = 1024;            // ids sorted at most
 
 enum PolicyOp : int { kOpDraw = 0, kOpProbs = 1, kOpSpec = 2 };
 
@@ -148,37 +164,45 @@ struct PsPowers {
 
 struct PsBox {  // one CTA's part of a cluster-wide reduction
   double mass;
-  uint32_t count, top;
-  uint32_t large, low;
+  uint32_t count, top, small, low;
 };
 
 struct PsCross {  // the bin in which a count or a mass is reached
-  double mass;    // ahead of it
+  double mass;     // ahead of it
   uint32_t count;  // ahead of it
-  uint32_t n;      // ids of it that are kept
+  uint32_t n;      // ids in it
   int bin;
 };
 
 struct PsShared {
   PsBox box[2][kPsMaxCluster];  // used alternately: one may still be read as the next is written
-  double part_mass[kPsWarps];
-  uint32_t part_count[kPsWarps], part_top[kPsWarps];
+  double part_mass[kPsWarps], part_high[kPsWarps];
+  uint32_t part_count[kPsWarps], part_top[kPsWarps], part_small[kPsWarps];
   // one entry per warp of the cluster, in id order; the second set holds what max(p - q, 0)
   // leaves
   double entry_mass[2][kPsEntries];
   uint32_t entry_ties[kPsEntries], entry_before[kPsEntries];
   PsPowers powers;
-  uint32_t part_large[kPsWarps], part_low[kPsWarps];
-  PsCross cross[2];  // of top-k, of top-p
+  PsCross cross[3];
+  uint32_t listed[kPsMaxCluster];  // ids that each CTA listed
+  uint32_t list_fill;
 };
 
-// dynamic shared memory: the histogram, the weights of its bins, the peaks of this CTA's ids
+// Dynamic shared memory: 32 KB that hold the CTA's histogram and the cluster's, or a list and
+// its sorted form, or in the end the weights of the bins; then the peaks of this CTA's ids.
 extern __shared__ __align__(16) unsigned char ps_dynamic[];
+constexpr size_t kPsArea = kPsBins * sizeof(uint32_t);
 __device__ __forceinline__ uint32_t* ps_hist() { return reinterpret_cast<uint32_t*>(ps_dynamic); }
-// weights of the bins: over the histogram where no other CTA reads it, else behind it
-__device__ __forceinline__ double* ps_table(int k) {
-  return reinterpret_cast<double*>(ps_dynamic + (k > 1 ? kPsBins * sizeof(uint32_t) : 0));
+__device__ __forceinline__ uint32_t* ps_merged() {
+  return reinterpret_cast<uint32_t*>(ps_dynamic + kPsArea);
 }
+__device__ __forceinline__ unsigned long long* ps_list() {
+  return reinterpret_cast<unsigned long long*>(ps_dynamic);
+}
+__device__ __forceinline__ unsigned long long* ps_sorted() {
+  return reinterpret_cast<unsigned long long*>(ps_dynamic + kPsArea);
+}
+__device__ __forceinline__ double* ps_table() { return reinterpret_cast<double*>(ps_dynamic); }
 
 // The part of a row that one warp owns, and how it is read.
 template <int DT>
@@ -243,6 +267,28 @@ struct RowView {
   __device__ __forceinline__ static float value_of(const Raw& r, int j) {
     return __uint_as_float(bits_of(r, j));
   }
+  // the same for a j that is not known when compiled
+  __device__ __forceinline__ static float value_at(const Raw& r, int j) {
+    if constexpr (DT == kF32) {
+      const uint4 h = j & 4 ? r.b : r.a;
+      const uint32_t lo = j & 1 ? h.y : h.x, hi = j & 1 ? h.w : h.z;
+      return __uint_as_float(j & 2 ? hi : lo);
+    } else {
+      const uint32_t lo = j & 2 ? r.a.y : r.a.x, hi = j & 2 ? r.a.w : r.a.z;
+      const uint32_t u = (j & 4 ? hi : lo) >> (16 * (j & 1)) & 0xFFFFu;
+      return DT == kBF16 ? bf16_bits_to_f32(u) : f16_bits_to_f32(u);
+    }
+  }
+
+  // f(j, whether this lane has one) for the set bits j of every lane's `set`, lowest first: as
+  // many turns as the fullest lane has bits. Whole warp.
+  template <class F>
+  __device__ __forceinline__ static void each_set(uint32_t set, F&& f) {
+    while (__any_sync(~0u, set)) {
+      f(set ? __ffs(set) - 1 : 0, set != 0u);
+      set &= set - 1u;
+    }
+  }
 
   // order code of the largest valid value, 0 without one; NaN above all
   __device__ __forceinline__ static uint32_t peak_of(const Raw& r) {
@@ -293,17 +339,17 @@ struct RowView {
       const uint32_t id = at + 8u * lane;
       const bool need = !peaks || peaks[(id - begin) >> 3] >= (code >> 16);
       if (!__any_sync(~0u, need)) continue;
-      f(id, load(need ? id : end));
+      const Raw r = load(need ? id : end);
+      f(id, r);
     }
   }
 };
 
-// 2^y for y <= 0 (below -1000: 0). Table-driven in the manner of Tang (ACM TOMS 15, 1989):
-// y = e + j/16 + f with |f| <= 1/32, 2^f by its Taylor polynomial of degree 6 (the next term
-// is below 5e-16 there), so about 1e-15 of the value. 12 float64 operations; the 16 entries
-// take the 16 pairs of banks, so lookups of a warp do not conflict.
-__device__ __forceinline__ double exp2_neg(double y, const PsPowers& powers) {
-  if (!(y > -1000.0)) return 0.0;
+// 2^y (below 2^-1000: 0, above 2^1000: +inf). Table-driven in the manner of Tang (ACM TOMS
+// 15, 1989): y = e + j/16 + f with |f| <= 1/32, 2^f by its Taylor polynomial of degree 6 (the
+// next term is below 5e-16 there), so about 1e-15 of the value. 12 float64 operations; the 16
+// entries take the 16 pairs of banks, so lookups of a warp do not conflict.
+__device__ __forceinline__ double exp2_table(double y, const PsPowers& powers) {
   const double shift = 0x1.8p48;  // its last place is 1/16
   const double t = y + shift;
   const int n = __double2loint(t);
@@ -316,35 +362,54 @@ __device__ __forceinline__ double exp2_neg(double y, const PsPowers& powers) {
   const double q = fma(fma(d, f2, b), f2, a) * f;
   const double w = powers.at[n & 15];
   const double r = fma(w, q, w);
-  return __hiloint2double(__double2hiint(r) + (n >> 4) * (1 << 20), __double2loint(r));
+  const double v = __hiloint2double(__double2hiint(r) + (n >> 4) * (1 << 20), __double2loint(r));
+  return y > -1000.0 ? (y < 1000.0 ? v : (double)INFINITY) : 0.0;
+}
+
+__device__ __forceinline__ float code_value(uint32_t code) {  // inverse of ord32
+  return __uint_as_float((code & 0x80000000u) ? code & 0x7FFFFFFFu : ~code);
 }
 
 // What decides which ids of the row are kept, and their weights.
 struct RowCut {
   double top, scale, inv_t, min_p;  // scale = log2(e) / T
   const PsPowers* powers;
-  uint32_t cut, take;  // ids above `cut`, and the first `take` ids equal to it
-  bool flat;           // every kept id weighs 1 (T = 0, or +inf present)
+  float cut;      // ids above it are kept,
+  uint32_t take;  // and of those equal to it the first `take`
+  bool flat;      // every kept id weighs 1 (T = 0, or +inf present)
 
   __device__ __forceinline__ double weight(float v) const {
-    return flat ? 1.0 : exp2_neg(((double)v - top) * scale, *powers);
+    return flat ? 1.0 : exp2_table(((double)v - top) * scale, *powers);
+  }
+  __device__ __forceinline__ void keep(float value, uint32_t first) {
+    cut = value;
+    take = first;
   }
   // the lowest order code that is kept
-  __device__ __forceinline__ uint32_t least() const { return take ? cut : cut + 1u; }
+  __device__ __forceinline__ uint32_t least() const { return ord32(cut); }
 
   // Weights below min_p are dropped one by one where they are summed; this raises the cut to
   // a bound below which none passes, which spares looking at them.
   __device__ __forceinline__ void bound_by_min_p() {
     if (flat || !(min_p > 0.0)) return;
     const double low = top + log(min_p) / inv_t * (1.0 + 1e-9) - fabs(top) * 1e-9;
-    const uint32_t code = ord32(__double2float_rd(low)) - 1u;
-    if (code >= cut) {
-      cut = code;
-      take = 0u;
-    }
-    if (take && weight(__uint_as_float(cut & 0x80000000u ? cut & 0x7FFFFFFFu : ~cut)) < min_p)
-      take = 0u;
+    const float bound = nextafterf(__double2float_rd(low), -INFINITY);
+    if (bound >= cut) keep(bound, 0u);
+    if (take && weight(cut) < min_p) take = 0u;
   }
+};
+
+// The mass that top-p has to reach. The sums that are held against it carry errors of some
+// 2^-50 of the total; the factor lets a mass that equals the goal (equal values: 270 of 300 ids
+// at 0.9) reach it whatever the order of summation.
+__device__ __forceinline__ double top_p_goal(double top_p, double total) {
+  return top_p * total * (1.0 - 0x1p-44);
+}
+
+// A range of order codes that holds the cut.
+struct PsRange {
+  uint32_t hi, lo;         // inclusive
+  uint32_t above, inside;  // ids above it, ids in it
 };
 
 template <int DT>
@@ -352,14 +417,16 @@ struct PolicyRow {
   using View = RowView<DT>;
   using Raw = typename View::Raw;
   PsShared& sh;
-  RowView<DT> view;
-  double* table = nullptr;  // weights of the kept bins, where the cut came from them
+  View view;
+  const double* table = nullptr;  // weights of the kept bins, where the cut came from them
   uint32_t rank, k;
   int warp, lane, entry;
   int parity = 0;
 
   __device__ PolicyRow(PsShared& s) : sh(s) {}
 
+  // What the CTAs of the cluster stored before it can be read after it. A buffer that other
+  // CTAs write or read is used again only after a publish() that lies behind its last use.
   __device__ __forceinline__ void publish() {
     if (k > 1) {
       ps_cluster_arrive();
@@ -369,27 +436,24 @@ struct PolicyRow {
     }
   }
 
-  // cluster-wide sums of the counts and of `mass`, and maximum of `top`
-  __device__ PsBox reduce(double mass, uint32_t count, uint32_t top, uint32_t large, uint32_t low) {
+  // cluster-wide sums, and the maximum of `top`
+  __device__ PsBox reduce(double mass, uint32_t count, uint32_t top, uint32_t small) {
     mass = warp_sum(mass);
     count = __reduce_add_sync(~0u, count);
     top = __reduce_max_sync(~0u, top);
-    large = __reduce_add_sync(~0u, large);
-    low = __reduce_add_sync(~0u, low);
+    small = __reduce_add_sync(~0u, small);
     if (lane == 0) {
-      sh.part_mass[warp] = mass, sh.part_count[warp] = count, sh.part_top[warp] = top;
-      sh.part_large[warp] = large, sh.part_low[warp] = low;
+      sh.part_mass[warp] = mass, sh.part_count[warp] = count;
+      sh.part_top[warp] = top, sh.part_small[warp] = small;
     }
     __syncthreads();
     if (warp == 0) {
+      const bool have = lane < kPsWarps;
       PsBox b = {};
-      for (int i = 0; i < kPsWarps; ++i) {
-        b.mass += sh.part_mass[i];
-        b.count += sh.part_count[i];
-        b.top = max(b.top, sh.part_top[i]);
-        b.large += sh.part_large[i];
-        b.low += sh.part_low[i];
-      }
+      b.mass = warp_sum(have ? sh.part_mass[lane] : 0.0);
+      b.count = __reduce_add_sync(~0u, have ? sh.part_count[lane] : 0u);
+      b.top = __reduce_max_sync(~0u, have ? sh.part_top[lane] : 0u);
+      b.small = __reduce_add_sync(~0u, have ? sh.part_small[lane] : 0u);
       if ((uint32_t)lane < k) *ps_remote(&sh.box[parity][rank], lane) = b;
     }
     publish();
@@ -399,220 +463,16 @@ struct PolicyRow {
       r.mass += b.mass;
       r.count += b.count;
       r.top = max(r.top, b.top);
-      r.large += b.large;
-      r.low += b.low;
+      r.small += b.small;
     }
     parity ^= 1;
     return r;
   }
 
-  // mass and count of the valid ids whose order code is at least `code`
-  __device__ PsBox at_least(const RowCut& c, uint32_t code) {
-    double mass = 0.0;
-    uint32_t count = 0;
-    view.each(lane, code, [&](uint32_t, const Raw& r) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if ((r.bits >> j & 1u) && ord32(View::value_of(r, j)) >= code) {
-          mass += c.weight(View::value_of(r, j));
-          ++count;
-        }
-    });
-    return reduce(mass, count, 0u, 0u, 0u);
-  }
-
-  // fills c.cut and c.take from the policy; `top` is the row's largest order code
-  __device__ void find_cut(RowCut& c, const RowPolicy& pol, uint32_t top) {
-    const uint32_t base = c.flat ? top - 1u : 0u;  // +inf present: those ids alone
-    c.cut = base;
-    c.take = 0;
-    PsBox above = {0.0, 0u, 0u};  // of the ids above the cut
-    bool by_k = false;
-    if (!(pol.temperature > 0.0)) {
-      c.cut = top;
-      c.take = 1;
-      return;
-    }
-    if (pol.top_k && pol.top_k < view.vocab) {
-      uint32_t lo = base, hi = top + 1u;
-      while (hi - lo > 1u) {
-        const uint32_t mid = lo + (hi - lo) / 2u;
-        const PsBox b = at_least(c, mid);
-        if (b.count >= pol.top_k) {
-          lo = mid;
-        } else {
-          hi = mid;
-          above = b;
-        }
-      }
-      if (lo > base) {
-        by_k = true;
-        c.cut = lo;
-        c.take = pol.top_k - above.count;
-      }
-    }
-    if (pol.top_p < 1.0) {
-      const double w_cut = by_k ? c.weight(code_value(c.cut)) : 0.0;
-      const double total = by_k ? above.mass + (double)c.take * w_cut : at_least(c, base + 1u).mass;
-      const double goal = pol.top_p * total;
-      uint32_t lo = c.cut, hi = top + 1u;
-      PsBox over = {0.0, 0u, 0u}, level = {0.0, 0u, 0u};
-      bool have = false;
-      while (hi - lo > 1u) {
-        const uint32_t mid = lo + (hi - lo) / 2u;
-        const PsBox b = at_least(c, mid);
-        if (b.mass >= goal) {
-          lo = mid;
-          level = b;
-          have = true;
-        } else {
-          hi = mid;
-          over = b;
-        }
-      }
-      const uint32_t most = have ? level.count - over.count : c.take;
-      if (by_k || have) {
-        const double w = c.weight(code_value(lo));
-        double t = ceil((goal - over.mass) / w);
-        t = t < 1.0 ? 1.0 : t > (double)most ? (double)most : t;
-        while (t > 1.0 && over.mass + (t - 1.0) * w >= goal) t -= 1.0;
-        while (t < (double)most && over.mass + t * w < goal) t += 1.0;
-        c.cut = lo;
-        c.take = (uint32_t)t;
-      }
-    }
-  }
-
-  // ---- the cut from the value histogram (bf16: a bin is one value) ----------------------
-  __device__ static float bin_value(int bin) {
-    const uint32_t bits = bin < kPsHalf ? kPsLow + (kPsHalf - 1 - bin)
-                                        : 0x8000u | (kPsLow + (bin - kPsHalf));
-    return __uint_as_float(bits << 16);
-  }
-
-  // counts a value's bin; false for the values that have none
-  __device__ __forceinline__ static bool count_bin(uint32_t* hist, uint32_t f32_bits) {
-    const uint32_t i = ((f32_bits >> 16) & 0x7FFFu) - kPsLow;
-    if (i >= (uint32_t)kPsHalf) return false;
-    const uint32_t positive = (uint32_t)((int32_t)~f32_bits >> 31);
-    atomicAdd(hist + kPsHalf + (int)(i ^ positive), 1u);
-    return true;
-  }
-
-  // Sets c.cut and c.take from the counts of every value; `sum` holds what lies outside the
-  // bins: `count` and `mass` of |v| < 2^-7, `large` of v >= 2^9, `low` of v <= -2^9. False
-  // where the bins do not decide the cut. Every CTA adds up the bins of all CTAs and finds the
-  // same cut for itself. `tab` gets the weights of the kept bins; with one CTA it may lie over
-  // the histogram.
-  __device__ bool find_cut_by_values(RowCut& c, const RowPolicy& pol, const PsBox& sum, double* tab) {
-    if (c.flat || sum.large) return false;
-    const int mine = threadIdx.x * kPsOwn;  // this thread's bins, in falling order of value
-    uint32_t n[kPsOwn] = {};
-    for (uint32_t r = 0; r < k; ++r) {
-      const uint4* h =
-          reinterpret_cast<const uint4*>((k > 1 ? ps_remote(ps_hist(), r) : ps_hist()) + mine);
-#pragma unroll
-      for (int i = 0; i < kPsOwn / 4; ++i) {
-        const uint4 x = h[i];
-        n[4 * i] += x.x, n[4 * i + 1] += x.y, n[4 * i + 2] += x.z, n[4 * i + 3] += x.w;
-      }
-    }
-    double w[kPsOwn], mass = 0.0;
-    uint32_t count = 0;
-    const bool by_mass = pol.top_p < 1.0;
-#pragma unroll
-    for (int j = 0; j < kPsOwn; ++j) {
-      w[j] = by_mass && n[j] ? c.weight(bin_value(mine + j)) : 0.0;
-      mass += (double)n[j] * w[j];
-      count += n[j];
-    }
-    if (threadIdx.x < 2) sh.cross[threadIdx.x].bin = -1;
-    double mass_before = 0.0, mass_end = 0.0;
-    if (by_mass) {
-      mass_end = block_scan(mass, sh.part_mass);
-      mass_before = __shfl_up_sync(~0u, mass_end, 1);
-      if (lane == 0) mass_before = warp ? sh.part_mass[warp - 1] : 0.0;
-    }
-    uint32_t count_before = block_scan(count, sh.part_count) - count;
-    if (mine >= kPsHalf) {  // the values next to zero lie between the halves
-      mass_before += sum.mass;
-      mass_end += sum.mass;
-      count_before += sum.count;
-    }
-    const uint32_t in_bins = sh.part_count[kPsWarps - 1] + sum.count;
-    const double all_mass = by_mass ? sh.part_mass[kPsWarps - 1] + sum.mass : 0.0;
-    // the values below -2^9 lie behind the bins; they may weigh nothing next to the rest
-    const bool low = sum.low && (c.top + 512.0) * c.inv_t < 60.0;
-
-    int cut_bin = kPsBins;
-    uint32_t take = 0;
-    double above = 0.0;
-    if (pol.top_k && pol.top_k < in_bins + sum.low) {
-      if (pol.top_k > in_bins) return false;
-      if (count_before < pol.top_k && pol.top_k <= count_before + count) {
-        PsCross x = {mass_before, count_before, 0u, -1};
-#pragma unroll
-        for (int j = 0; j < kPsOwn; ++j)
-          if (x.bin < 0) {
-            if (pol.top_k <= x.count + n[j]) {
-              x.bin = mine + j;
-            } else {
-              x.count += n[j];
-              x.mass += (double)n[j] * w[j];
-            }
-          }
-        sh.cross[0] = x;
-      }
-      __syncthreads();
-      if (sh.cross[0].bin < 0) return false;  // among the values next to zero
-      cut_bin = sh.cross[0].bin;
-      take = pol.top_k - sh.cross[0].count;
-      above = sh.cross[0].mass;
-    }
-    if (by_mass) {
-      const bool by_k = cut_bin < kPsBins;
-      if (!by_k && low) return false;
-      const double total = by_k ? above + (double)take * c.weight(bin_value(cut_bin)) : all_mass;
-      const double goal = pol.top_p * total;
-      if (count && mine <= cut_bin && mass_before < goal &&
-          (goal <= mass_end || cut_bin < mine + kPsOwn)) {
-        PsCross x = {mass_before, 0u, 0u, -1};  // the bin that reaches the goal, else the last
-        double run = mass_before, weight = 0.0;
-#pragma unroll
-        for (int j = 0; j < kPsOwn; ++j)
-          if (n[j] && mine + j <= cut_bin && run < goal) {
-            x = {run, 0u, mine + j == cut_bin ? take : n[j], mine + j};
-            weight = w[j];
-            run += (double)x.n * w[j];
-          }
-        double t = ceil((goal - x.mass) / weight);
-        t = t < 1.0 ? 1.0 : t > (double)x.n ? (double)x.n : t;
-        while (t > 1.0 && x.mass + (t - 1.0) * weight >= goal) t -= 1.0;
-        while (t < (double)x.n && x.mass + t * weight < goal) t += 1.0;
-        x.n = (uint32_t)t;
-        sh.cross[1] = x;
-      }
-      __syncthreads();
-      if (sh.cross[1].bin < 0) return false;  // among the values next to zero
-      cut_bin = sh.cross[1].bin;
-      take = sh.cross[1].n;
-    }
-    c.cut = cut_bin < kPsBins ? ord32(bin_value(cut_bin)) : 0u;
-    c.take = cut_bin < kPsBins ? take : 0u;
-    // the weights of the kept bins, for the passes that follow
-    table = tab;
-#pragma unroll
-    for (int j = 0; j < kPsOwn; ++j)
-      if (n[j] && mine + j <= cut_bin)
-        table[mine + j] = by_mass ? w[j] : c.weight(bin_value(mine + j));
-    __syncthreads();
-    return true;
-  }
-
   // inclusive scan over the CTA; part[w] becomes the sum up to and with warp w
   template <class T>
-  __device__ T block_scan(T v, T* part) {
-    T incl = warp_scan(v, lane);
+  __device__ __forceinline__ T block_scan(T v, T* part) {
+    const T incl = warp_scan(v, lane);
     if (lane == 31) part[warp] = incl;
     __syncthreads();
     if (warp == 0) {
@@ -623,11 +483,545 @@ struct PolicyRow {
     __syncthreads();
     return warp ? part[warp - 1] + incl : incl;
   }
-
-  __device__ static float code_value(uint32_t code) {
-    return __uint_as_float((code & 0x80000000u) ? code & 0x7FFFFFFFu : ~code);
+  // the same sums without this thread's: what the thread before it got, bit for bit
+  __device__ __forceinline__ double scan_before(double incl, const double* part) const {
+    const double prev = __shfl_up_sync(~0u, incl, 1);
+    return lane ? prev : warp ? part[warp - 1] : 0.0;
   }
 
+  __device__ __forceinline__ void clear_hist() {
+    for (int i = threadIdx.x; i < kPsBins / 4; i += kPsThreads)
+      reinterpret_cast<uint4*>(ps_hist())[i] = make_uint4(0u, 0u, 0u, 0u);
+    __syncthreads();
+  }
+
+  // After a reduce(): the cluster's counts of this thread's kPsOwn bins. Every CTA adds up its
+  // part of the bins and hands the sums to all.
+  __device__ __forceinline__ void merge_bins(uint32_t (&n)[kPsOwn]) {
+    const uint32_t* from = ps_hist();
+    if (k > 1) {
+      const int part = kPsBins / (int)k;
+      for (int i = threadIdx.x; i < part; i += kPsThreads) {
+        const int bin = (int)rank * part + i;
+        uint32_t x[kPsMaxCluster];
+#pragma unroll
+        for (uint32_t r = 0; r < kPsMaxCluster; ++r)
+          x[r] = r < k ? *ps_remote(ps_hist() + bin, r) : 0u;
+        uint32_t sum = 0;
+#pragma unroll
+        for (uint32_t r = 0; r < kPsMaxCluster; ++r) sum += x[r];
+#pragma unroll
+        for (uint32_t r = 0; r < kPsMaxCluster; ++r)
+          if (r < k) *ps_remote(ps_merged() + bin, r) = sum;
+      }
+      publish();
+      from = ps_merged();
+    }
+#pragma unroll
+    for (int i = 0; i < kPsOwn / 4; ++i) {
+      const uint4 x = reinterpret_cast<const uint4*>(from)[threadIdx.x * (kPsOwn / 4) + i];
+      n[4 * i] = x.x, n[4 * i + 1] = x.y, n[4 * i + 2] = x.z, n[4 * i + 3] = x.w;
+    }
+  }
+
+  // ---- the cut from the histogram of values ---------------------------------------------
+  __device__ __forceinline__ static uint32_t bin_bits(int bin) {  // of |v|, bfloat16
+    return bin < kPsHalf ? kPsLow + (kPsHalf - 1 - bin) : kPsLow + (bin - kPsHalf);
+  }
+  // the bin's value nearest to zero (bfloat16: its only one)
+  __device__ __forceinline__ static float bin_value(int bin) {
+    return __uint_as_float((bin_bits(bin) | (bin < kPsHalf ? 0u : 0x8000u)) << 16);
+  }
+  __device__ __forceinline__ static uint32_t bin_low_code(int bin) {
+    const uint32_t code = ord32(bin_value(bin));
+    return bin < kPsHalf ? code : code - 0xFFFFu;
+  }
+
+  // counts a value's bin, if it has one
+  __device__ __forceinline__ static void count_bin(uint32_t* hist, uint32_t f32_bits, bool valid) {
+    const uint32_t i = ((f32_bits >> 16) & 0x7FFFu) - kPsLow;
+    const uint32_t positive = (uint32_t)((int32_t)~f32_bits >> 31);
+    if (valid && i < (uint32_t)kPsHalf) atomicAdd(hist + kPsHalf + (int)(i ^ positive), 1u);
+  }
+
+  enum Found { kFound, kRange, kNothing };
+
+  // Looks for the cut in the bins. kFound: c has it. kRange: `range` holds it, and with top-k
+  // and top-p both also the k-th value. kNothing: the bins do not decide it. `sum` has the
+  // count of the valid ids, of those next to zero (bfloat16: and their mass; other types: the
+  // mass of all).
+  __device__ Found find_cut_in_bins(RowCut& c, const RowPolicy& pol, const PsBox& sum,
+                                    PsRange& range) {
+    constexpr bool kExact = DT == kBF16;  // a bin is one value
+    uint32_t n[kPsOwn];
+    merge_bins(n);
+    if (c.flat || !(c.top < kPsLarge)) return kNothing;
+    const int mine = threadIdx.x * kPsOwn;  // this thread's bins, in falling order of value
+    const bool by_mass = pol.top_p < 1.0;
+    // Bounds of the weights: of a bin's largest and smallest value. The values of 8 bins are
+    // equally spaced, their weights a geometric series; the series starts at the row's maximum
+    // in the bins that hold it (those above are empty).
+    double high[kPsOwn], low[kPsOwn], mass_high = 0.0, mass_low = 0.0;
+    uint32_t count = 0;
+#pragma unroll
+    for (int j = 0; j < kPsOwn; ++j) count += n[j];
+    if (by_mass) {
+      const float step = __uint_as_float(bin_bits(mine) << 16 & 0x7F800000u) * 0x1p-7f;
+      const double ratio = exp2_table(-(double)step * c.scale, *c.powers);
+      const float start = kExact || mine >= kPsHalf ? bin_value(mine) : bin_value(mine) + step;
+      int at = 0;
+      double w;
+      if ((double)start > c.top && count) {
+#pragma unroll
+        for (int j = kPsOwn - 1; j >= 0; --j)
+          if (n[j]) at = j;
+        const float v = bin_value(mine + at);
+        const float lowest = mine < kPsHalf ? v : v - step;
+        w = kExact ? 1.0 : c.weight(lowest);
+      } else {
+        w = c.weight(start);
+        if ((double)start > c.top) w = 0.0;  // all empty
+      }
+      const bool top_here = (double)start > c.top && !kExact;
+#pragma unroll
+      for (int j = 0; j < kPsOwn; ++j) {
+        high[j] = low[j] = 0.0;
+        if (j >= at) {
+          if (kExact) {
+            high[j] = low[j] = w;
+            w *= ratio;
+          } else if (top_here && j == at) {
+            high[j] = 1.0;
+            low[j] = w;
+          } else {
+            high[j] = w;
+            w *= ratio;
+            low[j] = w;
+          }
+        }
+        mass_high += (double)n[j] * high[j];
+        if (!kExact) mass_low += (double)n[j] * low[j];
+      }
+    }
+    if (threadIdx.x < 3) sh.cross[threadIdx.x].bin = -1;
+    uint32_t count_before = block_scan(count, sh.part_count) - count;
+    double high_end = 0.0, high_before = 0.0, low_end = 0.0, low_before = 0.0;
+    if (by_mass) {
+      high_end = block_scan(mass_high, sh.part_mass);
+      high_before = scan_before(high_end, sh.part_mass);
+      if (!kExact) {
+        low_end = block_scan(mass_low, sh.part_high);
+        low_before = scan_before(low_end, sh.part_high);
+      }
+    }
+    // the values next to zero, between the halves
+    const double small_high = kExact ? sum.mass : (double)sum.small * fmin(1.0, c.weight(kPsSmall));
+    const double small_low = kExact ? sum.mass : (double)sum.small * c.weight(-kPsSmall);
+    if (mine >= kPsHalf) {
+      count_before += sum.small;
+      high_before += small_high, high_end += small_high;
+      low_before += small_low, low_end += small_low;
+    }
+    if (kExact) low_before = high_before, low_end = high_end;
+    const uint32_t in_bins = sh.part_count[kPsWarps - 1] + sum.small;
+    // ids at and below -2^7 lie behind the bins; they may weigh nothing next to the rest
+    const uint32_t behind = sum.count - in_bins;
+    const bool behind_weighs = behind && c.weight(-kPsLarge) > 0x1p-80;
+
+    const double slack = kExact ? 0.0 : 1e-12;
+    const bool by_k = pol.top_k && pol.top_k < sum.count;
+    int k_bin = kPsBins;
+    double total = kExact ? (by_mass ? sh.part_mass[kPsWarps - 1] + sum.mass : 0.0) : sum.mass;
+    uint32_t k_count = 0;  // ids up to and with that bin
+    uint32_t k_take = 0;
+    if (by_k) {
+      if (pol.top_k > in_bins) return kNothing;
+      if (count_before < pol.top_k && pol.top_k <= count_before + count) {
+        PsCross x = {low_before, count_before, 0u, -1};
+#pragma unroll
+        for (int j = 0; j < kPsOwn; ++j)
+          if (x.bin < 0) {
+            if (pol.top_k <= x.count + n[j]) {
+              x.bin = mine + j;
+              x.n = n[j];
+              if (by_mass) x.mass += (double)(pol.top_k - x.count) * low[j];
+            } else {
+              x.count += n[j];
+              if (by_mass) x.mass += (double)n[j] * low[j];
+            }
+          }
+        sh.cross[0] = x;
+      }
+      __syncthreads();
+      const PsCross x = sh.cross[0];
+      if (x.bin < 0) return kNothing;  // among the values next to zero
+      k_bin = x.bin;
+      total = x.mass;
+      k_count = x.count + x.n;
+      k_take = pol.top_k - x.count;
+      if (!by_mass) {
+        range = {bin_low_code(k_bin) + 0xFFFFu, bin_low_code(k_bin), x.count, x.n};
+        if (kExact) c.keep(bin_value(k_bin), k_take);
+      }
+    }
+    if (by_mass) {
+      if (!by_k && behind_weighs) return kNothing;
+      const double goal = top_p_goal(pol.top_p, total);
+      // the first bin in which the mass can reach the goal ...
+      const double least = goal * (1.0 - slack);
+      if (count && mine <= k_bin && high_before < least &&
+          (least <= high_end || k_bin < mine + kPsOwn)) {
+        PsCross x = {high_before, count_before, 0u, -1};
+        double run = high_before, weight = 0.0;
+        uint32_t run_count = count_before;
+#pragma unroll
+        for (int j = 0; j < kPsOwn; ++j)
+          if (n[j] && mine + j <= k_bin && run < least) {
+            x = {run, run_count, kExact && mine + j == k_bin ? k_take : n[j], mine + j};
+            weight = high[j];
+            run += (double)x.n * high[j];
+            run_count += n[j];
+          }
+        if (kExact) x.n = ties_to_reach(goal - x.mass, weight, x.n, x.mass, goal);
+        sh.cross[1] = x;
+      }
+      // ... and the first in which it must have
+      const double most = goal * (1.0 + slack);
+      if (!kExact && !by_k && count && low_before < most && most <= low_end) {
+        PsCross x = {0.0, count_before, 0u, -1};
+        double run = low_before;
+#pragma unroll
+        for (int j = 0; j < kPsOwn; ++j)
+          if (n[j] && run < most) {
+            run += (double)n[j] * low[j];
+            x.count += n[j];
+            x.bin = mine + j;
+          }
+        sh.cross[2] = x;
+      }
+      __syncthreads();
+      const PsCross x = sh.cross[1];
+      if (x.bin < 0) return kNothing;  // among the values next to zero
+      if (kExact) {
+        c.keep(bin_value(x.bin), x.n);
+      } else {
+        const uint32_t hi = bin_low_code(x.bin) + 0xFFFFu;
+        if (by_k) {
+          range = {hi, bin_low_code(k_bin), x.count, k_count - x.count};
+        } else {
+          PsCross y = sh.cross[2];
+          if (y.bin < 0) y.bin = kPsBins - 1, y.count = in_bins;
+          range = {hi, bin_low_code(y.bin), x.count, y.count - x.count};
+        }
+      }
+    }
+    if (!kExact) return kRange;
+    // the weights of the kept bins, for the passes that follow
+    __syncthreads();  // the counts have been read
+    const float cut = c.cut;
+    double* weights = ps_table();
+#pragma unroll
+    for (int j = 0; j < kPsOwn; ++j)
+      if (n[j] && bin_value(mine + j) >= cut)
+        weights[mine + j] = by_mass ? high[j] : c.weight(bin_value(mine + j));
+    table = weights;
+    __syncthreads();
+    return kFound;
+  }
+
+  // Least number of ids of weight `w`, 1 to `most`, whose mass on top of `above` reaches `goal`.
+  __device__ __forceinline__ static uint32_t ties_to_reach(double need, double w, uint32_t most,
+                                                           double above, double goal) {
+    double t = ceil(need / w);
+    t = t >= 1.0 ? (t > (double)most ? (double)most : t) : 1.0;
+    while (t > 1.0 && above + (t - 1.0) * w >= goal) t -= 1.0;
+    while (t < (double)most && above + t * w < goal) t += 1.0;
+    return (uint32_t)t;
+  }
+
+  // ---- the cut from ranges of order codes -----------------------------------------------
+  // mass and count of the valid ids whose order code is at least `code`
+  __device__ PsBox at_least(const RowCut& c, uint32_t code) {
+    double mass = 0.0;
+    uint32_t count = 0;
+    view.each(lane, code, [&](uint32_t, const Raw& r) {
+      uint32_t set = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if ((r.bits >> j & 1u) && ord32(View::value_of(r, j)) >= code) set |= 1u << j;
+      count += __popc(set);
+      View::each_set(set, [&](int j, bool have) {
+        const double w = c.weight(View::value_at(r, j));
+        if (have) mass += w;
+      });
+    });
+    return reduce(mass, count, 0u, 0u);
+  }
+
+  // One turn of the histogram over the range: it shrinks to the bin that holds rank `rank_k`,
+  // or (rank_k 0) to the bins in which the mass can reach `goal`.
+  __device__ void refine(const RowCut& c, PsRange& range, uint32_t rank_k, double goal) {
+    const uint32_t width = range.hi - range.lo;
+    const int shift = max(0, 20 - __clz(width));  // width >> shift < 2^12
+    clear_hist();
+    uint32_t* hist = ps_hist();
+    double mass = 0.0;
+    view.each(lane, range.lo, [&](uint32_t, const Raw& r) {
+      uint32_t set = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t code = ord32(View::value_of(r, j));
+        const bool valid = r.bits >> j & 1u;
+        if (valid && code > range.hi) set |= 1u << j;
+        if (valid && range.hi - code <= width) atomicAdd(hist + ((range.hi - code) >> shift), 1u);
+      }
+      if (!rank_k)
+        View::each_set(set, [&](int j, bool have) {
+          const double w = c.weight(View::value_at(r, j));
+          if (have) mass += w;
+        });
+    });
+    const double above = reduce(mass, 0u, 0u, 0u).mass;
+    uint32_t n[kPsOwn], count = 0;
+    merge_bins(n);
+    const uint32_t mine = threadIdx.x * kPsOwn;
+    double mass_high = 0.0, mass_low = 0.0, high[kPsOwn], low[kPsOwn];
+#pragma unroll
+    for (int j = 0; j < kPsOwn; ++j) {
+      count += n[j];
+      high[j] = low[j] = 0.0;
+      if (!rank_k && n[j]) {
+        const uint32_t first = range.hi - ((mine + j) << shift);
+        const uint32_t span = min((1u << shift) - 1u, first - range.lo);
+        high[j] = c.weight(code_value(first));
+        low[j] = span ? c.weight(code_value(first - span)) : high[j];
+        mass_high += (double)n[j] * high[j];
+        mass_low += (double)n[j] * low[j];
+      }
+    }
+    if (threadIdx.x < 3) sh.cross[threadIdx.x].bin = -1;
+    const uint32_t before = range.above + block_scan(count, sh.part_count) - count;
+    PsCross first = {}, last = {};
+    if (rank_k) {
+      if (before < rank_k && rank_k <= before + count) {
+        PsCross x = {0.0, before, 0u, -1};
+#pragma unroll
+        for (int j = 0; j < kPsOwn; ++j)
+          if (x.bin < 0) {
+            if (rank_k <= x.count + n[j]) x.bin = (int)mine + j, x.n = n[j];
+            else x.count += n[j];
+          }
+        sh.cross[0] = x;
+      }
+      __syncthreads();
+      first = last = sh.cross[0];
+      last.count += last.n;
+    } else {
+      const double high_end = above + block_scan(mass_high, sh.part_mass);
+      const double high_before = __shfl_up_sync(~0u, high_end, 1);
+      const double hb = lane ? high_before : above + (warp ? sh.part_mass[warp - 1] : 0.0);
+      const double low_end = above + block_scan(mass_low, sh.part_high);
+      const double low_before = __shfl_up_sync(~0u, low_end, 1);
+      const double lb = lane ? low_before : above + (warp ? sh.part_high[warp - 1] : 0.0);
+      const double least = goal * (1.0 - 1e-12), most = goal * (1.0 + 1e-12);
+      if (count && hb < least && least <= high_end) {
+        PsCross x = {0.0, before, 0u, -1};
+        double run = hb;
+        uint32_t run_count = before;
+#pragma unroll
+        for (int j = 0; j < kPsOwn; ++j)
+          if (n[j] && run < least) {
+            x = {0.0, run_count, n[j], (int)mine + j};
+            run += (double)n[j] * high[j];
+            run_count += n[j];
+          }
+        sh.cross[0] = x;
+      }
+      if (count && lb < most && most <= low_end) {
+        PsCross x = {0.0, before, 0u, -1};
+        double run = lb;
+#pragma unroll
+        for (int j = 0; j < kPsOwn; ++j)
+          if (n[j] && run < most) {
+            run += (double)n[j] * low[j];
+            x.count += n[j];
+            x.bin = (int)mine + j;
+          }
+        sh.cross[1] = x;
+      }
+      __syncthreads();
+      first = sh.cross[0];
+      last = sh.cross[1];
+      if (first.bin < 0) first = {0.0, range.above, 0u, 0};
+      if (last.bin < 0) last = {0.0, range.above + range.inside, 0u, (int)(width >> shift)};
+    }
+    const uint32_t hi = range.hi - ((uint32_t)first.bin << shift);
+    const uint32_t end = range.hi - ((uint32_t)last.bin << shift);
+    const uint32_t span = min((1u << shift) - 1u, end - range.lo);
+    range = {hi, end - span, first.count, last.count - first.count};
+  }
+
+  // Halves the range by the exact mass above its middle.
+  __device__ void bisect(const RowCut& c, PsRange& range, double goal) {
+    const uint32_t mid = range.lo + (range.hi - range.lo + 1u) / 2u;
+    const PsBox b = at_least(c, mid);
+    if (b.mass >= goal) {
+      range = {range.hi, mid, range.above, b.count - range.above};
+    } else {
+      range = {mid - 1u, range.lo, b.count, range.above + range.inside - b.count};
+    }
+  }
+
+  // Lists the ids of the range (at most kPsList), sorted by value falling, and sets the cut:
+  // at rank `rank_k` (0: no bound), and with by_mass where the mass reaches top_p of `total`
+  // (with rank_k: of the mass of those ranks).
+  __device__ void cut_from_list(RowCut& c, const PsRange& range, uint32_t rank_k, bool by_mass,
+                                double top_p, double total) {
+    if (threadIdx.x == 0) sh.list_fill = 0u;
+    __syncthreads();
+    unsigned long long* list = ps_list();
+    double mass = 0.0;
+    view.each(lane, range.lo, [&](uint32_t id, const Raw& r) {
+      uint32_t set = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t code = ord32(View::value_of(r, j));
+        const bool valid = r.bits >> j & 1u;
+        if (valid && code > range.hi) set |= 1u << j;
+        if (valid && code >= range.lo && code <= range.hi) {
+          const uint32_t at = atomicAdd(&sh.list_fill, 1u);
+          // ascending keys: value falling, id rising
+          if (at < kPsList) list[at] = (unsigned long long)~code << 32 | (id + j);
+        }
+      }
+      if (by_mass)
+        View::each_set(set, [&](int j, bool have) {
+          const double w = c.weight(View::value_at(r, j));
+          if (have) mass += w;
+        });
+    });
+    __syncthreads();
+    if ((uint32_t)threadIdx.x < k)
+      *ps_remote(&sh.listed[rank], threadIdx.x) = min(sh.list_fill, kPsList);
+    const double above = reduce(mass, 0u, 0u, 0u).mass;
+    unsigned long long* sorted = ps_sorted();
+    uint32_t n = 0;
+    for (uint32_t r = 0; r < k; ++r) {
+      const uint32_t m = sh.listed[r];
+      const unsigned long long* from = k > 1 ? ps_remote(list, r) : list;
+      for (uint32_t i = threadIdx.x; i < m; i += kPsThreads)
+        if (n + i < kPsList) sorted[n + i] = from[i];
+      n += m;
+    }
+    n = min(n, kPsList);
+    uint32_t size = 2;
+    while (size < n) size <<= 1;
+    for (uint32_t i = n + threadIdx.x; i < size; i += kPsThreads) sorted[i] = ~0ull;
+    __syncthreads();
+    // bitonic sort; a warp's 64 keys need no more than the warp
+    for (uint32_t run = 2; run <= size; run <<= 1)
+      for (uint32_t d = run >> 1; d; d >>= 1) {
+        const uint32_t t = threadIdx.x;
+        if (t < size / 2) {
+          const uint32_t i = 2u * t - (t & (d - 1u));
+          const unsigned long long a = sorted[i], b = sorted[i + d];
+          if ((a > b) == ((i & run) == 0u)) sorted[i] = b, sorted[i + d] = a;
+        }
+        if (d > 32u || (d == 1u && run >= 64u)) __syncthreads();
+        else __syncwarp();
+      }
+    __syncthreads();
+    // two keys to a thread
+    const uint32_t at = 2u * threadIdx.x;
+    const uint32_t have = rank_k ? min(n, rank_k - range.above) : n;
+    if (have == 0u) {  // rounding put the goal past every id: all that was kept stays
+      publish();
+      return;
+    }
+    uint32_t pos = have - 1u;
+    if (by_mass) {
+      const double w0 = at < have ? c.weight(code_value(~(uint32_t)(sorted[at] >> 32))) : 0.0;
+      const double w1 =
+          at + 1u < have ? c.weight(code_value(~(uint32_t)(sorted[at + 1u] >> 32))) : 0.0;
+      const double end = block_scan(w0 + w1, sh.part_mass);
+      const double before = scan_before(end, sh.part_mass);
+      if (rank_k) total = above + sh.part_mass[kPsWarps - 1];
+      const double goal = top_p_goal(top_p, total);
+      uint32_t mine = have - 1u;
+      if (at < have && above + before + w0 >= goal) mine = at;
+      else if (at + 1u < have && above + end >= goal) mine = at + 1u;
+      mine = __reduce_min_sync(~0u, mine);
+      if (lane == 0) sh.part_count[warp] = mine;
+      __syncthreads();
+      for (int i = 0; i < kPsWarps; ++i) pos = min(pos, sh.part_count[i]);
+      __syncthreads();
+    }
+    const uint32_t code = ~(uint32_t)(sorted[pos] >> 32);
+    uint32_t same = 0;
+    if (at <= pos) same += ~(uint32_t)(sorted[at] >> 32) == code;
+    if (at + 1u <= pos) same += ~(uint32_t)(sorted[at + 1u] >> 32) == code;
+    same = __reduce_add_sync(~0u, same);
+    if (lane == 0) sh.part_small[warp] = same;
+    __syncthreads();
+    uint32_t take = 0;
+    for (int i = 0; i < kPsWarps; ++i) take += sh.part_small[i];
+    c.keep(code_value(code), take);
+    publish();
+  }
+
+  // The cut, starting from nothing but the row's maximum `top`, or from `found`, a range out of
+  // the bins. `total` is the mass of all ids, or negative where it is not known.
+  __device__ __noinline__ void find_cut(RowCut& c, const RowPolicy& pol, uint32_t top,
+                                        uint32_t valid, double total, const PsRange* found) {
+    if (!(pol.temperature > 0.0)) {
+      c.keep(code_value(top), 1u);
+      return;
+    }
+    c.keep(c.flat ? FLT_MAX : -INFINITY, 0u);
+    const bool by_mass = pol.top_p < 1.0;
+    PsRange range = {top, c.flat ? top : kOrd32NegInf, 0u, valid};
+    if (c.flat) range.inside = valid = at_least(c, top).count;  // the +inf ids
+    const bool by_k = pol.top_k && pol.top_k < valid;
+    if (!by_k && !by_mass) return;
+    if (found && found->inside <= kPsList) {
+      cut_from_list(c, *found, by_k ? pol.top_k : 0u, by_mass, pol.top_p, total);
+      return;
+    }
+    if (by_k) {
+      if (found && !by_mass) range = *found;
+      while (range.inside > kPsList && range.hi != range.lo) refine(c, range, pol.top_k, 0.0);
+      if (range.hi == range.lo) c.keep(code_value(range.hi), pol.top_k - range.above);
+      else cut_from_list(c, range, pol.top_k, false, 1.0, 0.0);
+      if (!by_mass) return;
+      const PsBox b = at_least(c, ord32(c.cut) + 1u);
+      const double w = c.weight(c.cut);
+      total = b.mass + (double)c.take * w;
+      const double goal = top_p_goal(pol.top_p, total);
+      if (b.mass < goal) {
+        c.take = ties_to_reach(goal - b.mass, w, c.take, b.mass, goal);
+        return;
+      }
+      range = {top, ord32(c.cut) + 1u, 0u, b.count};
+    } else {
+      if (total < 0.0) total = at_least(c, range.lo).mass;
+      if (found) range = *found;
+    }
+    const double goal = top_p_goal(pol.top_p, total);
+    while (range.inside > kPsList && range.hi != range.lo) {
+      const uint32_t width = range.hi - range.lo;
+      refine(c, range, 0u, goal);
+      if (range.hi - range.lo > width / 4u) bisect(c, range, goal);
+    }
+    if (range.hi == range.lo) {
+      const double above = at_least(c, range.hi + 1u).mass;
+      const double w = c.weight(code_value(range.hi));
+      c.keep(code_value(range.hi), ties_to_reach(goal - above, w, range.inside, above, goal));
+    } else {
+      cut_from_list(c, range, 0u, true, pol.top_p, total);
+    }
+  }
+
+  // ---- the kept mass and the draw -------------------------------------------------------
   struct Scan {  // of the entries of all warps, as this warp sees them
     double total, mass_before;  // kept mass; of it, before this warp
     uint32_t ties_before, draft_before;
@@ -728,68 +1122,70 @@ struct PolicyRow {
   }
 
   // weight of a kept value
-  __device__ __forceinline__ double weight(const RowCut& c, uint32_t f32_bits) const {
+  __device__ __forceinline__ double weight(const RowCut& c, float v) const {
     if (DT == kBF16 && table) {
-      const uint32_t i = ((f32_bits >> 16) & 0x7FFFu) - kPsLow;
-      const uint32_t positive = (uint32_t)((int32_t)~f32_bits >> 31);
+      const uint32_t bits = __float_as_uint(v);
+      const uint32_t i = ((bits >> 16) & 0x7FFFu) - kPsLow;
+      const uint32_t positive = (uint32_t)((int32_t)~bits >> 31);
       if (i < (uint32_t)kPsHalf) return table[kPsHalf + (int)(i ^ positive)];
     }
-    return c.weight(__uint_as_float(f32_bits));
+    return c.weight(v);
   }
 
-  // f(id, weights of the lane's 8 ids: 0 where not kept) over this warp's ids;
-  // `ties_before`: ids at the cut before this warp
+  // sets of the lane's 8 values: above the cut, equal to it
+  __device__ __forceinline__ static void split(const RowCut& c, const Raw& r, uint32_t& above,
+                                               uint32_t& tie) {
+    above = tie = 0u;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float v = View::value_of(r, j);
+      if (v > c.cut) above |= 1u << j;
+      if (v == c.cut) tie |= 1u << j;
+    }
+    above &= r.bits;
+    tie &= r.bits;
+  }
+
+  // f(id, raw values, set of the kept ones) over the vectors of this warp that may hold some;
+  // `ties_before`: ids at the cut before this warp. A kept id may still weigh less than min_p.
   template <class F>
   __device__ __forceinline__ void each_kept(const RowCut& c, uint32_t ties_before, F&& f) {
     uint32_t run = ties_before;
     view.each(lane, c.least(), [&](uint32_t id, const Raw& r) {
-      double w[8];
-      uint32_t tie = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t code = ord32(View::value_of(r, j));
-        const bool valid = r.bits >> j & 1u;
-        w[j] = 0.0;
-        if (valid && code == c.cut) tie |= 1u << j;
-        if (valid && code > c.cut) {
-          const double x = weight(c, View::bits_of(r, j));
-          if (x >= c.min_p) w[j] = x;
-        }
-      }
+      uint32_t set, tie;
+      split(c, r, set, tie);
       if (c.take && __any_sync(~0u, tie)) {
         const uint32_t n = __popc(tie);
         const uint32_t incl = warp_scan(n, lane);
         uint32_t at = run + incl - n;
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (tie >> j & 1u) {
-            if (at < c.take) w[j] = weight(c, View::bits_of(r, j));
-            ++at;
-          }
         run += __shfl_sync(~0u, incl, 31);
+        while (tie && at < c.take) {
+          set |= tie & (0u - tie);
+          tie &= tie - 1u;
+          ++at;
+        }
       }
-      f(id, w);
+      if (__any_sync(~0u, set)) f(id, r, set);
     });
   }
 
   // first id, in id order, whose cumulative weight exceeds `goal`; `start` is the mass before
-  // this warp; weigh(id, w[8]) may replace the kept weights. Whole warp; all lanes return it.
+  // this warp; weigh(id, kept weight) is the weight to use. Whole warp; all lanes return it.
   template <class W>
   __device__ int pick(const RowCut& c, uint32_t ties_before, double start, double goal,
                       W&& weigh) {
     int found = -1, last = -1;
     double run = start;
-    each_kept(c, ties_before, [&](uint32_t id, double* w) {
+    each_kept(c, ties_before, [&](uint32_t id, const Raw& r, uint32_t set) {
       if (found >= 0) return;  // uniform over the warp
-      weigh(id, w);
       double s = 0.0;
       int mine = -1;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        s += w[j];
-        if (w[j] > 0.0) mine = (int)id + j;
-      }
-      if (!__any_sync(~0u, mine >= 0)) return;
+      View::each_set(set, [&](int j, bool have) {
+        double w = weight(c, View::value_at(r, j));
+        w = have && w >= c.min_p ? weigh(id + j, w) : 0.0;
+        s += w;
+        if (w > 0.0) mine = (int)id + j;
+      });
       const double incl = warp_scan(s, lane);
       const uint32_t over = __ballot_sync(~0u, s > 0.0 && run + incl > goal);
       if (over) {
@@ -797,11 +1193,12 @@ struct PolicyRow {
         const double prev = __shfl_up_sync(~0u, incl, 1);
         double acc = run + (lane ? prev : 0.0);
         int at = -1;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          acc += w[j];
-          if (at < 0 && w[j] > 0.0 && acc > goal) at = (int)id + j;
-        }
+        View::each_set(set, [&](int j, bool have) {
+          double w = weight(c, View::value_at(r, j));
+          w = have && w >= c.min_p ? weigh(id + j, w) : 0.0;
+          acc += w;
+          if (at < 0 && w > 0.0 && acc > goal) at = (int)id + j;
+        });
         found = __shfl_sync(~0u, at < 0 ? mine : at, src);
         return;
       }
@@ -876,64 +1273,79 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
   RowCut c = {};
   c.inv_t = fmin(1.0 / pol.temperature, 1e300);  // 0 times it stays 0
   c.scale = c.inv_t * 1.4426950408889634;
-  c.powers = &sh.powers;
-  if (threadIdx.x < 16) sh.powers.at[threadIdx.x] = exp2((double)threadIdx.x / 16.0);
   c.min_p = pol.min_p;
+  c.powers = &sh.powers;
+  c.cut = -INFINITY;
+  if (threadIdx.x < 16) sh.powers.at[threadIdx.x] = exp2((double)threadIdx.x / 16.0);
   if (ok) {
-    // one pass over the row: its maximum, the peaks, and for bf16 the count of every value
-    const bool values = DT == kBF16 && pol.temperature > 0.0 && (pol.top_k || pol.top_p < 1.0);
+    using View = RowView<DT>;
+    const bool by_mass = pol.top_p < 1.0;
+    const bool bins = pol.temperature > 0.0 && (pol.top_k || by_mass);
+    // the mass of all ids, relative to a value of 0 (its maximum is not known yet)
+    const bool mass_of_all = DT != kBF16 && bins && by_mass && !pol.top_k;
     uint32_t* hist = ps_hist();
-    if (values) {
-      for (int i = threadIdx.x; i < kPsBins / 4; i += kPsThreads)
-        reinterpret_cast<uint4*>(hist)[i] = make_uint4(0u, 0u, 0u, 0u);
-      __syncthreads();
-    }
-    uint32_t top = 0, small = 0, large = 0, low = 0;
-    double small_mass = 0.0;  // relative to a value of 0
+    if (bins) row.clear_hist();
+    uint32_t top = 0, small = 0, count = 0;
+    double mass = 0.0;
     row.view.stream(row.lane, [&](uint32_t id, const auto& r) {
-      using View = RowView<DT>;
       const uint32_t peak = View::peak_of(r);
       if (row.view.peaks) row.view.peaks[(id - row.view.begin) >> 3] = (uint16_t)(peak >> 16);
       top = max(top, peak);
       if (OP == kOpProbs) clear_probs(p.out_probs + group * p.out_stride, id, row.view.end);
-      if (DT == kBF16 && values) {
-        uint32_t odd = 0;
+      if (!bins) return;
+      count += __popc(r.bits);
+      float near = INFINITY;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t bits = View::bits_of(r, j);
+        const bool valid = r.bits >> j & 1u;
+        PolicyRow<DT>::count_bin(hist, bits, valid);
+        near = fminf(near, valid ? fabsf(__uint_as_float(bits)) : INFINITY);
+      }
+      if (__any_sync(~0u, near < kPsSmall)) {
+        uint32_t set = 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          if (r.bits >> j & 1u)
-            if (!PolicyRow<DT>::count_bin(hist, View::bits_of(r, j))) odd |= 1u << j;
-        if (odd) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (odd >> j & 1u) {
-              const float v = View::value_of(r, j);
-              if (fabsf(v) < 1.0f) {
-                ++small;
-                small_mass += exp((double)v * c.inv_t);
-              } else if (v > 0.0f) {
-                ++large;
-              } else {
-                ++low;
-              }
-            }
-        }
+          if (fabsf(View::value_of(r, j)) < kPsSmall) set |= 1u << j;
+        set &= r.bits;
+        small += __popc(set);
+        if (DT == kBF16 && by_mass)
+          View::each_set(set, [&](int j, bool have) {
+            const double w = exp2_table((double)View::value_at(r, j) * c.scale, *c.powers);
+            if (have) mass += w;
+          });
       }
+      if (DT != kBF16 && mass_of_all)
+        View::each_set(r.bits, [&](int j, bool have) {
+          const double w = exp2_table((double)View::value_at(r, j) * c.scale, *c.powers);
+          if (have) mass += w;
+        });
     });
-    PsBox sum = row.reduce(small_mass, small, top, large, low);
+    PsBox sum = row.reduce(mass, count, top, small);
     top = sum.top;
     if (top == 0u) status = kStatusEmptyMask;
     if (top == kOrd32NaN) status = kStatusNanInSupport;
     if (top == kOrd32NegInf) status = kStatusAllNegInf;
     if (!status) {
-      const float best = PolicyRow<DT>::code_value(top);
-      c.flat = !(pol.temperature > 0.0) || best == INFINITY;
-      c.top = best;
-      sum.mass = sum.count ? sum.mass * exp(-c.top * c.inv_t) : 0.0;
-      // a small mass that left the range of doubles on the way
-      const bool lost = !(sum.mass >= 0.0 && sum.mass < INFINITY);
-      if (!(values && !lost && row.find_cut_by_values(c, pol, sum, ps_table(p.k)))) {
-        __syncthreads();  // the scans' results have been read
-        row.find_cut(c, pol, top);
+      c.top = code_value(top);
+      c.flat = !(pol.temperature > 0.0) || c.top == INFINITY;
+      // the masses relative to the maximum, where they did not leave the range of doubles
+      const double shift = -c.top * c.scale;
+      const bool in_range = fabs(shift) < 900.0;
+      sum.mass = sum.mass > 0.0 ? sum.mass * exp2_table(shift, sh.powers) : 0.0;
+      const double total = in_range && mass_of_all ? sum.mass : -1.0;
+      if (!bins) {
+        if (pol.temperature > 0.0) c.cut = c.flat ? FLT_MAX : -INFINITY;
+        else c.keep(code_value(top), 1u);
+      } else {
+        PsRange range;
+        auto found = PolicyRow<DT>::kNothing;
+        if (in_range) found = row.find_cut_in_bins(c, pol, sum, range);
+        if (found != PolicyRow<DT>::kFound) {
+          __syncthreads();  // what the scans left in shared memory has been read
+          row.find_cut(c, pol, top, sum.count, total,
+                       found == PolicyRow<DT>::kRange ? &range : nullptr);
+        }
       }
       c.bound_by_min_p();
     }
@@ -968,33 +1380,31 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
   uint32_t ties = 0, before = 0;
   row.view.each(row.lane, c.least(), [&](uint32_t id, const auto& r) {
     using View = RowView<DT>;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (!(r.bits >> j & 1u)) continue;
-      const uint32_t code = ord32(View::value_of(r, j));
-      if (code == c.cut) {
-        ++ties;
-        if (OP == kOpSpec && id + j < draft) ++before;
-      } else if (code > c.cut) {
-        const double w = row.weight(c, View::bits_of(r, j));
-        if (w >= c.min_p) mass += w;
-      }
-    }
+    uint32_t set, tie;
+    PolicyRow<DT>::split(c, r, set, tie);
+    ties += __popc(tie);
+    if (OP == kOpSpec && id < draft)
+      before += __popc(draft - id < 8u ? tie & ((1u << (draft - id)) - 1u) : tie);
+    View::each_set(set, [&](int j, bool have) {
+      const double w = row.weight(c, View::value_at(r, j));
+      if (have && w >= c.min_p) mass += w;
+    });
   });
   mass = warp_sum(mass);
   ties = __reduce_add_sync(~0u, ties);
   before = __reduce_add_sync(~0u, before);
-  const double w_tie = c.take ? c.weight(PolicyRow<DT>::code_value(c.cut)) : 0.0;
+  const double w_tie = c.take ? c.weight(c.cut) : 0.0;
   auto scan = row.scan_entries(0, mass, ties, before, c.take, w_tie);
   const double total = scan.total;
 
   if (OP == kOpProbs) {
     float* out = p.out_probs + group * p.out_stride;
     const double inv = 1.0 / total;
-    row.each_kept(c, scan.ties_before, [&](uint32_t id, double* w) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (w[j] > 0.0) out[id + j] = (float)(w[j] * inv);
+    row.each_kept(c, scan.ties_before, [&](uint32_t id, const auto& r, uint32_t set) {
+      RowView<DT>::each_set(set, [&](int j, bool have) {
+        const double w = row.weight(c, RowView<DT>::value_at(r, j));
+        if (have && w >= c.min_p) out[id + j] = (float)(w * inv);
+      });
     });
     if (first) p.out_status[item] = 0u;
     return;
@@ -1009,8 +1419,7 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
       if (q) q_d = fmax((double)q[draft], 0.0);
       const bool valid = !row.view.mask || (row.view.mask[draft >> 3] >> (draft & 7u) & 1u);
       const float v = Elem<DT>::to_f32(row.view.row, draft);
-      const uint32_t code = ord32(v);
-      if (valid && (code > c.cut || (code == c.cut && scan.draft_before < c.take))) {
+      if (valid && (v > c.cut || (v == c.cut && scan.draft_before < c.take))) {
         const double w = c.weight(v);
         if (w >= c.min_p) p_d = w / total;
       }
@@ -1024,21 +1433,17 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
 
   // what remains of p where the draft's probability is taken off
   const double inv = 1.0 / total;
-  auto rest = [&](uint32_t id, double* w) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (w[j] > 0.0) {
-        const double qj = q ? fmax((double)q[id + j], 0.0)
-                            : (drafted && id + j == draft ? 1.0 : 0.0);
-        w[j] = fmax(w[j] * inv - qj, 0.0);
-      }
+  auto rest = [&](uint32_t id, double w) {
+    const double q_id = q ? fmax((double)q[id], 0.0) : (drafted && id == draft ? 1.0 : 0.0);
+    return fmax(w * inv - q_id, 0.0);
   };
   if (OP == kOpSpec && residual) {
     double sum = 0.0;
-    row.each_kept(c, scan.ties_before, [&](uint32_t id, double* w) {
-      rest(id, w);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) sum += w[j];
+    row.each_kept(c, scan.ties_before, [&](uint32_t id, const auto& r, uint32_t set) {
+      RowView<DT>::each_set(set, [&](int j, bool have) {
+        const double w = row.weight(c, RowView<DT>::value_at(r, j));
+        if (have && w >= c.min_p) sum += rest(id + j, w);
+      });
     });
     sum = warp_sum(sum);
     const auto left = row.scan_entries(1, sum, ties, 0u, 0u, 0.0);
@@ -1052,7 +1457,7 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
     const int id = OP == kOpSpec && residual
                        ? row.pick(c, scan.ties_before, scan.mass_before, goal, rest)
                        : row.pick(c, scan.ties_before, scan.mass_before, goal,
-                                  [](uint32_t, double*) {});
+                                  [](uint32_t, double w) { return w; });
     if (row.lane == 0) {
       if (OP == kOpDraw) {
         p.out_idx[item] = id;
