@@ -217,7 +217,7 @@ ONYX_API int onyx_masked_sample(const void* logits, int dtype, int64_t rows, int
  * exceeds u times the kept total, u = uniforms[r * uniform_stride] in [0, 1), float or
  * double (uniform_dtype ONYX_DTYPE_F32 or ONYX_DTYPE_F64). Status as for onyx_masked_sample,
  * and BAD_POLICY for a policy or a uniform outside its range (the row's logits are not
- * looked at); the id is -1 with any of them.
+ * looked at); the id is -1 with any of them. vocab is at most 2^30 in the three calls.
  */
 ONYX_API int onyx_policy_sample(const void* logits, int dtype, int64_t rows, int64_t vocab,
                                 int64_t row_stride, const uint32_t* mask, int64_t mask_stride,

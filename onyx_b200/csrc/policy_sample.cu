@@ -52,7 +52,7 @@ static cudaError_t allow_shared(const void* fn, int which) {
   if (e != cudaSuccess) return e;
   if (dev >= 0 && dev < 64 && (done[dev].load(std::memory_order_acquire) >> which & 1)) return e;
   e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           (int)(2 * kPsArea + kPsMostPeaks));
+                           (int)(std::max(ps_fixed(kF32), ps_fixed(kBF16)) + kPsMostPeaks));
   if (e == cudaSuccess && dev >= 0 && dev < 64)
     done[dev].fetch_or((uint16_t)(1u << which), std::memory_order_release);
   return e;
@@ -66,8 +66,8 @@ static int launch_policy(int dtype, PolicyParams& p, int64_t rows, cudaStream_t 
   p.k = cluster_size(rows, p.vocab, sms);
   if (rows * p.k > 0x7FFFFFFFll) return ONYX_ERR_INVALID_ARGUMENT;
   const int64_t per = (int64_t)p.k * kPsWarps * kPsChunk;
-  p.warp_ids = (int32_t)((p.vocab + per - 1) / per * kPsChunk);
-  size_t smem = 2 * kPsArea;
+  p.warp_ids = (int32_t)((p.vocab + 7 + per - 1) / per * kPsChunk);  // up to 7 ids of offset
+  size_t smem = ps_fixed(dtype);
   const size_t peaks = (size_t)p.warp_ids / 8 * kPsWarps * sizeof(uint16_t);
   p.peaks = 0;
   if (peaks <= kPsMostPeaks) {
@@ -102,11 +102,13 @@ static int launch_policy(int dtype, PolicyParams& p, int64_t rows, cudaStream_t 
 
 static bool policy_dtype(int dt) { return dt == kF32 || dt == kF16 || dt == kBF16; }
 
+constexpr int64_t kPsMostVocab = 1ll << 30;  // positions are counted in 32 bits
+
 // The checks that the three entry points share; `rows` entries of the policies.
 static int policy_checks(const void* logits, int dtype, int64_t rows, int64_t vocab,
                          const double* policies, int64_t policy_stride) {
   if (!policy_dtype(dtype)) return ONYX_ERR_UNSUPPORTED_DTYPE;
-  if (rows < 0 || rows > 0x7FFFFFFFll || vocab <= 0 || vocab > 0x7FFFFFFFll - 1)
+  if (rows < 0 || rows > 0x7FFFFFFFll || vocab <= 0 || vocab > kPsMostVocab)
     return ONYX_ERR_INVALID_ARGUMENT;
   if (rows > 0 && (!logits || !policies)) return ONYX_ERR_INVALID_ARGUMENT;
   if (policy_stride != 0 && policy_stride < 4) return ONYX_ERR_INVALID_ARGUMENT;

@@ -50,7 +50,7 @@ constexpr int kPsWarps = kPsThreads / 32;
 constexpr int kPsMaxCluster = 8;
 constexpr int kPsEntries = kPsMaxCluster * kPsWarps;
 constexpr int kPsChunk = 256;  // ids a warp handles at a time, 8 to a lane
-constexpr int kPsAhead = 4;    // chunks whose loads the streaming pass has in flight
+constexpr int kPsUnits = 1024;  // pieces at most into which the drawing CTA cuts a warp's part
 
 // The value histogram: one bin for every bf16 value with 2^-9 <= |v| < 2^7, in falling order
 // of value; positive ones first. The values next to zero, |v| < 2^-9, lie between the halves.
@@ -188,8 +188,10 @@ struct PsShared {
   uint32_t list_fill;
 };
 
-// Dynamic shared memory: 32 KB that hold the CTA's histogram and the cluster's, or a list and
-// its sorted form, or in the end the weights of the bins; then the peaks of this CTA's ids.
+// Dynamic shared memory. While the row streams in: the CTA's histogram, then the rings through
+// which the warps copy it. After that the rings' first 16 KB hold the cluster's histogram; the
+// two histograms' 32 KB are used again for a list and its sorted form, and for the weights of
+// the bins; behind them the drawing CTA keeps the sums of its pieces. Last come the peaks.
 extern __shared__ __align__(16) unsigned char ps_dynamic[];
 constexpr size_t kPsArea = kPsBins * sizeof(uint32_t);
 __device__ __forceinline__ uint32_t* ps_hist() { return reinterpret_cast<uint32_t*>(ps_dynamic); }
@@ -203,53 +205,172 @@ __device__ __forceinline__ unsigned long long* ps_sorted() {
   return reinterpret_cast<unsigned long long*>(ps_dynamic + kPsArea);
 }
 __device__ __forceinline__ double* ps_table() { return reinterpret_cast<double*>(ps_dynamic); }
+__device__ __forceinline__ double* ps_unit_mass() {
+  return reinterpret_cast<double*>(ps_dynamic + 2 * kPsArea);
+}
+__device__ __forceinline__ uint32_t* ps_unit_ties() {
+  return reinterpret_cast<uint32_t*>(ps_dynamic + 2 * kPsArea + kPsUnits * sizeof(double));
+}
+// A warp's ring: kDepth slots of one chunk's values and mask words.
+__host__ __device__ constexpr int ps_depth(int dt) { return dt == kF32 ? 3 : 4; }
+__host__ __device__ constexpr int ps_slot(int dt) { return kPsChunk * (dt == kF32 ? 4 : 2) + 48; }
+__host__ __device__ constexpr size_t ps_ring(int dt) { return (size_t)ps_depth(dt) * ps_slot(dt); }
+// bytes ahead of the peaks
+__host__ __device__ constexpr size_t ps_fixed(int dt) {
+  return kPsArea + (kPsWarps * ps_ring(dt) > kPsArea + kPsUnits * 12u
+                        ? kPsWarps * ps_ring(dt)
+                        : kPsArea + kPsUnits * 12u);
+}
 
-// The part of a row that one warp owns, and how it is read.
+__device__ __forceinline__ void ps_copy16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                   (uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
+}
+// 4 bytes, or zeros
+__device__ __forceinline__ void ps_copy4(void* dst, const void* src, bool have) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(
+                   (uint32_t)__cvta_generic_to_shared(dst)), "l"(src), "r"(have ? 4 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void ps_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void ps_await() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// The part of a row that one warp owns, and how it is read. Ids are counted by positions:
+// position = id + off, where `off` values lie between the 16-byte boundary at or before the
+// row's start and the start. So 8 positions from a multiple of 8 are 16-byte vectors in memory
+// whatever the row's alignment; those with an id outside the row are read value by value.
 template <int DT>
 struct RowView {
   using S = typename Elem<DT>::storage;
+  static constexpr int kDepth = ps_depth(DT), kSlot = ps_slot(DT);
   const S* row;
-  const uint8_t* mask;  // bit t & 7 of byte t >> 3
-  uint16_t* peaks;      // of this warp: order code >> 16 of the maximum of every 8 ids, or null
-  uint32_t begin, end, vocab;
-  bool vec;  // 16-byte loads: the row starts on a 16-byte boundary
+  const uint32_t* mask;
+  uint16_t* peaks;  // of this CTA: order code >> 16 of the maximum of every 8, or null
+  uint32_t base;    // the CTA's first position
+  uint32_t begin, end;  // positions; multiples of kPsChunk, but for the row's end
+  int vocab, off;
 
-  struct Raw {  // 8 consecutive ids as loaded
+  struct Raw {  // the values at 8 positions as loaded
     uint4 a, b;
-    uint32_t bits;
+    uint32_t bits;  // which of them are valid
   };
 
-  __device__ __forceinline__ Raw load(uint32_t id) const {
+  __device__ __forceinline__ int id_of(uint32_t pos) const { return (int)pos - off; }
+
+  // of the 8 ids from `id` on, those inside the row
+  __device__ __forceinline__ uint32_t inside(int id) const {
+    uint32_t bits = 0xFFu;
+    if (id < 0) bits = 0xFFu << min(-id, 8) & 0xFFu;
+    const int left = vocab - id;
+    if (left < 8) bits &= left > 0 ? (1u << left) - 1u : 0u;
+    return bits;
+  }
+
+  __device__ __forceinline__ void load_edge(Raw& r, int id) const {
+    uint32_t u[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      u[j] = 0u;
+      if (id + j >= 0 && id + j < vocab) {
+        if constexpr (DT == kF32) u[j] = __float_as_uint(row[id + j]);
+        else u[j] = row[id + j];
+      }
+    }
+    if constexpr (DT == kF32) {
+      r.a = make_uint4(u[0], u[1], u[2], u[3]);
+      r.b = make_uint4(u[4], u[5], u[6], u[7]);
+    } else {
+      r.a = make_uint4(u[0] | u[1] << 16, u[2] | u[3] << 16, u[4] | u[5] << 16, u[6] | u[7] << 16);
+    }
+  }
+
+  // the values at 8 positions, from global memory; none for a position past the end
+  __device__ __forceinline__ Raw load(uint32_t pos) const {
     Raw r;
     r.a = make_uint4(0u, 0u, 0u, 0u);
     if (DT == kF32) r.b = r.a;
     r.bits = 0u;
-    if (id >= end) return r;
-    const uint32_t left = vocab - id;
-    r.bits = mask ? mask[id >> 3] : 0xFFu;
-    if (left < 8u) r.bits &= (1u << left) - 1u;
-    if (vec && left >= 8u) {
+    if (pos >= end) return r;
+    const int id = id_of(pos);
+    r.bits = inside(id);
+    if (r.bits == 0xFFu) {
       r.a = *reinterpret_cast<const uint4*>(row + id);
       if (DT == kF32) r.b = *reinterpret_cast<const uint4*>(row + id + 4);
     } else {
-      uint32_t u[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        u[j] = 0u;
-        if ((uint32_t)j < left) {
-          if constexpr (DT == kF32) u[j] = __float_as_uint(row[id + j]);
-          else u[j] = row[id + j];
-        }
-      }
-      if constexpr (DT == kF32) {
-        r.a = make_uint4(u[0], u[1], u[2], u[3]);
-        r.b = make_uint4(u[4], u[5], u[6], u[7]);
-      } else {
-        r.a = make_uint4(u[0] | u[1] << 16, u[2] | u[3] << 16, u[4] | u[5] << 16,
-                         u[6] | u[7] << 16);
-      }
+      load_edge(r, id);
+    }
+    if (mask) {
+      const int w = id >> 5, words = (vocab + 31) >> 5;
+      const uint32_t lo = w >= 0 ? mask[w] : 0u;
+      const uint32_t hi = (id & 31) > 24 && w + 1 < words ? mask[w + 1] : 0u;
+      r.bits &= __funnelshift_r(lo, hi, id & 31);
     }
     return r;
+  }
+
+  // Starts the copy of chunk i (of n) into its slot of the warp's ring.
+  __device__ __forceinline__ void copy_chunk(unsigned char* ring, int lane, int i, int n) const {
+    if (i < n) {
+      unsigned char* slot = ring + (i % kDepth) * kSlot;
+      const int id0 = id_of(begin + (uint32_t)i * kPsChunk);
+      constexpr int kVec = DT == kF32 ? 4 : 8;
+#pragma unroll
+      for (int h = 0; h < 8 / kVec; ++h) {
+        const int v = lane + 32 * h, id = id0 + v * kVec;
+        // float32: a lane's two vectors 512 bytes apart, so that reading them has no conflicts
+        const int to = DT == kF32 ? (v & 1) * 512 + (v >> 1) * 16 : v * 16;
+        if (id >= 0 && id + kVec <= vocab) ps_copy16(slot + to, row + id);
+      }
+      if (mask && lane < 10) {
+        const int w = (id0 >> 5) + lane;
+        const bool have = w >= 0 && w < (vocab + 31) >> 5;
+        ps_copy4(slot + kSlot - 48 + 4 * lane, mask + (have ? w : 0), have);
+      }
+    }
+    ps_commit();
+  }
+
+  __device__ __forceinline__ int chunks() const {
+    return (int)((end - begin + kPsChunk - 1) / kPsChunk);
+  }
+  __device__ __forceinline__ void start_stream(unsigned char* ring, int lane) const {
+    const int n = chunks();
+#pragma unroll
+    for (int i = 0; i < kDepth - 1; ++i) copy_chunk(ring, lane, i, n);
+  }
+
+  // f(position of the lane's first value, its values): the pass that reads the row from HBM,
+  // through the ring that start_stream() began to fill. Every lane makes every call.
+  template <class F>
+  __device__ __forceinline__ void stream(unsigned char* ring, int lane, F&& f) const {
+    const int n = chunks();
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
+      copy_chunk(ring, lane, i + kDepth - 1, n);
+      ps_await<kDepth - 1>();
+      __syncwarp();
+      const unsigned char* slot = ring + (i % kDepth) * kSlot;
+      const uint32_t pos = begin + (uint32_t)i * kPsChunk + 8u * lane;
+      const int id = id_of(pos);
+      Raw r;
+      r.bits = inside(id);
+      if (r.bits == 0xFFu) {
+        r.a = *reinterpret_cast<const uint4*>(slot + lane * 16);
+        if (DT == kF32) r.b = *reinterpret_cast<const uint4*>(slot + 512 + lane * 16);
+      } else {
+        load_edge(r, id);
+      }
+      if (mask) {
+        const uint32_t* words = reinterpret_cast<const uint32_t*>(slot + kSlot - 48);
+        const int w = (id >> 5) - ((id - 8 * lane) >> 5);
+        r.bits &= __funnelshift_r(words[w], words[w + 1], id & 31);
+      }
+      __syncwarp();  // the slot has been read
+      f(pos, r);
+    }
   }
 
   // float32 bits of value j
@@ -290,21 +411,33 @@ struct RowView {
     }
   }
 
-  // order code of the largest valid value, 0 without one; NaN above all
-  __device__ __forceinline__ static uint32_t peak_of(const Raw& r) {
-    if (!r.bits) return 0u;
+  // the 8 values cut to bfloat16 width, two to a word
+  __device__ __forceinline__ static void narrow(const Raw& r, uint32_t (&t)[4]) {
+    if constexpr (DT == kBF16) {
+      t[0] = r.a.x, t[1] = r.a.y, t[2] = r.a.z, t[3] = r.a.w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        t[i] = __byte_perm(bits_of(r, 2 * i), bits_of(r, 2 * i + 1), 0x7632);
+    }
+  }
+
+  // Order code >> 16 of the largest valid value, 0 without one; raises `top`, which a NaN turns
+  // into one. `t` and `v`: the values to bfloat16 width and masks of the valid ones.
+  __device__ __forceinline__ static uint32_t peak(const Raw& r, const uint32_t (&t)[4],
+                                                  const uint32_t (&v)[4], bool full, float& top) {
     float m;
     if constexpr (DT == kF32) {
-      m = -INFINITY;
+      float x[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        m = max_nan_f32(m, r.bits >> j & 1u ? value_of(r, j) : -INFINITY);
+        x[j] = full || (r.bits >> j & 1u) ? value_of(r, j) : -INFINITY;
+      m = max_nan_f32(max_nan_f32(max_nan_f32(x[0], x[1]), max_nan_f32(x[2], x[3])),
+                      max_nan_f32(max_nan_f32(x[4], x[5]), max_nan_f32(x[6], x[7])));
     } else {
       const uint32_t none = DT == kBF16 ? 0xFF80FF80u : 0xFC00FC00u;  // -inf twice
-      uint32_t m01, m23, m45, m67;
-      expand8_16(r.bits, m01, m23, m45, m67);
-      const uint32_t a = (r.a.x & m01) | (none & ~m01), b = (r.a.y & m23) | (none & ~m23);
-      const uint32_t d = (r.a.z & m45) | (none & ~m45), e = (r.a.w & m67) | (none & ~m67);
+      const uint32_t a = (r.a.x & v[0]) | (none & ~v[0]), b = (r.a.y & v[1]) | (none & ~v[1]);
+      const uint32_t d = (r.a.z & v[2]) | (none & ~v[2]), e = (r.a.w & v[3]) | (none & ~v[3]);
       if constexpr (DT == kBF16) {
         const uint32_t x = max_nan_bf16x2(max_nan_bf16x2(a, b), max_nan_bf16x2(d, e));
         m = max_nan_f32(bf16_bits_to_f32(x & 0xFFFFu), bf16_bits_to_f32(x >> 16));
@@ -313,34 +446,33 @@ struct RowView {
         m = max_nan_f32(f16_bits_to_f32(x & 0xFFFFu), f16_bits_to_f32(x >> 16));
       }
     }
-    return ord32(m);
+    if (r.bits == 0u) return 0u;
+    top = max_nan_f32(top, m);
+    return ord32(m) >> 16;
   }
 
-  // f(id of the lane's first value, its raw values): the pass that reads the row from HBM.
-  // Every lane of the warp makes every call.
-  template <class F>
-  __device__ __forceinline__ void stream(int lane, F&& f) const {
-    uint32_t at = begin;
-    for (; at < end; at += kPsAhead * kPsChunk) {
-      Raw r[kPsAhead];
-#pragma unroll
-      for (int i = 0; i < kPsAhead; ++i) r[i] = load(at + i * kPsChunk + 8u * lane);
-#pragma unroll
-      for (int i = 0; i < kPsAhead; ++i)
-        if (at + i * kPsChunk < end) f(at + i * kPsChunk + 8u * lane, r[i]);
-    }
-  }
-
-  // f(id, raw values) over the chunks that may hold order codes of at least `code`; lanes whose
-  // 8 ids hold none get no valid ids. Every lane of the warp makes every call.
+  // f(position, values) over the chunks that may hold order codes of at least `code`, the next
+  // one's loads in flight; lanes whose 8 values hold none get no valid ones. Every lane of the
+  // warp makes every call.
   template <class F>
   __device__ __forceinline__ void each(int lane, uint32_t code, F&& f) const {
-    for (uint32_t at = begin; at < end; at += kPsChunk) {
-      const uint32_t id = at + 8u * lane;
-      const bool need = !peaks || peaks[(id - begin) >> 3] >= (code >> 16);
-      if (!__any_sync(~0u, need)) continue;
-      const Raw r = load(need ? id : end);
-      f(id, r);
+    const uint32_t step = 8u * lane, first = code >> 16;
+    auto need = [&](uint32_t at) {
+      return !peaks || peaks[(at + step - base) >> 3] >= first;
+    };
+    auto next = [&](uint32_t at) {
+      while (at < end && !__any_sync(~0u, need(at))) at += kPsChunk;
+      return at;
+    };
+    uint32_t at = next(begin);
+    Raw r = load(at < end && need(at) ? at + step : end);
+#pragma unroll 1
+    while (at < end) {
+      const uint32_t then = next(at + kPsChunk);
+      const Raw more = load(then < end && need(then) ? then + step : end);
+      f(at + step, r);
+      at = then;
+      r = more;
     }
   }
 };
@@ -420,6 +552,7 @@ struct PolicyRow {
   View view;
   const double* table = nullptr;  // weights of the kept bins, where the cut came from them
   uint32_t rank, k;
+  uint32_t warp_ids, row_end;  // positions of a warp, and of the row
   int warp, lane, entry;
   int parity = 0;
 
@@ -469,24 +602,55 @@ struct PolicyRow {
     return r;
   }
 
-  // inclusive scan over the CTA; part[w] becomes the sum up to and with warp w
-  template <class T>
-  __device__ __forceinline__ T block_scan(T v, T* part) {
-    const T incl = warp_scan(v, lane);
-    if (lane == 31) part[warp] = incl;
-    __syncthreads();
-    if (warp == 0) {
-      const T x = lane < kPsWarps ? part[lane] : T(0);
-      const T y = warp_scan(x, lane);
-      if (lane < kPsWarps) part[lane] = y;
+  // Exclusive scans over the CTA's threads, and the totals. The end of one thread's part is the
+  // start of the next one's bit for bit: each goal lies in one thread's part only. The parts
+  // are read by every thread, so a __syncthreads() has to lie between two calls.
+  struct Scanned {
+    uint32_t count_before, count_all;
+    double high_before, high_end, high_all, low_before, low_end, low_all;
+  };
+  __device__ Scanned scan_parts(uint32_t count, double high, double low, bool masses,
+                                bool two) {
+    Scanned s = {};
+    const uint32_t count_incl = warp_scan(count, lane);
+    double high_incl = 0.0, low_incl = 0.0;
+    if (masses) high_incl = warp_scan(high, lane);
+    if (two) low_incl = warp_scan(low, lane);
+    if (lane == 31) {
+      sh.part_count[warp] = count_incl;
+      sh.part_mass[warp] = high_incl;
+      sh.part_high[warp] = low_incl;
     }
     __syncthreads();
-    return warp ? part[warp - 1] + incl : incl;
-  }
-  // the same sums without this thread's: what the thread before it got, bit for bit
-  __device__ __forceinline__ double scan_before(double incl, const double* part) const {
-    const double prev = __shfl_up_sync(~0u, incl, 1);
-    return lane ? prev : warp ? part[warp - 1] : 0.0;
+    const uint32_t c = lane < kPsWarps ? sh.part_count[lane] : 0u;
+    const uint32_t c_incl = warp_scan(c, lane);
+    s.count_all = __shfl_sync(~0u, c_incl, 31);
+    s.count_before = __shfl_sync(~0u, c_incl - c, warp) + count_incl - count;
+    if (masses) {
+      double run = 0.0, mine = 0.0;
+#pragma unroll
+      for (int i = 0; i < kPsWarps; ++i) {
+        if (i == warp) mine = run;
+        run += sh.part_mass[i];
+      }
+      const double prev = __shfl_up_sync(~0u, high_incl, 1);
+      s.high_all = run;
+      s.high_before = lane ? mine + prev : mine;
+      s.high_end = mine + high_incl;
+    }
+    if (two) {
+      double run = 0.0, mine = 0.0;
+#pragma unroll
+      for (int i = 0; i < kPsWarps; ++i) {
+        if (i == warp) mine = run;
+        run += sh.part_high[i];
+      }
+      const double prev = __shfl_up_sync(~0u, low_incl, 1);
+      s.low_all = run;
+      s.low_before = lane ? mine + prev : mine;
+      s.low_end = mine + low_incl;
+    }
+    return s;
   }
 
   __device__ __forceinline__ void clear_hist() {
@@ -496,8 +660,8 @@ struct PolicyRow {
   }
 
   // After a reduce(): the cluster's counts of this thread's kPsOwn bins. Every CTA adds up its
-  // part of the bins and hands the sums to all.
-  __device__ __forceinline__ void merge_bins(uint32_t (&n)[kPsOwn]) {
+  // part of the bins and hands the sums to all. by_magnitude: bins as count_bins() lays them.
+  __device__ void merge_bins(uint32_t (&n)[kPsOwn], bool by_magnitude) {
     const uint32_t* from = ps_hist();
     if (k > 1) {
       const int part = kPsBins / (int)k;
@@ -517,11 +681,13 @@ struct PolicyRow {
       publish();
       from = ps_merged();
     }
+    const int mine = threadIdx.x * kPsOwn;
+    const bool turned = by_magnitude && mine < kPsHalf;
+    const uint4* at = reinterpret_cast<const uint4*>(from + (turned ? kPsHalf - kPsOwn - mine : mine));
+    const uint4 x = at[0], y = at[1];
+    const uint32_t t[kPsOwn] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
 #pragma unroll
-    for (int i = 0; i < kPsOwn / 4; ++i) {
-      const uint4 x = reinterpret_cast<const uint4*>(from)[threadIdx.x * (kPsOwn / 4) + i];
-      n[4 * i] = x.x, n[4 * i + 1] = x.y, n[4 * i + 2] = x.z, n[4 * i + 3] = x.w;
-    }
+    for (int j = 0; j < kPsOwn; ++j) n[j] = turned ? t[kPsOwn - 1 - j] : t[j];
   }
 
   // ---- the cut from the histogram of values ---------------------------------------------
@@ -537,11 +703,18 @@ struct PolicyRow {
     return bin < kPsHalf ? code : code - 0xFFFFu;
   }
 
-  // counts a value's bin, if it has one
-  __device__ __forceinline__ static void count_bin(uint32_t* hist, uint32_t f32_bits, bool valid) {
-    const uint32_t i = ((f32_bits >> 16) & 0x7FFFu) - kPsLow;
-    const uint32_t positive = (uint32_t)((int32_t)~f32_bits >> 31);
-    if (valid && i < (uint32_t)kPsHalf) atomicAdd(hist + kPsHalf + (int)(i ^ positive), 1u);
+  // Counts the bins of two values, the bfloat16 halves of `u`, where `valid` has ones; returns
+  // bit 15 and bit 31 set for those next to zero. In memory the bins of either sign lie by
+  // rising magnitude, negative ones behind. With the sign bit set no half borrows from the
+  // other; the bin is right where bits 11 to 14 come out as zeros.
+  __device__ __forceinline__ static uint32_t count_bins(unsigned char* hist, uint32_t u,
+                                                        uint32_t valid) {
+    const uint32_t t = (u | 0x80008000u) - kPsLow * 0x10001u;
+    const uint32_t bad = (t & 0x78007800u) | ~valid;
+    const uint32_t at = ((t & 0x07FF07FFu) | ((u >> 4) & 0x08000800u)) << 2;
+    if ((bad & 0xFFFFu) == 0u) atomicAdd(reinterpret_cast<uint32_t*>(hist + (at & 0xFFFFu)), 1u);
+    if (bad < 0x10000u) atomicAdd(reinterpret_cast<uint32_t*>(hist + (at >> 16)), 1u);
+    return ~t & 0x80008000u & valid;
   }
 
   enum Found { kFound, kRange, kNothing };
@@ -554,7 +727,7 @@ struct PolicyRow {
                                     PsRange& range) {
     constexpr bool kExact = DT == kBF16;  // a bin is one value
     uint32_t n[kPsOwn];
-    merge_bins(n);
+    merge_bins(n, true);
     if (c.flat || !(c.top < kPsLarge)) return kNothing;
     const int mine = threadIdx.x * kPsOwn;  // this thread's bins, in falling order of value
     const bool by_mass = pol.top_p < 1.0;
@@ -604,16 +777,10 @@ struct PolicyRow {
       }
     }
     if (threadIdx.x < 3) sh.cross[threadIdx.x].bin = -1;
-    uint32_t count_before = block_scan(count, sh.part_count) - count;
-    double high_end = 0.0, high_before = 0.0, low_end = 0.0, low_before = 0.0;
-    if (by_mass) {
-      high_end = block_scan(mass_high, sh.part_mass);
-      high_before = scan_before(high_end, sh.part_mass);
-      if (!kExact) {
-        low_end = block_scan(mass_low, sh.part_high);
-        low_before = scan_before(low_end, sh.part_high);
-      }
-    }
+    const Scanned scan = scan_parts(count, mass_high, mass_low, by_mass, by_mass && !kExact);
+    uint32_t count_before = scan.count_before;
+    double high_before = scan.high_before, high_end = scan.high_end;
+    double low_before = scan.low_before, low_end = scan.low_end;
     // the values next to zero, between the halves
     const double small_high = kExact ? sum.mass : (double)sum.small * fmin(1.0, c.weight(kPsSmall));
     const double small_low = kExact ? sum.mass : (double)sum.small * c.weight(-kPsSmall);
@@ -623,7 +790,7 @@ struct PolicyRow {
       low_before += small_low, low_end += small_low;
     }
     if (kExact) low_before = high_before, low_end = high_end;
-    const uint32_t in_bins = sh.part_count[kPsWarps - 1] + sum.small;
+    const uint32_t in_bins = scan.count_all + sum.small;
     // ids at and below -2^7 lie behind the bins; they may weigh nothing next to the rest
     const uint32_t behind = sum.count - in_bins;
     const bool behind_weighs = behind && c.weight(-kPsLarge) > 0x1p-80;
@@ -631,7 +798,7 @@ struct PolicyRow {
     const double slack = kExact ? 0.0 : 1e-12;
     const bool by_k = pol.top_k && pol.top_k < sum.count;
     int k_bin = kPsBins;
-    double total = kExact ? (by_mass ? sh.part_mass[kPsWarps - 1] + sum.mass : 0.0) : sum.mass;
+    double total = kExact ? scan.high_all + sum.mass : sum.mass;
     uint32_t k_count = 0;  // ids up to and with that bin
     uint32_t k_take = 0;
     if (by_k) {
@@ -783,7 +950,7 @@ struct PolicyRow {
     });
     const double above = reduce(mass, 0u, 0u, 0u).mass;
     uint32_t n[kPsOwn], count = 0;
-    merge_bins(n);
+    merge_bins(n, false);
     const uint32_t mine = threadIdx.x * kPsOwn;
     double mass_high = 0.0, mass_low = 0.0, high[kPsOwn], low[kPsOwn];
 #pragma unroll
@@ -800,7 +967,8 @@ struct PolicyRow {
       }
     }
     if (threadIdx.x < 3) sh.cross[threadIdx.x].bin = -1;
-    const uint32_t before = range.above + block_scan(count, sh.part_count) - count;
+    const Scanned scan = scan_parts(count, mass_high, mass_low, !rank_k, !rank_k);
+    const uint32_t before = range.above + scan.count_before;
     PsCross first = {}, last = {};
     if (rank_k) {
       if (before < rank_k && rank_k <= before + count) {
@@ -817,12 +985,8 @@ struct PolicyRow {
       first = last = sh.cross[0];
       last.count += last.n;
     } else {
-      const double high_end = above + block_scan(mass_high, sh.part_mass);
-      const double high_before = __shfl_up_sync(~0u, high_end, 1);
-      const double hb = lane ? high_before : above + (warp ? sh.part_mass[warp - 1] : 0.0);
-      const double low_end = above + block_scan(mass_low, sh.part_high);
-      const double low_before = __shfl_up_sync(~0u, low_end, 1);
-      const double lb = lane ? low_before : above + (warp ? sh.part_high[warp - 1] : 0.0);
+      const double high_end = above + scan.high_end, hb = above + scan.high_before;
+      const double low_end = above + scan.low_end, lb = above + scan.low_before;
       const double least = goal * (1.0 - 1e-12), most = goal * (1.0 + 1e-12);
       if (count && hb < least && least <= high_end) {
         PsCross x = {0.0, before, 0u, -1};
@@ -881,7 +1045,8 @@ struct PolicyRow {
     __syncthreads();
     unsigned long long* list = ps_list();
     double mass = 0.0;
-    view.each(lane, range.lo, [&](uint32_t id, const Raw& r) {
+    view.each(lane, range.lo, [&](uint32_t pos, const Raw& r) {
+      const uint32_t id = (uint32_t)view.id_of(pos);
       uint32_t set = 0;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
@@ -943,18 +1108,17 @@ struct PolicyRow {
       const double w0 = at < have ? c.weight(code_value(~(uint32_t)(sorted[at] >> 32))) : 0.0;
       const double w1 =
           at + 1u < have ? c.weight(code_value(~(uint32_t)(sorted[at + 1u] >> 32))) : 0.0;
-      const double end = block_scan(w0 + w1, sh.part_mass);
-      const double before = scan_before(end, sh.part_mass);
-      if (rank_k) total = above + sh.part_mass[kPsWarps - 1];
+      const Scanned scan = scan_parts(0u, w0 + w1, 0.0, true, false);
+      const double end = scan.high_end, before = scan.high_before;
+      if (rank_k) total = above + scan.high_all;
       const double goal = top_p_goal(top_p, total);
       uint32_t mine = have - 1u;
       if (at < have && above + before + w0 >= goal) mine = at;
       else if (at + 1u < have && above + end >= goal) mine = at + 1u;
       mine = __reduce_min_sync(~0u, mine);
-      if (lane == 0) sh.part_count[warp] = mine;
+      if (lane == 0) sh.part_top[warp] = mine;
       __syncthreads();
-      for (int i = 0; i < kPsWarps; ++i) pos = min(pos, sh.part_count[i]);
-      __syncthreads();
+      for (int i = 0; i < kPsWarps; ++i) pos = min(pos, sh.part_top[i]);
     }
     const uint32_t code = ~(uint32_t)(sorted[pos] >> 32);
     uint32_t same = 0;
@@ -1022,46 +1186,22 @@ struct PolicyRow {
   }
 
   // ---- the kept mass and the draw -------------------------------------------------------
-  struct Scan {  // of the entries of all warps, as this warp sees them
-    double total, mass_before;  // kept mass; of it, before this warp
-    uint32_t ties_before, draft_before;
-  };
-
-  // Kept mass of the entries that lane `lane` holds: `per` of them, in id order.
+  // The entries of all warps, scanned by every warp for itself; a lane holds up to kPer of
+  // them, in id order.
   static constexpr int kPer = kPsEntries / 32;
-  struct Held {
-    double mass[kPer];
-    int first, n;
+  struct Scan {
+    double total;
+    double mass_before;     // kept mass before the owner's ids ...
+    uint32_t ties_before;   // ... and ids at the cut before them
+    uint32_t my_ties;       // ids at the cut before this warp's
+    uint32_t draft_before;  // ids at the cut before the draft
+    int owner;  // entry whose interval of kept mass holds u times the total
   };
-  __device__ __forceinline__ Held held(int set, uint32_t take, double w_tie, uint32_t* ties_run,
-                                       uint32_t* ties_at) {
-    Held h;
-    const int n = (int)k * kPsWarps, per = (n + 31) / 32;
-    h.first = lane * per;
-    h.n = max(0, min(per, n - h.first));
-    uint32_t t[kPer], sum = 0;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      t[i] = i < h.n ? sh.entry_ties[h.first + i] : 0u;
-      h.mass[i] = i < h.n ? sh.entry_mass[set][h.first + i] : 0.0;
-      sum += t[i];
-    }
-    uint32_t run = warp_scan(sum, lane) - sum;
-    *ties_run = run;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      ties_at[i] = run;
-      const uint32_t kept = run < take ? min(t[i], take - run) : 0u;
-      if (kept) h.mass[i] += (double)kept * w_tie;
-      run += t[i];
-    }
-    return h;
-  }
 
-  // Publishes this warp's entry to the cluster and scans all of them; every warp does so for
-  // itself. `w_tie` is the weight of an id at the cut, `mass` that above it.
+  // Publishes this warp's entry to the cluster and scans all of them. `w_tie` is the weight of
+  // an id at the cut, `mass` that above it; set 1 leaves the ties as set 0 published them.
   __device__ Scan scan_entries(int set, double mass, uint32_t ties, uint32_t before,
-                               uint32_t take, double w_tie) {
+                               uint32_t take, double w_tie, double u) {
     if ((uint32_t)lane < k) {
       PsShared* r = ps_remote(&sh, lane);
       r->entry_mass[set][entry] = mass;
@@ -1071,54 +1211,56 @@ struct PolicyRow {
       }
     }
     publish();
-    uint32_t run, at[kPer];
-    const Held h = held(set, take, w_tie, &run, at);
-    double sum = 0.0;
+    const int n = (int)k * kPsWarps, per = (n + 31) / 32, first = lane * per;
+    uint32_t t[kPer], tie_sum = 0, draft = 0;
+    double m[kPer], sum = 0.0;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) sum += h.mass[i];
+    for (int i = 0; i < kPer; ++i) {
+      const bool have = i < per && first + i < n;
+      t[i] = have ? sh.entry_ties[first + i] : 0u;
+      m[i] = have ? sh.entry_mass[set][first + i] : 0.0;
+      draft += have ? sh.entry_before[first + i] : 0u;
+      tie_sum += t[i];
+    }
+    const uint32_t tie_start = warp_scan(tie_sum, lane) - tie_sum;
+    uint32_t run = tie_start;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const uint32_t kept = run < take ? min(t[i], take - run) : 0u;
+      if (kept) m[i] += (double)kept * w_tie;
+      run += t[i];
+      sum += m[i];
+    }
     const double incl = warp_scan(sum, lane);
     double acc = __shfl_up_sync(~0u, incl, 1);
     if (lane == 0) acc = 0.0;
     Scan s;
     s.total = __shfl_sync(~0u, incl, 31);
-    const int per = ((int)k * kPsWarps + 31) / 32, src = entry / per;
-    double mine = 0.0;
-    uint32_t mine_ties = 0;
-    uint32_t b = 0;
+    s.draft_before = __reduce_add_sync(~0u, draft);
+    const double goal = u * s.total;
+    // the first entry that passes the goal; the last with mass, if rounding leaves none
+    int hit = kPsEntries, last = 0;
+    double hit_mass = 0.0, last_mass = 0.0;
+    uint32_t hit_ties = 0, last_ties = 0, own = 0;
+    run = tie_start;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      if (h.first + i == entry) mine = acc, mine_ties = at[i];
-      if (i < h.n) b += sh.entry_before[h.first + i];
-      acc += h.mass[i];
-    }
-    s.mass_before = __shfl_sync(~0u, mine, src);
-    s.ties_before = __shfl_sync(~0u, mine_ties, src);
-    s.draft_before = __reduce_add_sync(~0u, b);
-    return s;
-  }
-
-  // the entry whose interval of kept mass holds `goal` (the last with mass, if rounding leaves
-  // none)
-  __device__ int find_owner(int set, uint32_t take, double w_tie, double goal) {
-    uint32_t run, at[kPer];
-    const Held h = held(set, take, w_tie, &run, at);
-    double sum = 0.0;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) sum += h.mass[i];
-    const double incl = warp_scan(sum, lane);
-    double acc = __shfl_up_sync(~0u, incl, 1);
-    if (lane == 0) acc = 0.0;
-    int first = kPsEntries, last = 0;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i)
-      if (h.mass[i] > 0.0) {
-        last = h.first + i;
-        if (acc + h.mass[i] > goal) first = min(first, h.first + i);
-        acc += h.mass[i];
+      if (first + i == entry) own = run;
+      if (m[i] > 0.0) {
+        last = first + i, last_mass = acc, last_ties = run;
+        if (hit == kPsEntries && acc + m[i] > goal) hit = last, hit_mass = acc, hit_ties = run;
       }
-    first = __reduce_min_sync(~0u, first);
-    last = __reduce_max_sync(~0u, last);
-    return first < kPsEntries ? first : last;
+      acc += m[i];
+      run += t[i];
+    }
+    s.my_ties = __shfl_sync(~0u, own, entry / per);
+    const int winner = __reduce_min_sync(~0u, hit);
+    const bool passed = winner < kPsEntries;
+    s.owner = passed ? winner : __reduce_max_sync(~0u, last);
+    const int src = s.owner / per;
+    s.mass_before = __shfl_sync(~0u, passed ? hit_mass : last_mass, src);
+    s.ties_before = __shfl_sync(~0u, passed ? hit_ties : last_ties, src);
+    return s;
   }
 
   // weight of a kept value
@@ -1146,12 +1288,13 @@ struct PolicyRow {
     tie &= r.bits;
   }
 
-  // f(id, raw values, set of the kept ones) over the vectors of this warp that may hold some;
-  // `ties_before`: ids at the cut before this warp. A kept id may still weigh less than min_p.
+  // f(id, raw values, set of the kept ones) over the vectors of `part` that may hold some;
+  // `ties_before`: ids at the cut before it. A kept id may still weigh less than min_p.
   template <class F>
-  __device__ __forceinline__ void each_kept(const RowCut& c, uint32_t ties_before, F&& f) {
+  __device__ __forceinline__ void each_kept(const View& part, const RowCut& c,
+                                            uint32_t ties_before, F&& f) {
     uint32_t run = ties_before;
-    view.each(lane, c.least(), [&](uint32_t id, const Raw& r) {
+    part.each(lane, c.least(), [&](uint32_t pos, const Raw& r) {
       uint32_t set, tie;
       split(c, r, set, tie);
       if (c.take && __any_sync(~0u, tie)) {
@@ -1165,29 +1308,99 @@ struct PolicyRow {
           ++at;
         }
       }
-      if (__any_sync(~0u, set)) f(id, r, set);
+      if (__any_sync(~0u, set)) f(view.id_of(pos), r, set);
     });
   }
 
-  // first id, in id order, whose cumulative weight exceeds `goal`; `start` is the mass before
-  // this warp; weigh(id, kept weight) is the weight to use. Whole warp; all lanes return it.
+  // The draw, by all warps of the CTA that has the owner: its part is cut into pieces, whose
+  // sums the warps take in turn; the warp that summed the piece that holds the goal walks it.
+  // Returns the id in that warp, -1 in the others. weigh(id, kept weight) is the weight to use.
   template <class W>
-  __device__ int pick(const RowCut& c, uint32_t ties_before, double start, double goal,
-                      W&& weigh) {
-    int found = -1, last = -1;
-    double run = start;
-    each_kept(c, ties_before, [&](uint32_t id, const Raw& r, uint32_t set) {
+  __device__ int draw(const RowCut& c, const Scan& s, double goal, W&& weigh) {
+    View part = view;
+    const uint64_t begin = (uint64_t)s.owner * warp_ids;
+    part.begin = (uint32_t)min(begin, (uint64_t)row_end);
+    part.end = (uint32_t)min(begin + warp_ids, (uint64_t)row_end);
+    const uint32_t all = (part.end - part.begin + kPsChunk - 1) / kPsChunk;
+    uint32_t piece = 1;  // chunks
+    while ((all + piece - 1) / piece > kPsUnits) piece *= 2;
+    const int n = (int)((all + piece - 1) / piece);
+    const uint32_t first = part.begin, stop = part.end, wide = piece * kPsChunk;
+    auto cut_to = [&](int i) {
+      part.begin = first + (uint32_t)i * wide;
+      part.end = min(stop, part.begin + wide);
+    };
+    double* masses = ps_unit_mass();
+    uint32_t* ties = ps_unit_ties();
+    if (c.take) {
+      for (int i = warp; i < n; i += kPsWarps) {
+        cut_to(i);
+        uint32_t t = 0;
+        part.each(lane, c.least(), [&](uint32_t, const Raw& r) {
+          uint32_t set, tie;
+          split(c, r, set, tie);
+          t += __popc(tie);
+        });
+        t = __reduce_add_sync(~0u, t);
+        if (lane == 0) ties[i] = t;
+      }
+      __syncthreads();
+    }
+    auto ties_at = [&](int i) {
+      uint32_t t = 0;
+      if (c.take)
+        for (int j = lane; j < i; j += 32) t += ties[j];
+      return s.ties_before + __reduce_add_sync(~0u, t);
+    };
+    for (int i = warp; i < n; i += kPsWarps) {
+      cut_to(i);
+      double m = 0.0;
+      each_kept(part, c, ties_at(i), [&](int id, const Raw& r, uint32_t set) {
+        View::each_set(set, [&](int j, bool have) {
+          const double w = weight(c, View::value_at(r, j));
+          if (have && w >= c.min_p) m += weigh(id + j, w);
+        });
+      });
+      m = warp_sum(m);
+      if (lane == 0) masses[i] = m;
+    }
+    __syncthreads();
+    // the piece that holds the goal, and the mass before it
+    int hit = -1, last = 0;
+    double run = s.mass_before, hit_run = run, last_run = run;
+    for (int i = 0; i < n && hit < 0; i += 32) {
+      const double m = i + lane < n ? masses[i + lane] : 0.0;
+      const double incl = warp_scan(m, lane);
+      const double prev = __shfl_up_sync(~0u, incl, 1);
+      const double before = run + (lane ? prev : 0.0);
+      const uint32_t over = __ballot_sync(~0u, m > 0.0 && run + incl > goal);
+      const uint32_t some = __ballot_sync(~0u, m > 0.0);
+      if (over) {
+        hit = i + __ffs(over) - 1;
+        hit_run = __shfl_sync(~0u, before, __ffs(over) - 1);
+      } else if (some) {
+        last = i + 31 - __clz(some);
+        last_run = __shfl_sync(~0u, before, 31 - __clz(some));
+      }
+      run += __shfl_sync(~0u, incl, 31);
+    }
+    if (hit < 0) hit = last, hit_run = last_run;  // what rounding leaves
+    if (hit % kPsWarps != warp) return -1;
+    cut_to(hit);
+    run = hit_run;
+    int found = -1, final = -1;
+    each_kept(part, c, ties_at(hit), [&](int id, const Raw& r, uint32_t set) {
       if (found >= 0) return;  // uniform over the warp
-      double s = 0.0;
+      double sum = 0.0;
       int mine = -1;
       View::each_set(set, [&](int j, bool have) {
         double w = weight(c, View::value_at(r, j));
         w = have && w >= c.min_p ? weigh(id + j, w) : 0.0;
-        s += w;
-        if (w > 0.0) mine = (int)id + j;
+        sum += w;
+        if (w > 0.0) mine = id + j;
       });
-      const double incl = warp_scan(s, lane);
-      const uint32_t over = __ballot_sync(~0u, s > 0.0 && run + incl > goal);
+      const double incl = warp_scan(sum, lane);
+      const uint32_t over = __ballot_sync(~0u, sum > 0.0 && run + incl > goal);
       if (over) {
         const int src = __ffs(over) - 1;
         const double prev = __shfl_up_sync(~0u, incl, 1);
@@ -1197,36 +1410,37 @@ struct PolicyRow {
           double w = weight(c, View::value_at(r, j));
           w = have && w >= c.min_p ? weigh(id + j, w) : 0.0;
           acc += w;
-          if (at < 0 && w > 0.0 && acc > goal) at = (int)id + j;
+          if (at < 0 && w > 0.0 && acc > goal) at = id + j;
         });
         found = __shfl_sync(~0u, at < 0 ? mine : at, src);
         return;
       }
-      last = max(last, mine);
+      final = max(final, mine);
       run += __shfl_sync(~0u, incl, 31);
     });
-    if (found < 0) found = __reduce_max_sync(~0u, last);
-    return found;
+    return found >= 0 ? found : __reduce_max_sync(~0u, final);
   }
 };
 
-// zeros for a lane's 8 ids
-__device__ __forceinline__ void clear_probs(float* out, uint32_t id, uint32_t end) {
-  if (id + 8u <= end && (reinterpret_cast<uintptr_t>(out) & 15u) == 0) {
-    reinterpret_cast<float4*>(out + id)[0] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    reinterpret_cast<float4*>(out + id)[1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (id + j < end) out[id + j] = 0.0f;
-  }
+// zeros for the ids [begin, end) of a row of probabilities, by the threads of a CTA
+__device__ __forceinline__ void clear_probs(float* row, uint32_t begin, uint32_t end) {
+  const uint32_t lead = (uint32_t)(-(int)(reinterpret_cast<uintptr_t>(row + begin) >> 2)) & 3u;
+  const uint32_t body = min(end, begin + lead), vecs = (end - body) / 4u;
+  if (threadIdx.x < body - begin) row[begin + threadIdx.x] = 0.0f;
+  float4* v = reinterpret_cast<float4*>(row + body);
+  for (uint32_t i = threadIdx.x; i < vecs; i += kPsThreads)
+    v[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  const uint32_t tail = body + 4u * vecs;
+  if (threadIdx.x < end - tail) row[tail + threadIdx.x] = 0.0f;
 }
 
 template <int DT, int OP>
 __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParams p) {
+  using Row = PolicyRow<DT>;
+  using View = RowView<DT>;
   __shared__ PsShared sh;
   const uint32_t k = (uint32_t)p.k;
-  // the barrier's first phase: every CTA of the cluster runs before its boxes are written
+  // the barrier's first phase: every CTA of the cluster runs before its memory is written
   if (k > 1) ps_cluster_arrive();
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
@@ -1234,22 +1448,27 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
   const int64_t group = OP == kOpSpec ? item / p.per_group : item;
   const int sub = OP == kOpSpec ? (int)(item - group * p.per_group) : 0;
 
-  PolicyRow<DT> row(sh);
+  Row row(sh);
   row.rank = k > 1 ? ps_rank() : 0u;
   row.k = k;
   row.warp = threadIdx.x >> 5;
   row.lane = threadIdx.x & 31;
   row.entry = (int)row.rank * kPsWarps + row.warp;
+  View& view = row.view;
   using S = typename Elem<DT>::storage;
-  row.view.row = static_cast<const S*>(p.logits) + group * p.group_stride + sub * p.row_stride;
-  row.view.mask = reinterpret_cast<const uint8_t*>(
-      p.mask ? p.mask + group * p.mask_group_stride + sub * p.mask_row_stride : nullptr);
-  row.view.vocab = (uint32_t)p.vocab;
-  const uint64_t begin = (uint64_t)row.entry * (uint32_t)p.warp_ids;
-  row.view.begin = (uint32_t)min(begin, (uint64_t)p.vocab);
-  row.view.end = (uint32_t)min(begin + (uint32_t)p.warp_ids, (uint64_t)p.vocab);
-  row.view.vec = (reinterpret_cast<uintptr_t>(row.view.row) & 15u) == 0;
-  row.view.peaks = p.peaks ? reinterpret_cast<uint16_t*>(ps_dynamic + p.peaks) + row.warp * (p.warp_ids >> 3) : nullptr;
+  view.row = static_cast<const S*>(p.logits) + group * p.group_stride + sub * p.row_stride;
+  view.mask = p.mask ? p.mask + group * p.mask_group_stride + sub * p.mask_row_stride : nullptr;
+  view.vocab = (int)p.vocab;
+  view.off = (int)((reinterpret_cast<uintptr_t>(view.row) & 15u) / sizeof(S));
+  row.warp_ids = (uint32_t)p.warp_ids;
+  row.row_end = (uint32_t)p.vocab + (uint32_t)view.off;
+  const uint64_t begin = (uint64_t)row.entry * row.warp_ids;
+  view.base = row.rank * kPsWarps * row.warp_ids;
+  view.begin = (uint32_t)min(begin, (uint64_t)row.row_end);
+  view.end = (uint32_t)min(begin + row.warp_ids, (uint64_t)row.row_end);
+  view.peaks = p.peaks ? reinterpret_cast<uint16_t*>(ps_dynamic + p.peaks) : nullptr;
+  unsigned char* ring = ps_dynamic + kPsArea + row.warp * ps_ring(DT);
+  view.start_stream(ring, row.lane);  // the copies run while the policy is read
 
   const RowPolicy pol = load_policy(p.policies + group * p.policy_stride);
   bool ok = pol.ok;
@@ -1264,11 +1483,19 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
     ok = ok && len >= 0 && len < p.per_group && u_accept >= 0.0 && u_accept < 1.0;
   }
   if (OP != kOpProbs) ok = ok && u >= 0.0 && u < 1.0;
+  if (OP == kOpProbs) {
+    const uint64_t first = (uint64_t)row.rank * kPsWarps * row.warp_ids;
+    clear_probs(p.out_probs + group * p.out_stride, (uint32_t)min(first, (uint64_t)p.vocab),
+                (uint32_t)min(first + kPsWarps * row.warp_ids, (uint64_t)p.vocab));
+  }
   if (k > 1) ps_cluster_wait();
 
   const bool first = row.rank == 0 && threadIdx.x == 0;
   uint32_t status = ok ? 0u : kStatusBadPolicy;
-  if (OP == kOpSpec && ok && sub > len) return;  // a row past the entry's drafts
+  if (OP == kOpSpec && ok && sub > len) {  // a row past the entry's drafts
+    ps_await<0>();
+    return;
+  }
 
   RowCut c = {};
   c.inv_t = fmin(1.0 / pol.temperature, 1e300);  // 0 times it stays 0
@@ -1278,31 +1505,29 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
   c.cut = -INFINITY;
   if (threadIdx.x < 16) sh.powers.at[threadIdx.x] = exp2((double)threadIdx.x / 16.0);
   if (ok) {
-    using View = RowView<DT>;
     const bool by_mass = pol.top_p < 1.0;
     const bool bins = pol.temperature > 0.0 && (pol.top_k || by_mass);
-    // the mass of all ids, relative to a value of 0 (its maximum is not known yet)
+    // the mass of all ids, relative to a value of 0 (the maximum is not known yet)
     const bool mass_of_all = DT != kBF16 && bins && by_mass && !pol.top_k;
-    uint32_t* hist = ps_hist();
     if (bins) row.clear_hist();
-    uint32_t top = 0, small = 0, count = 0;
+    uint32_t count = 0, small = 0, top16 = 0;
+    float top_value = -INFINITY;
     double mass = 0.0;
-    row.view.stream(row.lane, [&](uint32_t id, const auto& r) {
-      const uint32_t peak = View::peak_of(r);
-      if (row.view.peaks) row.view.peaks[(id - row.view.begin) >> 3] = (uint16_t)(peak >> 16);
-      top = max(top, peak);
-      if (OP == kOpProbs) clear_probs(p.out_probs + group * p.out_stride, id, row.view.end);
+    view.stream(ring, row.lane, [&](uint32_t pos, const auto& r) {
+      // the values to bfloat16 width, two to a word, and masks of the valid ones
+      uint32_t v[4] = {~0u, ~0u, ~0u, ~0u}, t[4];
+      const bool full = __all_sync(~0u, r.bits == 0xFFu);
+      if (!full) expand8_16(r.bits, v[0], v[1], v[2], v[3]);
+      View::narrow(r, t);
+      const uint32_t peak = View::peak(r, t, v, full, top_value);
+      if (view.peaks) view.peaks[(pos - view.base) >> 3] = (uint16_t)peak;
+      top16 = max(top16, peak);
       if (!bins) return;
       count += __popc(r.bits);
-      float near = INFINITY;
+      uint32_t near = 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t bits = View::bits_of(r, j);
-        const bool valid = r.bits >> j & 1u;
-        PolicyRow<DT>::count_bin(hist, bits, valid);
-        near = fminf(near, valid ? fabsf(__uint_as_float(bits)) : INFINITY);
-      }
-      if (__any_sync(~0u, near < kPsSmall)) {
+      for (int i = 0; i < 4; ++i) near |= Row::count_bins(ps_dynamic, t[i], v[i]);
+      if (__any_sync(~0u, near)) {
         uint32_t set = 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j)
@@ -1315,12 +1540,21 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
             if (have) mass += w;
           });
       }
-      if (DT != kBF16 && mass_of_all)
-        View::each_set(r.bits, [&](int j, bool have) {
-          const double w = exp2_table((double)View::value_at(r, j) * c.scale, *c.powers);
-          if (have) mass += w;
-        });
+      if (DT != kBF16 && mass_of_all) {
+        if (full) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            mass += exp2_table((double)View::value_of(r, j) * c.scale, *c.powers);
+        } else {
+          View::each_set(r.bits, [&](int j, bool have) {
+            const double w = exp2_table((double)View::value_at(r, j) * c.scale, *c.powers);
+            if (have) mass += w;
+          });
+        }
+      }
     });
+    // the order code of the maximum: 0 without a valid id
+    uint32_t top = top16 ? ord32(top_value) : 0u;
     PsBox sum = row.reduce(mass, count, top, small);
     top = sum.top;
     if (top == 0u) status = kStatusEmptyMask;
@@ -1339,12 +1573,12 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
         else c.keep(code_value(top), 1u);
       } else {
         PsRange range;
-        auto found = PolicyRow<DT>::kNothing;
+        auto found = Row::kNothing;
         if (in_range) found = row.find_cut_in_bins(c, pol, sum, range);
-        if (found != PolicyRow<DT>::kFound) {
+        if (found != Row::kFound) {
           __syncthreads();  // what the scans left in shared memory has been read
           row.find_cut(c, pol, top, sum.count, total,
-                       found == PolicyRow<DT>::kRange ? &range : nullptr);
+                       found == Row::kRange ? &range : nullptr);
         }
       }
       c.bound_by_min_p();
@@ -1352,39 +1586,31 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
   }
 
   if (status) {
-    if (OP == kOpProbs) {
-      if (!ok)  // the other rows were cleared as they were read
-        for (uint32_t i = row.view.begin + row.lane; i < row.view.end; i += 32u)
-          p.out_probs[group * p.out_stride + i] = 0.0f;
-      if (first) p.out_status[item] = status;
-    } else if (first) {
-      if (OP == kOpDraw) {
-        p.out_idx[item] = -1;
-        p.out_status[item] = status;
-      } else {
-        p.results[item] = make_int4(kDecided, -1, (int)status, 0);
-      }
+    if (first) {
+      if (OP == kOpDraw) p.out_idx[item] = -1;
+      if (OP == kOpSpec) p.results[item] = make_int4(kDecided, -1, (int)status, 0);
+      else p.out_status[item] = status;
     }
+    ps_await<0>();  // a row that was not looked at: its copies have to land all the same
     return;
   }
 
   // the kept mass and the ties at the cut, by warps; for a drafted row also the ties before it
-  uint32_t draft = 0;
-  bool drafted = false;
+  int draft = -1;
   if (OP == kOpSpec && sub < len) {
-    const int32_t d = p.drafts[group * p.draft_stride + sub];
-    drafted = d >= 0 && d < (int64_t)p.vocab;
-    draft = drafted ? (uint32_t)d : 0u;
+    draft = p.drafts[group * p.draft_stride + sub];
+    if (draft < 0 || draft >= view.vocab) draft = -1;
   }
   double mass = 0.0;
   uint32_t ties = 0, before = 0;
-  row.view.each(row.lane, c.least(), [&](uint32_t id, const auto& r) {
-    using View = RowView<DT>;
+  view.each(row.lane, c.least(), [&](uint32_t pos, const auto& r) {
     uint32_t set, tie;
-    PolicyRow<DT>::split(c, r, set, tie);
+    Row::split(c, r, set, tie);
     ties += __popc(tie);
-    if (OP == kOpSpec && id < draft)
-      before += __popc(draft - id < 8u ? tie & ((1u << (draft - id)) - 1u) : tie);
+    if (OP == kOpSpec) {
+      const int ahead = draft - view.id_of(pos);
+      if (ahead > 0) before += __popc(ahead < 8 ? tie & ((1u << ahead) - 1u) : tie);
+    }
     View::each_set(set, [&](int j, bool have) {
       const double w = row.weight(c, View::value_at(r, j));
       if (have && w >= c.min_p) mass += w;
@@ -1394,15 +1620,14 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
   ties = __reduce_add_sync(~0u, ties);
   before = __reduce_add_sync(~0u, before);
   const double w_tie = c.take ? c.weight(c.cut) : 0.0;
-  auto scan = row.scan_entries(0, mass, ties, before, c.take, w_tie);
-  const double total = scan.total;
+  auto scan = row.scan_entries(0, mass, ties, before, c.take, w_tie, u);
+  const double inv = 1.0 / scan.total;
 
   if (OP == kOpProbs) {
     float* out = p.out_probs + group * p.out_stride;
-    const double inv = 1.0 / total;
-    row.each_kept(c, scan.ties_before, [&](uint32_t id, const auto& r, uint32_t set) {
-      RowView<DT>::each_set(set, [&](int j, bool have) {
-        const double w = row.weight(c, RowView<DT>::value_at(r, j));
+    row.each_kept(view, c, scan.my_ties, [&](int id, const auto& r, uint32_t set) {
+      View::each_set(set, [&](int j, bool have) {
+        const double w = row.weight(c, View::value_at(r, j));
         if (have && w >= c.min_p) out[id + j] = (float)(w * inv);
       });
     });
@@ -1413,18 +1638,18 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
   bool residual = false;
   const float* q = nullptr;
   if (OP == kOpSpec && sub < len) {
-    double p_d = 0.0, q_d = drafted ? 1.0 : 0.0;
+    double p_d = 0.0, q_d = 1.0;
     if (p.draft_probs) q = p.draft_probs + group * p.dp_group_stride + sub * p.dp_row_stride;
-    if (drafted) {
+    if (draft >= 0) {
       if (q) q_d = fmax((double)q[draft], 0.0);
-      const bool valid = !row.view.mask || (row.view.mask[draft >> 3] >> (draft & 7u) & 1u);
-      const float v = Elem<DT>::to_f32(row.view.row, draft);
+      const bool valid = !view.mask || (view.mask[draft >> 5] >> (draft & 31) & 1u);
+      const float v = Elem<DT>::to_f32(view.row, draft);
       if (valid && (v > c.cut || (v == c.cut && scan.draft_before < c.take))) {
         const double w = c.weight(v);
-        if (w >= c.min_p) p_d = w / total;
+        if (w >= c.min_p) p_d = w / scan.total;
       }
     }
-    if (drafted && u_accept * q_d < p_d) {
+    if (draft >= 0 && u_accept * q_d < p_d) {
       if (first) p.results[item] = make_int4(kAccepted, -1, 0, 0);
       return;
     }
@@ -1432,39 +1657,32 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
   }
 
   // what remains of p where the draft's probability is taken off
-  const double inv = 1.0 / total;
-  auto rest = [&](uint32_t id, double w) {
-    const double q_id = q ? fmax((double)q[id], 0.0) : (drafted && id == draft ? 1.0 : 0.0);
+  auto rest = [&](int id, double w) {
+    if (!residual) return w;
+    const double q_id = q ? fmax((double)q[id], 0.0) : id == draft ? 1.0 : 0.0;
     return fmax(w * inv - q_id, 0.0);
   };
   if (OP == kOpSpec && residual) {
     double sum = 0.0;
-    row.each_kept(c, scan.ties_before, [&](uint32_t id, const auto& r, uint32_t set) {
-      RowView<DT>::each_set(set, [&](int j, bool have) {
-        const double w = row.weight(c, RowView<DT>::value_at(r, j));
+    row.each_kept(view, c, scan.my_ties, [&](int id, const auto& r, uint32_t set) {
+      View::each_set(set, [&](int j, bool have) {
+        const double w = row.weight(c, View::value_at(r, j));
         if (have && w >= c.min_p) sum += rest(id + j, w);
       });
     });
     sum = warp_sum(sum);
-    const auto left = row.scan_entries(1, sum, ties, 0u, 0u, 0.0);
+    const auto left = row.scan_entries(1, sum, 0u, 0u, 0u, 0.0, u);
     residual = left.total > 0.0;  // else the draft covers p everywhere: draw from p itself
-    if (residual) scan.total = left.total, scan.mass_before = left.mass_before;
+    if (residual) scan = left;
   }
-  const double goal = u * scan.total;
-  const int owner = residual ? row.find_owner(1, 0u, 0.0, goal)
-                             : row.find_owner(0, c.take, w_tie, goal);
-  if (owner == row.entry) {
-    const int id = OP == kOpSpec && residual
-                       ? row.pick(c, scan.ties_before, scan.mass_before, goal, rest)
-                       : row.pick(c, scan.ties_before, scan.mass_before, goal,
-                                  [](uint32_t, double w) { return w; });
-    if (row.lane == 0) {
-      if (OP == kOpDraw) {
-        p.out_idx[item] = id;
-        p.out_status[item] = 0u;
-      } else {
-        p.results[item] = make_int4(kDecided, id, 0, 0);
-      }
+  if (scan.owner / kPsWarps != (int)row.rank) return;
+  const int id = row.draw(c, scan, u * scan.total, rest);
+  if (id >= 0 && row.lane == 0) {
+    if (OP == kOpDraw) {
+      p.out_idx[item] = id;
+      p.out_status[item] = 0u;
+    } else {
+      p.results[item] = make_int4(kDecided, id, 0, 0);
     }
   }
 }
