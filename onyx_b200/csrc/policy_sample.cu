@@ -27,15 +27,48 @@ static int device_sms(cudaError_t* err) {
   return sms;
 }
 
-// CTAs per row: a power of two, as many as the SMs hold two of, at least 4,096 ids each.
-static int cluster_size(int64_t rows, int64_t vocab, int sms) {
-  int k = 1;
-  while (k < kPsMaxCluster && rows * k * 2 <= 2ll * sms && vocab >= 2ll * k * 4096) k *= 2;
-  return k;
-}
+// How a launch lays out its rows: CTAs per row, positions per warp, dynamic shared memory.
+struct PolicyPlan {
+  int k;
+  int32_t warp_ids, peaks, keep, slots;
+  size_t smem;
+};
 
 // Shared memory spent on peaks at most; longer parts of rows do without.
-constexpr size_t kPsMostPeaks = 96 * 1024;
+constexpr size_t kPsMostPeaks = 64 * 1024;
+// Dynamic shared memory with which two CTAs fit an SM (228 KB, 1 KB of it for each CTA, and the
+// static part).
+constexpr size_t kPsTwoFit = 228 * 1024 / 2 - 1024 - sizeof(PsShared) - 512;
+
+static PolicyPlan plan_with(int k, int64_t vocab, int dtype, bool masked) {
+  PolicyPlan pl = {};
+  pl.k = k;
+  const int64_t per = (int64_t)k * kPsWarps * kPsChunk;
+  pl.warp_ids = (int32_t)((vocab + 7 + per - 1) / per * kPsChunk);  // up to 7 ids of offset
+  pl.smem = kPsFixed;
+  const size_t peaks = (size_t)pl.warp_ids / 8 * kPsWarps * sizeof(uint16_t);
+  pl.peaks = peaks <= kPsMostPeaks;
+  if (pl.peaks) pl.smem += peaks;
+  pl.slots = (int32_t)pl.smem;
+  const size_t slot = (size_t)ps_slot(dtype, masked);
+  const size_t all = (size_t)pl.warp_ids / kPsChunk * kPsWarps * slot;
+  pl.keep = pl.peaks && pl.smem + all <= kPsTwoFit;
+  pl.smem += pl.keep ? all : kPsWarps * ps_depth(dtype) * slot;
+  return pl;
+}
+
+// CTAs per row: a power of two, as many as the SMs hold two of, at least 4,096 ids each; and
+// as many as it takes to have two CTAs on an SM.
+static PolicyPlan make_plan(int64_t rows, int64_t vocab, int dtype, bool masked, int sms) {
+  int k = 1;
+  while (k < kPsMaxCluster && rows * k * 2 <= 2ll * sms && vocab >= 2ll * k * 4096) k *= 2;
+  PolicyPlan pl = plan_with(k, vocab, dtype, masked);
+  while (k < kPsMaxCluster && pl.smem > kPsTwoFit) {
+    k *= 2;
+    pl = plan_with(k, vocab, dtype, masked);
+  }
+  return pl;
+}
 
 template <int OP>
 static const void* policy_fn(int dtype) {
@@ -52,7 +85,7 @@ static cudaError_t allow_shared(const void* fn, int which) {
   if (e != cudaSuccess) return e;
   if (dev >= 0 && dev < 64 && (done[dev].load(std::memory_order_acquire) >> which & 1)) return e;
   e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           (int)(std::max(ps_fixed(kF32), ps_fixed(kBF16)) + kPsMostPeaks));
+                           (int)(kPsFixed + kPsMostPeaks + kPsWarps * std::max(ps_depth(kF32) * ps_slot(kF32, true), ps_depth(kBF16) * ps_slot(kBF16, true))));
   if (e == cudaSuccess && dev >= 0 && dev < 64)
     done[dev].fetch_or((uint16_t)(1u << which), std::memory_order_release);
   return e;
@@ -63,24 +96,20 @@ static int launch_policy(int dtype, PolicyParams& p, int64_t rows, cudaStream_t 
   cudaError_t e;
   const int sms = device_sms(&e);
   if (!sms) return finish_launch(e);
-  p.k = cluster_size(rows, p.vocab, sms);
+  const PolicyPlan pl = make_plan(rows, p.vocab, dtype, p.mask != nullptr, sms);
+  p.k = pl.k;
+  p.warp_ids = pl.warp_ids;
+  p.peaks = pl.peaks;
+  p.keep = pl.keep;
+  p.slots = pl.slots;
   if (rows * p.k > 0x7FFFFFFFll) return ONYX_ERR_INVALID_ARGUMENT;
-  const int64_t per = (int64_t)p.k * kPsWarps * kPsChunk;
-  p.warp_ids = (int32_t)((p.vocab + 7 + per - 1) / per * kPsChunk);  // up to 7 ids of offset
-  size_t smem = ps_fixed(dtype);
-  const size_t peaks = (size_t)p.warp_ids / 8 * kPsWarps * sizeof(uint16_t);
-  p.peaks = 0;
-  if (peaks <= kPsMostPeaks) {
-    p.peaks = (int32_t)smem;
-    smem += peaks;
-  }
   const void* fn = policy_fn<OP>(dtype);
   e = allow_shared(fn, OP * 3 + (dtype == kBF16 ? 0 : dtype == kF16 ? 1 : 2));
   if (e != cudaSuccess) return finish_launch(e);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(rows * p.k), 1, 1);
   cfg.blockDim = dim3(kPsThreads, 1, 1);
-  cfg.dynamicSmemBytes = smem;
+  cfg.dynamicSmemBytes = pl.smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   int n = 0;

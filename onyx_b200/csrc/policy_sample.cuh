@@ -50,7 +50,7 @@ constexpr int kPsWarps = kPsThreads / 32;
 constexpr int kPsMaxCluster = 8;
 constexpr int kPsEntries = kPsMaxCluster * kPsWarps;
 constexpr int kPsChunk = 256;  // ids a warp handles at a time, 8 to a lane
-constexpr int kPsUnits = 1024;  // pieces at most into which the drawing CTA cuts a warp's part
+constexpr int kPsUnits = 256;  // pieces at most into which the drawing CTA cuts a warp's part
 
 // The value histogram: one bin for every bf16 value with 2^-9 <= |v| < 2^7, in falling order
 // of value; positive ones first. The values next to zero, |v| < 2^-9, lie between the halves.
@@ -88,7 +88,9 @@ struct PolicyParams {
   int4* results;              // spec: {verdict, token, status, 0} of every row
   int32_t warp_ids;  // ids per warp, a multiple of kPsChunk
   int32_t k;         // CTAs per row
-  int32_t peaks;     // where in dynamic shared memory the peaks of every 8 ids lie (0: nowhere)
+  int32_t peaks;     // the peaks are kept (else their place is empty)
+  int32_t keep;      // shared memory holds all chunks of a CTA's part
+  int32_t slots;     // where in dynamic shared memory the chunks' slots begin
 };
 
 enum Verdict : int { kAccepted = 0, kDecided = 1 };
@@ -188,10 +190,11 @@ struct PsShared {
   uint32_t list_fill;
 };
 
-// Dynamic shared memory. While the row streams in: the CTA's histogram, then the rings through
-// which the warps copy it. After that the rings' first 16 KB hold the cluster's histogram; the
-// two histograms' 32 KB are used again for a list and its sorted form, and for the weights of
-// the bins; behind them the drawing CTA keeps the sums of its pieces. Last come the peaks.
+// Dynamic shared memory: the CTA's histogram and the cluster's; their 32 KB are used again for a
+// list and its sorted form, and for the weights of the bins. Then the sums of the pieces of a
+// draw, the peaks, and last the slots into which the warps copy their part of the row: all of
+// its chunks where they fit (the later passes read them there), else a ring of
+// ps_depth().
 extern __shared__ __align__(16) unsigned char ps_dynamic[];
 constexpr size_t kPsArea = kPsBins * sizeof(uint32_t);
 __device__ __forceinline__ uint32_t* ps_hist() { return reinterpret_cast<uint32_t*>(ps_dynamic); }
@@ -211,16 +214,13 @@ __device__ __forceinline__ double* ps_unit_mass() {
 __device__ __forceinline__ uint32_t* ps_unit_ties() {
   return reinterpret_cast<uint32_t*>(ps_dynamic + 2 * kPsArea + kPsUnits * sizeof(double));
 }
-// A warp's ring: kDepth slots of one chunk's values and mask words.
-__host__ __device__ constexpr int ps_depth(int dt) { return dt == kF32 ? 3 : 4; }
-__host__ __device__ constexpr int ps_slot(int dt) { return kPsChunk * (dt == kF32 ? 4 : 2) + 48; }
-__host__ __device__ constexpr size_t ps_ring(int dt) { return (size_t)ps_depth(dt) * ps_slot(dt); }
 // bytes ahead of the peaks
-__host__ __device__ constexpr size_t ps_fixed(int dt) {
-  return kPsArea + (kPsWarps * ps_ring(dt) > kPsArea + kPsUnits * 12u
-                        ? kPsWarps * ps_ring(dt)
-                        : kPsArea + kPsUnits * 12u);
+constexpr size_t kPsFixed = 2 * kPsArea + kPsUnits * (sizeof(double) + sizeof(uint32_t));
+// A slot: a chunk's values, and its mask words where there is a mask.
+__host__ __device__ constexpr int ps_slot(int dt, bool masked) {
+  return kPsChunk * (dt == kF32 ? 4 : 2) + (masked ? 48 : 0);
 }
+__host__ __device__ constexpr int ps_depth(int dt) { return dt == kF32 ? 2 : 4; }
 
 __device__ __forceinline__ void ps_copy16(void* dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
@@ -245,13 +245,16 @@ __device__ __forceinline__ void ps_await() {
 template <int DT>
 struct RowView {
   using S = typename Elem<DT>::storage;
-  static constexpr int kDepth = ps_depth(DT), kSlot = ps_slot(DT);
+  static constexpr int kData = kPsChunk * (int)sizeof(S), kDepth = ps_depth(DT);
   const S* row;
   const uint32_t* mask;
   uint16_t* peaks;  // of this CTA: order code >> 16 of the maximum of every 8, or null
   uint32_t base;    // the CTA's first position
   uint32_t begin, end;  // positions; multiples of kPsChunk, but for the row's end
   int vocab, off;
+  unsigned char* slots;  // of the CTA's chunks in order, if all are kept, else of the warp's ring
+  int slot_bytes;
+  bool kept;  // all chunks are kept
 
   struct Raw {  // the values at 8 positions as loaded
     uint4 a, b;
@@ -287,14 +290,38 @@ struct RowView {
     }
   }
 
-  // the values at 8 positions, from global memory; none for a position past the end
-  __device__ __forceinline__ Raw load(uint32_t pos) const {
+  // of the slot of the chunk that position `at` begins, lane's 8 values
+  __device__ __forceinline__ Raw from_slot(const unsigned char* slot, uint32_t at, int lane) const {
+    Raw r;
+    r.a = *reinterpret_cast<const uint4*>(slot + lane * 16);
+    if (DT == kF32) r.b = *reinterpret_cast<const uint4*>(slot + 512 + lane * 16);
+    r.bits = 0xFFu;
+    const int id0 = id_of(at), id = id0 + 8 * lane;
+    if (id0 < 0 || id0 + kPsChunk > vocab) {  // an end of the row
+      r.bits = inside(id);
+      if (r.bits != 0xFFu) load_edge(r, id);
+    }
+    if (mask) {
+      const uint32_t* words = reinterpret_cast<const uint32_t*>(slot + kData);
+      const int w = (id >> 5) - (id0 >> 5);
+      r.bits &= __funnelshift_r(words[w], words[w + 1], id & 31);
+    }
+    return r;
+  }
+
+  // the lane's 8 values of the chunk at `at`, none if it does not need them; `at` < end
+  __device__ __forceinline__ Raw load(uint32_t at, int lane, bool need) const {
+    if (kept) {
+      Raw r = from_slot(slots + (size_t)((at - base) / kPsChunk) * slot_bytes, at, lane);
+      if (!need) r.bits = 0u;
+      return r;
+    }
     Raw r;
     r.a = make_uint4(0u, 0u, 0u, 0u);
     if (DT == kF32) r.b = r.a;
     r.bits = 0u;
-    if (pos >= end) return r;
-    const int id = id_of(pos);
+    if (!need) return r;
+    const int id = id_of(at) + 8 * lane;
     r.bits = inside(id);
     if (r.bits == 0xFFu) {
       r.a = *reinterpret_cast<const uint4*>(row + id);
@@ -302,7 +329,7 @@ struct RowView {
     } else {
       load_edge(r, id);
     }
-    if (mask) {
+    if (mask && r.bits) {
       const int w = id >> 5, words = (vocab + 31) >> 5;
       const uint32_t lo = w >= 0 ? mask[w] : 0u;
       const uint32_t hi = (id & 31) > 24 && w + 1 < words ? mask[w + 1] : 0u;
@@ -311,65 +338,71 @@ struct RowView {
     return r;
   }
 
-  // Starts the copy of chunk i (of n) into its slot of the warp's ring.
-  __device__ __forceinline__ void copy_chunk(unsigned char* ring, int lane, int i, int n) const {
-    if (i < n) {
-      unsigned char* slot = ring + (i % kDepth) * kSlot;
-      const int id0 = id_of(begin + (uint32_t)i * kPsChunk);
-      constexpr int kVec = DT == kF32 ? 4 : 8;
+  // Starts the copy of the chunk at `at` into `slot`.
+  __device__ __forceinline__ void copy_chunk(unsigned char* slot, int lane, uint32_t at) const {
+    constexpr int kVec = DT == kF32 ? 4 : 8;
+    const int id0 = id_of(at);
+    const bool whole = id0 >= 0 && id0 + kPsChunk <= vocab;
+    const S* from = row + id0 + lane * kVec;
 #pragma unroll
-      for (int h = 0; h < 8 / kVec; ++h) {
-        const int v = lane + 32 * h, id = id0 + v * kVec;
-        // float32: a lane's two vectors 512 bytes apart, so that reading them has no conflicts
-        const int to = DT == kF32 ? (v & 1) * 512 + (v >> 1) * 16 : v * 16;
-        if (id >= 0 && id + kVec <= vocab) ps_copy16(slot + to, row + id);
-      }
-      if (mask && lane < 10) {
-        const int w = (id0 >> 5) + lane;
-        const bool have = w >= 0 && w < (vocab + 31) >> 5;
-        ps_copy4(slot + kSlot - 48 + 4 * lane, mask + (have ? w : 0), have);
-      }
+    for (int h = 0; h < 8 / kVec; ++h) {
+      const int v = lane + 32 * h, id = id0 + v * kVec;
+      // float32: a lane's two vectors 512 bytes apart, so that reading them has no conflicts
+      const int to = DT == kF32 ? (v & 1) * 512 + (v >> 1) * 16 : v * 16;
+      if (whole || (id >= 0 && id + kVec <= vocab)) ps_copy16(slot + to, from + 32 * kVec * h);
     }
-    ps_commit();
+    if (mask && lane < 10) {
+      const int w = (id0 >> 5) + lane;
+      const bool have = w >= 0 && w < (vocab + 31) >> 5;
+      ps_copy4(slot + kData + 4 * lane, mask + (have ? w : 0), have);
+    }
   }
 
   __device__ __forceinline__ int chunks() const {
     return (int)((end - begin + kPsChunk - 1) / kPsChunk);
   }
-  __device__ __forceinline__ void start_stream(unsigned char* ring, int lane) const {
-    const int n = chunks();
-#pragma unroll
-    for (int i = 0; i < kDepth - 1; ++i) copy_chunk(ring, lane, i, n);
+  // Starts all copies, or those that fill the ring but for one slot.
+  __device__ __forceinline__ void start_stream(int lane) const {
+    const int n = chunks(), now = kept ? n : min(n, kDepth - 1);
+    unsigned char* slot = slots + (kept ? (size_t)((begin - base) / kPsChunk) * slot_bytes : 0);
+#pragma unroll 1
+    for (int i = 0; i < (kept ? n : kDepth - 1); ++i) {
+      if (i < now) copy_chunk(slot, lane, begin + (uint32_t)i * kPsChunk);
+      ps_commit();
+      slot += slot_bytes;
+    }
   }
 
   // f(position of the lane's first value, its values): the pass that reads the row from HBM,
-  // through the ring that start_stream() began to fill. Every lane makes every call.
+  // behind the copies of start_stream(). Every lane makes every call.
   template <class F>
-  __device__ __forceinline__ void stream(unsigned char* ring, int lane, F&& f) const {
+  __device__ __forceinline__ void stream(int lane, F&& f) const {
     const int n = chunks();
+    unsigned char* slot = slots + (kept ? (size_t)((begin - base) / kPsChunk) * slot_bytes : 0);
+    unsigned char* const last = slots + (kDepth - 1) * slot_bytes;
+    unsigned char* fill = last;  // the ring's free slot
+    uint32_t at = begin;
 #pragma unroll 1
     for (int i = 0; i < n; ++i) {
-      copy_chunk(ring, lane, i + kDepth - 1, n);
-      ps_await<kDepth - 1>();
-      __syncwarp();
-      const unsigned char* slot = ring + (i % kDepth) * kSlot;
-      const uint32_t pos = begin + (uint32_t)i * kPsChunk + 8u * lane;
-      const int id = id_of(pos);
-      Raw r;
-      r.bits = inside(id);
-      if (r.bits == 0xFFu) {
-        r.a = *reinterpret_cast<const uint4*>(slot + lane * 16);
-        if (DT == kF32) r.b = *reinterpret_cast<const uint4*>(slot + 512 + lane * 16);
+      if (kept) {  // at most n - 1 - i copies may still be on their way
+        const int ahead = n - 1 - i;
+        if (ahead >= 8) ps_await<8>();
+        else if (ahead >= 4) ps_await<4>();
+        else if (ahead >= 2) ps_await<2>();
+        else if (ahead == 1) ps_await<1>();
+        else ps_await<0>();
       } else {
-        load_edge(r, id);
+        if (i + kDepth - 1 < n) copy_chunk(fill, lane, at + (kDepth - 1) * kPsChunk);
+        ps_commit();
+        fill = fill == last ? slots : fill + slot_bytes;
+        ps_await<kDepth - 1>();
       }
-      if (mask) {
-        const uint32_t* words = reinterpret_cast<const uint32_t*>(slot + kSlot - 48);
-        const int w = (id >> 5) - ((id - 8 * lane) >> 5);
-        r.bits &= __funnelshift_r(words[w], words[w + 1], id & 31);
-      }
+      __syncwarp();
+      const Raw r = from_slot(slot, at, lane);
       __syncwarp();  // the slot has been read
-      f(pos, r);
+      f(at + 8u * lane, r);
+      at += kPsChunk;
+      slot = !kept && slot == last ? slots : slot + slot_bytes;
     }
   }
 
@@ -465,37 +498,50 @@ struct RowView {
       return at;
     };
     uint32_t at = next(begin);
-    Raw r = load(at < end && need(at) ? at + step : end);
+    if (at >= end) return;
+    Raw r = load(at, lane, need(at));
 #pragma unroll 1
-    while (at < end) {
+    while (true) {
       const uint32_t then = next(at + kPsChunk);
-      const Raw more = load(then < end && need(then) ? then + step : end);
+      Raw more = r;
+      if (then < end) more = load(then, lane, need(then));
       f(at + step, r);
+      if (then >= end) break;
       at = then;
       r = more;
     }
   }
 };
 
-// 2^y (below 2^-1000: 0, above 2^1000: +inf). Table-driven in the manner of Tang (ACM TOMS
-// 15, 1989): y = e + j/16 + f with |f| <= 1/32, 2^f by its Taylor polynomial of degree 6 (the
-// next term is below 5e-16 there), so about 1e-15 of the value. 12 float64 operations; the 16
+// 2^(y/16) for |y| < 2^20. Table-driven in the manner of Tang (ACM TOMS 15, 1989): y = 16 e + j
+// + f with |f| <= 1/2, 2^(f/16) by its Taylor polynomial, the term of degree 6 folded into
+// those of degree 4 and 2 (Chebyshev): within 1e-14 of the value, and 1 for y = 0. The 16
 // entries take the 16 pairs of banks, so lookups of a warp do not conflict.
-__device__ __forceinline__ double exp2_table(double y, const PsPowers& powers) {
-  const double shift = 0x1.8p48;  // its last place is 1/16
-  const double t = y + shift;
+constexpr double kPsShift = 0x1.8p52;
+__device__ __forceinline__ double exp2_parts(double t, double f, const PsPowers& powers) {
   const int n = __double2loint(t);
-  const double f = y - (t - shift);
-  const double f2 = f * f;
-  // ln 2^k / k!
-  const double a = fma(0.2402265069591007, f, 0.6931471805599453);
-  const double b = fma(0.009618129107628477, f, 0.05550410866482158);
-  const double d = fma(0.00015403530393381608, f, 0.0013333558146428443);
-  const double q = fma(fma(d, f2, b), f2, a) * f;
+  // (ln 2 / 16)^k / k!
+  constexpr double c1 = 0.6931471805599453 / 16.0, c2 = c1 * c1 / 2.0, c3 = c2 * c1 / 3.0;
+  constexpr double c4 = c3 * c1 / 4.0, c5 = c4 * c1 / 5.0, c6 = c5 * c1 / 6.0;
+  double q = c5;
+  q = fma(q, f, c4 + c6 * 1.5 * 0.25);
+  q = fma(q, f, c3);
+  q = fma(q, f, c2 - c6 * 0.5625 * 0.0625);
+  q = fma(q, f, c1);
   const double w = powers.at[n & 15];
-  const double r = fma(w, q, w);
-  const double v = __hiloint2double(__double2hiint(r) + (n >> 4) * (1 << 20), __double2loint(r));
-  return y > -1000.0 ? (y < 1000.0 ? v : (double)INFINITY) : 0.0;
+  const double r = fma(w * f, q, w);
+  return __hiloint2double(__double2hiint(r) + (n >> 4) * (1 << 20), __double2loint(r));
+}
+// 2^(y/16), 0 below 2^-1000, +inf above 2^1000
+__device__ __forceinline__ double exp2_table(double y, const PsPowers& powers) {
+  const double t = y + kPsShift;
+  const double v = exp2_parts(t, y - (t - kPsShift), powers);
+  return y > -16000.0 ? (y < 16000.0 ? v : (double)INFINITY) : 0.0;
+}
+// 2^(v scale / 16) for v scale in (-16000, 16000)
+__device__ __forceinline__ double exp2_scaled(float v, double scale, const PsPowers& powers) {
+  const double x = (double)v, t = fma(x, scale, kPsShift);
+  return exp2_parts(t, fma(x, scale, kPsShift - t), powers);
 }
 
 __device__ __forceinline__ float code_value(uint32_t code) {  // inverse of ord32
@@ -504,9 +550,10 @@ __device__ __forceinline__ float code_value(uint32_t code) {  // inverse of ord3
 
 // What decides which ids of the row are kept, and their weights.
 struct RowCut {
-  double top, scale, inv_t, min_p;  // scale = log2(e) / T
+  double top, scale, inv_t, min_p;  // scale = 16 log2(e) / T
   const PsPowers* powers;
   float cut;      // ids above it are kept,
+  uint32_t cut2;  // (the same in a 16-bit type, twice, once the cut stands)
   uint32_t take;  // and of those equal to it the first `take`
   bool flat;      // every kept id weighs 1 (T = 0, or +inf present)
 
@@ -544,6 +591,12 @@ struct PsRange {
   uint32_t above, inside;  // ids above it, ids in it
 };
 
+// Weights summed so far: of the codes above `down_to`, this lane's part and the cluster's.
+struct PsSummed {
+  double lane, all;
+  uint32_t down_to;
+};
+
 template <int DT>
 struct PolicyRow {
   using View = RowView<DT>;
@@ -551,6 +604,7 @@ struct PolicyRow {
   PsShared& sh;
   View view;
   const double* table = nullptr;  // weights of the kept bins, where the cut came from them
+  PsSummed summed = {0.0, 0.0, ~0u};
   uint32_t rank, k;
   uint32_t warp_ids, row_end;  // positions of a warp, and of the row
   int warp, lane, entry;
@@ -656,7 +710,6 @@ struct PolicyRow {
   __device__ __forceinline__ void clear_hist() {
     for (int i = threadIdx.x; i < kPsBins / 4; i += kPsThreads)
       reinterpret_cast<uint4*>(ps_hist())[i] = make_uint4(0u, 0u, 0u, 0u);
-    __syncthreads();
   }
 
   // After a reduce(): the cluster's counts of this thread's kPsOwn bins. Every CTA adds up its
@@ -683,8 +736,8 @@ struct PolicyRow {
     }
     const int mine = threadIdx.x * kPsOwn;
     const bool turned = by_magnitude && mine < kPsHalf;
-    const uint4* at = reinterpret_cast<const uint4*>(from + (turned ? kPsHalf - kPsOwn - mine : mine));
-    const uint4 x = at[0], y = at[1];
+    const uint32_t* at = from + (turned ? kPsHalf - kPsOwn - mine : mine);
+    const uint4 x = reinterpret_cast<const uint4*>(at)[0], y = reinterpret_cast<const uint4*>(at)[1];
     const uint32_t t[kPsOwn] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
 #pragma unroll
     for (int j = 0; j < kPsOwn; ++j) n[j] = turned ? t[kPsOwn - 1 - j] : t[j];
@@ -707,13 +760,19 @@ struct PolicyRow {
   // bit 15 and bit 31 set for those next to zero. In memory the bins of either sign lie by
   // rising magnitude, negative ones behind. With the sign bit set no half borrows from the
   // other; the bin is right where bits 11 to 14 come out as zeros.
-  __device__ __forceinline__ static uint32_t count_bins(unsigned char* hist, uint32_t u,
+  __device__ __forceinline__ static uint32_t count_bins(uint32_t hist, uint32_t u,
                                                         uint32_t valid) {
     const uint32_t t = (u | 0x80008000u) - kPsLow * 0x10001u;
     const uint32_t bad = (t & 0x78007800u) | ~valid;
     const uint32_t at = ((t & 0x07FF07FFu) | ((u >> 4) & 0x08000800u)) << 2;
-    if ((bad & 0xFFFFu) == 0u) atomicAdd(reinterpret_cast<uint32_t*>(hist + (at & 0xFFFFu)), 1u);
-    if (bad < 0x10000u) atomicAdd(reinterpret_cast<uint32_t*>(hist + (at >> 16)), 1u);
+    // predicated, where the compiler would branch
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .b32 x;\n\t"
+        "and.b32 x, %2, 0xFFFF;\n\tsetp.eq.u32 p, x, 0;\n\tsetp.lt.u32 q, %2, 0x10000;\n\t"
+        "@p red.shared.add.u32 [%0], 1;\n\t@q red.shared.add.u32 [%1], 1;\n\t}" ::"r"(
+            hist + (at & 0xFFFFu)),
+        "r"(hist + (at >> 16)), "r"(bad)
+        : "memory");
     return ~t & 0x80008000u & valid;
   }
 
@@ -906,6 +965,67 @@ struct PolicyRow {
     return (uint32_t)t;
   }
 
+  // weight of a kept value; `bins`: the table, if there is one
+  __device__ __forceinline__ static double weigh(float v, double top, double scale, bool flat,
+                                                 const PsPowers& powers, const double* bins) {
+    if (DT == kBF16 && bins) {
+      const uint32_t bits = __float_as_uint(v);
+      const uint32_t i = ((bits >> 16) & 0x7FFFu) - kPsLow;
+      const uint32_t positive = (uint32_t)((int32_t)~bits >> 31);
+      if (i < (uint32_t)kPsHalf) return bins[kPsHalf + (int)(i ^ positive)];
+    }
+    return flat ? 1.0 : exp2_table(((double)v - top) * scale, powers);
+  }
+  __device__ __forceinline__ double weight(const RowCut& c, float v) const {
+    return weigh(v, c.top, c.scale, c.flat, *c.powers, table);
+  }
+
+  // f(j, weight) for the values j of the lane's `set` that weigh min_p at least. Whole warp.
+  // Few to a lane: one after the other; else all eight side by side, which hides the latency
+  // of the float64 chains.
+  template <class F>
+  __device__ __forceinline__ void each_weight(const RowCut& c, const Raw& r, uint32_t set,
+                                              F&& f) const {
+    if (__any_sync(~0u, __popc(set) > 2)) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const double w = weight(c, View::value_of(r, j));
+        if ((set >> j & 1u) && w >= c.min_p) f(j, w);
+      }
+    } else {
+      View::each_set(set, [&](int j, bool have) {
+        const double w = weight(c, View::value_at(r, j));
+        if (have && w >= c.min_p) f(j, w);
+      });
+    }
+  }
+  // the sum of those weights that are `least` at least; 0 without a call where no lane has one
+  __device__ __forceinline__ double sum_of(const RowCut& c, const Raw& r, uint32_t set,
+                                           double least) const {
+    if (!__any_sync(~0u, set)) return 0.0;
+    return sum_set(r, set, c.top, c.scale, least, c.flat, c.powers, table);
+  }
+  __device__ __noinline__ static double sum_set(const Raw r, uint32_t set, double top,
+                                                double scale, double least, bool flat,
+                                                const PsPowers* powers, const double* bins) {
+    double a = 0.0, b = 0.0;
+    if (__any_sync(~0u, __popc(set) > 2)) {
+#pragma unroll
+      for (int j = 0; j < 8; j += 2) {
+        const double w = weigh(View::value_of(r, j), top, scale, flat, *powers, bins);
+        const double x = weigh(View::value_of(r, j + 1), top, scale, flat, *powers, bins);
+        a += (set >> j & 1u) && w >= least ? w : 0.0;
+        b += (set >> j & 2u) && x >= least ? x : 0.0;
+      }
+    } else {
+      View::each_set(set, [&](int j, bool have) {
+        const double w = weigh(View::value_at(r, j), top, scale, flat, *powers, bins);
+        a += have && w >= least ? w : 0.0;
+      });
+    }
+    return a + b;
+  }
+
   // ---- the cut from ranges of order codes -----------------------------------------------
   // mass and count of the valid ids whose order code is at least `code`
   __device__ PsBox at_least(const RowCut& c, uint32_t code) {
@@ -917,12 +1037,20 @@ struct PolicyRow {
       for (int j = 0; j < 8; ++j)
         if ((r.bits >> j & 1u) && ord32(View::value_of(r, j)) >= code) set |= 1u << j;
       count += __popc(set);
-      View::each_set(set, [&](int j, bool have) {
-        const double w = c.weight(View::value_at(r, j));
-        if (have) mass += w;
-      });
+      mass += sum_of(c, r, set, 0.0);
     });
     return reduce(mass, count, 0u, 0u);
+  }
+
+  // After a pass that summed the codes above `hi` that were not summed yet (or none): the mass
+  // of all codes above `hi`.
+  __device__ double sum_up(double mass, uint32_t hi, bool did) {
+    const double more = reduce(mass, 0u, 0u, 0u).mass;
+    if (!did) return 0.0;
+    summed.lane += mass;
+    summed.all += more;
+    summed.down_to = hi;
+    return summed.all;
   }
 
   // One turn of the histogram over the range: it shrinks to the bin that holds rank `rank_k`,
@@ -931,6 +1059,7 @@ struct PolicyRow {
     const uint32_t width = range.hi - range.lo;
     const int shift = max(0, 20 - __clz(width));  // width >> shift < 2^12
     clear_hist();
+    __syncthreads();
     uint32_t* hist = ps_hist();
     double mass = 0.0;
     view.each(lane, range.lo, [&](uint32_t, const Raw& r) {
@@ -939,16 +1068,12 @@ struct PolicyRow {
       for (int j = 0; j < 8; ++j) {
         const uint32_t code = ord32(View::value_of(r, j));
         const bool valid = r.bits >> j & 1u;
-        if (valid && code > range.hi) set |= 1u << j;
+        if (valid && code > range.hi && code <= summed.down_to) set |= 1u << j;
         if (valid && range.hi - code <= width) atomicAdd(hist + ((range.hi - code) >> shift), 1u);
       }
-      if (!rank_k)
-        View::each_set(set, [&](int j, bool have) {
-          const double w = c.weight(View::value_at(r, j));
-          if (have) mass += w;
-        });
+      if (!rank_k) mass += sum_of(c, r, set, 0.0);
     });
-    const double above = reduce(mass, 0u, 0u, 0u).mass;
+    const double above = sum_up(mass, range.hi, !rank_k);
     uint32_t n[kPsOwn], count = 0;
     merge_bins(n, false);
     const uint32_t mine = threadIdx.x * kPsOwn;
@@ -1052,23 +1177,19 @@ struct PolicyRow {
       for (int j = 0; j < 8; ++j) {
         const uint32_t code = ord32(View::value_of(r, j));
         const bool valid = r.bits >> j & 1u;
-        if (valid && code > range.hi) set |= 1u << j;
+        if (valid && code > range.hi && code <= summed.down_to) set |= 1u << j;
         if (valid && code >= range.lo && code <= range.hi) {
           const uint32_t at = atomicAdd(&sh.list_fill, 1u);
           // ascending keys: value falling, id rising
           if (at < kPsList) list[at] = (unsigned long long)~code << 32 | (id + j);
         }
       }
-      if (by_mass)
-        View::each_set(set, [&](int j, bool have) {
-          const double w = c.weight(View::value_at(r, j));
-          if (have) mass += w;
-        });
+      if (by_mass) mass += sum_of(c, r, set, 0.0);
     });
     __syncthreads();
     if ((uint32_t)threadIdx.x < k)
       *ps_remote(&sh.listed[rank], threadIdx.x) = min(sh.list_fill, kPsList);
-    const double above = reduce(mass, 0u, 0u, 0u).mass;
+    const double above = sum_up(mass, range.hi, by_mass);
     unsigned long long* sorted = ps_sorted();
     uint32_t n = 0;
     for (uint32_t r = 0; r < k; ++r) {
@@ -1263,29 +1384,53 @@ struct PolicyRow {
     return s;
   }
 
-  // weight of a kept value
-  __device__ __forceinline__ double weight(const RowCut& c, float v) const {
-    if (DT == kBF16 && table) {
-      const uint32_t bits = __float_as_uint(v);
-      const uint32_t i = ((bits >> 16) & 0x7FFFu) - kPsLow;
-      const uint32_t positive = (uint32_t)((int32_t)~bits >> 31);
-      if (i < (uint32_t)kPsHalf) return table[kPsHalf + (int)(i ^ positive)];
-    }
-    return c.weight(v);
-  }
-
   // sets of the lane's 8 values: above the cut, equal to it
   __device__ __forceinline__ static void split(const RowCut& c, const Raw& r, uint32_t& above,
                                                uint32_t& tie) {
     above = tie = 0u;
+    if constexpr (DT == kF32) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float v = View::value_of(r, j);
-      if (v > c.cut) above |= 1u << j;
-      if (v == c.cut) tie |= 1u << j;
+      for (int j = 0; j < 8; ++j) {
+        const float v = View::value_of(r, j);
+        if (v > c.cut) above |= 1u << j;
+        if (v == c.cut) tie |= 1u << j;
+      }
+    } else {
+      // two values at a time; no value lies between the cut and the cut rounded down
+      const uint32_t w[4] = {r.a.x, r.a.y, r.a.z, r.a.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t at = 0x00020001u << (2 * i);
+        above |= greater2(w[i], c.cut2) & at;
+        tie |= equal2(w[i], c.cut2) & at;
+      }
+      above = (above | above >> 16) & 0xFFu;
+      tie = (tie | tie >> 16) & 0xFFu;
     }
     above &= r.bits;
     tie &= r.bits;
+  }
+  __device__ __forceinline__ static uint32_t greater2(uint32_t a, uint32_t b) {
+    uint32_t m;
+    if constexpr (DT == kBF16) asm("set.gt.u32.bf16x2 %0, %1, %2;" : "=r"(m) : "r"(a), "r"(b));
+    else asm("set.gt.u32.f16x2 %0, %1, %2;" : "=r"(m) : "r"(a), "r"(b));
+    return m;
+  }
+  __device__ __forceinline__ static uint32_t equal2(uint32_t a, uint32_t b) {
+    uint32_t m;
+    if constexpr (DT == kBF16) asm("set.eq.u32.bf16x2 %0, %1, %2;" : "=r"(m) : "r"(a), "r"(b));
+    else asm("set.eq.u32.f16x2 %0, %1, %2;" : "=r"(m) : "r"(a), "r"(b));
+    return m;
+  }
+  // the cut in the row's own type, rounded down, twice
+  __device__ __forceinline__ static uint32_t twice(float cut) {
+    if constexpr (DT == kBF16) {
+      return (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rd(cut)) * 0x10001u;
+    } else if constexpr (DT == kF16) {
+      return (uint32_t)__half_as_ushort(__float2half_rd(cut)) * 0x10001u;
+    } else {
+      return 0u;
+    }
   }
 
   // f(id, raw values, set of the kept ones) over the vectors of `part` that may hold some;
@@ -1356,10 +1501,7 @@ struct PolicyRow {
       cut_to(i);
       double m = 0.0;
       each_kept(part, c, ties_at(i), [&](int id, const Raw& r, uint32_t set) {
-        View::each_set(set, [&](int j, bool have) {
-          const double w = weight(c, View::value_at(r, j));
-          if (have && w >= c.min_p) m += weigh(id + j, w);
-        });
+        each_weight(c, r, set, [&](int j, double w) { m += weigh(id + j, w); });
       });
       m = warp_sum(m);
       if (lane == 0) masses[i] = m;
@@ -1393,9 +1535,8 @@ struct PolicyRow {
       if (found >= 0) return;  // uniform over the warp
       double sum = 0.0;
       int mine = -1;
-      View::each_set(set, [&](int j, bool have) {
-        double w = weight(c, View::value_at(r, j));
-        w = have && w >= c.min_p ? weigh(id + j, w) : 0.0;
+      each_weight(c, r, set, [&](int j, double w) {
+        w = weigh(id + j, w);
         sum += w;
         if (w > 0.0) mine = id + j;
       });
@@ -1406,9 +1547,8 @@ struct PolicyRow {
         const double prev = __shfl_up_sync(~0u, incl, 1);
         double acc = run + (lane ? prev : 0.0);
         int at = -1;
-        View::each_set(set, [&](int j, bool have) {
-          double w = weight(c, View::value_at(r, j));
-          w = have && w >= c.min_p ? weigh(id + j, w) : 0.0;
+        each_weight(c, r, set, [&](int j, double w) {
+          w = weigh(id + j, w);
           acc += w;
           if (at < 0 && w > 0.0 && acc > goal) at = id + j;
         });
@@ -1442,7 +1582,7 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
   const uint32_t k = (uint32_t)p.k;
   // the barrier's first phase: every CTA of the cluster runs before its memory is written
   if (k > 1) ps_cluster_arrive();
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" :::);
 
   const int64_t item = (int64_t)(blockIdx.x / k);
   const int64_t group = OP == kOpSpec ? item / p.per_group : item;
@@ -1466,9 +1606,17 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
   view.base = row.rank * kPsWarps * row.warp_ids;
   view.begin = (uint32_t)min(begin, (uint64_t)row.row_end);
   view.end = (uint32_t)min(begin + row.warp_ids, (uint64_t)row.row_end);
-  view.peaks = p.peaks ? reinterpret_cast<uint16_t*>(ps_dynamic + p.peaks) : nullptr;
-  unsigned char* ring = ps_dynamic + kPsArea + row.warp * ps_ring(DT);
-  view.start_stream(ring, row.lane);  // the copies run while the policy is read
+  view.peaks = p.peaks ? reinterpret_cast<uint16_t*>(ps_dynamic + kPsFixed) : nullptr;
+  view.kept = p.keep != 0;
+  view.slot_bytes = ps_slot(DT, view.mask != nullptr);
+  view.slots = ps_dynamic + p.slots + (view.kept ? 0 : row.warp * View::kDepth * view.slot_bytes);
+  row.clear_hist();
+  if (threadIdx.x < 16) sh.powers.at[threadIdx.x] = exp2((double)threadIdx.x / 16.0);
+  __syncthreads();
+
+  // what came before on the stream has written the inputs
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  view.start_stream(row.lane);  // the copies run while the policy is read
 
   const RowPolicy pol = load_policy(p.policies + group * p.policy_stride);
   bool ok = pol.ok;
@@ -1499,21 +1647,23 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
 
   RowCut c = {};
   c.inv_t = fmin(1.0 / pol.temperature, 1e300);  // 0 times it stays 0
-  c.scale = c.inv_t * 1.4426950408889634;
+  c.scale = c.inv_t * (16.0 * 1.4426950408889634);
   c.min_p = pol.min_p;
   c.powers = &sh.powers;
   c.cut = -INFINITY;
-  if (threadIdx.x < 16) sh.powers.at[threadIdx.x] = exp2((double)threadIdx.x / 16.0);
   if (ok) {
     const bool by_mass = pol.top_p < 1.0;
     const bool bins = pol.temperature > 0.0 && (pol.top_k || by_mass);
     // the mass of all ids, relative to a value of 0 (the maximum is not known yet)
     const bool mass_of_all = DT != kBF16 && bins && by_mass && !pol.top_k;
-    if (bins) row.clear_hist();
+    const uint32_t hist = (uint32_t)__cvta_generic_to_shared(ps_hist());
+    // values below it weigh nothing on the scale of 2^(v scale / 16) (nor do they count as much
+    // as the bound's 2^-937 there)
+    const float floor_value = (float)(-15000.0 / c.scale);
     uint32_t count = 0, small = 0, top16 = 0;
     float top_value = -INFINITY;
-    double mass = 0.0;
-    view.stream(ring, row.lane, [&](uint32_t pos, const auto& r) {
+    double mass = 0.0, mass2 = 0.0;
+    view.stream(row.lane, [&](uint32_t pos, const auto& r) {
       // the values to bfloat16 width, two to a word, and masks of the valid ones
       uint32_t v[4] = {~0u, ~0u, ~0u, ~0u}, t[4];
       const bool full = __all_sync(~0u, r.bits == 0xFFu);
@@ -1526,7 +1676,7 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
       count += __popc(r.bits);
       uint32_t near = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) near |= Row::count_bins(ps_dynamic, t[i], v[i]);
+      for (int i = 0; i < 4; ++i) near |= Row::count_bins(hist, t[i], v[i]);
       if (__any_sync(~0u, near)) {
         uint32_t set = 0;
 #pragma unroll
@@ -1543,11 +1693,14 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
       if (DT != kBF16 && mass_of_all) {
         if (full) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            mass += exp2_table((double)View::value_of(r, j) * c.scale, *c.powers);
+          for (int j = 0; j < 8; j += 2) {
+            mass += exp2_scaled(fmaxf(View::value_of(r, j), floor_value), c.scale, sh.powers);
+            mass2 += exp2_scaled(fmaxf(View::value_of(r, j + 1), floor_value), c.scale, sh.powers);
+          }
         } else {
           View::each_set(r.bits, [&](int j, bool have) {
-            const double w = exp2_table((double)View::value_at(r, j) * c.scale, *c.powers);
+            const double w =
+                exp2_scaled(fmaxf(View::value_at(r, j), floor_value), c.scale, sh.powers);
             if (have) mass += w;
           });
         }
@@ -1555,7 +1708,7 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
     });
     // the order code of the maximum: 0 without a valid id
     uint32_t top = top16 ? ord32(top_value) : 0u;
-    PsBox sum = row.reduce(mass, count, top, small);
+    PsBox sum = row.reduce(mass + mass2, count, top, small);
     top = sum.top;
     if (top == 0u) status = kStatusEmptyMask;
     if (top == kOrd32NaN) status = kStatusNanInSupport;
@@ -1565,16 +1718,18 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
       c.flat = !(pol.temperature > 0.0) || c.top == INFINITY;
       // the masses relative to the maximum, where they did not leave the range of doubles
       const double shift = -c.top * c.scale;
-      const bool in_range = fabs(shift) < 900.0;
+      const bool in_range = fabs(shift) < 14400.0;
       sum.mass = sum.mass > 0.0 ? sum.mass * exp2_table(shift, sh.powers) : 0.0;
-      const double total = in_range && mass_of_all ? sum.mass : -1.0;
+      const bool measured = mass_of_all && in_range && floor_value < -1e-30f;
+      const double total = measured ? sum.mass : -1.0;
       if (!bins) {
         if (pol.temperature > 0.0) c.cut = c.flat ? FLT_MAX : -INFINITY;
         else c.keep(code_value(top), 1u);
       } else {
         PsRange range;
         auto found = Row::kNothing;
-        if (in_range) found = row.find_cut_in_bins(c, pol, sum, range);
+        if (in_range && (measured || !mass_of_all))
+          found = row.find_cut_in_bins(c, pol, sum, range);
         if (found != Row::kFound) {
           __syncthreads();  // what the scans left in shared memory has been read
           row.find_cut(c, pol, top, sum.count, total,
@@ -1582,6 +1737,7 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
         }
       }
       c.bound_by_min_p();
+      c.cut2 = Row::twice(c.cut);
     }
   }
 
@@ -1601,7 +1757,10 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
     draft = p.drafts[group * p.draft_stride + sub];
     if (draft < 0 || draft >= view.vocab) draft = -1;
   }
-  double mass = 0.0;
+  // what finding the cut has summed already, if min_p takes nothing from it
+  const bool summed = !(c.min_p > 0.0);
+  const uint32_t down_to = summed ? row.summed.down_to : ~0u;
+  double mass = summed ? row.summed.lane : 0.0;
   uint32_t ties = 0, before = 0;
   view.each(row.lane, c.least(), [&](uint32_t pos, const auto& r) {
     uint32_t set, tie;
@@ -1611,10 +1770,12 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
       const int ahead = draft - view.id_of(pos);
       if (ahead > 0) before += __popc(ahead < 8 ? tie & ((1u << ahead) - 1u) : tie);
     }
-    View::each_set(set, [&](int j, bool have) {
-      const double w = row.weight(c, View::value_at(r, j));
-      if (have && w >= c.min_p) mass += w;
-    });
+    if (down_to != ~0u) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (ord32(View::value_of(r, j)) > down_to) set &= ~(1u << j);
+    }
+    mass += row.sum_of(c, r, set, c.min_p);
   });
   mass = warp_sum(mass);
   ties = __reduce_add_sync(~0u, ties);
@@ -1626,10 +1787,7 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
   if (OP == kOpProbs) {
     float* out = p.out_probs + group * p.out_stride;
     row.each_kept(view, c, scan.my_ties, [&](int id, const auto& r, uint32_t set) {
-      View::each_set(set, [&](int j, bool have) {
-        const double w = row.weight(c, View::value_at(r, j));
-        if (have && w >= c.min_p) out[id + j] = (float)(w * inv);
-      });
+      row.each_weight(c, r, set, [&](int j, double w) { out[id + j] = (float)(w * inv); });
     });
     if (first) p.out_status[item] = 0u;
     return;
@@ -1665,10 +1823,7 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
   if (OP == kOpSpec && residual) {
     double sum = 0.0;
     row.each_kept(view, c, scan.my_ties, [&](int id, const auto& r, uint32_t set) {
-      View::each_set(set, [&](int j, bool have) {
-        const double w = row.weight(c, View::value_at(r, j));
-        if (have && w >= c.min_p) sum += rest(id + j, w);
-      });
+      row.each_weight(c, r, set, [&](int j, double w) { sum += rest(id + j, w); });
     });
     sum = warp_sum(sum);
     const auto left = row.scan_entries(1, sum, 0u, 0u, 0u, 0.0, u);
