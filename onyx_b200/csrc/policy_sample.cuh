@@ -90,7 +90,8 @@ struct PolicyParams {
   int32_t k;         // CTAs per row
   int32_t peaks;     // the peaks are kept (else their place is empty)
   int32_t keep;      // shared memory holds all chunks of a CTA's part
-  int32_t slots;     // where in dynamic shared memory the chunks' slots begin
+  int32_t slots;     // where in dynamic shared memory the chunks' slots begin,
+  int32_t lists;     // and the lists of the warps (over a ring, which is done by then)
 };
 
 enum Verdict : int { kAccepted = 0, kDecided = 1 };
@@ -176,6 +177,14 @@ struct PsCross {  // the bin in which a count or a mass is reached
   int bin;
 };
 
+struct PsScan {  // of the entries of all warps
+  double total;
+  double mass_before;     // kept mass before the owner's ids ...
+  uint32_t ties_before;   // ... and ids at the cut before them
+  uint32_t draft_before;  // ids at the cut before the draft
+  int owner;  // entry whose interval of kept mass holds u times the total
+};
+
 struct PsShared {
   PsBox box[2][kPsMaxCluster];  // used alternately: one may still be read as the next is written
   double part_mass[kPsWarps], part_high[kPsWarps];
@@ -188,6 +197,10 @@ struct PsShared {
   PsCross cross[3];
   uint32_t listed[kPsMaxCluster];  // ids that each CTA listed
   uint32_t list_fill;
+  int listed_by[kPsWarps];  // vectors that each warp gathered for the passes after the cut
+  PsScan scan[2];
+  uint32_t ties_before[kPsWarps];
+  double sums_before[2][kPsWarps + 1];
 };
 
 // Dynamic shared memory: the CTA's histogram and the cluster's; their 32 KB are used again for a
@@ -248,7 +261,9 @@ struct RowView {
   static constexpr int kData = kPsChunk * (int)sizeof(S), kDepth = ps_depth(DT);
   const S* row;
   const uint32_t* mask;
-  uint16_t* peaks;  // of this CTA: order code >> 16 of the maximum of every 8, or null
+  uint16_t* peaks;  // of this CTA: the peaks (see peak()) of every 8 positions, or null
+  uint16_t* list;   // vectors of 8 of this part that the last gather() found,
+  int listed;       // so many (without peaks: all)
   uint32_t base;    // the CTA's first position
   uint32_t begin, end;  // positions; multiples of kPsChunk, but for the row's end
   int vocab, off;
@@ -309,32 +324,39 @@ struct RowView {
     return r;
   }
 
-  // the lane's 8 values of the chunk at `at`, none if it does not need them; `at` < end
-  __device__ __forceinline__ Raw load(uint32_t at, int lane, bool need) const {
-    if (kept) {
-      Raw r = from_slot(slots + (size_t)((at - base) / kPsChunk) * slot_bytes, at, lane);
-      if (!need) r.bits = 0u;
-      return r;
-    }
+  // the 8 values from position `pos` on, none if they are not wanted
+  __device__ __forceinline__ Raw load(uint32_t pos, bool wanted) const {
     Raw r;
     r.a = make_uint4(0u, 0u, 0u, 0u);
     if (DT == kF32) r.b = r.a;
     r.bits = 0u;
-    if (!need) return r;
-    const int id = id_of(at) + 8 * lane;
+    if (!wanted) return r;
+    const int id = id_of(pos);
     r.bits = inside(id);
-    if (r.bits == 0xFFu) {
-      r.a = *reinterpret_cast<const uint4*>(row + id);
-      if (DT == kF32) r.b = *reinterpret_cast<const uint4*>(row + id + 4);
+    uint32_t lo = ~0u, hi = ~0u;
+    if (kept) {
+      const uint32_t at = (pos - base) >> 3, lane = at & 31u;
+      const unsigned char* slot = slots + (size_t)(at >> 5) * slot_bytes;
+      r.a = *reinterpret_cast<const uint4*>(slot + lane * 16);
+      if (DT == kF32) r.b = *reinterpret_cast<const uint4*>(slot + 512 + lane * 16);
+      if (mask) {
+        const uint32_t* words = reinterpret_cast<const uint32_t*>(slot + kData);
+        const int w = (id >> 5) - ((id - 8 * (int)lane) >> 5);
+        lo = words[w], hi = words[w + 1];
+      }
     } else {
-      load_edge(r, id);
+      if (r.bits == 0xFFu) {
+        r.a = *reinterpret_cast<const uint4*>(row + id);
+        if (DT == kF32) r.b = *reinterpret_cast<const uint4*>(row + id + 4);
+      }
+      if (mask) {
+        const int w = id >> 5, words = (vocab + 31) >> 5;
+        lo = w >= 0 && w < words ? mask[w] : 0u;
+        hi = (id & 31) > 24 && w + 1 < words ? mask[w + 1] : 0u;
+      }
     }
-    if (mask && r.bits) {
-      const int w = id >> 5, words = (vocab + 31) >> 5;
-      const uint32_t lo = w >= 0 ? mask[w] : 0u;
-      const uint32_t hi = (id & 31) > 24 && w + 1 < words ? mask[w + 1] : 0u;
-      r.bits &= __funnelshift_r(lo, hi, id & 31);
-    }
+    if (r.bits != 0xFFu) load_edge(r, id);
+    r.bits &= __funnelshift_r(lo, hi, id & 31);
     return r;
   }
 
@@ -455,59 +477,115 @@ struct RowView {
     }
   }
 
-  // Order code >> 16 of the largest valid value, 0 without one; raises `top`, which a NaN turns
-  // into one. `t` and `v`: the values to bfloat16 width and masks of the valid ones.
-  __device__ __forceinline__ static uint32_t peak(const Raw& r, const uint32_t (&t)[4],
-                                                  const uint32_t (&v)[4], bool full, float& top) {
-    float m;
+  // The peak of 8 values: 16 bits that rise with the largest valid one (16-bit types: their
+  // own order code, float32: the upper half of it), 0 without one, 0xFFFF with a NaN. `v`:
+  // masks of the valid ones; float32 also raises `top`, which a NaN turns into one.
+  __device__ __forceinline__ static uint32_t peak(const Raw& r, const uint32_t (&v)[4], bool full,
+                                                  float& top) {
     if constexpr (DT == kF32) {
       float x[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j)
         x[j] = full || (r.bits >> j & 1u) ? value_of(r, j) : -INFINITY;
-      m = max_nan_f32(max_nan_f32(max_nan_f32(x[0], x[1]), max_nan_f32(x[2], x[3])),
-                      max_nan_f32(max_nan_f32(x[4], x[5]), max_nan_f32(x[6], x[7])));
+      const float m = max_nan_f32(max_nan_f32(max_nan_f32(x[0], x[1]), max_nan_f32(x[2], x[3])),
+                                  max_nan_f32(max_nan_f32(x[4], x[5]), max_nan_f32(x[6], x[7])));
+      if (r.bits == 0u) return 0u;
+      top = max_nan_f32(top, m);
+      return ord32(m) >> 16;
     } else {
       const uint32_t none = DT == kBF16 ? 0xFF80FF80u : 0xFC00FC00u;  // -inf twice
       const uint32_t a = (r.a.x & v[0]) | (none & ~v[0]), b = (r.a.y & v[1]) | (none & ~v[1]);
       const uint32_t d = (r.a.z & v[2]) | (none & ~v[2]), e = (r.a.w & v[3]) | (none & ~v[3]);
-      if constexpr (DT == kBF16) {
-        const uint32_t x = max_nan_bf16x2(max_nan_bf16x2(a, b), max_nan_bf16x2(d, e));
-        m = max_nan_f32(bf16_bits_to_f32(x & 0xFFFFu), bf16_bits_to_f32(x >> 16));
-      } else {
-        const uint32_t x = max_nan_f16x2(max_nan_f16x2(a, b), max_nan_f16x2(d, e));
-        m = max_nan_f32(f16_bits_to_f32(x & 0xFFFFu), f16_bits_to_f32(x >> 16));
-      }
+      const uint32_t x = max2(max2(a, b), max2(d, e));
+      const uint32_t h = max2(x, x >> 16) & 0xFFFFu;
+      return r.bits ? h ^ (h & 0x8000u ? 0xFFFFu : 0x8000u) : 0u;
     }
-    if (r.bits == 0u) return 0u;
-    top = max_nan_f32(top, m);
-    return ord32(m) >> 16;
+  }
+  __device__ __forceinline__ static uint32_t max2(uint32_t a, uint32_t b) {
+    return DT == kBF16 ? max_nan_bf16x2(a, b) : max_nan_f16x2(a, b);
+  }
+  // order code of the largest peak of a 16-bit row
+  __device__ __forceinline__ static uint32_t top_code(uint32_t peak) {
+    const uint32_t h = peak ^ (peak & 0x8000u ? 0x8000u : 0xFFFFu);
+    return ord32(DT == kBF16 ? bf16_bits_to_f32(h) : f16_bits_to_f32(h));
+  }
+  // the least peak of 8 values that hold an order code of at least `code`
+  __device__ __forceinline__ static uint32_t least_peak(uint32_t code) {
+    uint32_t peak = code >> 16;
+    if constexpr (DT == kF16) {
+      const uint32_t f = (code & 0x80000000u) ? code & 0x7FFFFFFFu : ~code;
+      const uint32_t h = __half_as_ushort(__float2half_rd(__uint_as_float(f)));
+      peak = h ^ (h & 0x8000u ? 0xFFFFu : 0x8000u);
+    }
+    return DT != kF32 && peak == 0x8000u ? 0x7FFFu : peak;  // -0 counts as 0
   }
 
-  // f(position, values) over the chunks that may hold order codes of at least `code`, the next
-  // one's loads in flight; lanes whose 8 values hold none get no valid ones. Every lane of the
-  // warp makes every call.
-  template <class F>
-  __device__ __forceinline__ void each(int lane, uint32_t code, F&& f) const {
-    const uint32_t step = 8u * lane, first = code >> 16;
-    auto need = [&](uint32_t at) {
-      return !peaks || peaks[(at + step - base) >> 3] >= first;
-    };
-    auto next = [&](uint32_t at) {
-      while (at < end && !__any_sync(~0u, need(at))) at += kPsChunk;
-      return at;
-    };
-    uint32_t at = next(begin);
-    if (at >= end) return;
-    Raw r = load(at, lane, need(at));
+  // Lists the vectors of this part that may hold order codes of at least `code`. Whole warp.
+  __device__ void gather(int lane, uint32_t code) {
+    if (!peaks) {
+      listed = (int)((end - begin + 7u) >> 3);
+      return;
+    }
+    const uint32_t least = least_peak(code);
+    const uint16_t* mine = peaks + ((begin - base) >> 3);
+    const int stop = chunks() * 32;
+    int n = 0;
 #pragma unroll 1
-    while (true) {
-      const uint32_t then = next(at + kPsChunk);
+    for (int i = 0; i < stop; i += 256) {
+      const int at = i + 8 * lane;
+      uint32_t set = 0;
+      if (at < stop) {
+        const uint4 x = *reinterpret_cast<const uint4*>(mine + at);
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if ((w[j] & 0xFFFFu) >= least) set |= 1u << (2 * j);
+          if (w[j] >> 16 >= least) set |= 2u << (2 * j);
+        }
+      }
+      const uint32_t c = __popc(set), incl = warp_scan(c, lane);
+      int to = n + (int)(incl - c);
+      while (set) {
+        list[to++] = (uint16_t)(at + __ffs(set) - 1);
+        set &= set - 1u;
+      }
+      n += (int)__shfl_sync(~0u, incl, 31);
+    }
+    __syncwarp();
+    listed = n;
+  }
+  // the entries [from, to) of the list alone
+  __device__ __forceinline__ RowView slice(int from, int to) const {
+    RowView part = *this;
+    part.listed = to - from;
+    if (peaks) part.list += from;
+    else part.begin += 8u * (uint32_t)from;
+    return part;
+  }
+
+  // f(position, values) over the list, a vector to a lane in rising order, the next one's loads
+  // in flight; lanes past its end get no valid values. Every lane of the warp makes every call.
+  template <class F>
+  __device__ __forceinline__ void each(int lane, F&& f) const {
+    if (listed == 0) return;
+    auto at = [&](int j) {
+      return begin + 8u * (j < listed ? (peaks ? (uint32_t)list[j] : (uint32_t)j) : 0u);
+    };
+    int j = lane;
+    uint32_t pos = at(j);
+    Raw r = load(pos, j < listed);
+    const int turns = (listed + 31) >> 5;
+#pragma unroll 1
+    for (int i = 0; i < turns; ++i) {
+      j += 32;
+      uint32_t pos2 = pos;
       Raw more = r;
-      if (then < end) more = load(then, lane, need(then));
-      f(at + step, r);
-      if (then >= end) break;
-      at = then;
+      if (i + 1 < turns) {
+        pos2 = at(j);
+        more = load(pos2, j < listed);
+      }
+      f(pos, r);
+      pos = pos2;
       r = more;
     }
   }
@@ -680,29 +758,30 @@ struct PolicyRow {
     const uint32_t c_incl = warp_scan(c, lane);
     s.count_all = __shfl_sync(~0u, c_incl, 31);
     s.count_before = __shfl_sync(~0u, c_incl - c, warp) + count_incl - count;
-    if (masses) {
-      double run = 0.0, mine = 0.0;
+    if (!masses) return s;
+    if (warp < (two ? 2 : 1)) {  // in order, so that the parts join
+      const double* part = warp ? sh.part_high : sh.part_mass;
+      double run = 0.0;
 #pragma unroll
       for (int i = 0; i < kPsWarps; ++i) {
-        if (i == warp) mine = run;
-        run += sh.part_mass[i];
+        const double x = part[i];
+        if (lane == i) sh.sums_before[warp][i] = run;
+        run += x;
       }
-      const double prev = __shfl_up_sync(~0u, high_incl, 1);
-      s.high_all = run;
-      s.high_before = lane ? mine + prev : mine;
-      s.high_end = mine + high_incl;
+      if (lane == 0) sh.sums_before[warp][kPsWarps] = run;
     }
+    __syncthreads();
+    const double prev = __shfl_up_sync(~0u, high_incl, 1);
+    const double mine = sh.sums_before[0][warp];
+    s.high_all = sh.sums_before[0][kPsWarps];
+    s.high_before = lane ? mine + prev : mine;
+    s.high_end = mine + high_incl;
     if (two) {
-      double run = 0.0, mine = 0.0;
-#pragma unroll
-      for (int i = 0; i < kPsWarps; ++i) {
-        if (i == warp) mine = run;
-        run += sh.part_high[i];
-      }
-      const double prev = __shfl_up_sync(~0u, low_incl, 1);
-      s.low_all = run;
-      s.low_before = lane ? mine + prev : mine;
-      s.low_end = mine + low_incl;
+      const double prev_low = __shfl_up_sync(~0u, low_incl, 1);
+      const double mine_low = sh.sums_before[1][warp];
+      s.low_all = sh.sums_before[1][kPsWarps];
+      s.low_before = lane ? mine_low + prev_low : mine_low;
+      s.low_end = mine_low + low_incl;
     }
     return s;
   }
@@ -1031,7 +1110,8 @@ struct PolicyRow {
   __device__ PsBox at_least(const RowCut& c, uint32_t code) {
     double mass = 0.0;
     uint32_t count = 0;
-    view.each(lane, code, [&](uint32_t, const Raw& r) {
+    view.gather(lane, code);
+    view.each(lane, [&](uint32_t, const Raw& r) {
       uint32_t set = 0;
 #pragma unroll
       for (int j = 0; j < 8; ++j)
@@ -1062,7 +1142,8 @@ struct PolicyRow {
     __syncthreads();
     uint32_t* hist = ps_hist();
     double mass = 0.0;
-    view.each(lane, range.lo, [&](uint32_t, const Raw& r) {
+    view.gather(lane, range.lo);
+    view.each(lane, [&](uint32_t, const Raw& r) {
       uint32_t set = 0;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
@@ -1170,7 +1251,8 @@ struct PolicyRow {
     __syncthreads();
     unsigned long long* list = ps_list();
     double mass = 0.0;
-    view.each(lane, range.lo, [&](uint32_t pos, const Raw& r) {
+    view.gather(lane, range.lo);
+    view.each(lane, [&](uint32_t pos, const Raw& r) {
       const uint32_t id = (uint32_t)view.id_of(pos);
       uint32_t set = 0;
 #pragma unroll
@@ -1307,22 +1389,12 @@ struct PolicyRow {
   }
 
   // ---- the kept mass and the draw -------------------------------------------------------
-  // The entries of all warps, scanned by every warp for itself; a lane holds up to kPer of
-  // them, in id order.
+  // Publishes this warp's entry to the cluster; the first warp of every CTA scans them all, a
+  // lane holding up to kPer in id order. `w_tie` is the weight of an id at the cut, `mass` that
+  // above it; set 1 leaves the ties as set 0 published them.
   static constexpr int kPer = kPsEntries / 32;
-  struct Scan {
-    double total;
-    double mass_before;     // kept mass before the owner's ids ...
-    uint32_t ties_before;   // ... and ids at the cut before them
-    uint32_t my_ties;       // ids at the cut before this warp's
-    uint32_t draft_before;  // ids at the cut before the draft
-    int owner;  // entry whose interval of kept mass holds u times the total
-  };
-
-  // Publishes this warp's entry to the cluster and scans all of them. `w_tie` is the weight of
-  // an id at the cut, `mass` that above it; set 1 leaves the ties as set 0 published them.
-  __device__ Scan scan_entries(int set, double mass, uint32_t ties, uint32_t before,
-                               uint32_t take, double w_tie, double u) {
+  __device__ PsScan scan_entries(int set, double mass, uint32_t ties, uint32_t before,
+                                 uint32_t take, double w_tie, double u) {
     if ((uint32_t)lane < k) {
       PsShared* r = ps_remote(&sh, lane);
       r->entry_mass[set][entry] = mass;
@@ -1332,56 +1404,61 @@ struct PolicyRow {
       }
     }
     publish();
-    const int n = (int)k * kPsWarps, per = (n + 31) / 32, first = lane * per;
-    uint32_t t[kPer], tie_sum = 0, draft = 0;
-    double m[kPer], sum = 0.0;
+    if (warp == 0) {
+      const int n = (int)k * kPsWarps, per = (n + 31) / 32, first = lane * per;
+      uint32_t t[kPer], tie_sum = 0, draft = 0;
+      double m[kPer], sum = 0.0;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const bool have = i < per && first + i < n;
-      t[i] = have ? sh.entry_ties[first + i] : 0u;
-      m[i] = have ? sh.entry_mass[set][first + i] : 0.0;
-      draft += have ? sh.entry_before[first + i] : 0u;
-      tie_sum += t[i];
-    }
-    const uint32_t tie_start = warp_scan(tie_sum, lane) - tie_sum;
-    uint32_t run = tie_start;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const uint32_t kept = run < take ? min(t[i], take - run) : 0u;
-      if (kept) m[i] += (double)kept * w_tie;
-      run += t[i];
-      sum += m[i];
-    }
-    const double incl = warp_scan(sum, lane);
-    double acc = __shfl_up_sync(~0u, incl, 1);
-    if (lane == 0) acc = 0.0;
-    Scan s;
-    s.total = __shfl_sync(~0u, incl, 31);
-    s.draft_before = __reduce_add_sync(~0u, draft);
-    const double goal = u * s.total;
-    // the first entry that passes the goal; the last with mass, if rounding leaves none
-    int hit = kPsEntries, last = 0;
-    double hit_mass = 0.0, last_mass = 0.0;
-    uint32_t hit_ties = 0, last_ties = 0, own = 0;
-    run = tie_start;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      if (first + i == entry) own = run;
-      if (m[i] > 0.0) {
-        last = first + i, last_mass = acc, last_ties = run;
-        if (hit == kPsEntries && acc + m[i] > goal) hit = last, hit_mass = acc, hit_ties = run;
+      for (int i = 0; i < kPer; ++i) {
+        const bool have = i < per && first + i < n;
+        t[i] = have ? sh.entry_ties[first + i] : 0u;
+        m[i] = have ? sh.entry_mass[set][first + i] : 0.0;
+        draft += have ? sh.entry_before[first + i] : 0u;
+        tie_sum += t[i];
       }
-      acc += m[i];
-      run += t[i];
+      const uint32_t tie_start = warp_scan(tie_sum, lane) - tie_sum;
+      uint32_t run = tie_start;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const uint32_t kept = run < take ? min(t[i], take - run) : 0u;
+        if (kept) m[i] += (double)kept * w_tie;
+        const int own = first + i - (int)rank * kPsWarps;  // a warp of this CTA
+        if (set == 0 && i < per && own >= 0 && own < kPsWarps) sh.ties_before[own] = run;
+        run += t[i];
+        sum += m[i];
+      }
+      const double incl = warp_scan(sum, lane);
+      double acc = __shfl_up_sync(~0u, incl, 1);
+      if (lane == 0) acc = 0.0;
+      const double total = __shfl_sync(~0u, incl, 31);
+      draft = __reduce_add_sync(~0u, draft);
+      const double goal = u * total;
+      // the first entry that passes the goal; the last with mass, if rounding leaves none
+      int hit = kPsEntries, last = -1;
+      double hit_mass = 0.0, last_mass = 0.0;
+      uint32_t hit_ties = 0, last_ties = 0;
+      run = tie_start;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        if (m[i] > 0.0) {
+          last = first + i, last_mass = acc, last_ties = run;
+          if (hit == kPsEntries && acc + m[i] > goal) hit = last, hit_mass = acc, hit_ties = run;
+        }
+        acc += m[i];
+        run += t[i];
+      }
+      const int winner = __reduce_min_sync(~0u, hit);
+      const int final = __reduce_max_sync(~0u, last);
+      if (lane == 0) sh.scan[set].total = total, sh.scan[set].draft_before = draft;
+      if (winner < kPsEntries ? hit == winner : final >= 0 ? last == final : lane == 0) {
+        const bool passed = winner < kPsEntries;
+        sh.scan[set].owner = passed ? hit : max(last, 0);
+        sh.scan[set].mass_before = passed ? hit_mass : last_mass;
+        sh.scan[set].ties_before = passed ? hit_ties : last_ties;
+      }
     }
-    s.my_ties = __shfl_sync(~0u, own, entry / per);
-    const int winner = __reduce_min_sync(~0u, hit);
-    const bool passed = winner < kPsEntries;
-    s.owner = passed ? winner : __reduce_max_sync(~0u, last);
-    const int src = s.owner / per;
-    s.mass_before = __shfl_sync(~0u, passed ? hit_mass : last_mass, src);
-    s.ties_before = __shfl_sync(~0u, passed ? hit_ties : last_ties, src);
-    return s;
+    __syncthreads();
+    return sh.scan[set];
   }
 
   // sets of the lane's 8 values: above the cut, equal to it
@@ -1439,7 +1516,7 @@ struct PolicyRow {
   __device__ __forceinline__ void each_kept(const View& part, const RowCut& c,
                                             uint32_t ties_before, F&& f) {
     uint32_t run = ties_before;
-    part.each(lane, c.least(), [&](uint32_t pos, const Raw& r) {
+    part.each(lane, [&](uint32_t pos, const Raw& r) {
       uint32_t set, tie;
       split(c, r, set, tie);
       if (c.take && __any_sync(~0u, tie)) {
@@ -1457,81 +1534,13 @@ struct PolicyRow {
     });
   }
 
-  // The draw, by all warps of the CTA that has the owner: its part is cut into pieces, whose
-  // sums the warps take in turn; the warp that summed the piece that holds the goal walks it.
-  // Returns the id in that warp, -1 in the others. weigh(id, kept weight) is the weight to use.
+  // The first id of `part`, in id order, at which the weights summed from `run` on exceed
+  // `goal` (the last with a weight, if rounding leaves none). Whole warp; all lanes return it.
   template <class W>
-  __device__ int draw(const RowCut& c, const Scan& s, double goal, W&& weigh) {
-    View part = view;
-    const uint64_t begin = (uint64_t)s.owner * warp_ids;
-    part.begin = (uint32_t)min(begin, (uint64_t)row_end);
-    part.end = (uint32_t)min(begin + warp_ids, (uint64_t)row_end);
-    const uint32_t all = (part.end - part.begin + kPsChunk - 1) / kPsChunk;
-    uint32_t piece = 1;  // chunks
-    while ((all + piece - 1) / piece > kPsUnits) piece *= 2;
-    const int n = (int)((all + piece - 1) / piece);
-    const uint32_t first = part.begin, stop = part.end, wide = piece * kPsChunk;
-    auto cut_to = [&](int i) {
-      part.begin = first + (uint32_t)i * wide;
-      part.end = min(stop, part.begin + wide);
-    };
-    double* masses = ps_unit_mass();
-    uint32_t* ties = ps_unit_ties();
-    if (c.take) {
-      for (int i = warp; i < n; i += kPsWarps) {
-        cut_to(i);
-        uint32_t t = 0;
-        part.each(lane, c.least(), [&](uint32_t, const Raw& r) {
-          uint32_t set, tie;
-          split(c, r, set, tie);
-          t += __popc(tie);
-        });
-        t = __reduce_add_sync(~0u, t);
-        if (lane == 0) ties[i] = t;
-      }
-      __syncthreads();
-    }
-    auto ties_at = [&](int i) {
-      uint32_t t = 0;
-      if (c.take)
-        for (int j = lane; j < i; j += 32) t += ties[j];
-      return s.ties_before + __reduce_add_sync(~0u, t);
-    };
-    for (int i = warp; i < n; i += kPsWarps) {
-      cut_to(i);
-      double m = 0.0;
-      each_kept(part, c, ties_at(i), [&](int id, const Raw& r, uint32_t set) {
-        each_weight(c, r, set, [&](int j, double w) { m += weigh(id + j, w); });
-      });
-      m = warp_sum(m);
-      if (lane == 0) masses[i] = m;
-    }
-    __syncthreads();
-    // the piece that holds the goal, and the mass before it
-    int hit = -1, last = 0;
-    double run = s.mass_before, hit_run = run, last_run = run;
-    for (int i = 0; i < n && hit < 0; i += 32) {
-      const double m = i + lane < n ? masses[i + lane] : 0.0;
-      const double incl = warp_scan(m, lane);
-      const double prev = __shfl_up_sync(~0u, incl, 1);
-      const double before = run + (lane ? prev : 0.0);
-      const uint32_t over = __ballot_sync(~0u, m > 0.0 && run + incl > goal);
-      const uint32_t some = __ballot_sync(~0u, m > 0.0);
-      if (over) {
-        hit = i + __ffs(over) - 1;
-        hit_run = __shfl_sync(~0u, before, __ffs(over) - 1);
-      } else if (some) {
-        last = i + 31 - __clz(some);
-        last_run = __shfl_sync(~0u, before, 31 - __clz(some));
-      }
-      run += __shfl_sync(~0u, incl, 31);
-    }
-    if (hit < 0) hit = last, hit_run = last_run;  // what rounding leaves
-    if (hit % kPsWarps != warp) return -1;
-    cut_to(hit);
-    run = hit_run;
+  __device__ int walk(const View& part, const RowCut& c, uint32_t ties_before, double run,
+                      double goal, W&& weigh) {
     int found = -1, final = -1;
-    each_kept(part, c, ties_at(hit), [&](int id, const Raw& r, uint32_t set) {
+    each_kept(part, c, ties_before, [&](int id, const Raw& r, uint32_t set) {
       if (found >= 0) return;  // uniform over the warp
       double sum = 0.0;
       int mine = -1;
@@ -1559,6 +1568,81 @@ struct PolicyRow {
       run += __shfl_sync(~0u, incl, 31);
     });
     return found >= 0 ? found : __reduce_max_sync(~0u, final);
+  }
+
+  // The draw, in the CTA that has the owner. A short list its owner walks alone. A long one is
+  // cut into pieces, whose sums the warps take in turn; the warp that summed the piece that
+  // holds the goal walks that. Returns the id in the walking warp, -1 in the others.
+  // weigh(id, kept weight) is the weight to use.
+  template <class W>
+  __device__ int draw(const RowCut& c, const PsScan& s, double goal, W&& weigh) {
+    const int own = s.owner % kPsWarps, all = sh.listed_by[own];
+    View list = view;
+    const uint64_t begin = (uint64_t)s.owner * warp_ids;
+    list.begin = (uint32_t)min(begin, (uint64_t)row_end);
+    list.end = (uint32_t)min(begin + warp_ids, (uint64_t)row_end);
+    list.list += (own - warp) * (int)(warp_ids >> 3);
+    list.listed = all;
+    if (all <= 64) {
+      if (warp != own) return -1;
+      return walk(list, c, s.ties_before, s.mass_before, goal, weigh);
+    }
+    int wide = 32;
+    while ((all + wide - 1) / wide > kPsUnits) wide *= 2;
+    const int n = (all + wide - 1) / wide;
+    auto piece = [&](int i) { return list.slice(i * wide, min(all, (i + 1) * wide)); };
+    double* masses = ps_unit_mass();
+    uint32_t* ties = ps_unit_ties();
+    if (c.take) {
+      for (int i = warp; i < n; i += kPsWarps) {
+        uint32_t t = 0;
+        piece(i).each(lane, [&](uint32_t, const Raw& r) {
+          uint32_t set, tie;
+          split(c, r, set, tie);
+          t += __popc(tie);
+        });
+        t = __reduce_add_sync(~0u, t);
+        if (lane == 0) ties[i] = t;
+      }
+      __syncthreads();
+    }
+    auto ties_at = [&](int i) {
+      uint32_t t = 0;
+      if (c.take)
+        for (int j = lane; j < i; j += 32) t += ties[j];
+      return s.ties_before + __reduce_add_sync(~0u, t);
+    };
+    for (int i = warp; i < n; i += kPsWarps) {
+      double m = 0.0;
+      each_kept(piece(i), c, ties_at(i), [&](int id, const Raw& r, uint32_t set) {
+        each_weight(c, r, set, [&](int j, double w) { m += weigh(id + j, w); });
+      });
+      m = warp_sum(m);
+      if (lane == 0) masses[i] = m;
+    }
+    __syncthreads();
+    // the piece that holds the goal, and the mass before it
+    int hit = -1, last = 0;
+    double run = s.mass_before, hit_run = run, last_run = run;
+    for (int i = 0; i < n && hit < 0; i += 32) {
+      const double m = i + lane < n ? masses[i + lane] : 0.0;
+      const double incl = warp_scan(m, lane);
+      const double prev = __shfl_up_sync(~0u, incl, 1);
+      const double before = run + (lane ? prev : 0.0);
+      const uint32_t over = __ballot_sync(~0u, m > 0.0 && run + incl > goal);
+      const uint32_t some = __ballot_sync(~0u, m > 0.0);
+      if (over) {
+        hit = i + __ffs(over) - 1;
+        hit_run = __shfl_sync(~0u, before, __ffs(over) - 1);
+      } else if (some) {
+        last = i + 31 - __clz(some);
+        last_run = __shfl_sync(~0u, before, 31 - __clz(some));
+      }
+      run += __shfl_sync(~0u, incl, 31);
+    }
+    if (hit < 0) hit = last, hit_run = last_run;  // what rounding leaves
+    if (hit % kPsWarps != warp) return -1;
+    return walk(piece(hit), c, ties_at(hit), hit_run, goal, weigh);
   }
 };
 
@@ -1607,6 +1691,8 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
   view.begin = (uint32_t)min(begin, (uint64_t)row.row_end);
   view.end = (uint32_t)min(begin + row.warp_ids, (uint64_t)row.row_end);
   view.peaks = p.peaks ? reinterpret_cast<uint16_t*>(ps_dynamic + kPsFixed) : nullptr;
+  view.list = reinterpret_cast<uint16_t*>(ps_dynamic + p.lists) + row.warp * (row.warp_ids >> 3);
+  view.listed = 0;
   view.kept = p.keep != 0;
   view.slot_bytes = ps_slot(DT, view.mask != nullptr);
   view.slots = ps_dynamic + p.slots + (view.kept ? 0 : row.warp * View::kDepth * view.slot_bytes);
@@ -1669,7 +1755,7 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
       const bool full = __all_sync(~0u, r.bits == 0xFFu);
       if (!full) expand8_16(r.bits, v[0], v[1], v[2], v[3]);
       View::narrow(r, t);
-      const uint32_t peak = View::peak(r, t, v, full, top_value);
+      const uint32_t peak = View::peak(r, v, full, top_value);
       if (view.peaks) view.peaks[(pos - view.base) >> 3] = (uint16_t)peak;
       top16 = max(top16, peak);
       if (!bins) return;
@@ -1706,8 +1792,8 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
         }
       }
     });
-    // the order code of the maximum: 0 without a valid id
-    uint32_t top = top16 ? ord32(top_value) : 0u;
+    // order code of the maximum, 0 without a valid id
+    uint32_t top = top16 == 0u ? 0u : DT == kF32 ? ord32(top_value) : View::top_code(top16);
     PsBox sum = row.reduce(mass + mass2, count, top, small);
     top = sum.top;
     if (top == 0u) status = kStatusEmptyMask;
@@ -1762,7 +1848,9 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
   const uint32_t down_to = summed ? row.summed.down_to : ~0u;
   double mass = summed ? row.summed.lane : 0.0;
   uint32_t ties = 0, before = 0;
-  view.each(row.lane, c.least(), [&](uint32_t pos, const auto& r) {
+  view.gather(row.lane, c.least());
+  if (row.lane == 0) sh.listed_by[row.warp] = view.listed;
+  view.each(row.lane, [&](uint32_t pos, const auto& r) {
     uint32_t set, tie;
     Row::split(c, r, set, tie);
     ties += __popc(tie);
@@ -1786,7 +1874,7 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
 
   if (OP == kOpProbs) {
     float* out = p.out_probs + group * p.out_stride;
-    row.each_kept(view, c, scan.my_ties, [&](int id, const auto& r, uint32_t set) {
+    row.each_kept(view, c, sh.ties_before[row.warp], [&](int id, const auto& r, uint32_t set) {
       row.each_weight(c, r, set, [&](int j, double w) { out[id + j] = (float)(w * inv); });
     });
     if (first) p.out_status[item] = 0u;
@@ -1822,7 +1910,7 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
   };
   if (OP == kOpSpec && residual) {
     double sum = 0.0;
-    row.each_kept(view, c, scan.my_ties, [&](int id, const auto& r, uint32_t set) {
+    row.each_kept(view, c, sh.ties_before[row.warp], [&](int id, const auto& r, uint32_t set) {
       row.each_weight(c, r, set, [&](int j, double w) { sum += rest(id + j, w); });
     });
     sum = warp_sum(sum);
