@@ -616,9 +616,10 @@ __device__ __forceinline__ double exp2_table(double y, const PsPowers& powers) {
   const double v = exp2_parts(t, y - (t - kPsShift), powers);
   return y > -16000.0 ? (y < 16000.0 ? v : (double)INFINITY) : 0.0;
 }
-// 2^(v scale / 16) for v scale in (-16000, 16000)
-__device__ __forceinline__ double exp2_scaled(float v, double scale, const PsPowers& powers) {
-  const double x = (double)v, t = fma(x, scale, kPsShift);
+// 2^((v - from) scale / 16) where that exponent lies within +-2^14
+__device__ __forceinline__ double exp2_from(float v, double from, double scale,
+                                            const PsPowers& powers) {
+  const double x = (double)v - from, t = fma(x, scale, kPsShift);
   return exp2_parts(t, fma(x, scale, kPsShift - t), powers);
 }
 
@@ -1087,20 +1088,41 @@ struct PolicyRow {
   __device__ __noinline__ static double sum_set(const Raw r, uint32_t set, double top,
                                                 double scale, double least, bool flat,
                                                 const PsPowers* powers, const double* bins) {
+    if (flat) return 1.0 >= least ? (double)__popc(set) : 0.0;
     double a = 0.0, b = 0.0;
-    if (__any_sync(~0u, __popc(set) > 2)) {
-#pragma unroll
-      for (int j = 0; j < 8; j += 2) {
-        const double w = weigh(View::value_of(r, j), top, scale, flat, *powers, bins);
-        const double x = weigh(View::value_of(r, j + 1), top, scale, flat, *powers, bins);
-        a += (set >> j & 1u) && w >= least ? w : 0.0;
-        b += (set >> j & 2u) && x >= least ? x : 0.0;
-      }
-    } else {
+    if (!__any_sync(~0u, __popc(set) > 2)) {
       View::each_set(set, [&](int j, bool have) {
-        const double w = weigh(View::value_at(r, j), top, scale, flat, *powers, bins);
+        const double w = weigh(View::value_at(r, j), top, scale, false, *powers, bins);
         a += have && w >= least ? w : 0.0;
       });
+      return a;
+    }
+    if (DT == kBF16 && bins) {
+      uint32_t missed = 0;  // values without a bin
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t bits = View::bits_of(r, j);
+        const uint32_t i = ((bits >> 16) & 0x7FFFu) - kPsLow;
+        const uint32_t positive = (uint32_t)((int32_t)~bits >> 31);
+        const bool has = i < (uint32_t)kPsHalf;
+        if (!has) missed |= 1u << j;
+        const double w = bins[has ? kPsHalf + (int)(i ^ positive) : 0];
+        a += (set >> j & 1u) && has && w >= least ? w : 0.0;
+      }
+      missed &= set;
+      if (__any_sync(~0u, missed))
+        View::each_set(missed, [&](int j, bool have) {
+          const double w = weigh(View::value_at(r, j), top, scale, false, *powers, nullptr);
+          b += have && w >= least ? w : 0.0;
+        });
+      return a + b;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+      const double w = exp2_table(((double)View::value_of(r, j) - top) * scale, *powers);
+      const double x = exp2_table(((double)View::value_of(r, j + 1) - top) * scale, *powers);
+      a += (set >> j & 1u) && w >= least ? w : 0.0;
+      b += (set >> j & 2u) && x >= least ? x : 0.0;
     }
     return a + b;
   }
@@ -1338,8 +1360,8 @@ struct PolicyRow {
 
   // The cut, starting from nothing but the row's maximum `top`, or from `found`, a range out of
   // the bins. `total` is the mass of all ids, or negative where it is not known.
-  __device__ __noinline__ void find_cut(RowCut& c, const RowPolicy& pol, uint32_t top,
-                                        uint32_t valid, double total, const PsRange* found) {
+  __device__ __forceinline__ void find_cut(RowCut& c, const RowPolicy& pol, uint32_t top,
+                                           uint32_t valid, double total, const PsRange* found) {
     if (!(pol.temperature > 0.0)) {
       c.keep(code_value(top), 1u);
       return;
@@ -1386,6 +1408,20 @@ struct PolicyRow {
     } else {
       cut_from_list(c, range, 0u, true, pol.top_p, total);
     }
+  }
+
+  // The same out of line, on copies: nothing of the caller's has to live in memory for it.
+  struct Outcome {
+    float cut;
+    uint32_t take;
+    int parity;
+    PsSummed summed;
+  };
+  __device__ __noinline__ static Outcome find_cut_apart(PolicyRow row, RowCut c, RowPolicy pol,
+                                                        uint32_t top, uint32_t valid,
+                                                        double total, bool have, PsRange range) {
+    row.find_cut(c, pol, top, valid, total, have ? &range : nullptr);
+    return {c.cut, c.take, row.parity, row.summed};
   }
 
   // ---- the kept mass and the draw -------------------------------------------------------
@@ -1740,12 +1776,16 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
   if (ok) {
     const bool by_mass = pol.top_p < 1.0;
     const bool bins = pol.temperature > 0.0 && (pol.top_k || by_mass);
-    // the mass of all ids, relative to a value of 0 (the maximum is not known yet)
-    const bool mass_of_all = DT != kBF16 && bins && by_mass && !pol.top_k;
+    // The mass of all ids is summed where top-p needs it and the bins do not give it, and where
+    // nothing is cut. The maximum is not known yet: it is summed relative to the value of id 0
+    // (the weights of equal values come out as 1), or to 0 if that one is far out.
+    const bool plain = pol.temperature > 0.0 && !bins && !(pol.min_p > 0.0);
+    const bool mass_of_all = plain || (DT != kBF16 && bins && by_mass && !pol.top_k);
+    const float first_value = Elem<DT>::to_f32(view.row, 0);
+    const double from = fabsf(first_value) < 512.0f ? (double)first_value : 0.0;
     const uint32_t hist = (uint32_t)__cvta_generic_to_shared(ps_hist());
-    // values below it weigh nothing on the scale of 2^(v scale / 16) (nor do they count as much
-    // as the bound's 2^-937 there)
-    const float floor_value = (float)(-15000.0 / c.scale);
+    // values below it weigh less than 2^-930 on that scale
+    const float floor_value = (float)(from - 15000.0 / c.scale);
     uint32_t count = 0, small = 0, top16 = 0;
     float top_value = -INFINITY;
     double mass = 0.0, mass2 = 0.0;
@@ -1758,6 +1798,24 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
       const uint32_t peak = View::peak(r, v, full, top_value);
       if (view.peaks) view.peaks[(pos - view.base) >> 3] = (uint16_t)peak;
       top16 = max(top16, peak);
+      if (mass_of_all) {
+        if (full) {
+#pragma unroll
+          for (int j = 0; j < 8; j += 2) {
+            const float x = View::value_of(r, j), y = View::value_of(r, j + 1);
+            const double a = exp2_from(fmaxf(x, floor_value), from, c.scale, sh.powers);
+            const double b = exp2_from(fmaxf(y, floor_value), from, c.scale, sh.powers);
+            mass += x >= floor_value ? a : 0.0;
+            mass2 += y >= floor_value ? b : 0.0;
+          }
+        } else {
+          View::each_set(r.bits, [&](int j, bool have) {
+            const float x = View::value_at(r, j);
+            const double a = exp2_from(fmaxf(x, floor_value), from, c.scale, sh.powers);
+            if (have && x >= floor_value) mass += a;
+          });
+        }
+      }
       if (!bins) return;
       count += __popc(r.bits);
       uint32_t near = 0;
@@ -1776,21 +1834,6 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
             if (have) mass += w;
           });
       }
-      if (DT != kBF16 && mass_of_all) {
-        if (full) {
-#pragma unroll
-          for (int j = 0; j < 8; j += 2) {
-            mass += exp2_scaled(fmaxf(View::value_of(r, j), floor_value), c.scale, sh.powers);
-            mass2 += exp2_scaled(fmaxf(View::value_of(r, j + 1), floor_value), c.scale, sh.powers);
-          }
-        } else {
-          View::each_set(r.bits, [&](int j, bool have) {
-            const double w =
-                exp2_scaled(fmaxf(View::value_at(r, j), floor_value), c.scale, sh.powers);
-            if (have) mass += w;
-          });
-        }
-      }
     });
     // order code of the maximum, 0 without a valid id
     uint32_t top = top16 == 0u ? 0u : DT == kF32 ? ord32(top_value) : View::top_code(top16);
@@ -1803,23 +1846,28 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
       c.top = code_value(top);
       c.flat = !(pol.temperature > 0.0) || c.top == INFINITY;
       // the masses relative to the maximum, where they did not leave the range of doubles
-      const double shift = -c.top * c.scale;
-      const bool in_range = fabs(shift) < 14400.0;
-      sum.mass = sum.mass > 0.0 ? sum.mass * exp2_table(shift, sh.powers) : 0.0;
-      const bool measured = mass_of_all && in_range && floor_value < -1e-30f;
+      const double shift = ((mass_of_all ? from : 0.0) - c.top) * c.scale;
+      const bool in_range = fabs(shift) < 14400.0 && fabs(c.top * c.scale) < 14400.0;
+      const double factor = in_range ? exp2_table(shift, sh.powers) : 0.0;
+      sum.mass = sum.mass > 0.0 ? sum.mass * factor : 0.0;
+      const bool measured = mass_of_all && in_range && (double)floor_value < from - 1e-30;
       const double total = measured ? sum.mass : -1.0;
       if (!bins) {
         if (pol.temperature > 0.0) c.cut = c.flat ? FLT_MAX : -INFINITY;
         else c.keep(code_value(top), 1u);
+        if (plain && measured && !c.flat) row.summed = {(mass + mass2) * factor, sum.mass, 0u};
       } else {
-        PsRange range;
+        PsRange range = {};
         auto found = Row::kNothing;
         if (in_range && (measured || !mass_of_all))
           found = row.find_cut_in_bins(c, pol, sum, range);
         if (found != Row::kFound) {
           __syncthreads();  // what the scans left in shared memory has been read
-          row.find_cut(c, pol, top, sum.count, total,
-                       found == Row::kRange ? &range : nullptr);
+          const auto o = Row::find_cut_apart(row, c, pol, top, sum.count, total,
+                                             found == Row::kRange, range);
+          c.keep(o.cut, o.take);
+          row.parity = o.parity;
+          row.summed = o.summed;
         }
       }
       c.bound_by_min_p();
@@ -1848,9 +1896,10 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
   const uint32_t down_to = summed ? row.summed.down_to : ~0u;
   double mass = summed ? row.summed.lane : 0.0;
   uint32_t ties = 0, before = 0;
+  if (c.cut == -INFINITY) view.peaks = nullptr;  // nothing is cut: every vector
   view.gather(row.lane, c.least());
   if (row.lane == 0) sh.listed_by[row.warp] = view.listed;
-  view.each(row.lane, [&](uint32_t pos, const auto& r) {
+  if (down_to != 0u) view.each(row.lane, [&](uint32_t pos, const auto& r) {
     uint32_t set, tie;
     Row::split(c, r, set, tie);
     ties += __popc(tie);
