@@ -187,7 +187,7 @@ struct PsScan {  // of the entries of all warps
 
 struct PsShared {
   PsBox box[2][kPsMaxCluster];  // used alternately: one may still be read as the next is written
-  double part_mass[kPsWarps], part_high[kPsWarps];
+  double part_mass[kPsWarps];
   uint32_t part_count[kPsWarps], part_top[kPsWarps], part_small[kPsWarps];
   // one entry per warp of the cluster, in id order; the second set holds what max(p - q, 0)
   // leaves
@@ -200,7 +200,8 @@ struct PsShared {
   int listed_by[kPsWarps];  // vectors that each warp gathered for the passes after the cut
   PsScan scan[2];
   uint32_t ties_before[kPsWarps];
-  double sums_before[2][kPsWarps + 1];
+  double sums_before[kPsWarps + 1];
+  uint32_t sample[2][4];
 };
 
 // Dynamic shared memory: the CTA's histogram and the cluster's; their 32 KB are used again for a
@@ -463,17 +464,6 @@ struct RowView {
     while (__any_sync(~0u, set)) {
       f(set ? __ffs(set) - 1 : 0, set != 0u);
       set &= set - 1u;
-    }
-  }
-
-  // the 8 values cut to bfloat16 width, two to a word
-  __device__ __forceinline__ static void narrow(const Raw& r, uint32_t (&t)[4]) {
-    if constexpr (DT == kBF16) {
-      t[0] = r.a.x, t[1] = r.a.y, t[2] = r.a.z, t[3] = r.a.w;
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        t[i] = __byte_perm(bits_of(r, 2 * i), bits_of(r, 2 * i + 1), 0x7632);
     }
   }
 
@@ -740,50 +730,34 @@ struct PolicyRow {
   // are read by every thread, so a __syncthreads() has to lie between two calls.
   struct Scanned {
     uint32_t count_before, count_all;
-    double high_before, high_end, high_all, low_before, low_end, low_all;
+    double mass_before, mass_end, mass_all;
   };
-  __device__ Scanned scan_parts(uint32_t count, double high, double low, bool masses,
-                                bool two) {
+  __device__ Scanned scan_parts(uint32_t count, double mass, bool masses) {
     Scanned s = {};
     const uint32_t count_incl = warp_scan(count, lane);
-    double high_incl = 0.0, low_incl = 0.0;
-    if (masses) high_incl = warp_scan(high, lane);
-    if (two) low_incl = warp_scan(low, lane);
-    if (lane == 31) {
-      sh.part_count[warp] = count_incl;
-      sh.part_mass[warp] = high_incl;
-      sh.part_high[warp] = low_incl;
-    }
+    const double incl = masses ? warp_scan(mass, lane) : 0.0;
+    if (lane == 31) sh.part_count[warp] = count_incl, sh.part_mass[warp] = incl;
     __syncthreads();
     const uint32_t c = lane < kPsWarps ? sh.part_count[lane] : 0u;
     const uint32_t c_incl = warp_scan(c, lane);
     s.count_all = __shfl_sync(~0u, c_incl, 31);
     s.count_before = __shfl_sync(~0u, c_incl - c, warp) + count_incl - count;
     if (!masses) return s;
-    if (warp < (two ? 2 : 1)) {  // in order, so that the parts join
-      const double* part = warp ? sh.part_high : sh.part_mass;
+    if (warp == 0) {  // in order, so that the parts join
       double run = 0.0;
 #pragma unroll
       for (int i = 0; i < kPsWarps; ++i) {
-        const double x = part[i];
-        if (lane == i) sh.sums_before[warp][i] = run;
+        const double x = sh.part_mass[i];
+        if (lane == i) sh.sums_before[i] = run;
         run += x;
       }
-      if (lane == 0) sh.sums_before[warp][kPsWarps] = run;
+      if (lane == 0) sh.sums_before[kPsWarps] = run;
     }
     __syncthreads();
-    const double prev = __shfl_up_sync(~0u, high_incl, 1);
-    const double mine = sh.sums_before[0][warp];
-    s.high_all = sh.sums_before[0][kPsWarps];
-    s.high_before = lane ? mine + prev : mine;
-    s.high_end = mine + high_incl;
-    if (two) {
-      const double prev_low = __shfl_up_sync(~0u, low_incl, 1);
-      const double mine_low = sh.sums_before[1][warp];
-      s.low_all = sh.sums_before[1][kPsWarps];
-      s.low_before = lane ? mine_low + prev_low : mine_low;
-      s.low_end = mine_low + low_incl;
-    }
+    const double prev = __shfl_up_sync(~0u, incl, 1), mine = sh.sums_before[warp];
+    s.mass_all = sh.sums_before[kPsWarps];
+    s.mass_before = lane ? mine + prev : mine;
+    s.mass_end = mine + incl;
     return s;
   }
 
@@ -823,25 +797,20 @@ struct PolicyRow {
     for (int j = 0; j < kPsOwn; ++j) n[j] = turned ? t[kPsOwn - 1 - j] : t[j];
   }
 
-  // ---- the cut from the histogram of values ---------------------------------------------
-  __device__ __forceinline__ static uint32_t bin_bits(int bin) {  // of |v|, bfloat16
+  // ---- bfloat16: the cut from a histogram with a bin for every value --------------------
+  __device__ __forceinline__ static uint32_t bin_bits(int bin) {  // of |v|
     return bin < kPsHalf ? kPsLow + (kPsHalf - 1 - bin) : kPsLow + (bin - kPsHalf);
   }
-  // the bin's value nearest to zero (bfloat16: its only one)
   __device__ __forceinline__ static float bin_value(int bin) {
     return __uint_as_float((bin_bits(bin) | (bin < kPsHalf ? 0u : 0x8000u)) << 16);
   }
-  __device__ __forceinline__ static uint32_t bin_low_code(int bin) {
-    const uint32_t code = ord32(bin_value(bin));
-    return bin < kPsHalf ? code : code - 0xFFFFu;
-  }
 
-  // Counts the bins of two values, the bfloat16 halves of `u`, where `valid` has ones; returns
-  // bit 15 and bit 31 set for those next to zero. In memory the bins of either sign lie by
-  // rising magnitude, negative ones behind. With the sign bit set no half borrows from the
-  // other; the bin is right where bits 11 to 14 come out as zeros.
-  __device__ __forceinline__ static uint32_t count_bins(uint32_t hist, uint32_t u,
-                                                        uint32_t valid) {
+  // Counts the bins of two values, the halves of `u`, where `valid` has ones; returns bit 15
+  // and bit 31 set for those next to zero. In memory the bins of either sign lie by rising
+  // magnitude, negative ones behind. With the sign bit set no half borrows from the other; the
+  // bin is right where bits 11 to 14 come out as zeros.
+  __device__ __forceinline__ static uint32_t count_values(uint32_t hist, uint32_t u,
+                                                          uint32_t valid) {
     const uint32_t t = (u | 0x80008000u) - kPsLow * 0x10001u;
     const uint32_t bad = (t & 0x78007800u) | ~valid;
     const uint32_t at = ((t & 0x07FF07FFu) | ((u >> 4) & 0x08000800u)) << 2;
@@ -856,183 +825,272 @@ struct PolicyRow {
     return ~t & 0x80008000u & valid;
   }
 
-  enum Found { kFound, kRange, kNothing };
-
-  // Looks for the cut in the bins. kFound: c has it. kRange: `range` holds it, and with top-k
-  // and top-p both also the k-th value. kNothing: the bins do not decide it. `sum` has the
-  // count of the valid ids, of those next to zero (bfloat16: and their mass; other types: the
-  // mass of all).
-  __device__ Found find_cut_in_bins(RowCut& c, const RowPolicy& pol, const PsBox& sum,
-                                    PsRange& range) {
-    constexpr bool kExact = DT == kBF16;  // a bin is one value
+  // Sets the cut and makes the table of weights; false where the bins do not decide it. `sum`
+  // has the count of the valid ids, and the count and mass of those next to zero.
+  __device__ bool cut_by_values(RowCut& c, const RowPolicy& pol, const PsBox& sum) {
     uint32_t n[kPsOwn];
     merge_bins(n, true);
-    if (c.flat || !(c.top < kPsLarge)) return kNothing;
+    if (c.flat || !(c.top < kPsLarge)) return false;
     const int mine = threadIdx.x * kPsOwn;  // this thread's bins, in falling order of value
     const bool by_mass = pol.top_p < 1.0;
-    // Bounds of the weights: of a bin's largest and smallest value. The values of 8 bins are
-    // equally spaced, their weights a geometric series; the series starts at the row's maximum
-    // in the bins that hold it (those above are empty).
-    double high[kPsOwn], low[kPsOwn], mass_high = 0.0, mass_low = 0.0;
+    // The mass of a bin is count times weight. The values of 8 bins are equally spaced, their
+    // weights a geometric series, which starts at the row's maximum in the bins that hold it
+    // (those above are empty).
+    double weight_of[kPsOwn], mass = 0.0;
     uint32_t count = 0;
 #pragma unroll
     for (int j = 0; j < kPsOwn; ++j) count += n[j];
     if (by_mass) {
       const float step = __uint_as_float(bin_bits(mine) << 16 & 0x7F800000u) * 0x1p-7f;
       const double ratio = exp2_table(-(double)step * c.scale, *c.powers);
-      const float start = kExact || mine >= kPsHalf ? bin_value(mine) : bin_value(mine) + step;
+      float from = bin_value(mine);
       int at = 0;
-      double w;
-      if ((double)start > c.top && count) {
+      if ((double)from > c.top) {
 #pragma unroll
         for (int j = kPsOwn - 1; j >= 0; --j)
           if (n[j]) at = j;
-        const float v = bin_value(mine + at);
-        const float lowest = mine < kPsHalf ? v : v - step;
-        w = kExact ? 1.0 : c.weight(lowest);
-      } else {
-        w = c.weight(start);
-        if ((double)start > c.top) w = 0.0;  // all empty
+        from = count ? bin_value(mine + at) : -INFINITY;
       }
-      const bool top_here = (double)start > c.top && !kExact;
+      double w = c.weight(from);
 #pragma unroll
       for (int j = 0; j < kPsOwn; ++j) {
-        high[j] = low[j] = 0.0;
-        if (j >= at) {
-          if (kExact) {
-            high[j] = low[j] = w;
-            w *= ratio;
-          } else if (top_here && j == at) {
-            high[j] = 1.0;
-            low[j] = w;
-          } else {
-            high[j] = w;
-            w *= ratio;
-            low[j] = w;
-          }
-        }
-        mass_high += (double)n[j] * high[j];
-        if (!kExact) mass_low += (double)n[j] * low[j];
+        weight_of[j] = j >= at ? w : 0.0;
+        if (j >= at) w *= ratio;
+        mass += (double)n[j] * weight_of[j];
       }
     }
-    if (threadIdx.x < 3) sh.cross[threadIdx.x].bin = -1;
-    const Scanned scan = scan_parts(count, mass_high, mass_low, by_mass, by_mass && !kExact);
+    if (threadIdx.x < 2) sh.cross[threadIdx.x].bin = -1;
+    const Scanned scan = scan_parts(count, mass, by_mass);
     uint32_t count_before = scan.count_before;
-    double high_before = scan.high_before, high_end = scan.high_end;
-    double low_before = scan.low_before, low_end = scan.low_end;
-    // the values next to zero, between the halves
-    const double small_high = kExact ? sum.mass : (double)sum.small * fmin(1.0, c.weight(kPsSmall));
-    const double small_low = kExact ? sum.mass : (double)sum.small * c.weight(-kPsSmall);
-    if (mine >= kPsHalf) {
+    double mass_before = scan.mass_before, mass_end = scan.mass_end;
+    if (mine >= kPsHalf) {  // the values next to zero lie between the halves
       count_before += sum.small;
-      high_before += small_high, high_end += small_high;
-      low_before += small_low, low_end += small_low;
+      mass_before += sum.mass, mass_end += sum.mass;
     }
-    if (kExact) low_before = high_before, low_end = high_end;
     const uint32_t in_bins = scan.count_all + sum.small;
     // ids at and below -2^7 lie behind the bins; they may weigh nothing next to the rest
-    const uint32_t behind = sum.count - in_bins;
-    const bool behind_weighs = behind && c.weight(-kPsLarge) > 0x1p-80;
+    const bool behind_weighs = sum.count > in_bins && c.weight(-kPsLarge) > 0x1p-80;
 
-    const double slack = kExact ? 0.0 : 1e-12;
+    int cut_bin = kPsBins;
+    uint32_t take = 0;
+    double total = scan.mass_all + sum.mass;
     const bool by_k = pol.top_k && pol.top_k < sum.count;
-    int k_bin = kPsBins;
-    double total = kExact ? scan.high_all + sum.mass : sum.mass;
-    uint32_t k_count = 0;  // ids up to and with that bin
-    uint32_t k_take = 0;
     if (by_k) {
-      if (pol.top_k > in_bins) return kNothing;
+      if (pol.top_k > in_bins) return false;
       if (count_before < pol.top_k && pol.top_k <= count_before + count) {
-        PsCross x = {low_before, count_before, 0u, -1};
+        PsCross x = {mass_before, count_before, 0u, -1};
 #pragma unroll
         for (int j = 0; j < kPsOwn; ++j)
           if (x.bin < 0) {
             if (pol.top_k <= x.count + n[j]) {
               x.bin = mine + j;
-              x.n = n[j];
-              if (by_mass) x.mass += (double)(pol.top_k - x.count) * low[j];
+              x.n = pol.top_k - x.count;
+              if (by_mass) x.mass += (double)x.n * weight_of[j];
             } else {
               x.count += n[j];
-              if (by_mass) x.mass += (double)n[j] * low[j];
+              if (by_mass) x.mass += (double)n[j] * weight_of[j];
             }
           }
         sh.cross[0] = x;
       }
       __syncthreads();
       const PsCross x = sh.cross[0];
-      if (x.bin < 0) return kNothing;  // among the values next to zero
-      k_bin = x.bin;
+      if (x.bin < 0) return false;  // among the values next to zero
+      cut_bin = x.bin;
+      take = x.n;
       total = x.mass;
-      k_count = x.count + x.n;
-      k_take = pol.top_k - x.count;
-      if (!by_mass) {
-        range = {bin_low_code(k_bin) + 0xFFFFu, bin_low_code(k_bin), x.count, x.n};
-        if (kExact) c.keep(bin_value(k_bin), k_take);
-      }
     }
     if (by_mass) {
-      if (!by_k && behind_weighs) return kNothing;
+      if (!by_k && behind_weighs) return false;
       const double goal = top_p_goal(pol.top_p, total);
-      // the first bin in which the mass can reach the goal ...
-      const double least = goal * (1.0 - slack);
-      if (count && mine <= k_bin && high_before < least &&
-          (least <= high_end || k_bin < mine + kPsOwn)) {
-        PsCross x = {high_before, count_before, 0u, -1};
-        double run = high_before, weight = 0.0;
-        uint32_t run_count = count_before;
+      if (count && mine <= cut_bin && mass_before < goal &&
+          (goal <= mass_end || cut_bin < mine + kPsOwn)) {
+        PsCross x = {mass_before, 0u, 0u, -1};  // the bin that reaches the goal, else the last
+        double run = mass_before, weight = 0.0;
 #pragma unroll
         for (int j = 0; j < kPsOwn; ++j)
-          if (n[j] && mine + j <= k_bin && run < least) {
-            x = {run, run_count, kExact && mine + j == k_bin ? k_take : n[j], mine + j};
-            weight = high[j];
-            run += (double)x.n * high[j];
-            run_count += n[j];
+          if (n[j] && mine + j <= cut_bin && run < goal) {
+            x = {run, 0u, by_k && mine + j == cut_bin ? take : n[j], mine + j};
+            weight = weight_of[j];
+            run += (double)x.n * weight;
           }
-        if (kExact) x.n = ties_to_reach(goal - x.mass, weight, x.n, x.mass, goal);
+        x.n = ties_to_reach(goal - x.mass, weight, x.n, x.mass, goal);
         sh.cross[1] = x;
       }
-      // ... and the first in which it must have
-      const double most = goal * (1.0 + slack);
-      if (!kExact && !by_k && count && low_before < most && most <= low_end) {
-        PsCross x = {0.0, count_before, 0u, -1};
-        double run = low_before;
+      __syncthreads();
+      const PsCross x = sh.cross[1];
+      if (x.bin < 0) return false;  // among the values next to zero
+      cut_bin = x.bin;
+      take = x.n;
+    }
+    if (cut_bin < kPsBins) c.keep(bin_value(cut_bin), take);
+    // the weights of the kept bins, for the passes that follow
+    __syncthreads();  // the counts have been read
+    double* weights = ps_table();
+#pragma unroll
+    for (int j = 0; j < kPsOwn; ++j)
+      if (n[j] && mine + j <= cut_bin)
+        weights[mine + j] = by_mass ? weight_of[j] : c.weight(bin_value(mine + j));
+    table = weights;
+    __syncthreads();
+    return true;
+  }
+
+  // ---- other types: the few bins that hold the cut ---------------------------------------
+  // Bins of equal width, 1/32 in the exponent of the weights, from 80 above the largest of a
+  // sample of the row's values to 48 below it, in falling order of value.
+  struct Linear {
+    float scale, shift;  // bin = round(shift - v scale) - 2^23
+    bool ok;
+  };
+  static constexpr float kBinsPerE = 32.0f, kBinsAbove = 2560.0f, kTwo23 = 8388608.0f;
+
+  __device__ __forceinline__ static uint32_t bin_of(const Linear& lin, float v) {
+    return __float_as_uint(fmaf(v, -lin.scale, lin.shift)) - 0x4B000000u;
+  }
+  __device__ __forceinline__ static void count_linear(uint32_t hist, const Linear& lin, float v,
+                                                      bool valid) {
+    const uint32_t bin = valid ? bin_of(lin, v) : ~0u;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.lt.u32 p, %1, %2;\n\t@p red.shared.add.u32 [%0], 1;\n\t}" ::"r"(
+            hist + (bin << 2)),
+        "r"(bin), "n"(kPsBins)
+        : "memory");
+  }
+  // Order code of the largest value whose bin is `bin` or a lower one (in value); 0 if that is
+  // not found within a few steps from where it should be.
+  __device__ __forceinline__ static uint32_t top_of_bin(const Linear& lin, int bin) {
+    auto reaches = [&](float x) {  // not NaN; bins past either end compare by the rounded value
+      return fmaf(x, -lin.scale, lin.shift) >= kTwo23 + (float)bin;
+    };
+    float x = (float)(((double)lin.shift - (double)kTwo23 - (double)bin + 0.5) / (double)lin.scale);
+    int steps = 0;
+    while (!reaches(x) && ++steps < 16) x = nextafterf(x, -INFINITY);
+    while (reaches(nextafterf(x, INFINITY)) && ++steps < 16) x = nextafterf(x, INFINITY);
+    return steps < 16 && x > -FLT_MAX && x < FLT_MAX ? ord32(x) : 0u;
+  }
+
+  // The bins for this row, and the value that its masses are relative to: the largest of 128
+  // samples, of the valid ones if there are any.
+  __device__ Linear sample_bins(float scale, double& from) {
+    if (warp < 4) {
+      const int id = (int)((int64_t)threadIdx.x * view.vocab >> 7);
+      const float v = Elem<DT>::to_f32(view.row, id);
+      const bool finite = fabsf(v) <= FLT_MAX;
+      const bool valid = !view.mask || (view.mask[id >> 5] >> (id & 31) & 1u);
+      const uint32_t any = __reduce_max_sync(~0u, finite ? ord32(v) : 0u);
+      const uint32_t best = __reduce_max_sync(~0u, finite && valid ? ord32(v) : 0u);
+      if (lane == 0) sh.sample[0][warp] = any, sh.sample[1][warp] = best;
+    }
+    __syncthreads();
+    uint32_t any = 0, best = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) any = max(any, sh.sample[0][i]), best = max(best, sh.sample[1][i]);
+    const uint32_t code = best ? best : any;
+    const float middle = code ? code_value(code) : 0.0f;
+    from = middle;
+    const bool ok = scale < 1e30f && fabsf(middle * scale) < 1e30f;
+    return {scale, fmaf(middle, scale, kTwo23 + kBinsAbove), ok};
+  }
+
+  // The range of codes that holds the cut, with top-k and top-p both also the k-th value; false
+  // where the bins do not tell. `total` is the mass of all ids, if top-p needs it.
+  __device__ bool range_by_bins(const RowCut& c, const RowPolicy& pol, const PsBox& sum,
+                                const Linear& lin, double total, PsRange& range) {
+    uint32_t n[kPsOwn];
+    merge_bins(n, false);
+    if (c.flat || !lin.ok || bin_of(lin, (float)c.top) >= (uint32_t)kPsBins) return false;
+    const int mine = threadIdx.x * kPsOwn;
+    const bool by_mass = pol.top_p < 1.0, by_k = pol.top_k && pol.top_k < sum.count;
+    // A bin's mass is its count times the weight of its middle, within 1/64 of it: the cut lies
+    // between the bins in which that mass reaches the goal less 1/60 and plus 1/60 of it (with
+    // top-k the goal itself is as far off, so twice that).
+    double mass = 0.0, weight_of[kPsOwn];
+    uint32_t count = 0;
+#pragma unroll
+    for (int j = 0; j < kPsOwn; ++j) count += n[j];
+    if (by_mass) {
+      const double middle =
+          ((double)lin.shift - (double)kTwo23 - (double)mine) / (double)lin.scale;
+      const double ratio = exp2_table(-c.scale / (double)lin.scale, *c.powers);
+      double w = exp2_table((middle - c.top) * c.scale, *c.powers);
+#pragma unroll
+      for (int j = 0; j < kPsOwn; ++j) {
+        weight_of[j] = w;
+        mass += (double)n[j] * w;
+        w *= ratio;
+      }
+    }
+    if (threadIdx.x < 3) sh.cross[threadIdx.x].bin = -1;
+    const Scanned scan = scan_parts(count, mass, by_mass);
+    uint32_t through = 0;  // ids up to and with the last bin of the range
+    int last = 0;
+    if (by_k) {
+      if (pol.top_k > scan.count_all) return false;
+      if (scan.count_before < pol.top_k && pol.top_k <= scan.count_before + count) {
+        PsCross x = {scan.mass_before, scan.count_before, 0u, -1};
+#pragma unroll
+        for (int j = 0; j < kPsOwn; ++j)
+          if (x.bin < 0) {
+            if (pol.top_k <= x.count + n[j]) {
+              x.bin = mine + j;
+              x.n = n[j];
+              if (by_mass) x.mass += (double)(pol.top_k - x.count) * weight_of[j];
+            } else {
+              x.count += n[j];
+              if (by_mass) x.mass += (double)n[j] * weight_of[j];
+            }
+          }
+        sh.cross[0] = x;
+      }
+      __syncthreads();
+      const PsCross x = sh.cross[0];
+      through = x.count + x.n;
+      last = x.bin;
+      total = x.mass;
+      if (!by_mass) range = {top_of_bin(lin, x.bin), 0u, x.count, x.n};
+    }
+    if (by_mass) {
+      const double goal = top_p_goal(pol.top_p, total);
+      const double least = goal * (by_k ? 1.0 - 2.0 / 60.0 : 1.0 - 1.0 / 60.0);
+      if (count && scan.mass_before < least && least <= scan.mass_end) {
+        PsCross x = {scan.mass_before, scan.count_before, 0u, -1};
+        double run = scan.mass_before;
+        uint32_t run_count = scan.count_before;
+#pragma unroll
+        for (int j = 0; j < kPsOwn; ++j)
+          if (n[j] && run < least) {
+            x = {run, run_count, n[j], mine + j};
+            run += (double)n[j] * weight_of[j];
+            run_count += n[j];
+          }
+        sh.cross[1] = x;
+      }
+      const double most = goal * (1.0 + 1.0 / 60.0);
+      if (!by_k && count && scan.mass_before < most && most <= scan.mass_end) {
+        PsCross x = {0.0, scan.count_before, 0u, -1};
+        double run = scan.mass_before;
 #pragma unroll
         for (int j = 0; j < kPsOwn; ++j)
           if (n[j] && run < most) {
-            run += (double)n[j] * low[j];
+            run += (double)n[j] * weight_of[j];
             x.count += n[j];
             x.bin = mine + j;
           }
         sh.cross[2] = x;
       }
       __syncthreads();
-      const PsCross x = sh.cross[1];
-      if (x.bin < 0) return kNothing;  // among the values next to zero
-      if (kExact) {
-        c.keep(bin_value(x.bin), x.n);
-      } else {
-        const uint32_t hi = bin_low_code(x.bin) + 0xFFFFu;
-        if (by_k) {
-          range = {hi, bin_low_code(k_bin), x.count, k_count - x.count};
-        } else {
-          PsCross y = sh.cross[2];
-          if (y.bin < 0) y.bin = kPsBins - 1, y.count = in_bins;
-          range = {hi, bin_low_code(y.bin), x.count, y.count - x.count};
-        }
+      const PsCross x = sh.cross[1], y = sh.cross[2];
+      if (x.bin < 0) return false;
+      if (!by_k) {
+        last = y.bin < 0 ? kPsBins - 1 : y.bin;
+        through = y.bin < 0 ? scan.count_all : y.count;
       }
+      range = {top_of_bin(lin, x.bin), 0u, x.count, through - x.count};
     }
-    if (!kExact) return kRange;
-    // the weights of the kept bins, for the passes that follow
-    __syncthreads();  // the counts have been read
-    const float cut = c.cut;
-    double* weights = ps_table();
-#pragma unroll
-    for (int j = 0; j < kPsOwn; ++j)
-      if (n[j] && bin_value(mine + j) >= cut)
-        weights[mine + j] = by_mass ? high[j] : c.weight(bin_value(mine + j));
-    table = weights;
-    __syncthreads();
-    return kFound;
+    const uint32_t below = top_of_bin(lin, last + 1);
+    range.lo = below + 1u;
+    return range.hi && below && range.lo <= range.hi;
   }
 
   // Least number of ids of weight `w`, 1 to `most`, whose mass on top of `above` reaches `goal`.
@@ -1194,8 +1252,8 @@ struct PolicyRow {
         mass_low += (double)n[j] * low[j];
       }
     }
-    if (threadIdx.x < 3) sh.cross[threadIdx.x].bin = -1;
-    const Scanned scan = scan_parts(count, mass_high, mass_low, !rank_k, !rank_k);
+    if (threadIdx.x < 2) sh.cross[threadIdx.x].bin = -1;
+    const Scanned scan = scan_parts(count, mass_high, !rank_k);
     const uint32_t before = range.above + scan.count_before;
     PsCross first = {}, last = {};
     if (rank_k) {
@@ -1213,8 +1271,10 @@ struct PolicyRow {
       first = last = sh.cross[0];
       last.count += last.n;
     } else {
-      const double high_end = above + scan.high_end, hb = above + scan.high_before;
-      const double low_end = above + scan.low_end, lb = above + scan.low_before;
+      __syncthreads();
+      const Scanned scan2 = scan_parts(0u, mass_low, true);
+      const double hb = above + scan.mass_before, high_end = above + scan.mass_end;
+      const double lb = above + scan2.mass_before, low_end = above + scan2.mass_end;
       const double least = goal * (1.0 - 1e-12), most = goal * (1.0 + 1e-12);
       if (count && hb < least && least <= high_end) {
         PsCross x = {0.0, before, 0u, -1};
@@ -1267,7 +1327,8 @@ struct PolicyRow {
   // Lists the ids of the range (at most kPsList), sorted by value falling, and sets the cut:
   // at rank `rank_k` (0: no bound), and with by_mass where the mass reaches top_p of `total`
   // (with rank_k: of the mass of those ranks).
-  __device__ void cut_from_list(RowCut& c, const PsRange& range, uint32_t rank_k, bool by_mass,
+  // False where the goal lies above the range or below it.
+  __device__ bool cut_from_list(RowCut& c, const PsRange& range, uint32_t rank_k, bool by_mass,
                                 double top_p, double total) {
     if (threadIdx.x == 0) sh.list_fill = 0u;
     __syncthreads();
@@ -1324,19 +1385,17 @@ struct PolicyRow {
     // two keys to a thread
     const uint32_t at = 2u * threadIdx.x;
     const uint32_t have = rank_k ? min(n, rank_k - range.above) : n;
-    if (have == 0u) {  // rounding put the goal past every id: all that was kept stays
-      publish();
-      return;
-    }
     uint32_t pos = have - 1u;
+    bool holds = have > 0u;
     if (by_mass) {
       const double w0 = at < have ? c.weight(code_value(~(uint32_t)(sorted[at] >> 32))) : 0.0;
       const double w1 =
           at + 1u < have ? c.weight(code_value(~(uint32_t)(sorted[at + 1u] >> 32))) : 0.0;
-      const Scanned scan = scan_parts(0u, w0 + w1, 0.0, true, false);
-      const double end = scan.high_end, before = scan.high_before;
-      if (rank_k) total = above + scan.high_all;
+      const Scanned scan = scan_parts(0u, w0 + w1, true);
+      const double end = scan.mass_end, before = scan.mass_before;
+      if (rank_k) total = above + scan.mass_all;
       const double goal = top_p_goal(top_p, total);
+      holds = holds && above < goal && (rank_k || above + scan.mass_all >= goal);
       uint32_t mine = have - 1u;
       if (at < have && above + before + w0 >= goal) mine = at;
       else if (at + 1u < have && above + end >= goal) mine = at + 1u;
@@ -1345,17 +1404,18 @@ struct PolicyRow {
       __syncthreads();
       for (int i = 0; i < kPsWarps; ++i) pos = min(pos, sh.part_top[i]);
     }
-    const uint32_t code = ~(uint32_t)(sorted[pos] >> 32);
+    const uint32_t code = ~(uint32_t)(sorted[holds ? pos : 0u] >> 32);
     uint32_t same = 0;
-    if (at <= pos) same += ~(uint32_t)(sorted[at] >> 32) == code;
-    if (at + 1u <= pos) same += ~(uint32_t)(sorted[at + 1u] >> 32) == code;
+    if (holds && at <= pos) same += ~(uint32_t)(sorted[at] >> 32) == code;
+    if (holds && at + 1u <= pos) same += ~(uint32_t)(sorted[at + 1u] >> 32) == code;
     same = __reduce_add_sync(~0u, same);
     if (lane == 0) sh.part_small[warp] = same;
     __syncthreads();
     uint32_t take = 0;
     for (int i = 0; i < kPsWarps; ++i) take += sh.part_small[i];
-    c.keep(code_value(code), take);
+    if (holds) c.keep(code_value(code), take);
     publish();
+    return holds;
   }
 
   // The cut, starting from nothing but the row's maximum `top`, or from `found`, a range out of
@@ -1373,8 +1433,8 @@ struct PolicyRow {
     const bool by_k = pol.top_k && pol.top_k < valid;
     if (!by_k && !by_mass) return;
     if (found && found->inside <= kPsList) {
-      cut_from_list(c, *found, by_k ? pol.top_k : 0u, by_mass, pol.top_p, total);
-      return;
+      if (cut_from_list(c, *found, by_k ? pol.top_k : 0u, by_mass, pol.top_p, total)) return;
+      summed = {0.0, 0.0, ~0u};  // the range may have lain too low
     }
     if (by_k) {
       if (found && !by_mass) range = *found;
@@ -1393,20 +1453,28 @@ struct PolicyRow {
       range = {top, ord32(c.cut) + 1u, 0u, b.count};
     } else {
       if (total < 0.0) total = at_least(c, range.lo).mass;
-      if (found) range = *found;
     }
     const double goal = top_p_goal(pol.top_p, total);
-    while (range.inside > kPsList && range.hi != range.lo) {
-      const uint32_t width = range.hi - range.lo;
-      refine(c, range, 0u, goal);
-      if (range.hi - range.lo > width / 4u) bisect(c, range, goal);
-    }
-    if (range.hi == range.lo) {
-      const double above = at_least(c, range.hi + 1u).mass;
-      const double w = c.weight(code_value(range.hi));
-      c.keep(code_value(range.hi), ties_to_reach(goal - above, w, range.inside, above, goal));
-    } else {
-      cut_from_list(c, range, 0u, true, pol.top_p, total);
+    const PsRange all = range;
+    for (bool guess = found && !by_k;; guess = false) {
+      range = guess ? *found : all;
+      while (range.inside > kPsList && range.hi != range.lo) {
+        const uint32_t width = range.hi - range.lo;
+        refine(c, range, 0u, goal);
+        if (range.hi - range.lo > width / 4u) bisect(c, range, goal);
+      }
+      if (range.hi == range.lo) {
+        const double above = at_least(c, range.hi + 1u).mass;
+        const double w = c.weight(code_value(range.hi));
+        if (!guess || (above < goal && above + (double)range.inside * w >= goal)) {
+          c.keep(code_value(range.hi), ties_to_reach(goal - above, w, range.inside, above, goal));
+          return;
+        }
+      } else if (cut_from_list(c, range, 0u, true, pol.top_p, total)) {
+        return;
+      }
+      if (!guess) return;  // rounding put the goal past every id: all that was kept stays
+      summed = {0.0, 0.0, ~0u};
     }
   }
 
@@ -1777,12 +1845,18 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
     const bool by_mass = pol.top_p < 1.0;
     const bool bins = pol.temperature > 0.0 && (pol.top_k || by_mass);
     // The mass of all ids is summed where top-p needs it and the bins do not give it, and where
-    // nothing is cut. The maximum is not known yet: it is summed relative to the value of id 0
-    // (the weights of equal values come out as 1), or to 0 if that one is far out.
+    // nothing is cut. The maximum is not known yet: it is summed relative to one of the row's
+    // values (the weights of equal values come out as 1).
     const bool plain = pol.temperature > 0.0 && !bins && !(pol.min_p > 0.0);
     const bool mass_of_all = plain || (DT != kBF16 && bins && by_mass && !pol.top_k);
-    const float first_value = Elem<DT>::to_f32(view.row, 0);
-    const double from = fabsf(first_value) < 512.0f ? (double)first_value : 0.0;
+    typename Row::Linear lin = {};
+    double from = 0.0;
+    if (DT != kBF16) {
+      lin = row.sample_bins((float)(c.inv_t * Row::kBinsPerE), from);
+    } else if (plain) {
+      const float x = Elem<DT>::to_f32(view.row, 0);
+      if (fabsf(x) < 512.0f) from = x;
+    }
     const uint32_t hist = (uint32_t)__cvta_generic_to_shared(ps_hist());
     // values below it weigh less than 2^-930 on that scale
     const float floor_value = (float)(from - 15000.0 / c.scale);
@@ -1790,11 +1864,9 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
     float top_value = -INFINITY;
     double mass = 0.0, mass2 = 0.0;
     view.stream(row.lane, [&](uint32_t pos, const auto& r) {
-      // the values to bfloat16 width, two to a word, and masks of the valid ones
-      uint32_t v[4] = {~0u, ~0u, ~0u, ~0u}, t[4];
       const bool full = __all_sync(~0u, r.bits == 0xFFu);
-      if (!full) expand8_16(r.bits, v[0], v[1], v[2], v[3]);
-      View::narrow(r, t);
+      uint32_t v[4] = {~0u, ~0u, ~0u, ~0u};  // masks of the valid ones, 16 bits each
+      if (DT != kF32 && !full) expand8_16(r.bits, v[0], v[1], v[2], v[3]);
       const uint32_t peak = View::peak(r, v, full, top_value);
       if (view.peaks) view.peaks[(pos - view.base) >> 3] = (uint16_t)peak;
       top16 = max(top16, peak);
@@ -1818,21 +1890,28 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
       }
       if (!bins) return;
       count += __popc(r.bits);
-      uint32_t near = 0;
+      if constexpr (DT == kBF16) {
+        const uint32_t near = Row::count_values(hist, r.a.x, v[0]) |
+                              Row::count_values(hist, r.a.y, v[1]) |
+                              Row::count_values(hist, r.a.z, v[2]) |
+                              Row::count_values(hist, r.a.w, v[3]);
+        if (__any_sync(~0u, near)) {
+          uint32_t set = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) near |= Row::count_bins(hist, t[i], v[i]);
-      if (__any_sync(~0u, near)) {
-        uint32_t set = 0;
+          for (int j = 0; j < 8; ++j)
+            if (fabsf(View::value_of(r, j)) < kPsSmall) set |= 1u << j;
+          set &= r.bits;
+          small += __popc(set);
+          if (by_mass)
+            View::each_set(set, [&](int j, bool have) {
+              const double w = exp2_table((double)View::value_at(r, j) * c.scale, *c.powers);
+              if (have) mass += w;
+            });
+        }
+      } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          if (fabsf(View::value_of(r, j)) < kPsSmall) set |= 1u << j;
-        set &= r.bits;
-        small += __popc(set);
-        if (DT == kBF16 && by_mass)
-          View::each_set(set, [&](int j, bool have) {
-            const double w = exp2_table((double)View::value_at(r, j) * c.scale, *c.powers);
-            if (have) mass += w;
-          });
+          Row::count_linear(hist, lin, View::value_of(r, j), full || (r.bits >> j & 1u));
       }
     });
     // order code of the maximum, 0 without a valid id
@@ -1846,8 +1925,8 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
       c.top = code_value(top);
       c.flat = !(pol.temperature > 0.0) || c.top == INFINITY;
       // the masses relative to the maximum, where they did not leave the range of doubles
-      const double shift = ((mass_of_all ? from : 0.0) - c.top) * c.scale;
-      const bool in_range = fabs(shift) < 14400.0 && fabs(c.top * c.scale) < 14400.0;
+      const double shift = (from - c.top) * c.scale;
+      const bool in_range = fabs(shift) < 14400.0;
       const double factor = in_range ? exp2_table(shift, sh.powers) : 0.0;
       sum.mass = sum.mass > 0.0 ? sum.mass * factor : 0.0;
       const bool measured = mass_of_all && in_range && (double)floor_value < from - 1e-30;
@@ -1858,13 +1937,15 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
         if (plain && measured && !c.flat) row.summed = {(mass + mass2) * factor, sum.mass, 0u};
       } else {
         PsRange range = {};
-        auto found = Row::kNothing;
-        if (in_range && (measured || !mass_of_all))
-          found = row.find_cut_in_bins(c, pol, sum, range);
-        if (found != Row::kFound) {
+        bool found = false;
+        if (in_range && (measured || !mass_of_all)) {
+          if constexpr (DT == kBF16) found = row.cut_by_values(c, pol, sum);
+          else found = row.range_by_bins(c, pol, sum, lin, total, range);
+        }
+        if (DT != kBF16 || !found) {
           __syncthreads();  // what the scans left in shared memory has been read
-          const auto o = Row::find_cut_apart(row, c, pol, top, sum.count, total,
-                                             found == Row::kRange, range);
+          const auto o =
+              Row::find_cut_apart(row, c, pol, top, sum.count, total, found, range);
           c.keep(o.cut, o.take);
           row.parity = o.parity;
           row.summed = o.summed;
