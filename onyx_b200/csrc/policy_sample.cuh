@@ -90,6 +90,7 @@ struct PolicyParams {
   int32_t k;         // CTAs per row
   int32_t peaks;     // the peaks are kept (else their place is empty)
   int32_t keep;      // shared memory holds all chunks of a CTA's part
+  int32_t depth;     // else: slots of a warp's ring
   int32_t slots;     // where in dynamic shared memory the chunks' slots begin,
   int32_t lists;     // and the lists of the warps (over a ring, which is done by then)
 };
@@ -208,7 +209,7 @@ struct PsShared {
 // list and its sorted form, and for the weights of the bins. Then the sums of the pieces of a
 // draw, the peaks, and last the slots into which the warps copy their part of the row: all of
 // its chunks where they fit (the later passes read them there), else a ring of
-// ps_depth().
+// 2 to 8 slots.
 extern __shared__ __align__(16) unsigned char ps_dynamic[];
 constexpr size_t kPsArea = kPsBins * sizeof(uint32_t);
 __device__ __forceinline__ uint32_t* ps_hist() { return reinterpret_cast<uint32_t*>(ps_dynamic); }
@@ -234,22 +235,43 @@ constexpr size_t kPsFixed = 2 * kPsArea + kPsUnits * (sizeof(double) + sizeof(ui
 __host__ __device__ constexpr int ps_slot(int dt, bool masked) {
   return kPsChunk * (dt == kF32 ? 4 : 2) + (masked ? 48 : 0);
 }
-__host__ __device__ constexpr int ps_depth(int dt) { return dt == kF32 ? 2 : 4; }
+// slots of a ring, the most that shared memory leaves room for
+constexpr int kPsDepths[] = {8, 4, 3, 2};
 
-__device__ __forceinline__ void ps_copy16(void* dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
-                   (uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
+__device__ __forceinline__ void ps_copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 // 4 bytes, or zeros
-__device__ __forceinline__ void ps_copy4(void* dst, const void* src, bool have) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(
-                   (uint32_t)__cvta_generic_to_shared(dst)), "l"(src), "r"(have ? 4 : 0)
+__device__ __forceinline__ void ps_copy4(uint32_t dst, const void* src, bool have) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src),
+               "r"(have ? 4 : 0)
                : "memory");
+}
+__device__ __forceinline__ uint4 ps_load16(uint32_t at) {
+  uint4 r;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+               : "r"(at)
+               : "memory");
+  return r;
+}
+__device__ __forceinline__ uint32_t ps_load4(uint32_t at) {
+  uint32_t r;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(r) : "r"(at) : "memory");
+  return r;
 }
 __device__ __forceinline__ void ps_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void ps_await() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+// waits until at most `ahead` of the latest copies are on their way (or fewer)
+__device__ __forceinline__ void ps_await_all_but(int ahead) {
+  if (ahead >= 7) ps_await<7>();
+  else if (ahead >= 3) ps_await<3>();
+  else if (ahead == 2) ps_await<2>();
+  else if (ahead == 1) ps_await<1>();
+  else ps_await<0>();
 }
 
 // The part of a row that one warp owns, and how it is read. Ids are counted by positions:
@@ -259,7 +281,7 @@ __device__ __forceinline__ void ps_await() {
 template <int DT>
 struct RowView {
   using S = typename Elem<DT>::storage;
-  static constexpr int kData = kPsChunk * (int)sizeof(S), kDepth = ps_depth(DT);
+  static constexpr int kData = kPsChunk * (int)sizeof(S);
   const S* row;
   const uint32_t* mask;
   uint16_t* peaks;  // of this CTA: the peaks (see peak()) of every 8 positions, or null
@@ -268,8 +290,8 @@ struct RowView {
   uint32_t base;    // the CTA's first position
   uint32_t begin, end;  // positions; multiples of kPsChunk, but for the row's end
   int vocab, off;
-  unsigned char* slots;  // of the CTA's chunks in order, if all are kept, else of the warp's ring
-  int slot_bytes;
+  uint32_t slots;  // of the CTA's chunks in order, if all are kept, else of the warp's ring
+  int slot_bytes, depth;
   bool kept;  // all chunks are kept
 
   struct Raw {  // the values at 8 positions as loaded
@@ -306,25 +328,6 @@ struct RowView {
     }
   }
 
-  // of the slot of the chunk that position `at` begins, lane's 8 values
-  __device__ __forceinline__ Raw from_slot(const unsigned char* slot, uint32_t at, int lane) const {
-    Raw r;
-    r.a = *reinterpret_cast<const uint4*>(slot + lane * 16);
-    if (DT == kF32) r.b = *reinterpret_cast<const uint4*>(slot + 512 + lane * 16);
-    r.bits = 0xFFu;
-    const int id0 = id_of(at), id = id0 + 8 * lane;
-    if (id0 < 0 || id0 + kPsChunk > vocab) {  // an end of the row
-      r.bits = inside(id);
-      if (r.bits != 0xFFu) load_edge(r, id);
-    }
-    if (mask) {
-      const uint32_t* words = reinterpret_cast<const uint32_t*>(slot + kData);
-      const int w = (id >> 5) - (id0 >> 5);
-      r.bits &= __funnelshift_r(words[w], words[w + 1], id & 31);
-    }
-    return r;
-  }
-
   // the 8 values from position `pos` on, none if they are not wanted
   __device__ __forceinline__ Raw load(uint32_t pos, bool wanted) const {
     Raw r;
@@ -337,13 +340,12 @@ struct RowView {
     uint32_t lo = ~0u, hi = ~0u;
     if (kept) {
       const uint32_t at = (pos - base) >> 3, lane = at & 31u;
-      const unsigned char* slot = slots + (size_t)(at >> 5) * slot_bytes;
-      r.a = *reinterpret_cast<const uint4*>(slot + lane * 16);
-      if (DT == kF32) r.b = *reinterpret_cast<const uint4*>(slot + 512 + lane * 16);
+      const uint32_t slot = slots + (at >> 5) * (uint32_t)slot_bytes;
+      r.a = ps_load16(slot + lane * 16u);
+      if (DT == kF32) r.b = ps_load16(slot + 512u + lane * 16u);
       if (mask) {
-        const uint32_t* words = reinterpret_cast<const uint32_t*>(slot + kData);
         const int w = (id >> 5) - ((id - 8 * (int)lane) >> 5);
-        lo = words[w], hi = words[w + 1];
+        lo = ps_load4(slot + kData + 4 * w), hi = ps_load4(slot + kData + 4 * w + 4);
       }
     } else {
       if (r.bits == 0xFFu) {
@@ -361,18 +363,17 @@ struct RowView {
     return r;
   }
 
-  // Starts the copy of the chunk at `at` into `slot`.
-  __device__ __forceinline__ void copy_chunk(unsigned char* slot, int lane, uint32_t at) const {
+  // Starts the copy of the chunk whose first id is `id0` into `slot`.
+  __device__ __forceinline__ void copy_chunk(uint32_t slot, int lane, int id0) const {
     constexpr int kVec = DT == kF32 ? 4 : 8;
-    const int id0 = id_of(at);
-    const bool whole = id0 >= 0 && id0 + kPsChunk <= vocab;
-    const S* from = row + id0 + lane * kVec;
+    const bool inner = id0 >= 0 && id0 + kPsChunk <= vocab;
+    const S* from = row + (id0 + lane * kVec);
 #pragma unroll
     for (int h = 0; h < 8 / kVec; ++h) {
       const int v = lane + 32 * h, id = id0 + v * kVec;
       // float32: a lane's two vectors 512 bytes apart, so that reading them has no conflicts
       const int to = DT == kF32 ? (v & 1) * 512 + (v >> 1) * 16 : v * 16;
-      if (whole || (id >= 0 && id + kVec <= vocab)) ps_copy16(slot + to, from + 32 * kVec * h);
+      if (inner || (id >= 0 && id + kVec <= vocab)) ps_copy16(slot + to, from + 32 * kVec * h);
     }
     if (mask && lane < 10) {
       const int w = (id0 >> 5) + lane;
@@ -384,48 +385,62 @@ struct RowView {
   __device__ __forceinline__ int chunks() const {
     return (int)((end - begin + kPsChunk - 1) / kPsChunk);
   }
+  __device__ __forceinline__ uint32_t first_slot() const {
+    return slots + (kept ? (begin - base) / kPsChunk * (uint32_t)slot_bytes : 0u);
+  }
   // Starts all copies, or those that fill the ring but for one slot.
   __device__ __forceinline__ void start_stream(int lane) const {
-    const int n = chunks(), now = kept ? n : min(n, kDepth - 1);
-    unsigned char* slot = slots + (kept ? (size_t)((begin - base) / kPsChunk) * slot_bytes : 0);
+    const int n = chunks(), groups = kept ? n : depth - 1;
+    uint32_t slot = first_slot();
 #pragma unroll 1
-    for (int i = 0; i < (kept ? n : kDepth - 1); ++i) {
-      if (i < now) copy_chunk(slot, lane, begin + (uint32_t)i * kPsChunk);
+    for (int i = 0; i < groups; ++i) {
+      if (i < n) copy_chunk(slot, lane, id_of(begin) + i * kPsChunk);
       ps_commit();
       slot += slot_bytes;
     }
   }
 
-  // f(position of the lane's first value, its values): the pass that reads the row from HBM,
-  // behind the copies of start_stream(). Every lane makes every call.
+  // f(peak index, the lane's 8 values, whether no lane misses one): the pass that reads the row
+  // from HBM, behind the copies of start_stream(). Every lane makes every call.
   template <class F>
   __device__ __forceinline__ void stream(int lane, F&& f) const {
     const int n = chunks();
-    unsigned char* slot = slots + (kept ? (size_t)((begin - base) / kPsChunk) * slot_bytes : 0);
-    unsigned char* const last = slots + (kDepth - 1) * slot_bytes;
-    unsigned char* fill = last;  // the ring's free slot
-    uint32_t at = begin;
+    const uint32_t ring = slots + (uint32_t)(depth * slot_bytes);
+    uint32_t slot = first_slot(), fill = ring - slot_bytes;  // the ring's free slot
+    uint32_t at = ((begin - base) >> 3) + lane;
+    int id0 = id_of(begin);
 #pragma unroll 1
     for (int i = 0; i < n; ++i) {
-      if (kept) {  // at most n - 1 - i copies may still be on their way
-        const int ahead = n - 1 - i;
-        if (ahead >= 8) ps_await<8>();
-        else if (ahead >= 4) ps_await<4>();
-        else if (ahead >= 2) ps_await<2>();
-        else if (ahead == 1) ps_await<1>();
-        else ps_await<0>();
+      if (kept) {
+        ps_await_all_but(n - 1 - i);
       } else {
-        if (i + kDepth - 1 < n) copy_chunk(fill, lane, at + (kDepth - 1) * kPsChunk);
+        if (i + depth - 1 < n) copy_chunk(fill, lane, id0 + (depth - 1) * kPsChunk);
         ps_commit();
-        fill = fill == last ? slots : fill + slot_bytes;
-        ps_await<kDepth - 1>();
+        fill += slot_bytes;
+        if (fill == ring) fill = slots;
+        ps_await_all_but(depth - 1);
       }
       __syncwarp();
-      const Raw r = from_slot(slot, at, lane);
+      Raw r;
+      r.a = ps_load16(slot + lane * 16);
+      if (DT == kF32) r.b = ps_load16(slot + 512 + lane * 16);
+      r.bits = 0xFFu;
+      const bool inner = id0 >= 0 && id0 + kPsChunk <= vocab;
+      if (!inner) {  // an end of the row
+        r.bits = inside(id0 + 8 * lane);
+        if (r.bits != 0xFFu) load_edge(r, id0 + 8 * lane);
+      }
+      if (mask) {
+        const int id = id0 + 8 * lane, w = (id >> 5) - (id0 >> 5);
+        const uint32_t word = slot + kData + 4 * w;
+        r.bits &= __funnelshift_r(ps_load4(word), ps_load4(word + 4), id & 31);
+      }
       __syncwarp();  // the slot has been read
-      f(at + 8u * lane, r);
-      at += kPsChunk;
-      slot = !kept && slot == last ? slots : slot + slot_bytes;
+      f(at, r, inner && !mask);
+      at += 32;
+      id0 += kPsChunk;
+      slot += slot_bytes;
+      if (!kept && slot == ring) slot = slots;
     }
   }
 
@@ -483,12 +498,15 @@ struct RowView {
       top = max_nan_f32(top, m);
       return ord32(m) >> 16;
     } else {
-      const uint32_t none = DT == kBF16 ? 0xFF80FF80u : 0xFC00FC00u;  // -inf twice
-      const uint32_t a = (r.a.x & v[0]) | (none & ~v[0]), b = (r.a.y & v[1]) | (none & ~v[1]);
-      const uint32_t d = (r.a.z & v[2]) | (none & ~v[2]), e = (r.a.w & v[3]) | (none & ~v[3]);
+      uint32_t a = r.a.x, b = r.a.y, d = r.a.z, e = r.a.w;
+      if (!full) {
+        const uint32_t none = DT == kBF16 ? 0xFF80FF80u : 0xFC00FC00u;  // -inf twice
+        a = (a & v[0]) | (none & ~v[0]), b = (b & v[1]) | (none & ~v[1]);
+        d = (d & v[2]) | (none & ~v[2]), e = (e & v[3]) | (none & ~v[3]);
+      }
       const uint32_t x = max2(max2(a, b), max2(d, e));
       const uint32_t h = max2(x, x >> 16) & 0xFFFFu;
-      return r.bits ? h ^ (h & 0x8000u ? 0xFFFFu : 0x8000u) : 0u;
+      return full || r.bits ? h ^ (h & 0x8000u ? 0xFFFFu : 0x8000u) : 0u;
     }
   }
   __device__ __forceinline__ static uint32_t max2(uint32_t a, uint32_t b) {
@@ -1369,6 +1387,19 @@ struct PolicyRow {
     while (size < n) size <<= 1;
     for (uint32_t i = n + threadIdx.x; i < size; i += kPsThreads) sorted[i] = ~0ull;
     __syncthreads();
+    if (n <= 256u) {
+      // each key's place is the count of the smaller ones, by up to 32 threads to a key (128
+      // keys: 0.4 us, where the bitonic sort takes 4)
+      const uint32_t group = min(32u, kPsThreads / max(size, 16u)), part = threadIdx.x % group;
+      const uint32_t i = threadIdx.x / group;
+      const unsigned long long key = i < n ? sorted[i] : 0ull;
+      uint32_t place = 0;
+      for (uint32_t j = part; j < n; j += group) place += sorted[j] < key;
+      for (uint32_t d = group / 2; d; d /= 2) place += __shfl_xor_sync(~0u, place, d);
+      sorted += kPsList;
+      if (i < n && part == 0) sorted[place] = key;
+      size = 0;  // nothing left to sort
+    }
     // bitonic sort; a warp's 64 keys need no more than the warp
     for (uint32_t run = 2; run <= size; run <<= 1)
       for (uint32_t d = run >> 1; d; d >>= 1) {
@@ -1799,7 +1830,9 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
   view.listed = 0;
   view.kept = p.keep != 0;
   view.slot_bytes = ps_slot(DT, view.mask != nullptr);
-  view.slots = ps_dynamic + p.slots + (view.kept ? 0 : row.warp * View::kDepth * view.slot_bytes);
+  view.depth = p.depth;
+  view.slots = (uint32_t)__cvta_generic_to_shared(ps_dynamic) + (uint32_t)p.slots +
+               (view.kept ? 0u : (uint32_t)(row.warp * p.depth * view.slot_bytes));
   row.clear_hist();
   if (threadIdx.x < 16) sh.powers.at[threadIdx.x] = exp2((double)threadIdx.x / 16.0);
   __syncthreads();
@@ -1863,12 +1896,11 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
     uint32_t count = 0, small = 0, top16 = 0;
     float top_value = -INFINITY;
     double mass = 0.0, mass2 = 0.0;
-    view.stream(row.lane, [&](uint32_t pos, const auto& r) {
-      const bool full = __all_sync(~0u, r.bits == 0xFFu);
+    view.stream(row.lane, [&](uint32_t at, const auto& r, bool full) {
       uint32_t v[4] = {~0u, ~0u, ~0u, ~0u};  // masks of the valid ones, 16 bits each
       if (DT != kF32 && !full) expand8_16(r.bits, v[0], v[1], v[2], v[3]);
       const uint32_t peak = View::peak(r, v, full, top_value);
-      if (view.peaks) view.peaks[(pos - view.base) >> 3] = (uint16_t)peak;
+      if (view.peaks) view.peaks[at] = (uint16_t)peak;
       top16 = max(top16, peak);
       if (mass_of_all) {
         if (full) {
