@@ -400,50 +400,6 @@ struct RowView {
     }
   }
 
-  // f(peak index, the lane's 8 values, whether no lane misses one): the pass that reads the row
-  // from HBM, behind the copies of start_stream(). Every lane makes every call.
-  template <class F>
-  __device__ __forceinline__ void stream(int lane, F&& f) const {
-    const int n = chunks();
-    const uint32_t ring = slots + (uint32_t)(depth * slot_bytes);
-    uint32_t slot = first_slot(), fill = ring - slot_bytes;  // the ring's free slot
-    uint32_t at = ((begin - base) >> 3) + lane;
-    int id0 = id_of(begin);
-#pragma unroll 1
-    for (int i = 0; i < n; ++i) {
-      if (kept) {
-        ps_await_all_but(n - 1 - i);
-      } else {
-        if (i + depth - 1 < n) copy_chunk(fill, lane, id0 + (depth - 1) * kPsChunk);
-        ps_commit();
-        fill += slot_bytes;
-        if (fill == ring) fill = slots;
-        ps_await_all_but(depth - 1);
-      }
-      __syncwarp();
-      Raw r;
-      r.a = ps_load16(slot + lane * 16);
-      if (DT == kF32) r.b = ps_load16(slot + 512 + lane * 16);
-      r.bits = 0xFFu;
-      const bool inner = id0 >= 0 && id0 + kPsChunk <= vocab;
-      if (!inner) {  // an end of the row
-        r.bits = inside(id0 + 8 * lane);
-        if (r.bits != 0xFFu) load_edge(r, id0 + 8 * lane);
-      }
-      if (mask) {
-        const int id = id0 + 8 * lane, w = (id >> 5) - (id0 >> 5);
-        const uint32_t word = slot + kData + 4 * w;
-        r.bits &= __funnelshift_r(ps_load4(word), ps_load4(word + 4), id & 31);
-      }
-      __syncwarp();  // the slot has been read
-      f(at, r, inner && !mask);
-      at += 32;
-      id0 += kPsChunk;
-      slot += slot_bytes;
-      if (!kept && slot == ring) slot = slots;
-    }
-  }
-
   // float32 bits of value j
   __device__ __forceinline__ static uint32_t bits_of(const Raw& r, int j) {
     const uint32_t a[4] = {r.a.x, r.a.y, r.a.z, r.a.w};
@@ -966,9 +922,10 @@ struct PolicyRow {
   __device__ __forceinline__ static uint32_t bin_of(const Linear& lin, float v) {
     return __float_as_uint(fmaf(v, -lin.scale, lin.shift)) - 0x4B000000u;
   }
-  __device__ __forceinline__ static void count_linear(uint32_t hist, const Linear& lin, float v,
-                                                      bool valid) {
-    const uint32_t bin = valid ? bin_of(lin, v) : ~0u;
+  __device__ __forceinline__ static void count_linear(uint32_t hist, float scale, float shift,
+                                                      float v, bool valid) {
+    const uint32_t at = __float_as_uint(fmaf(v, -scale, shift)) - 0x4B000000u;
+    const uint32_t bin = valid ? at : ~0u;
     asm volatile(
         "{\n\t.reg .pred p;\n\tsetp.lt.u32 p, %1, %2;\n\t@p red.shared.add.u32 [%0], 1;\n\t}" ::"r"(
             hist + (bin << 2)),
@@ -1159,11 +1116,20 @@ struct PolicyRow {
   __device__ __forceinline__ double sum_of(const RowCut& c, const Raw& r, uint32_t set,
                                            double least) const {
     if (!__any_sync(~0u, set)) return 0.0;
-    return sum_set(r, set, c.top, c.scale, least, c.flat, c.powers, table);
+    return sum_set(r.a.x, r.a.y, r.a.z, r.a.w, DT == kF32 ? r.b.x : 0u, DT == kF32 ? r.b.y : 0u,
+                   DT == kF32 ? r.b.z : 0u, DT == kF32 ? r.b.w : 0u, set, c.top, c.scale, least,
+                   c.flat, c.powers, table);
   }
-  __device__ __noinline__ static double sum_set(const Raw r, uint32_t set, double top,
-                                                double scale, double least, bool flat,
-                                                const PsPowers* powers, const double* bins) {
+  // (Scalars, for a struct that is passed by value lives in memory, and so do its copies.)
+  __device__ __noinline__ static double sum_set(uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                                uint32_t b0, uint32_t b1, uint32_t b2, uint32_t b3,
+                                                uint32_t set, double top, double scale,
+                                                double least, bool flat, const PsPowers* powers,
+                                                const double* bins) {
+    Raw r;
+    r.a = make_uint4(a0, a1, a2, a3);
+    r.b = make_uint4(b0, b1, b2, b3);
+    r.bits = set;
     if (flat) return 1.0 >= least ? (double)__popc(set) : 0.0;
     double a = 0.0, b = 0.0;
     if (!__any_sync(~0u, __popc(set) > 2)) {
@@ -1509,18 +1475,45 @@ struct PolicyRow {
     }
   }
 
-  // The same out of line, on copies: nothing of the caller's has to live in memory for it.
+  // The same out of line, on copies that are made field by field: nothing of the caller's has
+  // to live in memory for it (where every asynchronous copy would have it read again).
   struct Outcome {
     float cut;
     uint32_t take;
     int parity;
     PsSummed summed;
   };
-  __device__ __noinline__ static Outcome find_cut_apart(PolicyRow row, RowCut c, RowPolicy pol,
-                                                        uint32_t top, uint32_t valid,
-                                                        double total, bool have, PsRange range) {
-    row.find_cut(c, pol, top, valid, total, have ? &range : nullptr);
-    return {c.cut, c.take, row.parity, row.summed};
+  __device__ __noinline__ static void find_cut_on(PolicyRow* row, RowCut* c, const RowPolicy* pol,
+                                                  uint32_t top, uint32_t valid, double total,
+                                                  const PsRange* range) {
+    row->find_cut(*c, *pol, top, valid, total, range);
+  }
+  __device__ __forceinline__ Outcome find_cut_apart(const RowCut& c, const RowPolicy& pol,
+                                                    uint32_t top, uint32_t valid, double total,
+                                                    bool have, const PsRange& range) const {
+    PolicyRow r(sh);
+    r.view.row = view.row, r.view.mask = view.mask;
+    r.view.peaks = view.peaks, r.view.list = view.list, r.view.listed = view.listed;
+    r.view.base = view.base, r.view.begin = view.begin, r.view.end = view.end;
+    r.view.vocab = view.vocab, r.view.off = view.off;
+    r.view.slots = view.slots, r.view.slot_bytes = view.slot_bytes, r.view.depth = view.depth;
+    r.view.kept = view.kept;
+    r.rank = rank, r.k = k, r.warp_ids = warp_ids, r.row_end = row_end;
+    r.warp = warp, r.lane = lane, r.entry = entry, r.parity = parity;
+    RowCut x;
+    x.top = c.top, x.scale = c.scale, x.inv_t = c.inv_t, x.min_p = c.min_p;
+    x.powers = c.powers, x.cut = c.cut, x.cut2 = c.cut2, x.take = c.take, x.flat = c.flat;
+    RowPolicy y;
+    y.temperature = pol.temperature, y.top_p = pol.top_p, y.min_p = pol.min_p;
+    y.top_k = pol.top_k, y.ok = pol.ok;
+    PsRange z;
+    z.hi = range.hi, z.lo = range.lo, z.above = range.above, z.inside = range.inside;
+    find_cut_on(&r, &x, &y, top, valid, total, have ? &z : nullptr);
+    Outcome o;
+    o.cut = x.cut, o.take = x.take, o.parity = r.parity;
+    o.summed.lane = r.summed.lane, o.summed.all = r.summed.all;
+    o.summed.down_to = r.summed.down_to;
+    return o;
   }
 
   // ---- the kept mass and the draw -------------------------------------------------------
@@ -1781,6 +1774,149 @@ struct PolicyRow {
   }
 };
 
+// What the pass that reads the row from HBM finds in a lane's values.
+struct PsFirst {
+  uint32_t peak;  // of 16-bit types: the largest peak
+  float top;      // float32: the largest value, a NaN with a NaN
+  uint32_t count, small;  // valid ids; bfloat16: those next to zero
+  double mass;    // MASS: of all ids relative to `from`; bfloat16 with small_mass: of those
+                  // next to zero relative to 0
+};
+
+// The pass behind the copies of start_stream(): peaks, and with BINS the histogram, with MASS
+// the weights. One loop for each of the four, on scalars of its own: the first version, a
+// lambda called from a method of the view, took 150 instructions a chunk where this takes 35
+// (256 rows of 128,256, the maximum alone: 34 us, now 15).
+template <int DT, bool BINS, bool MASS>
+__device__ __forceinline__ PsFirst first_pass(const RowView<DT>& view, int lane,
+                                              const typename PolicyRow<DT>::Linear& bins,
+                                              double from, double scale, bool small_mass,
+                                              const PsPowers& powers) {
+  using View = RowView<DT>;
+  using Row = PolicyRow<DT>;
+  using S = typename Elem<DT>::storage;
+  constexpr int kVec = DT == kF32 ? 4 : 8;
+  const S* const row = view.row;
+  const uint32_t* const mask = view.mask;
+  const int vocab = view.vocab, n = view.chunks(), words = (vocab + 31) >> 5;
+  const uint32_t bytes = (uint32_t)view.slot_bytes;
+  const bool kept = view.kept;
+  const int depth = kept ? n + 1 : view.depth;  // copies of a kept part are all on their way
+  const uint32_t start = view.slots;
+  const uint32_t stop = kept ? 0xFFFFFFFFu : start + (uint32_t)view.depth * bytes;
+  uint32_t slot = view.first_slot();
+  uint32_t fill = stop - bytes;
+  int id0 = view.id_of(view.begin), fill_id = id0 + (depth - 1) * kPsChunk;
+  uint32_t peak_at = 0;
+  if (view.peaks)
+    peak_at = (uint32_t)__cvta_generic_to_shared(view.peaks) +
+              2u * (((view.begin - view.base) >> 3) + (uint32_t)lane);
+  const uint32_t hist = (uint32_t)__cvta_generic_to_shared(ps_hist());
+  const float scale_b = bins.scale, shift_b = bins.shift;
+  const float floor_value = (float)(from - 15000.0 / scale);  // less than 2^-930 below it
+  PsFirst out = {0u, -INFINITY, 0u, 0u, 0.0};
+  double mass2 = 0.0;
+
+#pragma unroll 1
+  for (int i = 0; i < n; ++i) {
+    if (i + depth - 1 < n) {
+      const bool inner = fill_id >= 0 && fill_id + kPsChunk <= vocab;
+      const S* src = row + (fill_id + lane * kVec);
+#pragma unroll
+      for (int h = 0; h < 8 / kVec; ++h) {
+        const int v = lane + 32 * h, id = fill_id + v * kVec;
+        const int to = DT == kF32 ? (v & 1) * 512 + (v >> 1) * 16 : v * 16;
+        if (inner || (id >= 0 && id + kVec <= vocab)) ps_copy16(fill + to, src + 32 * kVec * h);
+      }
+      if (mask && lane < 10) {
+        const int w = (fill_id >> 5) + lane;
+        const bool have = w >= 0 && w < words;
+        ps_copy4(fill + View::kData + 4 * lane, mask + (have ? w : 0), have);
+      }
+      fill_id += kPsChunk;
+      fill += bytes;
+      if (fill == stop) fill = start;
+    }
+    if (!kept) ps_commit();
+    ps_await_all_but(kept ? n - 1 - i : depth - 1);
+    __syncwarp();
+    typename View::Raw r;
+    r.a = ps_load16(slot + lane * 16);
+    if (DT == kF32) r.b = ps_load16(slot + 512 + lane * 16);
+    r.bits = 0xFFu;
+    bool full = true;
+    if (id0 < 0 || id0 + kPsChunk > vocab) {  // an end of the row
+      r.bits = view.inside(id0 + 8 * lane);
+      if (r.bits != 0xFFu) view.load_edge(r, id0 + 8 * lane);
+      full = false;
+    }
+    if (mask) {
+      const int id = id0 + 8 * lane, w = (id >> 5) - (id0 >> 5);
+      const uint32_t word = slot + View::kData + 4 * w;
+      r.bits &= __funnelshift_r(ps_load4(word), ps_load4(word + 4), id & 31);
+      full = false;
+    }
+    __syncwarp();  // the slot has been read
+    id0 += kPsChunk;
+    slot += bytes;
+    if (slot == stop) slot = start;
+
+    uint32_t v[4] = {~0u, ~0u, ~0u, ~0u};  // masks of the valid ones, 16 bits each
+    if (DT != kF32 && !full) expand8_16(r.bits, v[0], v[1], v[2], v[3]);
+    const uint32_t peak = View::peak(r, v, full, out.top);
+    if (peak_at)
+      asm volatile("st.shared.u16 [%0], %1;" ::"r"(peak_at), "h"((uint16_t)peak) : "memory");
+    peak_at += peak_at ? 64u : 0u;
+    out.peak = max(out.peak, peak);
+    if (MASS) {
+      if (full) {
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+          const float x = View::value_of(r, j), y = View::value_of(r, j + 1);
+          const double a = exp2_from(fmaxf(x, floor_value), from, scale, powers);
+          const double b = exp2_from(fmaxf(y, floor_value), from, scale, powers);
+          out.mass += x >= floor_value ? a : 0.0;
+          mass2 += y >= floor_value ? b : 0.0;
+        }
+      } else {
+        View::each_set(r.bits, [&](int j, bool have) {
+          const float x = View::value_at(r, j);
+          const double a = exp2_from(fmaxf(x, floor_value), from, scale, powers);
+          if (have && x >= floor_value) out.mass += a;
+        });
+      }
+    }
+    if (BINS) {
+      out.count += __popc(r.bits);
+      if constexpr (DT == kBF16) {
+        const uint32_t near =
+            Row::count_values(hist, r.a.x, v[0]) | Row::count_values(hist, r.a.y, v[1]) |
+            Row::count_values(hist, r.a.z, v[2]) | Row::count_values(hist, r.a.w, v[3]);
+        if (__any_sync(~0u, near)) {
+          uint32_t set = 0;
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (fabsf(View::value_of(r, j)) < kPsSmall) set |= 1u << j;
+          set &= r.bits;
+          out.small += __popc(set);
+          if (small_mass)
+            View::each_set(set, [&](int j, bool have) {
+              const double w = exp2_table((double)View::value_at(r, j) * scale, powers);
+              if (have) out.mass += w;
+            });
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          Row::count_linear(hist, scale_b, shift_b, View::value_of(r, j),
+                            full || (r.bits >> j & 1u));
+      }
+    }
+  }
+  out.mass += mass2;
+  return out;
+}
+
 // zeros for the ids [begin, end) of a row of probabilities, by the threads of a CTA
 __device__ __forceinline__ void clear_probs(float* row, uint32_t begin, uint32_t end) {
   const uint32_t lead = (uint32_t)(-(int)(reinterpret_cast<uintptr_t>(row + begin) >> 2)) & 3u;
@@ -1890,65 +2026,20 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
       const float x = Elem<DT>::to_f32(view.row, 0);
       if (fabsf(x) < 512.0f) from = x;
     }
-    const uint32_t hist = (uint32_t)__cvta_generic_to_shared(ps_hist());
-    // values below it weigh less than 2^-930 on that scale
-    const float floor_value = (float)(from - 15000.0 / c.scale);
-    uint32_t count = 0, small = 0, top16 = 0;
-    float top_value = -INFINITY;
-    double mass = 0.0, mass2 = 0.0;
-    view.stream(row.lane, [&](uint32_t at, const auto& r, bool full) {
-      uint32_t v[4] = {~0u, ~0u, ~0u, ~0u};  // masks of the valid ones, 16 bits each
-      if (DT != kF32 && !full) expand8_16(r.bits, v[0], v[1], v[2], v[3]);
-      const uint32_t peak = View::peak(r, v, full, top_value);
-      if (view.peaks) view.peaks[at] = (uint16_t)peak;
-      top16 = max(top16, peak);
-      if (mass_of_all) {
-        if (full) {
-#pragma unroll
-          for (int j = 0; j < 8; j += 2) {
-            const float x = View::value_of(r, j), y = View::value_of(r, j + 1);
-            const double a = exp2_from(fmaxf(x, floor_value), from, c.scale, sh.powers);
-            const double b = exp2_from(fmaxf(y, floor_value), from, c.scale, sh.powers);
-            mass += x >= floor_value ? a : 0.0;
-            mass2 += y >= floor_value ? b : 0.0;
-          }
-        } else {
-          View::each_set(r.bits, [&](int j, bool have) {
-            const float x = View::value_at(r, j);
-            const double a = exp2_from(fmaxf(x, floor_value), from, c.scale, sh.powers);
-            if (have && x >= floor_value) mass += a;
-          });
-        }
-      }
-      if (!bins) return;
-      count += __popc(r.bits);
-      if constexpr (DT == kBF16) {
-        const uint32_t near = Row::count_values(hist, r.a.x, v[0]) |
-                              Row::count_values(hist, r.a.y, v[1]) |
-                              Row::count_values(hist, r.a.z, v[2]) |
-                              Row::count_values(hist, r.a.w, v[3]);
-        if (__any_sync(~0u, near)) {
-          uint32_t set = 0;
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (fabsf(View::value_of(r, j)) < kPsSmall) set |= 1u << j;
-          set &= r.bits;
-          small += __popc(set);
-          if (by_mass)
-            View::each_set(set, [&](int j, bool have) {
-              const double w = exp2_table((double)View::value_at(r, j) * c.scale, *c.powers);
-              if (have) mass += w;
-            });
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          Row::count_linear(hist, lin, View::value_of(r, j), full || (r.bits >> j & 1u));
-      }
-    });
+    PsFirst f;
+    if (bins && mass_of_all) {
+      if constexpr (DT != kBF16)
+        f = first_pass<DT, true, true>(view, row.lane, lin, from, c.scale, false, sh.powers);
+    } else if (bins) {
+      f = first_pass<DT, true, false>(view, row.lane, lin, from, c.scale, by_mass, sh.powers);
+    } else if (mass_of_all) {
+      f = first_pass<DT, false, true>(view, row.lane, lin, from, c.scale, false, sh.powers);
+    } else {
+      f = first_pass<DT, false, false>(view, row.lane, lin, from, c.scale, false, sh.powers);
+    }
     // order code of the maximum, 0 without a valid id
-    uint32_t top = top16 == 0u ? 0u : DT == kF32 ? ord32(top_value) : View::top_code(top16);
-    PsBox sum = row.reduce(mass + mass2, count, top, small);
+    uint32_t top = f.peak == 0u ? 0u : DT == kF32 ? ord32(f.top) : View::top_code(f.peak);
+    PsBox sum = row.reduce(f.mass, f.count, top, f.small);
     top = sum.top;
     if (top == 0u) status = kStatusEmptyMask;
     if (top == kOrd32NaN) status = kStatusNanInSupport;
@@ -1961,12 +2052,14 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
       const bool in_range = fabs(shift) < 14400.0;
       const double factor = in_range ? exp2_table(shift, sh.powers) : 0.0;
       sum.mass = sum.mass > 0.0 ? sum.mass * factor : 0.0;
-      const bool measured = mass_of_all && in_range && (double)floor_value < from - 1e-30;
+      // (not if the temperature is so low that the pass could not tell `from` from its floor)
+      const bool measured =
+          mass_of_all && in_range && (double)(float)(from - 15000.0 / c.scale) < from - 1e-30;
       const double total = measured ? sum.mass : -1.0;
       if (!bins) {
         if (pol.temperature > 0.0) c.cut = c.flat ? FLT_MAX : -INFINITY;
         else c.keep(code_value(top), 1u);
-        if (plain && measured && !c.flat) row.summed = {(mass + mass2) * factor, sum.mass, 0u};
+        if (plain && measured && !c.flat) row.summed = {f.mass * factor, sum.mass, 0u};
       } else {
         PsRange range = {};
         bool found = false;
@@ -1977,7 +2070,7 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
         if (DT != kBF16 || !found) {
           __syncthreads();  // what the scans left in shared memory has been read
           const auto o =
-              Row::find_cut_apart(row, c, pol, top, sum.count, total, found, range);
+              row.find_cut_apart(c, pol, top, sum.count, total, found, range);
           c.keep(o.cut, o.take);
           row.parity = o.parity;
           row.summed = o.summed;
