@@ -30,7 +30,7 @@ static int device_sms(cudaError_t* err) {
 // How a launch lays out its rows: CTAs per row, positions per warp, dynamic shared memory.
 struct PolicyPlan {
   int k;
-  int32_t warp_ids, peaks, keep, depth, slots, lists;
+  int32_t warp_ids, peaks, keep, slots, lists;
   size_t smem;
 };
 
@@ -55,14 +55,8 @@ static PolicyPlan plan_with(int k, int64_t vocab, int dtype, bool masked) {
   pl.keep = pl.peaks && pl.smem + lists + all <= kPsTwoFit;
   pl.lists = (int32_t)pl.smem;
   pl.slots = (int32_t)(pl.smem + (pl.keep ? lists : 0));
-  for (int depth : kPsDepths) {
-    const size_t ring = std::max((size_t)kPsWarps * depth * slot, lists);
-    pl.depth = depth;
-    if (pl.smem + ring <= kPsTwoFit || depth == kPsDepths[3]) {
-      pl.smem += pl.keep ? lists + all : ring;
-      break;
-    }
-  }
+  const size_t ring = std::max((size_t)kPsWarps * ps_depth(dtype) * slot, lists);
+  pl.smem += pl.keep ? lists + all : ring;
   return pl;
 }
 
@@ -94,7 +88,7 @@ static cudaError_t allow_shared(const void* fn, int which) {
   if (e != cudaSuccess) return e;
   if (dev >= 0 && dev < 64 && (done[dev].load(std::memory_order_acquire) >> which & 1)) return e;
   e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           (int)(kPsFixed + 2 * kPsMostPeaks + 2 * kPsWarps * ps_slot(kF32, true)));
+                           (int)(kPsFixed + 2 * kPsMostPeaks + kPsWarps * ps_depth(kF32) * ps_slot(kF32, true)));
   if (e == cudaSuccess && dev >= 0 && dev < 64)
     done[dev].fetch_or((uint16_t)(1u << which), std::memory_order_release);
   return e;
@@ -110,7 +104,6 @@ static int launch_policy(int dtype, PolicyParams& p, int64_t rows, cudaStream_t 
   p.warp_ids = pl.warp_ids;
   p.peaks = pl.peaks;
   p.keep = pl.keep;
-  p.depth = pl.depth;
   p.slots = pl.slots;
   p.lists = pl.lists;
   if (rows * p.k > 0x7FFFFFFFll) return ONYX_ERR_INVALID_ARGUMENT;

@@ -90,7 +90,6 @@ struct PolicyParams {
   int32_t k;         // CTAs per row
   int32_t peaks;     // the peaks are kept (else their place is empty)
   int32_t keep;      // shared memory holds all chunks of a CTA's part
-  int32_t depth;     // else: slots of a warp's ring
   int32_t slots;     // where in dynamic shared memory the chunks' slots begin,
   int32_t lists;     // and the lists of the warps (over a ring, which is done by then)
 };
@@ -209,7 +208,7 @@ struct PsShared {
 // list and its sorted form, and for the weights of the bins. Then the sums of the pieces of a
 // draw, the peaks, and last the slots into which the warps copy their part of the row: all of
 // its chunks where they fit (the later passes read them there), else a ring of
-// 2 to 8 slots.
+// ps_depth().
 extern __shared__ __align__(16) unsigned char ps_dynamic[];
 constexpr size_t kPsArea = kPsBins * sizeof(uint32_t);
 __device__ __forceinline__ uint32_t* ps_hist() { return reinterpret_cast<uint32_t*>(ps_dynamic); }
@@ -235,8 +234,8 @@ constexpr size_t kPsFixed = 2 * kPsArea + kPsUnits * (sizeof(double) + sizeof(ui
 __host__ __device__ constexpr int ps_slot(int dt, bool masked) {
   return kPsChunk * (dt == kF32 ? 4 : 2) + (masked ? 48 : 0);
 }
-// slots of a ring, the most that shared memory leaves room for
-constexpr int kPsDepths[] = {8, 4, 3, 2};
+// slots of a ring
+__host__ __device__ constexpr int ps_depth(int dt) { return dt == kF32 ? 3 : 4; }
 
 __device__ __forceinline__ void ps_copy16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -265,11 +264,11 @@ template <int N>
 __device__ __forceinline__ void ps_await() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-// waits until at most `ahead` of the latest copies are on their way (or fewer)
+// waits until at most `ahead` of the latest groups are on their way (or fewer)
 __device__ __forceinline__ void ps_await_all_but(int ahead) {
-  if (ahead >= 7) ps_await<7>();
-  else if (ahead >= 3) ps_await<3>();
-  else if (ahead == 2) ps_await<2>();
+  if (ahead >= 8) ps_await<8>();
+  else if (ahead >= 4) ps_await<4>();
+  else if (ahead >= 2) ps_await<2>();
   else if (ahead == 1) ps_await<1>();
   else ps_await<0>();
 }
@@ -281,7 +280,7 @@ __device__ __forceinline__ void ps_await_all_but(int ahead) {
 template <int DT>
 struct RowView {
   using S = typename Elem<DT>::storage;
-  static constexpr int kData = kPsChunk * (int)sizeof(S);
+  static constexpr int kData = kPsChunk * (int)sizeof(S), kDepth = ps_depth(DT);
   const S* row;
   const uint32_t* mask;
   uint16_t* peaks;  // of this CTA: the peaks (see peak()) of every 8 positions, or null
@@ -291,7 +290,7 @@ struct RowView {
   uint32_t begin, end;  // positions; multiples of kPsChunk, but for the row's end
   int vocab, off;
   uint32_t slots;  // of the CTA's chunks in order, if all are kept, else of the warp's ring
-  int slot_bytes, depth;
+  int slot_bytes;
   bool kept;  // all chunks are kept
 
   struct Raw {  // the values at 8 positions as loaded
@@ -375,7 +374,11 @@ struct RowView {
       const int to = DT == kF32 ? (v & 1) * 512 + (v >> 1) * 16 : v * 16;
       if (inner || (id >= 0 && id + kVec <= vocab)) ps_copy16(slot + to, from + 32 * kVec * h);
     }
-    if (mask && lane < 10) {
+    if (mask) copy_words(slot, lane, id0);
+  }
+  // the mask words of the chunk
+  __device__ __forceinline__ void copy_words(uint32_t slot, int lane, int id0) const {
+    if (lane < 10) {
       const int w = (id0 >> 5) + lane;
       const bool have = w >= 0 && w < (vocab + 31) >> 5;
       ps_copy4(slot + kData + 4 * lane, mask + (have ? w : 0), have);
@@ -390,7 +393,7 @@ struct RowView {
   }
   // Starts all copies, or those that fill the ring but for one slot.
   __device__ __forceinline__ void start_stream(int lane) const {
-    const int n = chunks(), groups = kept ? n : depth - 1;
+    const int n = chunks(), groups = kept ? n : kDepth - 1;
     uint32_t slot = first_slot();
 #pragma unroll 1
     for (int i = 0; i < groups; ++i) {
@@ -1496,7 +1499,7 @@ struct PolicyRow {
     r.view.peaks = view.peaks, r.view.list = view.list, r.view.listed = view.listed;
     r.view.base = view.base, r.view.begin = view.begin, r.view.end = view.end;
     r.view.vocab = view.vocab, r.view.off = view.off;
-    r.view.slots = view.slots, r.view.slot_bytes = view.slot_bytes, r.view.depth = view.depth;
+    r.view.slots = view.slots, r.view.slot_bytes = view.slot_bytes;
     r.view.kept = view.kept;
     r.rank = rank, r.k = k, r.warp_ids = warp_ids, r.row_end = row_end;
     r.warp = warp, r.lane = lane, r.entry = entry, r.parity = parity;
@@ -1795,78 +1798,80 @@ __device__ __forceinline__ PsFirst first_pass(const RowView<DT>& view, int lane,
   using View = RowView<DT>;
   using Row = PolicyRow<DT>;
   using S = typename Elem<DT>::storage;
-  constexpr int kVec = DT == kF32 ? 4 : 8;
-  const S* const row = view.row;
+  constexpr int kVec = DT == kF32 ? 4 : 8, kDepth = View::kDepth;
   const uint32_t* const mask = view.mask;
-  const int vocab = view.vocab, n = view.chunks(), words = (vocab + 31) >> 5;
+  const int n = view.chunks();
   const uint32_t bytes = (uint32_t)view.slot_bytes;
   const bool kept = view.kept;
-  const int depth = kept ? n + 1 : view.depth;  // copies of a kept part are all on their way
+  // chunks inside the row; the others are copied and read with care
+  const int id_first = view.id_of(view.begin);
+  const int inner_from = id_first < 0 ? 1 : 0;
+  const int inner_to = inner_from + max(0, (view.vocab - (id_first + inner_from * kPsChunk)) / kPsChunk);
   const uint32_t start = view.slots;
-  const uint32_t stop = kept ? 0xFFFFFFFFu : start + (uint32_t)view.depth * bytes;
-  uint32_t slot = view.first_slot();
-  uint32_t fill = stop - bytes;
-  int id0 = view.id_of(view.begin), fill_id = id0 + (depth - 1) * kPsChunk;
-  uint32_t peak_at = 0;
-  if (view.peaks)
+  const uint32_t stop = kept ? 0xFFFFFFFFu : start + kDepth * bytes;
+  uint32_t slot = view.first_slot(), fill = stop - bytes;
+  const S* src = view.row + (id_first + (kDepth - 1) * kPsChunk + lane * kVec);
+  const int ahead = kept ? n : kDepth - 1;  // copies started when a chunk is read
+  const int half = kept ? n / 2 : -1;
+  uint32_t peak_at = (uint32_t)__cvta_generic_to_shared(ps_unit_ties()), peak_step = 0u;
+  if (view.peaks) {  // (else all go to a place that is not read before it is written again)
     peak_at = (uint32_t)__cvta_generic_to_shared(view.peaks) +
               2u * (((view.begin - view.base) >> 3) + (uint32_t)lane);
+    peak_step = 64u;
+  }
   const uint32_t hist = (uint32_t)__cvta_generic_to_shared(ps_hist());
   const float scale_b = bins.scale, shift_b = bins.shift;
   const float floor_value = (float)(from - 15000.0 / scale);  // less than 2^-930 below it
   PsFirst out = {0u, -INFINITY, 0u, 0u, 0.0};
   double mass2 = 0.0;
+  if (kept) ps_await_all_but(n - half);
 
 #pragma unroll 1
   for (int i = 0; i < n; ++i) {
-    if (i + depth - 1 < n) {
-      const bool inner = fill_id >= 0 && fill_id + kPsChunk <= vocab;
-      const S* src = row + (fill_id + lane * kVec);
-#pragma unroll
-      for (int h = 0; h < 8 / kVec; ++h) {
-        const int v = lane + 32 * h, id = fill_id + v * kVec;
-        const int to = DT == kF32 ? (v & 1) * 512 + (v >> 1) * 16 : v * 16;
-        if (inner || (id >= 0 && id + kVec <= vocab)) ps_copy16(fill + to, src + 32 * kVec * h);
+    if (!kept) {
+      const int next = i + ahead;
+      if (next >= inner_from && next < inner_to) {
+        ps_copy16(fill + (DT == kF32 ? (lane & 1) * 512 + (lane >> 1) * 16 : lane * 16), src);
+        if (DT == kF32)
+          ps_copy16(fill + (lane & 1) * 512 + (lane >> 1) * 16 + 256, src + 32 * kVec);
+        if (mask) view.copy_words(fill, lane, id_first + next * kPsChunk);
+      } else if (next < n) {
+        view.copy_chunk(fill, lane, id_first + next * kPsChunk);
       }
-      if (mask && lane < 10) {
-        const int w = (fill_id >> 5) + lane;
-        const bool have = w >= 0 && w < words;
-        ps_copy4(fill + View::kData + 4 * lane, mask + (have ? w : 0), have);
-      }
-      fill_id += kPsChunk;
+      src += kPsChunk;
       fill += bytes;
       if (fill == stop) fill = start;
+      ps_commit();
+      ps_await<kDepth - 1>();
+    } else if (i == half) {
+      ps_await<0>();
     }
-    if (!kept) ps_commit();
-    ps_await_all_but(kept ? n - 1 - i : depth - 1);
-    __syncwarp();
+    if (DT == kF32 || mask) __syncwarp();  // else a lane reads what it copied itself
     typename View::Raw r;
     r.a = ps_load16(slot + lane * 16);
     if (DT == kF32) r.b = ps_load16(slot + 512 + lane * 16);
     r.bits = 0xFFu;
-    bool full = true;
-    if (id0 < 0 || id0 + kPsChunk > vocab) {  // an end of the row
-      r.bits = view.inside(id0 + 8 * lane);
-      if (r.bits != 0xFFu) view.load_edge(r, id0 + 8 * lane);
+    bool full = !mask;
+    if (i < inner_from || i >= inner_to) {
+      const int id = id_first + i * kPsChunk + 8 * lane;
+      r.bits = view.inside(id);
+      if (r.bits != 0xFFu) view.load_edge(r, id);
       full = false;
     }
     if (mask) {
-      const int id = id0 + 8 * lane, w = (id >> 5) - (id0 >> 5);
+      const int id0 = id_first + i * kPsChunk, id = id0 + 8 * lane, w = (id >> 5) - (id0 >> 5);
       const uint32_t word = slot + View::kData + 4 * w;
       r.bits &= __funnelshift_r(ps_load4(word), ps_load4(word + 4), id & 31);
-      full = false;
     }
-    __syncwarp();  // the slot has been read
-    id0 += kPsChunk;
+    if (DT == kF32 || mask) __syncwarp();  // the slot has been read
     slot += bytes;
     if (slot == stop) slot = start;
 
     uint32_t v[4] = {~0u, ~0u, ~0u, ~0u};  // masks of the valid ones, 16 bits each
     if (DT != kF32 && !full) expand8_16(r.bits, v[0], v[1], v[2], v[3]);
     const uint32_t peak = View::peak(r, v, full, out.top);
-    if (peak_at)
-      asm volatile("st.shared.u16 [%0], %1;" ::"r"(peak_at), "h"((uint16_t)peak) : "memory");
-    peak_at += peak_at ? 64u : 0u;
+    asm volatile("st.shared.u16 [%0], %1;" ::"r"(peak_at), "h"((uint16_t)peak) : "memory");
+    peak_at += peak_step;
     out.peak = max(out.peak, peak);
     if (MASS) {
       if (full) {
@@ -1966,9 +1971,8 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
   view.listed = 0;
   view.kept = p.keep != 0;
   view.slot_bytes = ps_slot(DT, view.mask != nullptr);
-  view.depth = p.depth;
   view.slots = (uint32_t)__cvta_generic_to_shared(ps_dynamic) + (uint32_t)p.slots +
-               (view.kept ? 0u : (uint32_t)(row.warp * p.depth * view.slot_bytes));
+               (view.kept ? 0u : (uint32_t)(row.warp * View::kDepth * view.slot_bytes));
   row.clear_hist();
   if (threadIdx.x < 16) sh.powers.at[threadIdx.x] = exp2((double)threadIdx.x / 16.0);
   __syncthreads();
