@@ -1344,11 +1344,13 @@ struct PolicyRow {
     const double above = sum_up(mass, range.hi, by_mass);
     unsigned long long* sorted = ps_sorted();
     uint32_t n = 0;
-    for (uint32_t r = 0; r < k; ++r) {
-      const uint32_t m = sh.listed[r];
-      const unsigned long long* from = k > 1 ? ps_remote(list, r) : list;
-      for (uint32_t i = threadIdx.x; i < m; i += kPsThreads)
-        if (n + i < kPsList) sorted[n + i] = from[i];
+    for (uint32_t r = 0; r < k; ++r) {  // a warp or two to each CTA's list
+      const uint32_t m = sh.listed[r], warps = kPsWarps / k;
+      if ((uint32_t)warp / warps == r) {
+        const unsigned long long* from = k > 1 ? ps_remote(list, r) : list;
+        for (uint32_t i = threadIdx.x % (32u * warps); i < m; i += 32u * warps)
+          if (n + i < kPsList) sorted[n + i] = from[i];
+      }
       n += m;
     }
     n = min(n, kPsList);
@@ -1432,10 +1434,6 @@ struct PolicyRow {
     if (c.flat) range.inside = valid = at_least(c, top).count;  // the +inf ids
     const bool by_k = pol.top_k && pol.top_k < valid;
     if (!by_k && !by_mass) return;
-    if (found && found->inside <= kPsList) {
-      if (cut_from_list(c, *found, by_k ? pol.top_k : 0u, by_mass, pol.top_p, total)) return;
-      summed = {0.0, 0.0, ~0u};  // the range may have lain too low
-    }
     if (by_k) {
       if (found && !by_mass) range = *found;
       while (range.inside > kPsList && range.hi != range.lo) refine(c, range, pol.top_k, 0.0);
@@ -2066,13 +2064,21 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
         if (plain && measured && !c.flat) row.summed = {f.mass * factor, sum.mass, 0u};
       } else {
         PsRange range = {};
-        bool found = false;
+        bool found = false, listless = false;
         if (in_range && (measured || !mass_of_all)) {
           if constexpr (DT == kBF16) found = row.cut_by_values(c, pol, sum);
           else found = row.range_by_bins(c, pol, sum, lin, total, range);
         }
-        if (DT != kBF16 || !found) {
+        if (DT != kBF16 && found && range.inside <= kPsList) {
           __syncthreads();  // what the scans left in shared memory has been read
+          const bool by_k = pol.top_k && pol.top_k < sum.count;
+          found = row.cut_from_list(c, range, by_k ? pol.top_k : 0u, by_mass, pol.top_p, total);
+          if (!found) row.summed = {0.0, 0.0, ~0u};  // the range may have lain too low
+        } else if (DT != kBF16 || !found) {
+          __syncthreads();
+          listless = true;
+        }
+        if (listless || !found) {
           const auto o =
               row.find_cut_apart(c, pol, top, sum.count, total, found, range);
           c.keep(o.cut, o.take);
