@@ -194,7 +194,7 @@ struct PsShared {
   double entry_mass[2][kPsEntries];
   uint32_t entry_ties[kPsEntries], entry_before[kPsEntries];
   PsPowers powers;
-  PsCross cross[3];
+  PsCross cross[5];
   uint32_t listed[kPsMaxCluster];  // ids that each CTA listed
   uint32_t list_fill;
   int listed_by[kPsWarps];  // vectors that each warp gathered for the passes after the cut
@@ -982,7 +982,8 @@ struct PolicyRow {
     const bool by_mass = pol.top_p < 1.0, by_k = pol.top_k && pol.top_k < sum.count;
     // A bin's mass is its count times the weight of its middle, within 1/64 of it: the cut lies
     // between the bins in which that mass reaches the goal less 1/60 and plus 1/60 of it (with
-    // top-k the goal itself is as far off, so twice that).
+    // top-k the goal itself is as far off, so twice that). Where those hold many ids, no few of
+    // them carry the mass, the errors of the bins cancel, and 1/256 is some ten deviations.
     double mass = 0.0, weight_of[kPsOwn];
     uint32_t count = 0;
 #pragma unroll
@@ -999,7 +1000,7 @@ struct PolicyRow {
         w *= ratio;
       }
     }
-    if (threadIdx.x < 3) sh.cross[threadIdx.x].bin = -1;
+    if (threadIdx.x < 5) sh.cross[threadIdx.x].bin = -1;
     const Scanned scan = scan_parts(count, mass, by_mass);
     uint32_t through = 0;  // ids up to and with the last bin of the range
     int last = 0;
@@ -1030,39 +1031,40 @@ struct PolicyRow {
     }
     if (by_mass) {
       const double goal = top_p_goal(pol.top_p, total);
-      const double least = goal * (by_k ? 1.0 - 2.0 / 60.0 : 1.0 - 1.0 / 60.0);
-      if (count && scan.mass_before < least && least <= scan.mass_end) {
-        PsCross x = {scan.mass_before, scan.count_before, 0u, -1};
-        double run = scan.mass_before;
-        uint32_t run_count = scan.count_before;
+      // cross[at]: the bin in which the mass reaches `mark`, ids before it and in it
+      auto mark_bin = [&](int at, double mark) {
+        if (count && scan.mass_before < mark && mark <= scan.mass_end) {
+          PsCross x = {0.0, scan.count_before, 0u, -1};
+          double run = scan.mass_before;
 #pragma unroll
-        for (int j = 0; j < kPsOwn; ++j)
-          if (n[j] && run < least) {
-            x = {run, run_count, n[j], mine + j};
-            run += (double)n[j] * weight_of[j];
-            run_count += n[j];
-          }
-        sh.cross[1] = x;
-      }
-      const double most = goal * (1.0 + 1.0 / 60.0);
-      if (!by_k && count && scan.mass_before < most && most <= scan.mass_end) {
-        PsCross x = {0.0, scan.count_before, 0u, -1};
-        double run = scan.mass_before;
-#pragma unroll
-        for (int j = 0; j < kPsOwn; ++j)
-          if (n[j] && run < most) {
-            run += (double)n[j] * weight_of[j];
-            x.count += n[j];
-            x.bin = mine + j;
-          }
-        sh.cross[2] = x;
+          for (int j = 0; j < kPsOwn; ++j)
+            if (n[j] && run < mark) {
+              x.count += x.n;
+              x.n = n[j];
+              x.bin = mine + j;
+              run += (double)n[j] * weight_of[j];
+            }
+          sh.cross[at] = x;
+        }
+      };
+      mark_bin(1, goal * (by_k ? 1.0 - 2.0 / 60.0 : 1.0 - 1.0 / 60.0));
+      if (!by_k) {
+        mark_bin(2, goal * (1.0 + 1.0 / 60.0));
+        mark_bin(3, goal * (1.0 - 1.0 / 256.0));
+        mark_bin(4, goal * (1.0 + 1.0 / 256.0));
       }
       __syncthreads();
-      const PsCross x = sh.cross[1], y = sh.cross[2];
+      PsCross x = sh.cross[1];
       if (x.bin < 0) return false;
       if (!by_k) {
-        last = y.bin < 0 ? kPsBins - 1 : y.bin;
-        through = y.bin < 0 ? scan.count_all : y.count;
+        PsCross y = sh.cross[2];
+        if (y.bin < 0) y = {0.0, scan.count_all, 0u, kPsBins - 1};
+        if (y.count + y.n - x.count > kPsList && sh.cross[3].bin >= 0) {
+          x = sh.cross[3];
+          if (sh.cross[4].bin >= 0) y = sh.cross[4];
+        }
+        last = y.bin;
+        through = y.count + y.n;
       }
       range = {top_of_bin(lin, x.bin), 0u, x.count, through - x.count};
     }
