@@ -194,7 +194,7 @@ struct PsShared {
   double entry_mass[2][kPsEntries];
   uint32_t entry_ties[kPsEntries], entry_before[kPsEntries];
   PsPowers powers;
-  PsCross cross[5];
+  PsCross cross[7];
   uint32_t listed[kPsMaxCluster];  // ids that each CTA listed
   uint32_t list_fill;
   int listed_by[kPsWarps];  // vectors that each warp gathered for the passes after the cut
@@ -914,13 +914,13 @@ struct PolicyRow {
   }
 
   // ---- other types: the few bins that hold the cut ---------------------------------------
-  // Bins of equal width, 1/32 in the exponent of the weights, from 80 above the largest of a
-  // sample of the row's values to 48 below it, in falling order of value.
+  // Bins of equal width, 1/64 in the exponent of the weights, from 40 above the largest of a
+  // sample of the row's values to 24 below it, in falling order of value.
   struct Linear {
     float scale, shift;  // bin = round(shift - v scale) - 2^23
     bool ok;
   };
-  static constexpr float kBinsPerE = 32.0f, kBinsAbove = 2560.0f, kTwo23 = 8388608.0f;
+  static constexpr float kBinsPerE = 64.0f, kBinsAbove = 2560.0f, kTwo23 = 8388608.0f;
 
   __device__ __forceinline__ static uint32_t bin_of(const Linear& lin, float v) {
     return __float_as_uint(fmaf(v, -lin.scale, lin.shift)) - 0x4B000000u;
@@ -980,10 +980,12 @@ struct PolicyRow {
     if (c.flat || !lin.ok || bin_of(lin, (float)c.top) >= (uint32_t)kPsBins) return false;
     const int mine = threadIdx.x * kPsOwn;
     const bool by_mass = pol.top_p < 1.0, by_k = pol.top_k && pol.top_k < sum.count;
-    // A bin's mass is its count times the weight of its middle, within 1/64 of it: the cut lies
-    // between the bins in which that mass reaches the goal less 1/60 and plus 1/60 of it (with
-    // top-k the goal itself is as far off, so twice that). Where those hold many ids, no few of
-    // them carry the mass, the errors of the bins cancel, and 1/256 is some ten deviations.
+    // A bin's mass is its count times the weight of its middle, within 1/128 of it (the row's
+    // maximum counts as it is): the cut lies between the bins in which that mass reaches the
+    // goal less 1/120 and plus 1/120 of it (with top-k the goal itself is as far off, so twice
+    // that). Many ids there mean that few of them carry the mass alone; then the errors of the
+    // bins cancel, to some 3e-4 of the goal with a list of 200 by that bound and to 1e-4 where
+    // 1/512 still holds over 1,024: those rows take 1/512 and 1/1536, and the list is checked.
     double mass = 0.0, weight_of[kPsOwn];
     uint32_t count = 0;
 #pragma unroll
@@ -999,8 +1001,18 @@ struct PolicyRow {
         mass += (double)n[j] * w;
         w *= ratio;
       }
+      const int top_bin = (int)bin_of(lin, (float)c.top) - mine;
+      if (top_bin >= 0 && top_bin < kPsOwn) {
+#pragma unroll
+        for (int j = 0; j < kPsOwn; ++j)
+          if (j == top_bin) {
+            const double extra = (1.0 - weight_of[j]) / (double)n[j];
+            weight_of[j] += extra;
+            mass += (double)n[j] * extra;
+          }
+      }
     }
-    if (threadIdx.x < 5) sh.cross[threadIdx.x].bin = -1;
+    if (threadIdx.x < 7) sh.cross[threadIdx.x].bin = -1;
     const Scanned scan = scan_parts(count, mass, by_mass);
     uint32_t through = 0;  // ids up to and with the last bin of the range
     int last = 0;
@@ -1047,11 +1059,13 @@ struct PolicyRow {
           sh.cross[at] = x;
         }
       };
-      mark_bin(1, goal * (by_k ? 1.0 - 2.0 / 60.0 : 1.0 - 1.0 / 60.0));
+      mark_bin(1, goal * (by_k ? 1.0 - 2.0 / 120.0 : 1.0 - 1.0 / 120.0));
       if (!by_k) {
-        mark_bin(2, goal * (1.0 + 1.0 / 60.0));
-        mark_bin(3, goal * (1.0 - 1.0 / 256.0));
-        mark_bin(4, goal * (1.0 + 1.0 / 256.0));
+        mark_bin(2, goal * (1.0 + 1.0 / 120.0));
+        mark_bin(3, goal * (1.0 - 1.0 / 512.0));
+        mark_bin(4, goal * (1.0 + 1.0 / 512.0));
+        mark_bin(5, goal * (1.0 - 1.0 / 1536.0));
+        mark_bin(6, goal * (1.0 + 1.0 / 1536.0));
       }
       __syncthreads();
       PsCross x = sh.cross[1];
@@ -1059,10 +1073,11 @@ struct PolicyRow {
       if (!by_k) {
         PsCross y = sh.cross[2];
         if (y.bin < 0) y = {0.0, scan.count_all, 0u, kPsBins - 1};
-        if (y.count + y.n - x.count > kPsList && sh.cross[3].bin >= 0) {
-          x = sh.cross[3];
-          if (sh.cross[4].bin >= 0) y = sh.cross[4];
-        }
+#pragma unroll
+        for (int at = 3; at <= 5; at += 2)
+          if (y.count + y.n - x.count > (at == 3 ? 192u : kPsList) && sh.cross[at].bin >= 0 &&
+              sh.cross[at + 1].bin >= 0)
+            x = sh.cross[at], y = sh.cross[at + 1];
         last = y.bin;
         through = y.count + y.n;
       }
