@@ -101,6 +101,23 @@ def pack_policies(policies: SamplingPolicy | Iterable[SamplingPolicy],
     return (rows[0] if single else rows).to(device)
 
 
+# the current stream's handle without a Stream object around it (2 us a call less)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _call(name: str, index: int, *args: object) -> None:
+    """One C call on device ``index``, on its current stream; raises on an error code."""
+    lib = _lib.load()
+    if torch.cuda.current_device() == index:
+        code = getattr(lib, name)(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            code = getattr(lib, name)(*args, _raw_stream(index))
+    if code:
+        _lib.check(name, code)
+
+
 def _logit_code(dtype: torch.dtype) -> int:
     code = _LOGIT_DTYPES.get(dtype)
     if code is None:
@@ -176,21 +193,11 @@ def policy_sample(logits: torch.Tensor, bitmask: torch.Tensor | None, policies: 
         uniforms = uniforms.contiguous()
     idx = torch.empty(rows, dtype=torch.int32, device=device)
     status = torch.empty(rows, dtype=torch.int32, device=device)
-    if rows == 0:
-        return _ms.MaskedArgmaxResult(idx, status)
-    lib = _lib.load()
-    with torch.cuda.device(device):
-        stream = torch.cuda.current_stream(device)
-        _lib.check(
-            "onyx_policy_sample",
-            lib.onyx_policy_sample(
-                x.data_ptr(), code, rows, vocab, x.stride(0) if rows > 1 else vocab,
-                None if m is None else m.data_ptr(), 0 if m is None else m.stride(0),
-                pol.data_ptr(), pol_stride, uniforms.data_ptr(), u_code,
-                uniforms.stride(0) if rows > 1 else 1, idx.data_ptr(), status.data_ptr(),
-                stream.cuda_stream,
-            ),
-        )
+    if rows:
+        _call("onyx_policy_sample", device.index, x.data_ptr(), code, rows, vocab,
+              x.stride(0) if rows > 1 else vocab, None if m is None else m.data_ptr(),
+              0 if m is None else m.stride(0), pol.data_ptr(), pol_stride, uniforms.data_ptr(),
+              u_code, uniforms.stride(0) if rows > 1 else 1, idx.data_ptr(), status.data_ptr())
     return _ms.MaskedArgmaxResult(idx, status)
 
 
@@ -217,20 +224,11 @@ def policy_probs(logits: torch.Tensor, bitmask: torch.Tensor | None, policies: t
             raise ValueError("out must not share memory with logits")
     device = _ms._same_device(x, pol, out, *(() if m is None else (m,)))
     status = torch.empty(rows, dtype=torch.int32, device=device)
-    if rows == 0:
-        return out, status
-    lib = _lib.load()
-    with torch.cuda.device(device):
-        stream = torch.cuda.current_stream(device)
-        _lib.check(
-            "onyx_policy_probs",
-            lib.onyx_policy_probs(
-                x.data_ptr(), code, rows, vocab, x.stride(0) if rows > 1 else vocab,
-                None if m is None else m.data_ptr(), 0 if m is None else m.stride(0),
-                pol.data_ptr(), pol_stride, out.data_ptr(), out.stride(0) if rows > 1 else vocab,
-                status.data_ptr(), stream.cuda_stream,
-            ),
-        )
+    if rows:
+        _call("onyx_policy_probs", device.index, x.data_ptr(), code, rows, vocab,
+              x.stride(0) if rows > 1 else vocab, None if m is None else m.data_ptr(),
+              0 if m is None else m.stride(0), pol.data_ptr(), pol_stride, out.data_ptr(),
+              out.stride(0) if rows > 1 else vocab, status.data_ptr())
     return out, status
 
 
@@ -302,28 +300,17 @@ def spec_sample(logits: torch.Tensor, bitmasks: torch.Tensor | None, drafts: tor
     accept = torch.empty(batch, dtype=torch.int32, device=device)
     token = torch.empty(batch, dtype=torch.int32, device=device)
     status = torch.empty(batch, dtype=torch.int32, device=device)
-    if batch == 0:
-        return _ms.SpecVerifyResult(accept, token, status)
-    lib = _lib.load()
-    with torch.cuda.device(device):
-        stream = torch.cuda.current_stream(device)
-        ws = torch.empty(lib.onyx_spec_sample_workspace_size(batch, gamma), dtype=torch.uint8,
-                         device=device)
-        _lib.check(
-            "onyx_spec_sample",
-            lib.onyx_spec_sample(
-                logits.data_ptr(), code, batch, gamma, vocab,
-                logits.stride(0) if batch > 1 else 0, logits.stride(1),
-                None if bitmasks is None else bitmasks.data_ptr(),
-                0 if bitmasks is None or batch == 1 else bitmasks.stride(0),
-                0 if bitmasks is None else bitmasks.stride(1), drafts.data_ptr(),
-                drafts.stride(0) if batch > 1 else gamma, None if q is None else q.data_ptr(),
-                0 if q is None or batch == 1 else q.stride(0),
-                vocab if q is None or gamma == 1 else q.stride(1),
-                None if draft_lens is None else draft_lens.data_ptr(), pol.data_ptr(),
-                pol_stride, uniforms.data_ptr(), u_code,
-                uniforms.stride(0) if batch > 1 else g1, accept.data_ptr(), token.data_ptr(),
-                status.data_ptr(), ws.data_ptr(), ws.numel(), stream.cuda_stream,
-            ),
-        )
+    if batch:
+        ws = torch.empty(batch * g1 * 16, dtype=torch.uint8, device=device)
+        _call("onyx_spec_sample", device.index, logits.data_ptr(), code, batch, gamma, vocab,
+              logits.stride(0) if batch > 1 else 0, logits.stride(1),
+              None if bitmasks is None else bitmasks.data_ptr(),
+              0 if bitmasks is None or batch == 1 else bitmasks.stride(0),
+              0 if bitmasks is None else bitmasks.stride(1), drafts.data_ptr(),
+              drafts.stride(0) if batch > 1 else gamma, None if q is None else q.data_ptr(),
+              0 if q is None or batch == 1 else q.stride(0),
+              vocab if q is None or gamma == 1 else q.stride(1),
+              None if draft_lens is None else draft_lens.data_ptr(), pol.data_ptr(), pol_stride,
+              uniforms.data_ptr(), u_code, uniforms.stride(0) if batch > 1 else g1,
+              accept.data_ptr(), token.data_ptr(), status.data_ptr(), ws.data_ptr(), ws.numel())
     return _ms.SpecVerifyResult(accept, token, status)
