@@ -60,11 +60,14 @@ static PolicyPlan plan_with(int k, int64_t vocab, int dtype, bool masked) {
   return pl;
 }
 
-// CTAs per row: a power of two, as many as the SMs hold two of, at least 4,096 ids each; and
-// as many as it takes to have two CTAs on an SM.
+// CTAs per row: a power of two, as many as the SMs hold two of, at least 2,048 ids each (one
+// row of 32,000: 23 us with 4, 22 with 8); two at least for long rows, for a batch waits for
+// its slowest rows, those whose kept ids are many (256 rows of 128,256 under mixed policies: 94
+// us with 1, 85 with 2; 64 x 8 float16 rows: 273 and 185); and as many as it takes to have two
+// CTAs on an SM.
 static PolicyPlan make_plan(int64_t rows, int64_t vocab, int dtype, bool masked, int sms) {
-  int k = 1;
-  while (k < kPsMaxCluster && rows * k * 2 <= 2ll * sms && vocab >= 2ll * k * 4096) k *= 2;
+  int k = vocab > 65536 ? 2 : 1;
+  while (k < kPsMaxCluster && rows * k * 2 <= 2ll * sms && vocab >= 2ll * k * 1950) k *= 2;
   PolicyPlan pl = plan_with(k, vocab, dtype, masked);
   while (k < kPsMaxCluster && pl.smem > kPsTwoFit) {
     k *= 2;
