@@ -268,8 +268,19 @@ int onyx_spec_sample(const void* logits, int dtype, int64_t batch, int64_t gamma
   p.dp_row_stride = dp_row_stride;
   p.draft_lens = draft_lens;
   p.results = static_cast<int4*>(workspace);
-  const int rc2 = launch_policy<kOpSpec>(dtype, p, batch * (gamma + 1), (cudaStream_t)stream);
-  if (rc2 != ONYX_OK) return rc2;
+  // As many rows of every entry to a launch as the SMs hold at once (two CTAs each, two to a
+  // row): the rows behind a refusal need not be read, and the next launch sees it.
+  cudaError_t e;
+  const int sms = device_sms(&e);
+  if (!sms) return finish_launch(e);
+  const int64_t together = std::max<int64_t>(1, 2ll * sms / batch);
+  for (int64_t from = 0; from <= gamma; from += together) {
+    p.sub_from = (int32_t)from;
+    p.sub_count = (int32_t)std::min<int64_t>(together, gamma + 1 - from);
+    const int rc2 =
+        launch_policy<kOpSpec>(dtype, p, batch * p.sub_count, (cudaStream_t)stream);
+    if (rc2 != ONYX_OK) return rc2;
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((batch + 127) / 128), 1, 1);
   cfg.blockDim = dim3(128, 1, 1);

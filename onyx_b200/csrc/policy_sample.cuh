@@ -76,6 +76,7 @@ struct PolicyParams {
   int64_t uniform_stride;
   int32_t uniform_f64;
   int32_t per_group;  // rows per entry: 1, or gamma + 1
+  int32_t sub_from, sub_count;  // spec: rows of every entry that this launch takes
   int32_t* out_idx;
   uint32_t* out_status;
   float* out_probs;
@@ -2013,9 +2014,13 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
   if (k > 1) ps_cluster_arrive();
   asm volatile("griddepcontrol.launch_dependents;" :::);
 
-  const int64_t item = (int64_t)(blockIdx.x / k);
-  const int64_t group = OP == kOpSpec ? item / p.per_group : item;
-  const int sub = OP == kOpSpec ? (int)(item - group * p.per_group) : 0;
+  int64_t item = (int64_t)(blockIdx.x / k), group = item;
+  int sub = 0;
+  if (OP == kOpSpec) {
+    group = item / p.sub_count;
+    sub = p.sub_from + (int)(item - group * p.sub_count);
+    item = group * p.per_group + sub;
+  }
 
   Row row(sh);
   row.rank = k > 1 ? ps_rank() : 0u;
@@ -2048,6 +2053,18 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
 
   // what came before on the stream has written the inputs
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (OP == kOpSpec && p.sub_from > 0) {
+    // an earlier launch may have decided the entry (rows past its drafts wrote nothing)
+    const int rows =
+        min(p.sub_from, p.draft_lens ? p.draft_lens[group] + 1 : p.per_group);
+    bool decided = false;
+    for (int i = 0; i < rows; ++i)
+      decided |= p.results[group * p.per_group + i].x == kDecided;
+    if (decided) {
+      if (k > 1) ps_cluster_wait();
+      return;
+    }
+  }
   view.start_stream(row.lane);  // the copies run while the policy is read
 
   const RowPolicy pol = load_policy(p.policies + group * p.policy_stride);
