@@ -206,8 +206,8 @@ ONYX_API int onyx_masked_sample(const void* logits, int dtype, int64_t rows, int
  * exp((v - max) / temperature) in float64; where any value is +inf the +inf ids share the
  * mass alone; temperature 0 keeps the first maximum alone. Ids are ranked by value, the
  * lowest id first among equals. top_k keeps the first k of the ranking; top_p the shortest
- * prefix of those whose mass reaches top_p times their mass (1: off; within 2^-44 of it has
- * reached it, which covers what the float64 sums round); min_p the ids whose
+ * prefix of those whose mass reaches top_p times their mass (1: off; float32 and float16: a
+ * mass within 2^-48 of that has reached it, which covers what the sums round); min_p the ids whose
  * weight is at least min_p times the largest. With top_k = 0 and min_p = 0 this is the
  * distribution of onyx_masked_sample, the reference's _filtered_reference_weights
  * (onyx_cuda/src/onyx_cuda/selection.py); only where the mass reaches top_p exactly (equal

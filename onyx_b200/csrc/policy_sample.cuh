@@ -168,7 +168,7 @@ struct PsPowers {
 
 struct PsBox {  // one CTA's part of a cluster-wide reduction
   double mass;
-  uint32_t count, top, small, low;
+  uint32_t count, top, small;
 };
 
 struct PsCross {  // the bin in which a count or a mass is reached
@@ -560,19 +560,19 @@ struct RowView {
 };
 
 // 2^(y/16) for |y| < 2^20. Table-driven in the manner of Tang (ACM TOMS 15, 1989): y = 16 e + j
-// + f with |f| <= 1/2, 2^(f/16) by its Taylor polynomial, the term of degree 6 folded into
-// those of degree 4 and 2 (Chebyshev): within 1e-14 of the value, and 1 for y = 0. The 16
-// entries take the 16 pairs of banks, so lookups of a warp do not conflict.
+// + f with |f| <= 1/2, 2^(f/16) by its Taylor polynomial of degree 6 (the next term is below
+// 5e-16): within 2^-50 of the value, and 1 for y = 0. The 16 entries take the 16 pairs of
+// banks, so lookups of a warp do not conflict.
 constexpr double kPsShift = 0x1.8p52;
 __device__ __forceinline__ double exp2_parts(double t, double f, const PsPowers& powers) {
   const int n = __double2loint(t);
   // (ln 2 / 16)^k / k!
   constexpr double c1 = 0.6931471805599453 / 16.0, c2 = c1 * c1 / 2.0, c3 = c2 * c1 / 3.0;
   constexpr double c4 = c3 * c1 / 4.0, c5 = c4 * c1 / 5.0, c6 = c5 * c1 / 6.0;
-  double q = c5;
-  q = fma(q, f, c4 + c6 * 1.5 * 0.25);
+  double q = fma(c6, f, c5);
+  q = fma(q, f, c4);
   q = fma(q, f, c3);
-  q = fma(q, f, c2 - c6 * 0.5625 * 0.0625);
+  q = fma(q, f, c2);
   q = fma(q, f, c1);
   const double w = powers.at[n & 15];
   const double r = fma(w * f, q, w);
@@ -624,13 +624,6 @@ struct RowCut {
     if (take && weight(cut) < min_p) take = 0u;
   }
 };
-
-// The mass that top-p has to reach. The sums that are held against it carry errors of some
-// 2^-50 of the total; the factor lets a mass that equals the goal (equal values: 270 of 300 ids
-// at 0.9) reach it whatever the order of summation.
-__device__ __forceinline__ double top_p_goal(double top_p, double total) {
-  return top_p * total * (1.0 - 0x1p-44);
-}
 
 // A range of order codes that holds the cut.
 struct PsRange {
@@ -880,7 +873,7 @@ struct PolicyRow {
     }
     if (by_mass) {
       if (!by_k && behind_weighs) return false;
-      const double goal = top_p_goal(pol.top_p, total);
+      const double goal = pol.top_p * total;
       if (count && mine <= cut_bin && mass_before < goal &&
           (goal <= mass_end || cut_bin < mine + kPsOwn)) {
         PsCross x = {mass_before, 0u, 0u, -1};  // the bin that reaches the goal, else the last
@@ -1043,7 +1036,7 @@ struct PolicyRow {
       if (!by_mass) range = {top_of_bin(lin, x.bin), 0u, x.count, x.n};
     }
     if (by_mass) {
-      const double goal = top_p_goal(pol.top_p, total);
+      const double goal = pol.top_p * total;
       // cross[at]: the bin in which the mass reaches `mark`, ids before it and in it
       auto mark_bin = [&](int at, double mark) {
         if (count && scan.mass_before < mark && mark <= scan.mass_end) {
@@ -1468,7 +1461,7 @@ struct PolicyRow {
       const Scanned scan = scan_parts(0u, w0 + w1, true);
       const double end = scan.mass_end, before = scan.mass_before;
       if (rank_k) total = above + scan.mass_all;
-      const double goal = top_p_goal(top_p, total);
+      const double goal = top_p * total;
       holds = holds && above < goal && (rank_k || above + scan.mass_all >= goal);
       uint32_t mine = have - 1u;
       if (at < have && above + before + w0 >= goal) mine = at;
@@ -1515,7 +1508,7 @@ struct PolicyRow {
       const PsBox b = at_least(c, ord32(c.cut) + 1u);
       const double w = c.weight(c.cut);
       total = b.mass + (double)c.take * w;
-      const double goal = top_p_goal(pol.top_p, total);
+      const double goal = pol.top_p * total;
       if (b.mass < goal) {
         c.take = ties_to_reach(goal - b.mass, w, c.take, b.mass, goal);
         return;
@@ -1524,7 +1517,7 @@ struct PolicyRow {
     } else {
       if (total < 0.0) total = at_least(c, range.lo).mass;
     }
-    const double goal = top_p_goal(pol.top_p, total);
+    const double goal = pol.top_p * total;
     const PsRange all = range;
     for (bool guess = found && !by_k;; guess = false) {
       range = guess ? *found : all;
@@ -2150,7 +2143,10 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
       // (not if the temperature is so low that the pass could not tell `from` from its floor)
       const bool measured =
           mass_of_all && in_range && (double)(float)(from - 15000.0 / c.scale) < from - 1e-30;
-      const double total = measured ? sum.mass : -1.0;
+      // What top-p measures by. Relative to the maximum equal values weigh exactly 1, and a mass
+      // that equals its goal (270 of 300 equal ids at 0.9) has reached it; the sums relative to
+      // `from` round each weight, by some 2^-51 of it, and the factor keeps that so.
+      const double total = measured ? sum.mass * (1.0 - 0x1p-48) : -1.0;
       if (!cuts) {
         if (pol.temperature > 0.0) c.cut = c.flat ? FLT_MAX : -INFINITY;
         else c.keep(code_value(top), 1u);
