@@ -225,6 +225,53 @@ def test_ties_at_the_cut(dtype, cuda_lib):
             check(x, None, dtype, table(policy, 4), np.full(4, u), probs=u == 0.25)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+def test_ways_to_the_cut(dtype, cuda_lib):
+    """Rows and policies that take each way to the cut: log-probabilities (all negative), one id
+    far above the rest, most ids at the type's lowest value, values next to zero, steps of many
+    equal values, wide and narrow ones; temperatures that keep one id and tens of thousands;
+    top-k below, at and past the lengths of the lists."""
+    rng = np.random.default_rng(70 + len(dtype))
+    vocab = 30011
+    x = rng.standard_normal((9, vocab)) * 3
+    x[1] -= np.log(np.exp(x[1]).sum()) + 30
+    x[2, 12345] = 45.0
+    x[3, rng.random(vocab) < 0.8] = -65504.0
+    x[4] *= 1e-4
+    x[5] = np.round(x[5])
+    x[6] *= 20
+    x[7] = rng.random(vocab) * 0.1 + 200.0
+    x[8, :20000] = -np.inf
+    x = rounded(x, dtype)
+    m = workloads.bernoulli_masks(rng, np.full(9, 0.3), vocab)
+    for policy in ((0.8, 0, 0.9, 0.0), (1.2, 0, 0.95, 0.0), (3.0, 0, 0.99, 0.0), (0.05, 0, 0.9, 0.0),
+                   (1.0, 512, 0.9, 0.0), (1.0, 513, 0.9, 0.0), (1.0, 1500, 1.0, 0.0),
+                   (2.0, 5000, 0.7, 0.01), (1.0, 0, 0.999999, 0.0), (0.7, 3, 0.5, 0.0)):
+        check(x, None, dtype, table(policy, 9), rng.random(9), probs=policy[0] != 3.0)
+        check(x, m, dtype, table(policy, 9), rng.random(9), probs=policy[0] == 2.0)
+
+
+def test_rows_past_the_peaks(cuda_lib):
+    """2.2 million ids: parts of a row too long for their peaks, read whole in every pass."""
+    rng = np.random.default_rng(81)
+    for dtype in ("bf16", "f32"):
+        x = normal(rng, (1, 2_200_003), dtype)
+        check(x, None, dtype, table(POLICIES["top_p"], 1), rng.random(1), probs=False)
+        check(x, None, dtype, table(POLICIES["all"], 1), rng.random(1), probs=False)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_rows_of_every_alignment(dtype, cuda_lib):
+    """Rows that follow each other without padding start at every offset from 16 bytes."""
+    rng = np.random.default_rng(90)
+    for vocab in (1001, 20003, 70001):
+        x = normal(rng, (9, vocab), dtype)
+        m = workloads.bernoulli_masks(rng, rng.uniform(0.1, 0.9, 9), vocab)
+        for policy in ("top_p", "all", "plain"):
+            check(x, m, dtype, table(POLICIES[policy], 9), rng.random(9), probs=policy == "all")
+            check(x, None, dtype, table(POLICIES[policy], 9), rng.random(9), probs=False)
+
+
 def test_nearly_equal_float32_values(cuda_lib):
     """float32 values that agree in all but their last bits, thousands in the same place."""
     rng = np.random.default_rng(12)
@@ -446,7 +493,8 @@ def test_spec_accepts_and_refuses(cuda_lib):
 
 
 @pytest.mark.parametrize("batch,gamma,vocab", [(1, 1, 5), (1, 1, 40000), (1, 7, 20000),
-                                               (3, 255, 70), (150, 1, 300), (40, 4, 9001)])
+                                               (3, 255, 70), (150, 1, 300), (40, 4, 9001),
+                                               (500, 3, 700)])
 def test_spec_shapes(batch, gamma, vocab, cuda_lib):
     rng = np.random.default_rng(batch * 1000 + gamma)
     x, m, q, d, u = spec_inputs(rng, batch, gamma, vocab, "bf16", noise=0.1)
@@ -599,6 +647,29 @@ def test_streams_and_graph_replay(cuda_lib):
             assert torch.equal(got, want)
         for got, want in zip(other, eager[2]):
             assert torch.equal(got, want)
+
+
+def test_calls_at_once_on_two_streams(cuda_lib):
+    """Each call has a workspace of its own, so calls on two streams may overlap."""
+    rng = np.random.default_rng(55)
+    x, m, q, d, u = spec_inputs(rng, 6, 3, 40009, "f16", noise=0.2)
+    pol = gpu(np.stack([POLICIES[n] for n in ("top_p", "all", "plain", "top_k", "greedy",
+                                              "min_p")]))
+    args = (to_device(x, "f16"), masks_to_device(m), torch.from_numpy(d).cuda(), pol, gpu(u))
+    qt = torch.from_numpy(q).cuda()
+    want = ox.spec_sample(*args, draft_probs=qt)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for _ in range(10):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(ox.spec_sample(*args, draft_probs=qt))
+    torch.cuda.synchronize()
+    for r in got:
+        for a, b in zip((r.accept_len, r.correction, r.status),
+                        (want.accept_len, want.correction, want.status)):
+            assert torch.equal(a, b)
 
 
 def test_repeated_calls_give_the_same_bits(cuda_lib):
