@@ -195,7 +195,7 @@ struct PsShared {
   double entry_mass[2][kPsEntries];
   uint32_t entry_ties[kPsEntries], entry_before[kPsEntries];
   PsPowers powers;
-  PsCross cross[7];
+  PsCross cross[9];
   uint32_t listed[kPsMaxCluster];  // ids that each CTA listed
   uint32_t list_fill;
   int listed_by[kPsWarps];  // vectors that each warp gathered for the passes after the cut
@@ -966,9 +966,10 @@ struct PolicyRow {
   }
 
   // The range of codes that holds the cut, with top-k and top-p both also the k-th value; false
-  // where the bins do not tell. `total` is the mass of all ids, if top-p needs it.
+  // where the bins do not tell. `total` is the mass of all ids, if top-p needs it. `safe` holds
+  // it surely, `range` in all likelihood.
   __device__ bool range_by_bins(const RowCut& c, const RowPolicy& pol, const PsBox& sum,
-                                const Linear& lin, double total, PsRange& range) {
+                                const Linear& lin, double total, PsRange& range, PsRange& safe) {
     uint32_t n[kPsOwn];
     merge_bins(n, false);
     if (c.flat || !lin.ok || bin_of(lin, (float)c.top) >= (uint32_t)kPsBins) return false;
@@ -978,8 +979,9 @@ struct PolicyRow {
     // maximum counts as it is): the cut lies between the bins in which that mass reaches the
     // goal less 1/120 and plus 1/120 of it (with top-k the goal itself is as far off, so twice
     // that). Many ids there mean that few of them carry the mass alone; then the errors of the
-    // bins cancel, to some 3e-4 of the goal with a list of 200 by that bound and to 1e-4 where
-    // 1/512 still holds over 1,024: those rows take 1/512 and 1/1536, and the list is checked.
+    // bins cancel: to some 5e-4 of the goal with a list of 200 by that bound, to 2e-4 where 1/320
+    // still holds over 1,024. Such rows take the widest of 1/320, 1/700 and 1/1536 that makes a
+    // list, and the list is checked (of 96,000 rows some 20 fail there).
     double mass = 0.0, weight_of[kPsOwn];
     uint32_t count = 0;
 #pragma unroll
@@ -1006,7 +1008,7 @@ struct PolicyRow {
           }
       }
     }
-    if (threadIdx.x < 7) sh.cross[threadIdx.x].bin = -1;
+    if (threadIdx.x < 9) sh.cross[threadIdx.x].bin = -1;
     const Scanned scan = scan_parts(count, mass, by_mass);
     uint32_t through = 0;  // ids up to and with the last bin of the range
     int last = 0;
@@ -1056,10 +1058,12 @@ struct PolicyRow {
       mark_bin(1, goal * (by_k ? 1.0 - 2.0 / 120.0 : 1.0 - 1.0 / 120.0));
       if (!by_k) {
         mark_bin(2, goal * (1.0 + 1.0 / 120.0));
-        mark_bin(3, goal * (1.0 - 1.0 / 512.0));
-        mark_bin(4, goal * (1.0 + 1.0 / 512.0));
-        mark_bin(5, goal * (1.0 - 1.0 / 1536.0));
-        mark_bin(6, goal * (1.0 + 1.0 / 1536.0));
+        mark_bin(3, goal * (1.0 - 1.0 / 320.0));
+        mark_bin(4, goal * (1.0 + 1.0 / 320.0));
+        mark_bin(5, goal * (1.0 - 1.0 / 700.0));
+        mark_bin(6, goal * (1.0 + 1.0 / 700.0));
+        mark_bin(7, goal * (1.0 - 1.0 / 1536.0));
+        mark_bin(8, goal * (1.0 + 1.0 / 1536.0));
       }
       __syncthreads();
       PsCross x = sh.cross[1];
@@ -1067,8 +1071,12 @@ struct PolicyRow {
       if (!by_k) {
         PsCross y = sh.cross[2];
         if (y.bin < 0) y = {0.0, scan.count_all, 0u, kPsBins - 1};
+        safe.above = x.count;
+        safe.inside = y.count + y.n - x.count;
+        safe.hi = top_of_bin(lin, x.bin);
+        safe.lo = top_of_bin(lin, y.bin + 1) + 1u;
 #pragma unroll
-        for (int at = 3; at <= 5; at += 2)
+        for (int at = 3; at <= 7; at += 2)
           if (y.count + y.n - x.count > (at == 3 ? 192u : kPsList) && sh.cross[at].bin >= 0 &&
               sh.cross[at + 1].bin >= 0)
             x = sh.cross[at], y = sh.cross[at + 1];
@@ -1079,7 +1087,8 @@ struct PolicyRow {
     }
     const uint32_t below = top_of_bin(lin, last + 1);
     range.lo = below + 1u;
-    return range.hi && below && range.lo <= range.hi;
+    if (by_k || !by_mass) safe = range;
+    return range.hi && below && range.lo <= range.hi && safe.hi && safe.lo > 1u;
   }
 
   // ---- top-k by the peaks ----------------------------------------------------------------
@@ -2152,27 +2161,32 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
         else c.keep(code_value(top), 1u);
         if (plain && measured && !c.flat) row.summed = {f.mass * factor, sum.mass, 0u};
       } else {
-        PsRange range = {};
-        bool found = false, listless = false;
+        PsRange range = {}, safe = {};
+        bool found = false, near = false;
         if (by_peaks) {
           if constexpr (DT != kBF16)
             found = !c.flat && row.range_by_peaks(pol, top, sum.count, range);
         } else if (in_range && (measured || !mass_of_all)) {
           if constexpr (DT == kBF16) found = row.cut_by_values(c, pol, sum);
-          else found = row.range_by_bins(c, pol, sum, lin, total, range);
+          else found = row.range_by_bins(c, pol, sum, lin, total, range, safe);
         }
         if (DT != kBF16 && found && (by_peaks || range.inside <= kPsList)) {
           __syncthreads();  // what the scans left in shared memory has been read
           const bool by_k = by_peaks || (pol.top_k && pol.top_k < sum.count);
           found = row.cut_from_list(c, range, by_k ? pol.top_k : 0u, by_mass, pol.top_p, total);
-          if (!found) row.summed = {0.0, 0.0, ~0u};  // the range may have lain too low
+          if (!found) {  // the range lay too low, or was too long for a list
+            row.summed = {0.0, 0.0, ~0u};
+            near = !by_peaks && !by_k;
+            range = safe;
+          }
         } else if (DT != kBF16 || !found) {
-          __syncthreads();
-          listless = true;
+          near = found;
+          found = false;
         }
-        if (listless || !found) {
+        if (!found) {
+          __syncthreads();  // (as above)
           const auto o =
-              row.find_cut_apart(c, pol, top, sum.count, total, found, range);
+              row.find_cut_apart(c, pol, top, sum.count, total, near, range);
           c.keep(o.cut, o.take);
           row.parity = o.parity;
           row.summed = o.summed;
