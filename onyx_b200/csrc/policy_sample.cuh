@@ -17,26 +17,42 @@
 // about one row in a hundred.
 //
 // Shape of the work. One cluster of k CTAs per row (k = 1, 2, 4 or 8, the more the fewer the
-// rows); CTA ranks, the warps of a CTA and the 256-id chunks of a warp follow id order, a lane
-// holding 8 consecutive ids.
-//   1  One pass reads the row from HBM: its maximum, the maximum of every 8 ids (the peaks,
-//      kept in shared memory), and a histogram with a bin for every value of bfloat16
-//      precision, |v| in [2^-9, 2^7) -- 4,096 bins. For float32 and float16 rows whose top-p
-//      needs the whole mass it also sums the weights.
+// rows), 512 threads each, two CTAs to an SM; CTA ranks, the warps of a CTA and the 256-id
+// chunks of a warp follow id order, a lane holding 8 consecutive ids (one or two 16-byte
+// vectors in memory, whatever the row's alignment).
+//   1  first_pass(): each warp copies its part of the row into shared memory (cp.async, all of
+//      it at once where it fits, else through a ring) and finds the maximum, the maximum of
+//      every 8 ids (the peaks, which stay in shared memory) and, as the policy asks, a
+//      histogram of 4,096 bins and the sum of the weights. The only pass over all values.
 //   2  The histograms of the CTAs are added up (each CTA a part of the bins, over distributed
-//      shared memory) and every CTA scans all bins in falling order of value. For bfloat16 a
-//      bin is one value, count times weight its mass, and the scan yields the cut. For the
-//      other types it yields the few bins that hold the cut.
-//   3  Those bins' ids (a few dozen as a rule) are listed, sorted by value and id and summed
-//      exactly. Where the list would be long the same histogram is taken again over the
-//      remaining range of order codes, a 4096th of it to a bin.
-//   4  The kept mass is summed by warps (the peaks name the vectors to read again, from L1 or
-//      L2), the warps' sums are scanned, and the warp whose interval holds u draws.
-// Rows that step 2 cannot serve (values of 2^7 and more, a cut among values next to zero)
-// start step 3 from the whole range of codes. No row length is bound to shared memory.
+//      shared memory) and every CTA scans the bins in falling order of value.
+//      bfloat16 (cut_by_values): a bin is one value, its mass count times weight, and the scan
+//      yields the cut. No weight is computed for an id: 8 bins share two exponentials.
+//      float32, float16 (range_by_bins): bins of 1/64 in the exponent around a sample of the
+//      row. They yield the few bins that hold the cut; a small top-k takes a histogram of the
+//      peaks instead (range_by_peaks).
+//   3  cut_from_list(), float32 and float16: the ids of those bins (a few dozen to a few
+//      hundred) are listed, sorted by value and summed exactly.
+//   4  The kept mass is summed by warps over lists of the vectors whose peak reaches the cut,
+//      the warps' sums are scanned, and the warp whose interval holds u draws (a long list is
+//      drawn by all warps of its CTA, piece by piece).
+// Rows that steps 2 and 3 cannot serve (bfloat16 values of 2^7 and more, a cut among values
+// next to zero, float32 maxima 40 T above the sample, lists over 1,024 ids) go through
+// find_cut(): the histogram over ranges of order codes, each turn a 4096th of the last. No row
+// length is bound to shared memory.
 //
 // Every CTA of a cluster computes the same totals from the same parts in the same order, so
-// all take the same branches, and the result does not depend on timing.
+// all take the same branches, and the result does not depend on timing. (Histograms are counts,
+// whose sums do not depend on the order of the atomics; lists are sorted by value and id.)
+//
+// What bounds it. 256 rows of 128,256 bfloat16 (65.7 MB, 10.2 us of copying at 6,464 GB/s), one
+// policy for all: instructions. The maximum alone takes 31 us and 154 warp instructions a chunk of
+// 256 ids, over the whole kernel; with top-k 50, so with the histogram and its cut, 65 us and
+// 345, the histogram's atomics meeting 2.8 bank conflicts each; DRAM is 20 and 11 % busy, the
+// issue slots 58 and 65 %. One row of 128,256 takes 15 us under top-p 0.9: a chain of latencies,
+// 8 us of it without any histogram. A batch under mixed policies waits for its slowest rows,
+// those that keep tens of thousands of ids (T = 1.2, top-p 0.95: 139 us, against 75 under
+// T = 0.8, top-p 0.9).
 #pragma once
 
 #include <cfloat>
@@ -1433,8 +1449,8 @@ struct PolicyRow {
     for (uint32_t i = n + threadIdx.x; i < size; i += kPsThreads) sorted[i] = ~0ull;
     __syncthreads();
     if (n <= 256u) {
-      // each key's place is the count of the smaller ones, by up to 32 threads to a key (128
-      // keys: 0.4 us, where the bitonic sort takes 4)
+      // each key's place is the count of the smaller ones, by up to 32 threads to a key: one
+      // pass over the keys, where the sort below has up to 36 steps that wait for one another
       const uint32_t group = min(32u, kPsThreads / max(size, 16u)), part = threadIdx.x % group;
       const uint32_t i = threadIdx.x / group;
       const unsigned long long key = i < n ? sorted[i] : 0ull;
@@ -1859,9 +1875,9 @@ struct PsFirst {
 };
 
 // The pass behind the copies of start_stream(): peaks, and with BINS the histogram, with MASS
-// the weights. One loop for each of the four, on scalars of its own: the first version, a
-// lambda called from a method of the view, took 150 instructions a chunk where this takes 35
-// (256 rows of 128,256, the maximum alone: 34 us, now 15).
+// the weights. One loop for each of the four, on scalars of its own, and the chunks at the edges
+// of a row apart from it: as one lambda called from a method of the view, 256 rows of 128,256
+// bfloat16 took 34 us for the maximum alone with one CTA a row, and 23 so.
 template <int DT, bool BINS, bool MASS>
 __device__ __forceinline__ PsFirst first_pass(const RowView<DT>& view, int lane,
                                               const typename PolicyRow<DT>::Linear& bins,
@@ -2057,8 +2073,8 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (OP == kOpSpec && p.sub_from > 0) {
     // an earlier launch may have decided the entry (rows past its drafts wrote nothing)
-    const int rows =
-        min(p.sub_from, p.draft_lens ? p.draft_lens[group] + 1 : p.per_group);
+    const int last = p.draft_lens ? p.draft_lens[group] : p.per_group - 1;
+    const int rows = last < p.sub_from ? last + 1 : p.sub_from;
     bool decided = false;
     for (int i = 0; i < rows; ++i)
       decided |= p.results[group * p.per_group + i].x == kDecided;
@@ -2106,8 +2122,8 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
     const bool by_mass = pol.top_p < 1.0;
     const bool cuts = pol.temperature > 0.0 && (pol.top_k || by_mass);
     // A small top-k goes by the peaks, not the bins. (One float32 row of 32,000: 19.2 -> 17.5 us.
-    // Not bfloat16, whose bins need no list: 256 rows of 128,256 took 85 us by the peaks, 51 by
-    // the bins.)
+    // Not bfloat16, whose bins need no list: 256 rows of 128,256, top-k 50, took 85 us by the
+    // peaks, 65 by the bins.)
     const bool by_peaks = DT != kBF16 && cuts && pol.top_k && pol.top_k <= kPsList / 2;
     const bool bins = cuts && !by_peaks;
     // The mass of all ids is summed where top-p needs it and the bins do not give it, and where

@@ -156,7 +156,7 @@ def _uniform_code(uniforms: torch.Tensor, shape: tuple[int, ...]) -> int:
 
 
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether the byte ranges that the two 2-d tensors span meet."""
+    """Whether the byte ranges that the two tensors span meet."""
     def span(t: torch.Tensor) -> tuple[int, int]:
         last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
         return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
@@ -220,8 +220,8 @@ def policy_probs(logits: torch.Tensor, bitmask: torch.Tensor | None, policies: t
                              f"got {out.dtype} {list(out.shape)}")
         if (vocab > 1 and out.stride(1) != 1) or (rows > 1 and out.stride(0) < vocab):
             raise ValueError("out must have contiguous rows that do not overlap")
-        if rows and _overlap(x, out):
-            raise ValueError("out must not share memory with logits")
+        if rows and any(_overlap(t, out) for t in (x, m, pol) if t is not None):
+            raise ValueError("out must not share memory with an input")
     device = _ms._same_device(x, pol, out, *(() if m is None else (m,)))
     status = torch.empty(rows, dtype=torch.int32, device=device)
     if rows:

@@ -679,3 +679,40 @@ def test_repeated_calls_give_the_same_bits(cuda_lib):
     first = ox.policy_probs(x, None, pol)[0].clone()
     for _ in range(5):
         assert torch.equal(ox.policy_probs(x, None, pol)[0], first)
+
+
+def test_probs_refuses_outputs_over_its_inputs(cuda_lib):
+    x = torch.zeros(2, 64, device="cuda")
+    pol = gpu(table((1.0, 0, 1.0, 0.0), 2))
+    words = torch.full((130,), -1, dtype=torch.int32, device="cuda")
+    over_mask = words.view(torch.float32)[:128].view(2, 64)
+    with pytest.raises(ValueError):
+        ox.policy_probs(x, words[:4].view(2, 2), pol, out=over_mask)
+    over_policies = torch.zeros(64, dtype=torch.float64, device="cuda")
+    with pytest.raises(ValueError):
+        ox.policy_probs(x, None, over_policies[:8].view(2, 4),
+                        out=over_policies.view(torch.float32).view(2, 64))
+    with pytest.raises(ValueError):
+        ox.policy_probs(x, None, pol, out=x)
+
+
+def test_lengths_out_of_range_in_a_batch_of_several_launches(cuda_lib):
+    """More rows than one launch takes: every entry's later rows look at what the earlier ones
+    decided, and a length may be anything that 32 bits hold."""
+    batch, gamma, vocab = 300, 3, 500
+    rng = np.random.default_rng(61)
+    x = to_device(normal(rng, (batch * (gamma + 1), vocab), "f32"), "f32")
+    x = x.view(batch, gamma + 1, vocab)
+    d = torch.from_numpy(rng.integers(0, vocab, (batch, gamma)).astype(np.int32)).cuda()
+    lens = torch.from_numpy(rng.integers(0, gamma + 1, batch).astype(np.int32))
+    bad = {0: 2**31 - 1, 7: -(2**31), 150: -1, 299: gamma + 1}
+    for i, n in bad.items():
+        lens[i] = n
+    pol = gpu(table((1.0, 0, 0.9, 0.0), batch))
+    u = gpu(rng.random((batch, gamma + 1)))
+    r = ox.spec_sample(x, None, d, pol, u, draft_lens=lens.cuda())
+    status = r.status.cpu().numpy()
+    for i in range(batch):
+        assert status[i] == (ox.STATUS_BAD_POLICY if i in bad else 0)
+    assert (r.correction.cpu().numpy()[list(bad)] == -1).all()
+    assert (r.accept_len.cpu().numpy()[list(bad)] == 0).all()
