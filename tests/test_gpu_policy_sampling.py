@@ -716,3 +716,22 @@ def test_lengths_out_of_range_in_a_batch_of_several_launches(cuda_lib):
         assert status[i] == (ox.STATUS_BAD_POLICY if i in bad else 0)
     assert (r.correction.cpu().numpy()[list(bad)] == -1).all()
     assert (r.accept_len.cpu().numpy()[list(bad)] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", ("f32", "f16", "bf16"))
+@pytest.mark.parametrize("scale", (20.0, 45.0, 400.0))
+@pytest.mark.parametrize("rows,vocab", ((1, 20011), (24, 100003), (3, 700)))
+def test_peaked_rows(cuda_lib, rows, vocab, scale, dtype):
+    """Logits far above the temperature: the maximum lies past the bins, and a few ids among
+    the largest peaks hold the mass; also with many of them tied, and under masks."""
+    rng = np.random.default_rng(int(scale) + vocab)
+    v = rng.standard_normal((rows, vocab)) * scale
+    v[:, 3] += scale  # a maximum far above the others
+    v[rows // 2, 5:900:2] = v[rows // 2].max()  # equal ones, more than fit the short list
+    x = rounded(v, dtype)
+    m = workloads.bernoulli_masks(rng, rng.uniform(0.05, 0.9, rows), vocab)
+    u = rng.random(rows)
+    for policy in ((1.0, 0, 0.9, 0.0), (0.1, 0, 0.95, 0.02), (1.3, 40, 0.99, 0.0),
+                   (8.0, 0, 0.7, 0.0), (1.0, 2000, 0.97, 0.0)):
+        check(x, None, dtype, table(policy, rows), u)
+        check(x, m, dtype, table(policy, rows), u)
