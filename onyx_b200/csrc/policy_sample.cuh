@@ -38,8 +38,9 @@
 //      drawn by all warps of its CTA, piece by piece).
 // Rows that steps 2 and 3 cannot serve (bfloat16 values of 2^7 and more, a cut among values
 // next to zero, float32 maxima 40 T above the sample, lists over 1,024 ids) go through
-// find_cut(): the histogram over ranges of order codes, each turn a 4096th of the last. No row
-// length is bound to shared memory.
+// find_cut(): a list of the ids of the largest peaks, and where that does not reach the goal the
+// histogram over ranges of order codes, each turn a 4096th of the last. No row length is bound
+// to shared memory.
 //
 // Every CTA of a cluster computes the same totals from the same parts in the same order, so
 // all take the same branches, and the result does not depend on timing. (Histograms are counts,
