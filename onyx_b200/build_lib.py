@@ -27,7 +27,8 @@ def _stale() -> bool:
     if not LIB.exists():
         return True
     mtime = LIB.stat().st_mtime
-    deps = sources() + sorted(CSRC.glob("*.cuh")) + [ROOT / "include" / "onyx_b200.h"]
+    deps = sources() + sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h"))
+    deps.append(ROOT / "include" / "onyx_b200.h")
     return any(p.stat().st_mtime > mtime for p in deps)
 
 

@@ -92,3 +92,27 @@ def test_missing_library_fails_loudly(tmp_path):
 
     with pytest.raises(_lib.OnyxLibraryUnavailableError):
         _lib.load(tmp_path / "libonyx_b200.so")
+
+
+def test_a_newer_header_makes_the_library_stale(tmp_path, monkeypatch):
+    """Every kind of file that the sources include counts, not the .cuh alone."""
+    import os
+
+    from onyx_b200 import build_lib
+
+    csrc, include = tmp_path / "csrc", tmp_path / "include"
+    csrc.mkdir()
+    include.mkdir()
+    files = [csrc / "a.cu", csrc / "b.cuh", csrc / "c.h", include / "onyx_b200.h"]
+    lib = tmp_path / "lib.so"
+    monkeypatch.setattr(build_lib, "CSRC", csrc)
+    monkeypatch.setattr(build_lib, "ROOT", tmp_path)
+    monkeypatch.setattr(build_lib, "LIB", lib)
+    for f in (*files, lib):
+        f.touch()
+        os.utime(f, (100, 100))
+    assert not build_lib._stale()
+    for f in files:
+        os.utime(f, (200, 200))
+        assert build_lib._stale(), f.name
+        os.utime(f, (100, 100))
