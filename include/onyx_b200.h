@@ -267,6 +267,15 @@ ONYX_API int onyx_spec_sample(const void* logits, int dtype, int64_t batch, int6
                               void* stream);
 
 /*
+ * How the three calls lay out `rows` rows on a device of `sms` multiprocessors (spec: the rows
+ * of one launch): layout[0] CTAs per row, [1] ids per warp, [2] 1 if the largest of every 8 ids
+ * is kept in shared memory, [3] 1 if the whole row is (else it streams through a ring of
+ * slots), [4] bytes of dynamic shared memory. On the host alone, for profiles and tests.
+ */
+ONYX_API int onyx_policy_layout(int64_t rows, int64_t vocab, int dtype, int masked, int sms,
+                                int32_t* layout);
+
+/*
  * Valid-token bitmasks of DFA states (the mask producer): row r of `out` (out_stride >=
  * ceil(vocab/32) words) is the packed mask of states[r] -- bit t set iff token t is
  * non-empty and walking its bytes through `trans` ([n_states][256] next-state ids) from

@@ -76,6 +76,7 @@ SIGNATURES: dict[str, tuple[object, list]] = {
     "onyx_spec_sample": (
         _i32, [_vp, _i32, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64,
                _i64, _vp, _vp, _i64, _vp, _i32, _i64, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "onyx_policy_layout": (_i32, [_i64, _i64, _i32, _i32, _i32, _vp]),
     "onyx_dfa_state_masks": (
         _i32, [_vp, _i32, _i32, _i32, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp]),
     "onyx_ipc_handle_bytes": (_sz, []),

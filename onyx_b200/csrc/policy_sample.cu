@@ -215,6 +215,20 @@ int onyx_policy_probs(const void* logits, int dtype, int64_t rows, int64_t vocab
   return launch_policy<kOpProbs>(dtype, p, rows, (cudaStream_t)stream);
 }
 
+int onyx_policy_layout(int64_t rows, int64_t vocab, int dtype, int masked, int sms,
+                       int32_t* layout) {
+  if (!policy_dtype(dtype)) return ONYX_ERR_UNSUPPORTED_DTYPE;
+  if (rows < 1 || rows > 0x7FFFFFFFll || vocab < 1 || vocab > kPsMostVocab || sms < 1 || !layout)
+    return ONYX_ERR_INVALID_ARGUMENT;
+  const PolicyPlan pl = make_plan(rows, vocab, dtype, masked != 0, sms);
+  layout[0] = pl.k;
+  layout[1] = pl.warp_ids;
+  layout[2] = pl.peaks;
+  layout[3] = pl.keep;
+  layout[4] = (int32_t)pl.smem;
+  return ONYX_OK;
+}
+
 size_t onyx_spec_sample_workspace_size(int64_t batch, int64_t gamma) {
   if (batch <= 0 || gamma < 1 || gamma > 255) return 0;
   return (size_t)batch * (size_t)(gamma + 1) * sizeof(int4);

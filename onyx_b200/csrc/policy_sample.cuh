@@ -59,6 +59,7 @@
 #include <cfloat>
 
 #include "onyx_common.cuh"
+#include "policy_ring.cuh"
 
 namespace onyx {
 
@@ -109,7 +110,7 @@ struct PolicyParams {
   int32_t peaks;     // the peaks are kept (else their place is empty)
   int32_t keep;      // shared memory holds all chunks of a CTA's part
   int32_t slots;     // where in dynamic shared memory the chunks' slots begin,
-  int32_t lists;     // and the lists of the warps (over a ring, which is done by then)
+  int32_t lists;     // and the lists of the warps (over a ring, whose copies have landed by then)
 };
 
 enum Verdict : int { kAccepted = 0, kDecided = 1 };
@@ -1909,8 +1910,7 @@ __device__ __forceinline__ PsFirst first_pass(const RowView<DT>& view, int lane,
   const bool kept = view.kept;
   // chunks inside the row; the others are copied and read with care
   const int id_first = view.id_of(view.begin);
-  const int inner_from = id_first < 0 ? 1 : 0;
-  const int inner_to = inner_from + max(0, (view.vocab - (id_first + inner_from * kPsChunk)) / kPsChunk);
+  const PsInner inner = ps_inner_chunks(id_first, n, view.vocab, kPsChunk);
   const uint32_t start = view.slots;
   const uint32_t stop = kept ? 0xFFFFFFFFu : start + kDepth * bytes;
   uint32_t slot = view.first_slot(), fill = stop - bytes;
@@ -1934,12 +1934,13 @@ __device__ __forceinline__ PsFirst first_pass(const RowView<DT>& view, int lane,
   for (int i = 0; i < n; ++i) {
     if (!kept) {
       const int next = i + ahead;
-      if (next >= inner_from && next < inner_to) {
+      const PsCopy what = ps_copy_at(next, n, inner);
+      if (what == kCopyWhole) {
         ps_copy16(fill + (DT == kF32 ? (lane & 1) * 512 + (lane >> 1) * 16 : lane * 16), src);
         if (DT == kF32)
           ps_copy16(fill + (lane & 1) * 512 + (lane >> 1) * 16 + 256, src + 32 * kVec);
         if (mask) view.copy_words(fill, lane, id_first + next * kPsChunk);
-      } else if (next < n) {
+      } else if (what == kCopyEdge) {
         view.copy_chunk(fill, lane, id_first + next * kPsChunk);
       }
       src += kPsChunk;
@@ -1956,7 +1957,7 @@ __device__ __forceinline__ PsFirst first_pass(const RowView<DT>& view, int lane,
     if (DT == kF32) r.b = ps_load16(slot + 512 + lane * 16);
     r.bits = 0xFFu;
     bool full = !mask;
-    if (i < inner_from || i >= inner_to) {
+    if (i < inner.from || i >= inner.to) {
       const int id = id_first + i * kPsChunk + 8 * lane;
       r.bits = view.inside(id);
       if (r.bits != 0xFFu) view.load_edge(r, id);
@@ -2022,6 +2023,7 @@ __device__ __forceinline__ PsFirst first_pass(const RowView<DT>& view, int lane,
       }
     }
   }
+  if (!kept) ps_await<0>();  // the last groups are empty; what follows writes over the ring
   out.mass += mass2;
   return out;
 }

@@ -15,12 +15,14 @@ relative, plus its sums' error and, below float32's smallest normal number, 2^-1
 
 from __future__ import annotations
 
+import ctypes
+
 import numpy as np
 import pytest
 import torch
 
 import onyx_b200 as ox
-from onyx_b200 import workloads
+from onyx_b200 import _lib, workloads
 from oracle import policy as opol
 from oracle import sampling as osamp
 from tests.gpu_util import host, masks_to_device, requires_cuda, to_device
@@ -735,3 +737,152 @@ def test_peaked_rows(cuda_lib, rows, vocab, scale, dtype):
                    (8.0, 0, 0.7, 0.0), (1.0, 2000, 0.97, 0.0)):
         check(x, None, dtype, table(policy, rows), u)
         check(x, m, dtype, table(policy, rows), u)
+
+
+# --------------------------------------------------------------------------------------
+# rows that stream through a ring of slots, over which the lists of later passes lie
+# --------------------------------------------------------------------------------------
+RING = {  # rows, vocabulary, views of a row padded by so many ids, mask
+    "masked_64": (64, 128256, 0, True), "one_cta_256": (256, 32000, 0, False),
+    "one_cta_masked": (300, 33333, 5, True), "odd_64": (64, 151665, 3, False),
+    "one_row": (1, 300007, 0, True), "large_256": (256, 128256, 0, False),
+}
+RING_POLICIES = ("greedy", "min_p", "top_p", "top_k", "plain", "all")
+
+
+def assert_ring(rows, vocab, dtype, masked):
+    code = {"f32": _lib.DTYPE_F32, "f16": _lib.DTYPE_F16, "bf16": _lib.DTYPE_BF16}[dtype]
+    out = (ctypes.c_int32 * 5)()
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    assert _lib.load().onyx_policy_layout(rows, vocab, code, int(masked), sms, out) == _lib.OK
+    assert out[2] and not out[3], "these rows are kept whole: the case tests something else"
+
+
+def ring_rows(rows, vocab, pad, masked, dtype, seed):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    full = torch.randn(rows, vocab + pad, generator=gen, device="cuda").mul_(3.0)
+    x = full.to({"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}[dtype])
+    m = None
+    if masked:  # from half of the ids down to one in 64
+        words = torch.full((rows, (vocab + 31) // 32), -1, dtype=torch.int32, device="cuda")
+        depth = torch.arange(rows, device="cuda").view(-1, 1) % 6
+        for i in range(6):
+            more = torch.randint(-2**31, 2**31, words.shape, generator=gen, device="cuda",
+                                 dtype=torch.int32)
+            words = torch.where(depth >= i, words & more, words)
+        m = words
+    u = torch.rand(rows, generator=gen, device="cuda", dtype=torch.float64)
+    return x[:, :vocab], m, u
+
+
+def oracle_row(x, m, policy, u, got):
+    """One row on the host: whether `got` is the draw."""
+    v = x.float().cpu().numpy().astype(np.float64)
+    valid = np.ones(v.size, bool) if m is None else osamp.unpack_mask(
+        host(m).view(np.uint32), v.size)
+    status, w = opol.kept_weights(v, valid, policy)
+    assert status == 0
+    want = opol.choose(w, u)
+    assert got == want or on_boundary(w, u, got, want), (policy, got, want)
+    return w
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("shape", list(RING))
+def test_ring_rows(shape, dtype, cuda_lib):
+    """Policies mixed over a batch, against the oracle; then the same call again, which gives
+    the same draws, alone and while another stream keeps memory busy."""
+    rows, vocab, pad, masked = RING[shape]
+    assert_ring(rows, vocab, dtype, masked)
+    x, m, u = ring_rows(rows, vocab, pad, masked, dtype, rows + vocab)
+    policies = np.stack([POLICIES[RING_POLICIES[r % 6]] for r in range(rows)])
+    pol = gpu(policies)
+    first = ox.policy_sample(x, m, pol, u)
+    assert not first.status.any()
+    probs, status = ox.policy_probs(x, m, pol)
+    assert not status.any()
+    some = sorted({0, rows - 1, *range(min(rows, 6)), *range(rows // 2, min(rows, rows // 2 + 6))})
+    ids, numbers = host(first.token_ids), host(u)
+    for r in some:
+        w = oracle_row(x[r], None if m is None else m[r], policies[r], numbers[r], ids[r])
+        assert_probs(probs[r], w / w.sum())
+    side, junk = torch.cuda.Stream(), torch.empty(1 << 28, dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    again = []
+    for i in range(16):
+        if i >= 8:
+            with torch.cuda.stream(side):
+                junk.add_(1)
+        again.append(ox.policy_sample(x, m, pol, u))
+    p = ox.policy_probs(x, m, pol)[0]
+    torch.cuda.synchronize()
+    for a in again:
+        assert torch.equal(a.token_ids, first.token_ids) and torch.equal(a.status, first.status)
+    assert torch.equal(p, probs)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("shape", list(RING))
+def test_ring_rows_greedy(shape, dtype, cuda_lib):
+    """A whole batch at temperature 0, where the least lies between the first pass and the
+    lists: the ids of masked_argmax, every time."""
+    rows, vocab, pad, masked = RING[shape]
+    x, m, u = ring_rows(rows, vocab, pad, masked, dtype, rows * 3 + vocab)
+    want = ox.masked_argmax(x, m).token_ids
+    pol = gpu((0.0, 0, 1.0, 0.0))
+    got = [ox.policy_sample(x, m, pol, u) for _ in range(24)]
+    for g in got:
+        assert torch.equal(g.token_ids, want) and not g.status.any()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+def test_ring_rows_min_p_alone(dtype, cuda_lib):
+    """min-p without another cut: no histogram, the lists follow the first pass at once."""
+    rows, vocab, pad, masked = RING["masked_64"]
+    x, m, u = ring_rows(rows, vocab, pad, masked, dtype, 17)
+    policy = (1.0, 0, 1.0, 0.02)
+    got = [ox.policy_sample(x, m, gpu(policy), u).token_ids for _ in range(24)]
+    for g in got:
+        assert torch.equal(g, got[0])
+    for r in range(0, rows, 9):
+        oracle_row(x[r], m[r], policy, host(u)[r], host(got[0])[r])
+
+
+@pytest.mark.parametrize("with_q", [True, False])
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+def test_ring_spec(dtype, with_q, cuda_lib):
+    """A speculative batch of 32 x 5 rows under every policy, against the oracle."""
+    batch, gamma, vocab = 32, 4, 151936
+    rows = batch * (gamma + 1)
+    assert_ring(batch * (gamma + 1), vocab, dtype, True)
+    x, m, _ = ring_rows(rows, vocab, 0, True, dtype, 5 + with_q)
+    x, m = x.view(batch, gamma + 1, vocab), m.view(batch, gamma + 1, -1)
+    policies = np.stack([POLICIES[RING_POLICIES[b % 6]] for b in range(batch)])
+    pol = gpu(policies)
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    q = torch.empty(batch, gamma, vocab, device="cuda")
+    d = torch.empty(batch, gamma, dtype=torch.int32, device="cuda")
+    for i in range(gamma):
+        near = (x[:, i].float() + 0.3 * torch.randn(batch, vocab, generator=gen, device="cuda")
+                ).to(x.dtype)
+        ox.policy_probs(near, m[:, i], pol, out=q[:, i])
+        u = torch.rand(batch, generator=gen, device="cuda", dtype=torch.float64)
+        d[:, i] = ox.policy_sample(near, m[:, i], pol, u).token_ids
+    u = torch.rand(batch, gamma + 1, generator=gen, device="cuda", dtype=torch.float64)
+    q = q if with_q else None
+    first = ox.spec_sample(x, m, d, pol, u, draft_probs=q)
+    again = [ox.spec_sample(x, m, d, pol, u, draft_probs=q) for _ in range(8)]
+    for a in again:
+        for got, want in zip((a.accept_len, a.correction, a.status),
+                             (first.accept_len, first.correction, first.status)):
+            assert torch.equal(got, want)
+    taken, token = host(first.accept_len), host(first.correction)
+    assert not first.status.any()
+    for b in range(0, batch, 3):
+        drawn = {}
+        want = opol.spec(x[b:b + 1].float().cpu().numpy().astype(np.float64),
+                         host(m[b:b + 1]).view(np.uint32), host(d[b:b + 1]), policies[b:b + 1],
+                         host(u[b:b + 1]), None if q is None else host(q[b:b + 1]), None, drawn)
+        assert taken[b] == want[0][0]
+        if token[b] != want[1][0]:
+            assert on_boundary(drawn[0], float(u[b, -1]), token[b], want[1][0])

@@ -3,8 +3,11 @@ fixtures and by brute force, and the refusals of the C entry points and the Pyth
 
 from __future__ import annotations
 
+import ctypes
 import itertools
 import math
+import subprocess
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -180,3 +183,77 @@ def test_calls_refuse_host_tensors():
         ox.spec_sample(x[None], None, torch.zeros(1, 1, dtype=torch.int32), pol, torch.zeros(1, 2))
     with pytest.raises(TypeError):
         ox.policy_sample([1.0], None, pol, torch.zeros(1))
+
+
+# --------------------------------------------------------------------------------------
+# rows that stream through a ring of slots in shared memory
+# --------------------------------------------------------------------------------------
+DTYPE_SIZES = {_lib.DTYPE_F32: 4, _lib.DTYPE_F16: 2, _lib.DTYPE_BF16: 2}
+
+
+def layout_of(lib, rows, vocab, dtype, masked):
+    out = (ctypes.c_int32 * 5)()
+    assert lib.onyx_policy_layout(rows, vocab, dtype, int(masked), 148, out) == _lib.OK
+    return dict(zip(("k", "warp_ids", "peaks", "keep", "smem"), out))
+
+
+@pytest.fixture(scope="session")
+def ring_copies(tmp_path_factory):
+    """The ring's schedule, as the kernel compiles it, on the host."""
+    src = Path(__file__).resolve().parent / "native" / "ring_copies.cpp"
+    lib = tmp_path_factory.mktemp("ring") / "ring_copies.so"
+    subprocess.run(["g++", "-O1", "-std=c++17", "-shared", "-fPIC", str(src), "-o", str(lib)],
+                   check=True)
+    fn = ctypes.CDLL(str(lib)).ring_copies
+
+    def call(id_first, n, vocab, depth):
+        out = (ctypes.c_int64 * 3)()
+        fn(id_first, n, vocab, 256, depth, out)
+        return tuple(out)
+
+    return call
+
+
+@pytest.mark.parametrize("rows,vocab,dtype,masked", [
+    (64, 128256, _lib.DTYPE_BF16, True), (256, 128256, _lib.DTYPE_BF16, False),
+    (256, 32000, _lib.DTYPE_F32, False), (1, 256000, _lib.DTYPE_F16, True),
+    (64, 151665, _lib.DTYPE_F32, False), (160, 151936, _lib.DTYPE_BF16, True),
+    (1, 1500001, _lib.DTYPE_F32, False), (300, 33333, _lib.DTYPE_F16, True),
+])
+def test_ring_starts_its_own_chunks_alone(rows, vocab, dtype, masked, cuda_lib, ring_copies):
+    """A warp copies each chunk of its part once, before it is read; no chunk of another
+    warp's, and nothing is on its way when the slots become the lists of later passes."""
+    plan = layout_of(cuda_lib, rows, vocab, dtype, masked)
+    assert not plan["keep"]
+    depth = 3 if dtype == _lib.DTYPE_F32 else 4
+    for off in range(16 // DTYPE_SIZES[dtype]):
+        end = vocab + off
+        for warp in range(16 * plan["k"]):
+            begin = min(warp * plan["warp_ids"], end)
+            stop = min(begin + plan["warp_ids"], end)
+            n = (stop - begin + 255) // 256
+            assert ring_copies(begin - off, n, vocab, depth) == (0, 0, 0), (off, warp, n)
+
+
+def test_layouts(cuda_lib):
+    """Small batches keep their rows in shared memory; serving batches stream them."""
+    bf16, f32 = _lib.DTYPE_BF16, _lib.DTYPE_F32
+    assert layout_of(cuda_lib, 1, 128256, bf16, False) == dict(
+        k=8, warp_ids=1024, peaks=1, keep=1, smem=layout_of(cuda_lib, 1, 128256, bf16, False)["smem"])
+    assert layout_of(cuda_lib, 256, 128256, bf16, False)["k"] == 2
+    assert layout_of(cuda_lib, 256, 32000, bf16, False)["k"] == 1
+    assert not layout_of(cuda_lib, 1, 2_200_003, f32, False)["peaks"]
+    for rows in (1, 2, 37, 64, 149, 1024):
+        for vocab in (1, 255, 32000, 151936, 1 << 20, 1 << 30):
+            for dtype in DTYPE_SIZES:
+                for masked in (False, True):
+                    p = layout_of(cuda_lib, rows, vocab, dtype, masked)
+                    assert p["k"] in (1, 2, 4, 8) and p["warp_ids"] % 256 == 0
+                    assert 16 * p["k"] * p["warp_ids"] >= vocab + 7
+                    assert p["smem"] + 8192 <= 227 * 1024
+    f = cuda_lib.onyx_policy_layout
+    out, bad = (ctypes.c_int32 * 5)(), _lib.ERR_INVALID_ARGUMENT
+    assert f(1, 100, 3, 0, 148, out) == _lib.ERR_UNSUPPORTED_DTYPE
+    for args in ((0, 100, 0, 0, 148, out), (1, 0, 0, 0, 148, out), (1, 1 << 31, 0, 0, 148, out),
+                 (1, 100, 0, 0, 0, out), (1, 100, 0, 0, 148, None)):
+        assert f(*args) == bad
