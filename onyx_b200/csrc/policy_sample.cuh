@@ -1925,7 +1925,8 @@ __device__ __forceinline__ PsFirst first_pass(const RowView<DT>& view, int lane,
   }
   const uint32_t hist = (uint32_t)__cvta_generic_to_shared(ps_hist());
   const float scale_b = bins.scale, shift_b = bins.shift;
-  const float floor_value = (float)(from - 15000.0 / scale);  // less than 2^-930 below it
+  // less than 2^-930 below it, but finite: a value of -inf counts at no temperature
+  const float floor_value = fmaxf((float)(from - 15000.0 / scale), -FLT_MAX);
   PsFirst out = {0u, -INFINITY, 0u, 0u, 0.0};
   double mass2 = 0.0;
   if (kept) ps_await_all_but(n - half);

@@ -886,3 +886,23 @@ def test_ring_spec(dtype, with_q, cuda_lib):
         assert taken[b] == want[0][0]
         if token[b] != want[1][0]:
             assert on_boundary(drawn[0], float(u[b, -1]), token[b], want[1][0])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("temperature", [1e30, 6e35, 1e37, 1e300, 1.7e308])
+def test_very_high_temperatures(temperature, dtype, cuda_lib):
+    """Every finite value weighs 1 there, and a logit of -inf still nothing."""
+    rng = np.random.default_rng(101)
+    x = rng.standard_normal((5, 5003)) * 3
+    x[1, rng.random(5003) < 0.4] = -np.inf
+    x[2, 1::2] = -np.inf
+    x[3, :5000] = -np.inf
+    x[4, 0] = -np.inf
+    x = rounded(x, dtype)
+    m = workloads.bernoulli_masks(rng, np.full(5, 0.5), 5003)
+    m[:, 0] |= np.uint32(3)
+    m[:, -1] |= np.uint32(1 << 10)
+    for policy in ((temperature, 0, 1.0, 0.0), (temperature, 0, 0.77123, 0.0),
+                   (temperature, 700, 0.5123, 0.0), (temperature, 0, 1.0, 0.3)):
+        check(x, None, dtype, table(policy, 5), rng.random(5))
+        check(x, m, dtype, table(policy, 5), rng.random(5))
