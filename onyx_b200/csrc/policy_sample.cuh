@@ -1891,6 +1891,13 @@ struct PsFirst {
                   // next to zero relative to 0
 };
 
+// The least value whose weight the first pass adds up, relative to `from`: 2^-937.5 at least,
+// which exp2_from() can form. Rounded up, for next to a `from` of 10^10 T the float below the
+// bound lies past that range; and finite, so that a value of -inf counts at no temperature.
+__device__ __forceinline__ float mass_floor(double from, double scale) {
+  return fmaxf(__double2float_ru(from - 15000.0 / scale), -FLT_MAX);
+}
+
 // The pass behind the copies of start_stream(): peaks, and with BINS the histogram, with MASS
 // the weights. One loop for each of the four, on scalars of its own, and the chunks at the edges
 // of a row apart from it: as one lambda called from a method of the view, 256 rows of 128,256
@@ -1925,8 +1932,7 @@ __device__ __forceinline__ PsFirst first_pass(const RowView<DT>& view, int lane,
   }
   const uint32_t hist = (uint32_t)__cvta_generic_to_shared(ps_hist());
   const float scale_b = bins.scale, shift_b = bins.shift;
-  // less than 2^-930 below it, but finite: a value of -inf counts at no temperature
-  const float floor_value = fmaxf((float)(from - 15000.0 / scale), -FLT_MAX);
+  const float floor_value = mass_floor(from, scale);
   PsFirst out = {0u, -INFINITY, 0u, 0u, 0.0};
   double mass2 = 0.0;
   if (kept) ps_await_all_but(n - half);
@@ -2186,7 +2192,7 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
       sum.mass = sum.mass > 0.0 ? sum.mass * factor : 0.0;
       // (not if the temperature is so low that the pass could not tell `from` from its floor)
       const bool measured =
-          mass_of_all && in_range && (double)(float)(from - 15000.0 / c.scale) < from - 1e-30;
+          mass_of_all && in_range && (double)mass_floor(from, c.scale) < from - 1e-30;
       // What top-p measures by. Relative to the maximum equal values weigh exactly 1, and a mass
       // that equals its goal (270 of 300 equal ids at 0.9) has reached it; the sums relative to
       // `from` round each weight, by some 2^-51 of it, and the factor keeps that so.

@@ -906,3 +906,17 @@ def test_very_high_temperatures(temperature, dtype, cuda_lib):
                    (temperature, 700, 0.5123, 0.0), (temperature, 0, 1.0, 0.3)):
         check(x, None, dtype, table(policy, 5), rng.random(5))
         check(x, m, dtype, table(policy, 5), rng.random(5))
+
+
+@pytest.mark.parametrize("policy", [(1.0, 0, 1.0, 0.0), (1.0, 0, 0.9, 0.0), (1.3, 0, 1.0, 0.0)])
+def test_values_of_ten_billion_temperatures(policy, cuda_lib):
+    """float32 values whose spacing is wider than the range of weights that are summed: the
+    next value below the largest weighs nothing."""
+    rng = np.random.default_rng(102)
+    x = (1.1e10 + 1024.0 * rng.integers(-4, 4, (6, 7001))).astype(np.float32)
+    x[3] = -x[3]
+    x[4] = np.float32(1.7e10) + 1024.0 * rng.integers(-2, 1, 7001)
+    x[5, 4000:] = np.float32(2.0**33)
+    check(x, None, "f32", table(policy, 6), rng.random(6))
+    m = workloads.bernoulli_masks(rng, np.full(6, 0.5), 7001)
+    check(x, m, "f32", table(policy, 6), rng.random(6))
