@@ -2185,9 +2185,11 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
     if (!status) {
       c.top = code_value(top);
       c.flat = !(pol.temperature > 0.0) || c.top == INFINITY;
-      // the masses relative to the maximum, where they did not leave the range of doubles
+      // The masses relative to the maximum, where they did not leave the range of doubles. Where
+      // `from` lies above it (a masked id), the floor below `from` must leave out nothing that
+      // counts: 2000 above the floor, it leaves out weights below 2^-125.
       const double shift = (from - c.top) * c.scale;
-      const bool in_range = fabs(shift) < 14400.0;
+      const bool in_range = shift > -14400.0 && shift < (mass_of_all ? 13000.0 : 14400.0);
       const double factor = in_range ? exp2_table(shift, sh.powers) : 0.0;
       sum.mass = sum.mass > 0.0 ? sum.mass * factor : 0.0;
       // (not if the temperature is so low that the pass could not tell `from` from its floor)

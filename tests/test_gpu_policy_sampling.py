@@ -16,6 +16,7 @@ relative, plus its sums' error and, below float32's smallest normal number, 2^-1
 from __future__ import annotations
 
 import ctypes
+import math
 
 import numpy as np
 import pytest
@@ -920,3 +921,51 @@ def test_values_of_ten_billion_temperatures(policy, cuda_lib):
     check(x, None, "f32", table(policy, 6), rng.random(6))
     m = workloads.bernoulli_masks(rng, np.full(6, 0.5), 7001)
     check(x, m, "f32", table(policy, 6), rng.random(6))
+
+
+def raw_sample(x, m, dtype, policies, u):
+    """policy_sample by its C entry, into outputs that hold -7: a row that nothing is written
+    for shows."""
+    xt, mt = to_device(x, dtype), None if m is None else masks_to_device(m)
+    pol, ut = gpu(policies), gpu(u)
+    rows, vocab = xt.shape
+    ids = torch.full((rows,), -7, dtype=torch.int32, device="cuda")
+    status = torch.full((rows,), -7, dtype=torch.int32, device="cuda")
+    code = {"f32": _lib.DTYPE_F32, "f16": _lib.DTYPE_F16, "bf16": _lib.DTYPE_BF16}[dtype]
+    _lib.check("onyx_policy_sample", _lib.load().onyx_policy_sample(
+        xt.data_ptr(), code, rows, vocab, vocab, None if mt is None else mt.data_ptr(),
+        0 if mt is None else mt.stride(0), pol.data_ptr(), 4, ut.data_ptr(), _lib.DTYPE_F64, 1,
+        ids.data_ptr(), status.data_ptr(), torch.cuda.current_stream().cuda_stream))
+    return host(ids), host(status)
+
+
+@pytest.mark.parametrize("dtype,high,t,low", [("f32", 619.0, 1.0, -32.0), ("f16", 619.0, 1.0, -32.0),
+                                              ("bf16", 500.0, 0.81, -27.0),
+                                              ("f32", 700.0, 1.0, -32.0),
+                                              ("f32", 560.0, 1.0, -32.0)])
+def test_masked_ids_far_above_the_valid_ones(dtype, high, t, low, cuda_lib):
+    """Ids that the mask takes out, hundreds of T above the rest, at the places that the kernel
+    samples: what is summed relative to them must still hold the valid ids' small weights.
+    n of these, of weight w, follow the largest one (weight 1), and u lies in their share. The
+    draw is the one whose rank passes (u (1 + n w) - 1) / w. Two sums of n weights, each within
+    n 2^-53 of its value, decide it, and as many the cut that top-p makes: 4 n 2^-53 / w ranks."""
+    vocab = 200000
+    x = np.full((2, vocab), low)
+    x[:, 1] = 0.0
+    at = np.arange(128) * vocab >> 7
+    x[:, at] = high
+    valid = np.ones(vocab, bool)
+    valid[at] = False
+    words = np.packbits(np.pad(valid, (0, -vocab % 32)), bitorder="little").view(np.uint32)
+    valid[1] = False
+    lows, w = np.flatnonzero(valid), math.exp(low / t)
+    n = lows.size
+    for p in (1.0, 1.0 - n * w * 0.02):
+        kept = n if p == 1.0 else math.ceil((p - 1.0 + p * n * w) / w)
+        u = np.array([1.0 - n * w * 0.5, 1.0 - n * w * 0.1])
+        ids, status = raw_sample(rounded(x, dtype), np.stack([words, words]), dtype,
+                                 table((t, 0, p, 0.0), 2), u)
+        assert (status == 0).all()
+        want = (u - 1.0 + u * kept * w) / w
+        assert np.isin(ids, lows).all(), ids
+        assert (np.abs(np.searchsorted(lows, ids) - want) <= 4 * n * 2.0**-53 / w + 2).all()
