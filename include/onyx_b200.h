@@ -203,7 +203,7 @@ ONYX_API int onyx_masked_sample(const void* logits, int dtype, int64_t rows, int
  * r * policy_stride (0: one policy for every row, else >= 4).
  *
  * The distribution of a row. Ids are the mask's (NULL: every id). Weights are
- * exp((v - max) / temperature) in float64; where any value is +inf the +inf ids share the
+ * exp((v - max) / temperature) in float64, 0 below 2^-1000; where any value is +inf the +inf ids share the
  * mass alone; temperature 0 keeps the first maximum alone. Ids are ranked by value, the
  * lowest id first among equals. top_k keeps the first k of the ranking; top_p the shortest
  * prefix of those whose mass reaches top_p times their mass (1: off; float32 and float16: a

@@ -2202,7 +2202,11 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
       if (!cuts) {
         if (pol.temperature > 0.0) c.cut = c.flat ? FLT_MAX : -INFINITY;
         else c.keep(code_value(top), 1u);
-        if (plain && measured && !c.flat) row.summed = {f.mass * factor, sum.mass, 0u};
+        // The warps' parts of it serve the draw where every weight that they hold is one relative
+        // to the maximum too (not below 2^-1000, which counts as 0 there), and where none that
+        // lies below the floor can be drawn.
+        const bool drawable = shift > -990.0 && (OP == kOpProbs || u >= 0x1p-64);
+        if (plain && measured && !c.flat && drawable) row.summed = {f.mass * factor, sum.mass, 0u};
       } else {
         PsRange range = {}, safe = {};
         bool found = false, near = false;

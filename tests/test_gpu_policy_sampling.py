@@ -969,3 +969,27 @@ def test_masked_ids_far_above_the_valid_ones(dtype, high, t, low, cuda_lib):
         want = (u - 1.0 + u * kept * w) / w
         assert np.isin(ids, lows).all(), ids
         assert (np.abs(np.searchsorted(lows, ids) - want) <= 4 * n * 2.0**-53 / w + 2).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_weights_that_underflow_are_not_drawn(dtype, cuda_lib):
+    """Weights below 2^-1000 count as 0. The largest value lies far above those that the first
+    pass measures by; the parts of the row before it hold ids that weigh nothing."""
+    vocab = 40000
+    x = np.zeros((4, vocab))
+    x[:, :5000] = -550.0
+    x[:, 20001] = 160.0
+    x[:, 39000:] = -550.0
+    x[1, :5000] = -540.0     # 700 T below
+    x[2, :5000] = -530.0     # 690 T below: 2^-995
+    x[3, 20001] = 100.0
+    x = rounded(x, dtype)
+    v = f64(x, dtype)
+    u = np.array([0.0, 1e-320, 2.0**-400, 1.0 - 2.0**-53])
+    for ui in u:
+        ids, status = raw_sample(x, None, dtype, table((1.0, 0, 1.0, 0.0), 4), np.full(4, ui))
+        assert (status == 0).all()
+        for r in range(4):
+            w = np.exp(v[r] - v[r].max())
+            w[w < 2.0**-1000] = 0.0
+            assert ids[r] == opol.choose(w, ui), (r, ui)
