@@ -639,7 +639,6 @@ struct RowCut {
     const double low = top + log(min_p) / inv_t * (1.0 + 1e-9) - fabs(top) * 1e-9;
     const float bound = nextafterf(__double2float_rd(low), -INFINITY);
     if (bound >= cut) keep(bound, 0u);
-    if (take && weight(cut) < min_p) take = 0u;
   }
 };
 
@@ -2265,6 +2264,10 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
   const uint32_t down_to = summed ? row.summed.down_to : ~0u;
   double mass = summed ? row.summed.lane : 0.0;
   uint32_t ties = 0, before = 0;
+  // An id at the cut weighs what the passes below take it for: a weight out of the table differs
+  // from the formula's in the last places, and min_p may lie between them.
+  const double w_tie = c.take ? row.weight(c, c.cut) : 0.0;
+  if (w_tie < c.min_p) c.take = 0u;
   if (c.cut == -INFINITY) view.peaks = nullptr;  // nothing is cut: every vector
   view.gather(row.lane, c.least());
   if (row.lane == 0) sh.listed_by[row.warp] = view.listed;
@@ -2286,7 +2289,6 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
   mass = warp_sum(mass);
   ties = __reduce_add_sync(~0u, ties);
   before = __reduce_add_sync(~0u, before);
-  const double w_tie = c.take ? c.weight(c.cut) : 0.0;
   auto scan = row.scan_entries(0, mass, ties, before, c.take, w_tie, u);
   const double inv = 1.0 / scan.total;
 
@@ -2309,7 +2311,7 @@ __global__ void __launch_bounds__(kPsThreads, 2) policy_kernel(const PolicyParam
       const bool valid = !view.mask || (view.mask[draft >> 5] >> (draft & 31) & 1u);
       const float v = Elem<DT>::to_f32(view.row, draft);
       if (valid && (v > c.cut || (v == c.cut && scan.draft_before < c.take))) {
-        const double w = c.weight(v);
+        const double w = row.weight(c, v);
         if (w >= c.min_p) p_d = w / scan.total;
       }
     }

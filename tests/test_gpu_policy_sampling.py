@@ -993,3 +993,30 @@ def test_weights_that_underflow_are_not_drawn(dtype, cuda_lib):
             w = np.exp(v[r] - v[r].max())
             w[w < 2.0**-1000] = 0.0
             assert ids[r] == opol.choose(w, ui), (r, ui)
+
+
+def test_min_p_at_the_weight_of_the_cut(cuda_lib):
+    """min_p next to the weight of the value that top-k cuts at, which lies in a part of the row
+    of its own: that id is kept or not, and in either case something is drawn."""
+    vocab, top = 9001, 8000
+    rows, policies = [], []
+    for j in range(1, 161):
+        low = 10.0 - j / 16.0
+        w = math.exp(low - 10.0)
+        for steps in range(-4, 5):
+            row = np.full(vocab, -100.0)
+            row[[0, 1, top]] = low, low, 10.0
+            rows.append(row)
+            policies.append((1.0, 2, 0.9999999, w * (1.0 + steps * 2.0**-52)))
+    policies = np.array(policies)
+    x = rounded(np.stack(rows), "bf16")
+    for dtype, values in (("bf16", x), ("f32", f64(x, "bf16").astype(np.float32))):
+        ids, status = raw_sample(values, None, dtype, policies, np.zeros(len(rows)))
+        assert (status == 0).all()
+        assert np.isin(ids, (0, top)).all()
+        p, st = ox.policy_probs(to_device(values, dtype), None, gpu(policies))
+        p = host(p).astype(np.float64)
+        assert not host(st).any()
+        # what is drawn at u = 0 is what has a probability, and they sum to 1
+        np.testing.assert_array_equal(np.where(p[:, 0] > 0, 0, top), ids)
+        assert (np.abs(p.sum(1) - 1.0) <= 2.0**-23).all()
