@@ -1020,3 +1020,31 @@ def test_min_p_at_the_weight_of_the_cut(cuda_lib):
         # what is drawn at u = 0 is what has a probability, and they sum to 1
         np.testing.assert_array_equal(np.where(p[:, 0] > 0, 0, top), ids)
         assert (np.abs(p.sum(1) - 1.0) <= 2.0**-23).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("lows", [1, 3, 8])
+def test_min_p_at_the_weight_of_an_id(lows, dtype, cuda_lib):
+    """min_p next to the weight of ids that have a part of the row to themselves: the passes that
+    sum and the one that draws agree on whether they are kept, one to a lane or many."""
+    vocab, top = 9001, 8000
+    rows, weights = [], []
+    for j in range(1, 161):
+        low = 10.0 - j / 16.0
+        w = math.exp(low - 10.0)
+        for steps in range(-6, 7):
+            row = np.full(vocab, -100.0)
+            row[:lows], row[top] = low, 10.0
+            rows.append(row)
+            weights.append(w * (1.0 + steps * 2.0**-52))
+    values, n = rounded(np.stack(rows), dtype), len(rows)
+    for k, p in ((0, 1.0), (0, 0.9999999), (20, 1.0), (600, 0.9999999)):
+        policies = np.stack([np.ones(n), np.full(n, k), np.full(n, p), weights], axis=1)
+        ids, status = raw_sample(values, None, dtype, policies, np.zeros(n))
+        assert (status == 0).all() and np.isin(ids, (0, top)).all()
+        probs, st = ox.policy_probs(to_device(values, dtype), None, gpu(policies))
+        probs = host(probs).astype(np.float64)
+        assert not host(st).any()
+        np.testing.assert_array_equal(np.where(probs[:, 0] > 0, 0, top), ids)
+        # each of the 9 probabilities at most is rounded by 2^-24 of itself
+        assert (np.abs(probs.sum(1) - 1.0) <= 2.0**-23).all()
