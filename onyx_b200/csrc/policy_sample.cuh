@@ -60,6 +60,7 @@
 
 #include "onyx_common.cuh"
 #include "policy_ring.cuh"
+#include "warp_prefix.cuh"
 
 namespace onyx {
 
@@ -178,6 +179,19 @@ __device__ __forceinline__ uint32_t warp_scan(uint32_t v, int lane) {  // inclus
   }
   return v;
 }
+
+struct PsLane {  // of ps_prefix_sum()
+  double x;
+  int lane;
+  __device__ __forceinline__ PsLane add_up(int d) const {
+    const double o = __shfl_up_sync(~0u, x, d);
+    return {lane >= d ? x + o : x, lane};
+  }
+  __device__ __forceinline__ PsLane max_up(int d) const {
+    const double o = __shfl_up_sync(~0u, x, d);
+    return {lane >= d && o > x ? o : x, lane};
+  }
+};
 
 // 2^(j/16), filled by every CTA when it starts.
 struct PsPowers {
@@ -714,8 +728,9 @@ struct PolicyRow {
   }
 
   // Exclusive scans over the CTA's threads, and the totals. The end of one thread's part is the
-  // start of the next one's bit for bit: each goal lies in one thread's part only. The parts
-  // are read by every thread, so a __syncthreads() has to lie between two calls.
+  // start of the next one's bit for bit, and no end lies below its start: each goal lies in one
+  // thread's part only, which alone writes where it is reached. The parts are read by every
+  // thread, so a __syncthreads() has to lie between two calls.
   struct Scanned {
     uint32_t count_before, count_all;
     double mass_before, mass_end, mass_all;
@@ -723,7 +738,7 @@ struct PolicyRow {
   __device__ Scanned scan_parts(uint32_t count, double mass, bool masses) {
     Scanned s = {};
     const uint32_t count_incl = warp_scan(count, lane);
-    const double incl = masses ? warp_scan(mass, lane) : 0.0;
+    const double incl = masses ? ps_prefix_sum(PsLane{mass, lane}).x : 0.0;
     if (lane == 31) sh.part_count[warp] = count_incl, sh.part_mass[warp] = incl;
     __syncthreads();
     const uint32_t c = lane < kPsWarps ? sh.part_count[lane] : 0u;
