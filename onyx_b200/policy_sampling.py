@@ -156,13 +156,24 @@ def _uniform_code(uniforms: torch.Tensor, shape: tuple[int, ...]) -> int:
 
 
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether the byte ranges that the two tensors span meet."""
-    def span(t: torch.Tensor) -> tuple[int, int]:
-        last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
-        return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+    """Whether a row (last dimension) of the one shares memory with a row of the other."""
+    def layout(t: torch.Tensor) -> tuple[int, int, int, int]:  # first byte, step, rows, length
+        size = t.element_size()
+        step, count = (t.stride(0) * size, t.shape[0]) if t.dim() > 1 else (0, 1)
+        return t.data_ptr(), step, count, t.shape[-1] * size
 
-    (a0, a1), (b0, b1) = span(a), span(b)
-    return a.device == b.device and a0 < b1 and b0 < a1
+    (a0, a_step, a_rows, a_len), (b0, b_step, b_rows, b_len) = layout(a), layout(b)
+    if (a.device != b.device or a0 + (a_rows - 1) * a_step + a_len <= b0
+            or b0 + (b_rows - 1) * b_step + b_len <= a0):
+        return False
+    while a_rows and b_rows:  # the spans meet: row by row, in rising order of address
+        if a0 < b0 + b_len and b0 < a0 + a_len:
+            return True
+        if a0 < b0:
+            a0, a_rows = a0 + a_step, a_rows - 1
+        else:
+            b0, b_rows = b0 + b_step, b_rows - 1
+    return False
 
 
 def _rows_of(logits: torch.Tensor, bitmask: torch.Tensor | None):

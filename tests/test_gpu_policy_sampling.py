@@ -1048,3 +1048,20 @@ def test_min_p_at_the_weight_of_an_id(lows, dtype, cuda_lib):
         np.testing.assert_array_equal(np.where(probs[:, 0] > 0, 0, top), ids)
         # each of the 9 probabilities at most is rounded by 2^-24 of itself
         assert (np.abs(probs.sum(1) - 1.0) <= 2.0**-23).all()
+
+
+def test_probs_beside_the_logits_in_one_buffer(cuda_lib):
+    """Logits and probabilities as two columns of one float32 buffer share no memory."""
+    rng = np.random.default_rng(111)
+    x = normal(rng, (6, 3001), "f32")
+    both = torch.full((6, 2, 3010), 7.0, device="cuda")
+    both[:, 0, :3001] = to_device(x, "f32")
+    policies = table(POLICIES["all"], 6)
+    p, status = ox.policy_probs(both[:, 0, :3001], None, gpu(policies), out=both[:, 1, 4:3005])
+    assert not status.any()
+    assert_probs(p, opol.probs(f64(x, "f32"), None, policies)[0])
+    np.testing.assert_array_equal(host(both[:, 0, :3001]), x)
+    assert (host(both[:, 0, 3001:]) == 7).all() and (host(both[:, 1, :4]) == 7).all()
+    assert (host(both[:, 1, 3005:]) == 7).all()
+    with pytest.raises(ValueError, match="share memory"):
+        ox.policy_probs(both[:, 0, :3001], None, gpu(policies), out=both.view(6, -1)[:, 3000:6001])

@@ -296,3 +296,31 @@ def test_prefix_sums_never_fall(warp_prefix):
         for i in range(32):
             want = math.fsum(v[: i + 1])
             assert abs(got[i] - want) <= 31 * 2.0**-53 * want
+
+
+# --------------------------------------------------------------------------------------
+# outputs that share memory with an input
+# --------------------------------------------------------------------------------------
+def test_overlap_is_that_of_rows():
+    """Rows that lie between each other's share nothing, though the spans do."""
+    from onyx_b200.policy_sampling import _overlap
+
+    both = torch.zeros(5, 2, 40)
+    assert not _overlap(both[:, 0], both[:, 1])
+    assert not _overlap(both[:, 1], both[:, 0])
+    assert _overlap(both[:, 0], both[:, 0])
+    flat = torch.zeros(5, 100)
+    assert not _overlap(flat[:, :30], flat[:, 30:60])
+    assert _overlap(flat[:, :31], flat[:, 30:60])
+    assert _overlap(flat[:, 30:60], flat[:, :31])
+    assert _overlap(flat[4:], flat) and _overlap(flat, flat[2:3])
+    assert not _overlap(flat[:2], flat[2:]) and not _overlap(flat[3:], flat[:3])
+    assert not _overlap(flat, torch.zeros(5, 100))
+    # rows of other types and other distances
+    words = flat.view(torch.int32)
+    assert not _overlap(words[:, 60:64], flat[:, :60]) and _overlap(words[:, 59:64], flat[:, :60])
+    line = torch.zeros(400, dtype=torch.float64)
+    assert _overlap(line[:8].view(2, 4), line.view(torch.float32)[8:80].view(2, 36))
+    assert not _overlap(line[:8].view(2, 4), line.view(torch.float32)[16:80].view(2, 32))
+    assert not _overlap(line[20:24], line.view(torch.float32)[:320].view(4, 80)[:, :40])
+    assert _overlap(line[18:24], line.view(torch.float32)[:320].view(4, 80)[:, :40])
