@@ -16,6 +16,7 @@ relative, plus its sums' error and, below float32's smallest normal number, 2^-1
 from __future__ import annotations
 
 import ctypes
+import decimal
 import math
 
 import numpy as np
@@ -1065,3 +1066,114 @@ def test_probs_beside_the_logits_in_one_buffer(cuda_lib):
     assert (host(both[:, 1, 3005:]) == 7).all()
     with pytest.raises(ValueError, match="share memory"):
         ox.policy_probs(both[:, 0, :3001], None, gpu(policies), out=both.view(6, -1)[:, 3000:6001])
+
+
+# --------------------------------------------------------------------------------------
+# the accuracy of a weight
+# --------------------------------------------------------------------------------------
+def weight_by_bisection(low, top, dtype, policy):
+    """The largest u at which id 0 of the row [low, top] is drawn, for every `low`: the kernel
+    draws it while w > u (w + 1), so u = w / (w + 1). Bits of float64 numbers are halved."""
+    values = rounded(np.stack([low, np.full(low.size, top)], axis=1), dtype)
+    x, pol = to_device(values, dtype), gpu(policy)
+    lo = torch.zeros(low.size, dtype=torch.int64, device="cuda")
+    hi = torch.full_like(lo, int(np.float64(0.75).view(np.int64)))
+    for _ in range(63):
+        mid = lo + (hi - lo) // 2
+        r = ox.policy_sample(x, None, pol, mid.view(torch.float64))
+        drawn = r.token_ids == 0
+        lo, hi = torch.where(drawn, mid, lo), torch.where(drawn, hi, mid)
+    assert (hi - lo <= 1).all()
+    return f64(values, dtype)[:, 0], host(lo.view(torch.float64))
+
+
+def weight_error(low, top, t, u):
+    """For every id x = (low - top) / t and the relative distance of u from w / (w + 1), w = exp(x),
+    with 40 digits."""
+    with decimal.localcontext() as ctx:
+        ctx.prec = 40
+        for a, b in zip(low.tolist(), u.tolist()):
+            x = (decimal.Decimal(a) - decimal.Decimal(top)) / decimal.Decimal(t)
+            w = x.exp()
+            yield float(x), float(decimal.Decimal(b) * (w + 1) / w - 1)
+
+
+@pytest.mark.parametrize("t", [1.0, 0.7, 3.3, 0.01])
+def test_accuracy_of_a_weight(t, cuda_lib):
+    """exp2_table() is within 2^-50. Its argument (v - max) log2(e) 16 / T is rounded by four
+    operations (1 / T, the constant, their product, the last product), each by 2^-53 of it: a
+    relative error of |x| 4 2^-53 of w = exp(x). The sum w + 1, its product with u and the last
+    place of u add 4 2^-53."""
+    rng = np.random.default_rng(120)
+    low = -rng.uniform(0.0, 690.0 * t, 2000)
+    low[:400] = -rng.uniform(0.0, 2.0 * t, 400)
+    low, u = weight_by_bisection(low, 0.0, "f32", (t, 0, 1.0, 1e-305))
+    for x, err in weight_error(low, 0.0, t, u):
+        assert abs(err) <= 2.0**-50 + abs(x) * 2.0**-51 + 2.0**-51, (x, err * 2.0**50)
+
+
+@pytest.mark.parametrize("t", [1.0, 0.7, 1.3])
+def test_accuracy_of_a_weight_from_the_table(t, cuda_lib):
+    """bfloat16 rows under top-p: a weight is the first of 8 times a ratio up to 7 times, each of
+    the eight factors within 2^-50 and their products rounded: 2^-47 + 7 2^-53, beside the
+    argument's part and 4 2^-53 for the sum, the product and u."""
+    low = 10.0 - np.arange(1, int(15 * t * 16)) / 16.0
+    low, u = weight_by_bisection(low, 10.0, "bf16", (t, 0, 0.9999999, 0.0))
+    for x, err in weight_error(low, 10.0, t, u):
+        assert abs(err) <= 2.0**-47 + abs(x) * 2.0**-51 + 11 * 2.0**-53, (x, err * 2.0**50)
+
+
+# --------------------------------------------------------------------------------------
+# the largest sizes
+# --------------------------------------------------------------------------------------
+@pytest.mark.parametrize("vocab", [1 << 30, (1 << 30) - 5])
+def test_longest_rows(vocab, cuda_lib):
+    """The longest row, whole and from an odd offset: the first maximum, the first k of the
+    ranking, and draws by float64 sums of pieces. Two sums of n weights decide a draw, each
+    within n 2^-53 of its value: the mass up to the id drawn is within 2 n 2^-53 of u times the
+    total, but for that id's own weight."""
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    x = torch.empty(1, 1 << 30, dtype=torch.bfloat16, device="cuda")
+    for part in x[0].split(1 << 27):
+        part.copy_(torch.randn(part.numel(), generator=gen, device="cuda").mul_(3.0))
+    x = x[:, (1 << 30) - vocab:]
+    top = x.max()
+    pol = gpu((0.0, 0, 1.0, 0.0))
+    half = torch.full((1,), 0.5, dtype=torch.float64, device="cuda")
+    want = int((x[0] == top).nonzero()[0])
+    assert int(ox.policy_sample(x, None, pol, half).token_ids) == want
+    # the first three of the ranking: values falling, ids rising among equals
+    levels = torch.cat([p.topk(3)[0] for p in x[0].split(1 << 27)]).sort(descending=True)[0][:3]
+    some = (x[0] >= levels[-1]).nonzero().squeeze(1)
+    first = sorted(some.tolist(), key=lambda i: (-float(x[0, i]), i))[:3]
+    got = [int(ox.policy_sample(x, None, gpu((1.0, 3, 1.0, 0.0)),
+                                torch.tensor([u], device="cuda")).token_ids)
+           for u in (0.0, 0.5, 1.0 - 2.0**-24)]
+    assert set(got) <= set(first) and got[0] == min(first) and got[-1] == max(first)
+    masses = torch.stack([torch.exp(p.double() - top.double()).sum()
+                          for p in x[0].split(1 << 24)]).cumsum(0)
+    for u in (1e-9, 0.37, 0.9999):
+        r = ox.policy_sample(x, None, gpu((1.0, 0, 1.0, 0.0)), half * 0 + u)
+        at = int(r.token_ids)
+        assert not r.status.any() and 0 <= at < vocab
+        piece = at >> 24
+        w = torch.exp(x[0, piece << 24: at + 1].double() - top.double())
+        through = float(w.sum()) + (float(masses[piece - 1]) if piece else 0.0)
+        total = float(masses[-1])
+        slack = 2 * vocab * 2.0**-53 * total
+        assert through - float(w[-1]) - slack <= u * total <= through + slack
+
+
+def test_many_short_rows(cuda_lib):
+    """More rows than 16 bits count, of 3 ids each."""
+    rng = np.random.default_rng(130)
+    rows = 70001
+    x = normal(rng, (rows, 3), "f32")
+    policies = np.stack([POLICIES[n] for n in ("plain", "greedy", "top_k1", "top_p", "min_p")])
+    policies = policies[np.arange(rows) % 5]
+    u = rng.random(rows)
+    ids, status = raw_sample(x, None, "f32", policies, u)
+    assert (status == 0).all()
+    some = np.concatenate([np.arange(500), np.arange(rows - 500, rows)])
+    want = opol.sample(f64(x[some], "f32"), None, policies[some], u[some])[0]
+    np.testing.assert_array_equal(ids[some], want)
