@@ -180,19 +180,6 @@ __device__ __forceinline__ uint32_t warp_scan(uint32_t v, int lane) {  // inclus
   return v;
 }
 
-struct PsLane {  // of ps_prefix_sum()
-  double x;
-  int lane;
-  __device__ __forceinline__ PsLane add_up(int d) const {
-    const double o = __shfl_up_sync(~0u, x, d);
-    return {lane >= d ? x + o : x, lane};
-  }
-  __device__ __forceinline__ PsLane max_up(int d) const {
-    const double o = __shfl_up_sync(~0u, x, d);
-    return {lane >= d && o > x ? o : x, lane};
-  }
-};
-
 // 2^(j/16), filled by every CTA when it starts.
 struct PsPowers {
   double at[16];
@@ -728,17 +715,22 @@ struct PolicyRow {
   }
 
   // Exclusive scans over the CTA's threads, and the totals. The end of one thread's part is the
-  // start of the next one's bit for bit, and no end lies below its start: each goal lies in one
-  // thread's part only, which alone writes where it is reached. The parts are read by every
-  // thread, so a __syncthreads() has to lie between two calls.
+  // start of the next one's; first_to_reach() tells which one reaches a goal. The parts are read
+  // by every thread, so a __syncthreads() has to lie between two calls.
   struct Scanned {
     uint32_t count_before, count_all;
+    double mass_start;  // of the warp's first thread
     double mass_before, mass_end, mass_all;
   };
+  // Whether this thread is the one to write where the sum reaches `goal`; one thread at most is.
+  // Whole warp; `start` is the warp's, `reached` whether the thread's end is at the goal.
+  __device__ __forceinline__ bool first_to_reach(bool reached, double start, double goal) const {
+    return ps_first_to_reach(__ballot_sync(~0u, reached), lane, start, goal);
+  }
   __device__ Scanned scan_parts(uint32_t count, double mass, bool masses) {
     Scanned s = {};
     const uint32_t count_incl = warp_scan(count, lane);
-    const double incl = masses ? ps_prefix_sum(PsLane{mass, lane}).x : 0.0;
+    const double incl = masses ? warp_scan(mass, lane) : 0.0;
     if (lane == 31) sh.part_count[warp] = count_incl, sh.part_mass[warp] = incl;
     __syncthreads();
     const uint32_t c = lane < kPsWarps ? sh.part_count[lane] : 0u;
@@ -759,8 +751,9 @@ struct PolicyRow {
     __syncthreads();
     const double prev = __shfl_up_sync(~0u, incl, 1), mine = sh.sums_before[warp];
     s.mass_all = sh.sums_before[kPsWarps];
+    s.mass_start = mine;
     s.mass_before = lane ? mine + prev : mine;
-    s.mass_end = mine + incl;
+    s.mass_end = ps_part_end(mine, incl, sh.sums_before[warp + 1]);
     return s;
   }
 
@@ -865,10 +858,11 @@ struct PolicyRow {
     if (threadIdx.x < 2) sh.cross[threadIdx.x].bin = -1;
     const Scanned scan = scan_parts(count, mass, by_mass);
     uint32_t count_before = scan.count_before;
-    double mass_before = scan.mass_before, mass_end = scan.mass_end;
+    double mass_start = scan.mass_start, mass_before = scan.mass_before;
+    double mass_end = scan.mass_end;
     if (mine >= kPsHalf) {  // the values next to zero lie between the halves
       count_before += sum.small;
-      mass_before += sum.mass, mass_end += sum.mass;
+      mass_start += sum.mass, mass_before += sum.mass, mass_end += sum.mass;
     }
     const uint32_t in_bins = scan.count_all + sum.small;
     // ids at and below -2^7 lie behind the bins; they may weigh nothing next to the rest
@@ -906,8 +900,9 @@ struct PolicyRow {
     if (by_mass) {
       if (!by_k && behind_weighs) return false;
       const double goal = pol.top_p * total;
-      if (count && mine <= cut_bin && mass_before < goal &&
-          (goal <= mass_end || cut_bin < mine + kPsOwn)) {
+      // the bins of this thread reach it, or hold the last of the k
+      const bool ends = goal <= mass_end || (mine <= cut_bin && cut_bin < mine + kPsOwn);
+      if (first_to_reach(ends, mass_start, goal) && count && mine <= cut_bin) {
         PsCross x = {mass_before, 0u, 0u, -1};  // the bin that reaches the goal, else the last
         double run = mass_before, weight = 0.0;
 #pragma unroll
@@ -1073,7 +1068,7 @@ struct PolicyRow {
       const double goal = pol.top_p * total;
       // cross[at]: the bin in which the mass reaches `mark`, ids before it and in it
       auto mark_bin = [&](int at, double mark) {
-        if (count && scan.mass_before < mark && mark <= scan.mass_end) {
+        if (first_to_reach(mark <= scan.mass_end, scan.mass_start, mark) && count) {
           PsCross x = {0.0, scan.count_before, 0u, -1};
           double run = scan.mass_before;
 #pragma unroll
@@ -1366,8 +1361,9 @@ struct PolicyRow {
       const Scanned scan2 = scan_parts(0u, mass_low, true);
       const double hb = above + scan.mass_before, high_end = above + scan.mass_end;
       const double lb = above + scan2.mass_before, low_end = above + scan2.mass_end;
+      const double high_start = above + scan.mass_start, low_start = above + scan2.mass_start;
       const double least = goal * (1.0 - 1e-12), most = goal * (1.0 + 1e-12);
-      if (count && hb < least && least <= high_end) {
+      if (first_to_reach(least <= high_end, high_start, least) && count) {
         PsCross x = {0.0, before, 0u, -1};
         double run = hb;
         uint32_t run_count = before;
@@ -1380,7 +1376,7 @@ struct PolicyRow {
           }
         sh.cross[0] = x;
       }
-      if (count && lb < most && most <= low_end) {
+      if (first_to_reach(most <= low_end, low_start, most) && count) {
         PsCross x = {0.0, before, 0u, -1};
         double run = lb;
 #pragma unroll

@@ -1,28 +1,32 @@
-// Inclusive sums over the 32 lanes of a warp, of masses that are not negative. The steps are
-// written over a value per lane `L` with add_up(d) (each lane adds what the lane d below had)
-// and max_up(d) (the larger of the two), so that the host's checks run the same lines on 32
-// numbers.
-// The lanes' sums are added up in trees that differ, so that one may come out a last place below
-// that of the lane before it; the second loop takes that back. So no goal lies in the parts of two
-// lanes. (Rounding keeps order: fl(a + b) <= fl(a + c) for b <= c, so offsets added to all of them
-// do too.)
+// Where a running sum of masses reaches a goal, over the threads of a CTA: which thread says so.
+// Plain C++ on a lane's numbers; the kernel and the host's checks run the same lines.
+//
+// A warp's lanes hold inclusive sums of their masses by a shuffle scan, whose sums are added up in
+// trees that differ: one may come out a last place below that of the lane before it, and an inner
+// one above the warp's whole sum. So a test of each lane's own interval can hold for two lanes, or
+// for lanes of two warps. Here the warps' starts, which are added up one after the other and never
+// fall, choose the warp, and the first lane whose end reaches the goal is the one.
 #pragma once
 
+#include <cstdint>
+
 #ifdef __CUDACC__
-#define PS_LANES __device__ __forceinline__
+#define PS_HOST_DEVICE __host__ __device__ __forceinline__
 #else
-#define PS_LANES inline
+#define PS_HOST_DEVICE inline
 #endif
 
 namespace onyx {
 
-template <class L>
-PS_LANES L ps_prefix_sum(L v) {
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) v = v.add_up(d);
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) v = v.max_up(d);
-  return v;
+// End of a lane's part: the warp's start and the lane's sum, no later than the warp's end.
+PS_HOST_DEVICE double ps_part_end(double warp_start, double incl, double warp_end) {
+  const double end = warp_start + incl;
+  return end < warp_end ? end : warp_end;
+}
+
+// `reached`: the lanes whose end is at the goal or past it.
+PS_HOST_DEVICE bool ps_first_to_reach(uint32_t reached, int lane, double warp_start, double goal) {
+  return warp_start < goal && (reached & (0u - reached)) == 1u << lane;
 }
 
 }  // namespace onyx

@@ -260,42 +260,51 @@ def test_layouts(cuda_lib):
 
 
 # --------------------------------------------------------------------------------------
-# prefix sums of masses
+# where a running sum reaches a goal
 # --------------------------------------------------------------------------------------
 @pytest.fixture(scope="session")
-def warp_prefix(tmp_path_factory):
-    """The kernel's prefix sum over a warp, on the host."""
+def crossings(tmp_path_factory):
+    """Which of 512 threads say that the sum of their masses reaches a goal, on the host; and
+    which would if each tested its own interval."""
     src = Path(__file__).resolve().parent / "native" / "warp_prefix.cpp"
     lib = tmp_path_factory.mktemp("prefix") / "warp_prefix.so"
     subprocess.run(["g++", "-O1", "-std=c++17", "-shared", "-fPIC", "-ffp-contract=off",
                     str(src), "-o", str(lib)], check=True)
-    fn = ctypes.CDLL(str(lib)).warp_prefix
-    pointer = ctypes.POINTER(ctypes.c_double)
+    fn = ctypes.CDLL(str(lib)).crossings
 
-    def call(values):
-        values, out = np.ascontiguousarray(values, np.float64), np.empty(32)
-        fn(values.ctypes.data_as(pointer), out.ctypes.data_as(pointer))
-        return out
+    def call(mass, goal):
+        here, own = (ctypes.c_int32 * 512)(), (ctypes.c_int32 * 512)()
+        fn(mass.ctypes.data_as(ctypes.c_void_p), ctypes.c_double(goal), here, own)
+        return np.flatnonzero(here), np.flatnonzero(own)
 
     return call
 
 
-def test_prefix_sums_never_fall(warp_prefix):
-    """Each lane's sum is at least that of the lane below it: then every goal lies between the
-    ends of one lane's part alone, and one thread writes where it is reached. And each is within
-    31 2^-53 of the exact sum, relative: 5 additions to a lane, of sums of at most 32 numbers."""
+def test_one_thread_reaches_a_goal(crossings):
+    """Goals next to the ends of lanes and warps, where rounding decides: one thread writes where
+    the sum reaches it, whose part ends within 512 2^-53 of there. (Of the threads' own
+    intervals, some hold the same goal.)"""
     rng = np.random.default_rng(0)
-    for trial in range(3000):
-        v = rng.random(32) ** rng.integers(1, 12)
+    twice = 0
+    for trial in range(60):
+        mass = rng.random(512) ** rng.integers(1, 12)
         if trial % 3 == 1:
-            v = np.exp(-rng.random(32) * 40)
+            mass = np.exp(-rng.random(512) * 40)
         if trial % 3 == 2:
-            v[rng.random(32) < 0.5] = 0.0
-        got = warp_prefix(v)
-        assert (np.diff(got) >= 0).all(), trial
-        for i in range(32):
-            want = math.fsum(v[: i + 1])
-            assert abs(got[i] - want) <= 31 * 2.0**-53 * want
+            mass[rng.random(512) < 0.5] = 0.0
+        cum = np.cumsum(mass)
+        for at in (*range(20, 44), *rng.integers(0, 511, 20)):
+            for steps in range(-3, 4):
+                goal = cum[at] * (1.0 + steps * 2.0**-53)
+                here, own = crossings(mass, goal)
+                twice += own.size > 1
+                assert here.size == 1, (trial, at, steps, here)
+                i = int(here[0])
+                slack = 512 * 2.0**-53 * cum[-1]
+                assert cum[i] + slack >= goal >= (cum[i - 1] if i else 0.0) - slack
+    assert twice  # else the masses test nothing
+    assert crossings(mass, cum[-1] * 1.01)[0].size == 0
+    assert crossings(mass, 0.0)[0].size == 0
 
 
 # --------------------------------------------------------------------------------------
