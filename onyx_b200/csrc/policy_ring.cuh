@@ -26,12 +26,12 @@ PS_HOST_DEVICE PsInner ps_inner_chunks(int id_first, int n, int vocab, int chunk
   return in;
 }
 
-// What the ring starts when chunk `next` comes up: a chunk inside the row, one at its edge, or
-// nothing.
-enum PsCopy : int { kCopyNone = 0, kCopyWhole = 1, kCopyEdge = 2 };
-PS_HOST_DEVICE PsCopy ps_copy_at(int next, int n, const PsInner& in) {
-  if (next >= in.from && next < in.to) return kCopyWhole;
-  return next < n ? kCopyEdge : kCopyNone;
+// Whether the ring copies chunk `next` when it comes up, as one inside the row, or else as one of
+// its own at an edge of the row. (Two tests in the loop: with the answer as one value of three,
+// 1,024 rows of 256,000 bfloat16 took 396 us, so 387.)
+PS_HOST_DEVICE bool ps_copies_inner(int next, const PsInner& in) {
+  return next >= in.from && next < in.to;
 }
+PS_HOST_DEVICE bool ps_copies_edge(int next, int n) { return next < n; }
 
 }  // namespace onyx

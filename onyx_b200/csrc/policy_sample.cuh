@@ -1951,13 +1951,12 @@ __device__ __forceinline__ PsFirst first_pass(const RowView<DT>& view, int lane,
   for (int i = 0; i < n; ++i) {
     if (!kept) {
       const int next = i + ahead;
-      const PsCopy what = ps_copy_at(next, n, inner);
-      if (what == kCopyWhole) {
+      if (ps_copies_inner(next, inner)) {
         ps_copy16(fill + (DT == kF32 ? (lane & 1) * 512 + (lane >> 1) * 16 : lane * 16), src);
         if (DT == kF32)
           ps_copy16(fill + (lane & 1) * 512 + (lane >> 1) * 16 + 256, src + 32 * kVec);
         if (mask) view.copy_words(fill, lane, id_first + next * kPsChunk);
-      } else if (what == kCopyEdge) {
+      } else if (ps_copies_edge(next, n)) {
         view.copy_chunk(fill, lane, id_first + next * kPsChunk);
       }
       src += kPsChunk;

@@ -16,7 +16,7 @@ extern "C" void ring_copies(int id_first, int n, int vocab, int chunk, int depth
   size_t landed = 0;
   for (int i = 0; i < n; ++i) {
     const int next = i + depth - 1;
-    const bool some = ps_copy_at(next, n, in) != kCopyNone;
+    const bool some = ps_copies_inner(next, in) || ps_copies_edge(next, n);
     groups.push_back(some ? next : -1);
     out[0] += some && next >= n;
     landed = groups.size() - (depth - 1);  // all but the latest depth - 1
