@@ -637,7 +637,8 @@ struct RowCut {
   // a bound below which none passes, which spares looking at them.
   __device__ __forceinline__ void bound_by_min_p() {
     if (flat || !(min_p > 0.0)) return;
-    const double low = top + log(min_p) / inv_t * (1.0 + 1e-9) - fabs(top) * 1e-9;
+    // (1e-9 for what the weights round: at a high temperature many values weigh exactly 1)
+    const double low = top + (log(min_p) * (1.0 + 1e-9) - 1e-9) / inv_t - fabs(top) * 1e-9;
     const float bound = nextafterf(__double2float_rd(low), -INFINITY);
     if (bound >= cut) keep(bound, 0u);
   }

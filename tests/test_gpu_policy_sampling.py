@@ -1177,3 +1177,24 @@ def test_many_short_rows(cuda_lib):
     some = np.concatenate([np.arange(500), np.arange(rows - 500, rows)])
     want = opol.sample(f64(x[some], "f32"), None, policies[some], u[some])[0]
     np.testing.assert_array_equal(ids[some], want)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+def test_min_p_where_weights_round_to_equal(dtype, cuda_lib):
+    """min_p keeps the ids whose float64 weight reaches it: values that differ by less than
+    2^-56 T weigh exactly 1, as the largest does."""
+    rng = np.random.default_rng(140)
+    x = rng.standard_normal((4, 5003)) * 3
+    x[1, ::3] = -np.inf
+    x[2] = np.round(x[2])
+    x[3] += 100.0
+    x = rounded(x, dtype)
+    m = workloads.bernoulli_masks(rng, np.full(4, 0.5), 5003)
+    for policy in ((1e20, 0, 1.0, 1.0), (1e300, 0, 0.5123, 1.0), (1e30, 700, 1.0, 1.0),
+                   (1e30, 20, 0.77, 1.0), (1e38, 0, 1.0, 0.999)):
+        check(x, None, dtype, table(policy, 4), rng.random(4))
+        check(x, m, dtype, table(policy, 4), rng.random(4))
+    tiny = rounded(rng.standard_normal((4, 5003)) * (1e-5 if dtype == "f16" else 1e-25), dtype)
+    t = 1e13 if dtype == "f16" else 1.0
+    for policy in ((t, 0, 1.0, 1.0), (t, 0, 0.5123, 1.0), (t, 30, 1.0, 1.0)):
+        check(tiny, m, dtype, table(policy, 4), rng.random(4))
