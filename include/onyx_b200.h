@@ -203,13 +203,16 @@ ONYX_API int onyx_masked_sample(const void* logits, int dtype, int64_t rows, int
  * r * policy_stride (0: one policy for every row, else >= 4).
  *
  * The distribution of a row. Ids are the mask's (NULL: every id). Weights are
- * exp((v - max) / temperature) in float64, 0 below 2^-1000; where any value is +inf the +inf ids share the
- * mass alone; temperature 0 keeps the first maximum alone. Ids are ranked by value, the
- * lowest id first among equals. top_k keeps the first k of the ranking; top_p the shortest
- * prefix of those whose mass reaches top_p times their mass (1: off; float32 and float16: a
- * mass within 2^-48 of that has reached it, which covers what the sums round); min_p the ids whose
- * weight is at least min_p times the largest. With top_k = 0 and min_p = 0 this is the
- * distribution of onyx_masked_sample, the reference's _filtered_reference_weights
+ * exp((v - max) / temperature) in float64, 0 below 2^-1000; where any value is +inf the +inf
+ * ids share the mass alone; temperature 0 keeps the first maximum alone. Ids are ranked by
+ * value, the lowest id first among equals. top_k keeps the first k of the ranking; top_p the
+ * shortest prefix of those whose mass reaches top_p times their mass (1: off; float32 and
+ * float16 without a top_k, where the first pass summed all weights: a mass within 2^-48 of that
+ * has reached it, which covers what that sum rounds); min_p the ids whose weight is at least
+ * min_p times the largest. A comparison that only the rounding of a float64 sum decides may
+ * fall either way, and another way with another number of rows: the order of the sums follows
+ * the layout (onyx_policy_layout). With top_k = 0 and min_p = 0 this is the distribution of
+ * onyx_masked_sample, the reference's _filtered_reference_weights
  * (onyx_cuda/src/onyx_cuda/selection.py); only where the mass reaches top_p exactly (equal
  * values) that one's sum of rounded shares may keep one id more.
  *

@@ -47,13 +47,19 @@
 // whose sums do not depend on the order of the atomics; lists are sorted by value and id.)
 //
 // What bounds it. 256 rows of 128,256 bfloat16 (65.7 MB, 10.2 us of copying at 6,464 GB/s), one
-// policy for all: instructions. The maximum alone takes 31 us and 154 warp instructions a chunk of
-// 256 ids, over the whole kernel; with top-k 50, so with the histogram and its cut, 65 us and
-// 345, the histogram's atomics meeting 2.8 bank conflicts each; DRAM is 20 and 11 % busy, the
-// issue slots 58 and 65 %. One row of 128,256 takes 15 us under top-p 0.9: a chain of latencies,
-// 8 us of it without any histogram. A batch under mixed policies waits for its slowest rows,
-// those that keep tens of thousands of ids (T = 1.2, top-p 0.95: 139 us, against 75 under
-// T = 0.8, top-p 0.9).
+// policy for all: instructions, and CTAs that fill 1.73 waves of the 296 that fit. The maximum
+// alone takes 32 us and 153 warp instructions a chunk of 256 ids, over the whole kernel; with
+// top-k 50, so with the histogram and its cut, 65 us and 341, the histogram's atomics meeting 2.8
+// bank conflicts each; DRAM is 20 and 11 % busy, the issue slots 57 and 64 %. 64 rows of 151,664
+// float32 (0.86 waves) take 24 us for the maximum, 37 with the sum of the weights and 69 under
+// top-p 0.9, 963 instructions a chunk, 131 of them float64. One bfloat16 row of 128,256 takes
+// 15.6 us under top-p 0.9: a chain of latencies, 8 us of it without any histogram. A batch under
+// mixed policies waits for its slowest rows, those that keep tens of thousands of ids (256
+// rows at T = 1.2, top-p 0.95: 138 us, against 75 under T = 0.8, top-p 0.9).
+//
+// Registers. Two CTAs of 512 threads leave 64 to a thread, and the kernels spill: bytes stored and
+// reloaded a thread, of draw, probs and spec, float32 132/868, 140/620, 388/1,700; float16 224/960,
+// 232/608, 332/1,596; bfloat16 16/104, 60/232, 56/148. Other widths have not been measured.
 #pragma once
 
 #include <cfloat>
@@ -580,8 +586,9 @@ struct RowView {
 
 // 2^(y/16) for |y| < 2^20. Table-driven in the manner of Tang (ACM TOMS 15, 1989): y = 16 e + j
 // + f with |f| <= 1/2, 2^(f/16) by its Taylor polynomial of degree 6 (the next term is below
-// 5e-16): within 2^-50 of the value, and 1 for y = 0. The 16 entries take the 16 pairs of
-// banks, so lookups of a warp do not conflict.
+// 5e-16): within 2^-50 of 2^(y/16), and 1 for y = 0. (A weight exp(x) has the rounding of y on top,
+// up to |x| 2^-51 of it: 1/T, the constant, their product and y are rounded.) The 16 entries take
+// the 16 pairs of banks, so lookups of a warp do not conflict.
 constexpr double kPsShift = 0x1.8p52;
 __device__ __forceinline__ double exp2_parts(double t, double f, const PsPowers& powers) {
   const int n = __double2loint(t);
@@ -832,7 +839,7 @@ struct PolicyRow {
     const bool by_mass = pol.top_p < 1.0;
     // The mass of a bin is count times weight. The values of 8 bins are equally spaced, their
     // weights a geometric series, which starts at the row's maximum in the bins that hold it
-    // (those above are empty).
+    // (those above are empty). Up to eight factors, each within 2^-50: a weight within 2^-47.
     double weight_of[kPsOwn], mass = 0.0;
     uint32_t count = 0;
 #pragma unroll
@@ -1009,7 +1016,7 @@ struct PolicyRow {
     // that). Many ids there mean that few of them carry the mass alone; then the errors of the
     // bins cancel: to some 5e-4 of the goal with a list of 200 by that bound, to 2e-4 where 1/320
     // still holds over 1,024. Such rows take the widest of 1/320, 1/700 and 1/1536 that makes a
-    // list, and the list is checked (of 96,000 rows some 20 fail there).
+    // list, and the list is checked.
     double mass = 0.0, weight_of[kPsOwn];
     uint32_t count = 0;
 #pragma unroll

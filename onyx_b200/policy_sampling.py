@@ -21,7 +21,8 @@ the columns temperature, top_k, top_p, min_p: :func:`pack_policies` makes it fro
 may be rewritten in place between calls or graph replays. Values outside their ranges, which
 the host cannot see, are reported per row as ``STATUS_BAD_POLICY``.
 
-Nothing here synchronises the device; results stay on the GPU.
+The three calls do not synchronise the device, and their results stay on the GPU;
+:func:`pack_policies` copies from the host, which waits for the current stream.
 """
 
 from __future__ import annotations
@@ -218,7 +219,7 @@ def policy_probs(logits: torch.Tensor, bitmask: torch.Tensor | None, policies: t
 
     0 for ids that are not kept, and throughout a row with a status. ``out``: a float32
     tensor of that shape to write to, its rows at any stride of at least V (a draft step's
-    ``draft_probs[:, i]``)."""
+    ``draft_probs[:, i]``); no row of it may share memory with one of an input."""
     x, m, code, rows, vocab = _rows_of(logits, bitmask)
     pol, pol_stride = _policy_rows(policies, rows)
     if out is None:
