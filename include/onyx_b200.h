@@ -230,7 +230,8 @@ ONYX_API int onyx_policy_sample(const void* logits, int dtype, int64_t rows, int
 
 /*
  * The distribution itself: out + r * out_stride gets row r's vocab probabilities, rounded
- * once to float, 0 for the ids that are not kept and for every id of a row with a status.
+ * once to float, 0 for the ids that are not kept and for every id of a row with a status. Rows of
+ * out must not share memory with one another or with rows of an input.
  */
 ONYX_API int onyx_policy_probs(const void* logits, int dtype, int64_t rows, int64_t vocab,
                                int64_t row_stride, const uint32_t* mask, int64_t mask_stride,

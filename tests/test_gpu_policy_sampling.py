@@ -1198,3 +1198,44 @@ def test_min_p_where_weights_round_to_equal(dtype, cuda_lib):
     t = 1e13 if dtype == "f16" else 1.0
     for policy in ((t, 0, 1.0, 1.0), (t, 0, 0.5123, 1.0), (t, 30, 1.0, 1.0)):
         check(tiny, m, dtype, table(policy, 4), rng.random(4))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("rows,vocab", [(6, 50021), (70, 128256)])
+def test_masks_of_a_grammar(rows, vocab, dtype, cuda_lib):
+    """A handful of valid ids, one, a long run, two runs far apart, all but a run, and a run that
+    ends with the row; NaN and infinities in masked places. Kept rows and streamed ones."""
+    if rows == 70:
+        assert_ring(rows, vocab, dtype, True)
+    rng = np.random.default_rng(150 + rows)
+    x, _, u = ring_rows(rows, vocab, 0, False, dtype, 151)
+    valid = np.zeros((rows, vocab), bool)
+    for r in range(rows):
+        a = int(rng.integers(0, vocab - 20000))
+        kind = r % 6
+        if kind == 0:
+            valid[r, rng.integers(0, vocab, 10)] = True
+        elif kind == 1:
+            valid[r, a] = True
+        elif kind == 2:
+            valid[r, a: a + 17001] = True
+        elif kind == 3:
+            valid[r, :37] = valid[r, vocab - 5000:] = True
+        elif kind == 4:
+            valid[r] = True
+            valid[r, a: a + 9000] = False
+        else:
+            valid[r, vocab - 3:] = True
+    x = torch.where(torch.from_numpy(valid).cuda(), x, float("nan"))
+    x[::2] = torch.where(x[::2].isnan(), float("inf"), x[::2])
+    m = np.packbits(np.pad(valid, ((0, 0), (0, -vocab % 32))), axis=1, bitorder="little")
+    m = masks_to_device(m.view(np.uint32))
+    for shift in range(3):
+        policies = np.stack([POLICIES[RING_POLICIES[(r // 6 + shift) % 6]] for r in range(rows)])
+        r1 = ox.policy_sample(x, m, gpu(policies), u)
+        probs, status = ox.policy_probs(x, m, gpu(policies))
+        assert not r1.status.any() and not status.any()
+        ids, numbers = host(r1.token_ids), host(u)
+        for r in range(shift, rows, 1 if rows < 10 else 7):
+            w = oracle_row(x[r], m[r], policies[r], numbers[r], ids[r])
+            assert_probs(probs[r], w / w.sum())
